@@ -18,8 +18,10 @@ from .fused_ops import (
     run_gqa_decode_splitkv_turboquant_fused_out,
     run_paged_gqa_decode_fused,
 )
+from .page_copy import run_page_copy, run_page_gather
 from .pools import Qwen3PagedLayerAllocator, TurboQuantLayerPool, resolve_value_group_size
 from .prefix_block_cache import PrefixBlockPool
+from .rotary import run_multi_axis_rotary, run_rotary_paged_kv_write
 from .turboquant import VALID_KV_CACHE_QUANT_BITS, TurboQuantKVRow, TurboQuantTensorRow, turboquant_is_available
 
 __all__ = [
@@ -30,4 +32,5 @@ __all__ = [
     "gqa_decode_splitkv_turboquant_fused_out_is_available", "paged_gqa_decode_fused_is_available",
     "run_gqa_decode_fused", "run_gqa_decode_splitkv_fused", "run_gqa_decode_splitkv_fused_out",
     "run_gqa_decode_splitkv_turboquant_fused_out", "run_paged_gqa_decode_fused", "grouped_query_attention",
+    "run_multi_axis_rotary", "run_rotary_paged_kv_write", "run_page_copy", "run_page_gather",
 ]

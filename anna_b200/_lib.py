@@ -34,6 +34,12 @@ class TqLayout(ctypes.Structure):
         return {name: int(getattr(self, name)) for name, _ in self._fields_}
 
 
+class PagePool(ctypes.Structure):
+    """``anna_page_pool``: one pool of an ``anna_page_copy`` call."""
+    _fields_ = [("src", c_ptr), ("dst", c_ptr), ("page_bytes", c_i64), ("src_pages", ctypes.c_int32),
+                ("dst_pages", ctypes.c_int32), ("first_pair", ctypes.c_int32), ("count", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); the order is the declaration order of include/anna_b200_kv.h
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "anna_kv_last_error": (ctypes.c_char_p, []),
@@ -48,6 +54,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "anna_decode_plan": (c_i32, [c_i32, c_i32, c_i64, ctypes.POINTER(c_i32), ctypes.POINTER(c_i32)]),
     "anna_paged_kv_write": (c_i32, [c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_i32,
                                     c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_i32, c_ptr, c_ptr]),
+    "anna_multi_axis_rotary": (c_i32, [c_ptr, c_i64, c_i64, c_i64] * 4 + [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_f32] +
+                               [c_i32] * 7 + [c_ptr]),
+    "anna_rotary_paged_kv_write": (c_i32, [c_ptr, c_i64, c_i64, c_i64] * 4 + [c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr] +
+                                   [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_f32] + [c_i32] * 7 +
+                                   [c_i64, c_i64, c_i32, c_ptr, c_ptr]),
+    "anna_page_copy_max_pairs": (c_i32, []),
+    "anna_page_copy": (c_i32, [c_ptr, c_i32, c_ptr, c_i64, c_ptr, c_ptr, c_ptr]),
     "anna_block_table_patch": (c_i32, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i32, c_ptr]),
     "anna_paged_kv_gather": (c_i32, [c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i32, c_i32,
                                      c_i32, c_i32, c_i64, c_i64, c_i64, c_i32, c_ptr]),

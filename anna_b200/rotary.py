@@ -1,0 +1,246 @@
+"""Rotary positions with several axes (time, height and width of images and video) on queries and keys, and the same fused with
+the write of keys and values into un-quantized pages.
+
+Stands in for the rotary part of ``Qwen3Attention._forward_attention`` (``src/anna/model/ops.py:1900-1914``): pair ``i`` of a
+head is its dims ``(i, i + rotary_dim / 2)``, which a token turns by ``positions[axis(i)] * theta ** (-2 i / rotary_dim)``; the
+dims behind ``rotary_dim`` stay as they are.  ``sections`` says how many pairs belong to each axis, one section after the other
+or, with ``interleaved``, in turns: pair ``i`` belongs to axis ``a = i % n`` while ``i < n * sections[a]``, else to the first.
+The angles are exact to 32 bits for positions up to 2^31 (they are reduced to one turn in 64 bits).
+"""
+from __future__ import annotations
+
+import math
+import threading
+from collections.abc import Sequence
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .fused_ops import _require_cuda, dtype_code, on_device, ptr, stream_ptr
+
+
+@dataclass(frozen=True)
+class RotaryTables:
+    axis_count: int
+    rates: torch.Tensor  # float64 [rotary_dim / 2], turns per position
+    axes: torch.Tensor   # int32 [rotary_dim / 2]
+
+
+_TABLES: dict[tuple, RotaryTables] = {}
+_LOCK = threading.Lock()
+
+
+def pair_axes(rotary_dim: int, sections: Sequence[int] | None, interleaved: bool) -> list[int]:
+    """Axis of every pair of rotated dims."""
+    pairs = rotary_dim // 2
+    if sections is None:
+        return [0] * pairs
+    sections = [int(s) for s in sections]
+    if not sections or min(sections) < 0 or sum(sections) != pairs:
+        raise ValueError(f"sections {tuple(sections)} must be counts of pairs that add up to rotary_dim / 2 = {pairs}")
+    if interleaved:
+        count = len(sections)
+        return [i % count if i < count * sections[i % count] else 0 for i in range(pairs)]
+    return [axis for axis, size in enumerate(sections) for _ in range(size)]
+
+
+def rotary_tables(rotary_dim: int, *, theta: float = 10000.0, sections: Sequence[int] | None = None, interleaved: bool = False,
+                  inverse_frequencies: Sequence[float] | None = None, device: torch.device) -> RotaryTables:
+    """Rates and axes of the pairs on the device, made once for each set of parameters.  ``inverse_frequencies`` (radians per
+    position, one for each pair) stands in for the powers of ``theta``."""
+    key = (rotary_dim, theta, None if sections is None else tuple(sections), bool(interleaved),
+           None if inverse_frequencies is None else tuple(inverse_frequencies), device)
+    found = _TABLES.get(key)
+    if found is not None:
+        return found
+    if rotary_dim < 2 or rotary_dim % 2 != 0:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    pairs = rotary_dim // 2
+    axes = pair_axes(rotary_dim, sections, interleaved)
+    if inverse_frequencies is None:
+        if not theta > 0 or not math.isfinite(theta):
+            raise ValueError(f"theta must be positive, got {theta}")
+        frequencies = [float(theta) ** (-i / pairs) for i in range(pairs)]
+    else:
+        frequencies = [float(f) for f in inverse_frequencies]
+        if len(frequencies) != pairs:
+            raise ValueError(f"inverse_frequencies must hold rotary_dim / 2 = {pairs} values, got {len(frequencies)}")
+    with on_device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call with new rotary parameters uploads their tables: make it outside graph capture")
+    with _LOCK:
+        if len(_TABLES) >= 1024:  # parameters that change from call to call are not a model's
+            _TABLES.clear()
+        tables = RotaryTables(axis_count=1 if sections is None else len(sections),
+                              rates=torch.tensor([f / (2.0 * math.pi) for f in frequencies], dtype=torch.float64, device=device),
+                              axes=torch.tensor(axes, dtype=torch.int32, device=device))
+        _TABLES[key] = tables
+    return tables
+
+
+def _check_rows(name: str, query: torch.Tensor, key: torch.Tensor) -> None:
+    if query.dim() != 4 or key.dim() != 4:
+        raise RuntimeError(f"{name}: query and key must be [batch, heads, tokens, head_dim]")
+    if query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2] or query.shape[3] != key.shape[3]:
+        raise RuntimeError(f"{name}: query and key must agree in batch, tokens and head_dim")
+    if query.dtype != key.dtype:
+        raise RuntimeError(f"{name}: query and key must share the dtype")
+    dtype_code(query.dtype)
+
+
+def _check_positions(name: str, positions: torch.Tensor, axes: int, batch: int, tokens: int) -> tuple[int, int, int]:
+    """Element strides per axis, batch and token."""
+    if positions.dtype != torch.long:
+        raise RuntimeError(f"{name}: positions must be int64")
+    if tuple(positions.shape) == (batch, tokens) and positions.dim() == 2:
+        return 0, positions.stride(0), positions.stride(1)
+    if tuple(positions.shape) != (axes, batch, tokens):
+        raise RuntimeError(f"{name}: positions must be [{axes}, {batch}, {tokens}] (axes, batch, tokens) or [{batch}, {tokens}], "
+                           f"got {list(positions.shape)}")
+    return positions.stride(0), positions.stride(1), positions.stride(2)
+
+
+def _extent(tensor: torch.Tensor) -> tuple[int, int]:
+    last = sum((size - 1) * stride for size, stride in zip(tensor.shape, tensor.stride()))
+    return tensor.data_ptr(), tensor.data_ptr() + (last + 1) * tensor.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (begin, end), (other_begin, other_end) = _extent(a), _extent(b)
+    return begin < other_end and other_begin < end
+
+
+def _output(name: str, label: str, given: torch.Tensor | None, source: torch.Tensor, others: list[torch.Tensor]) -> torch.Tensor:
+    """The tensor that receives the turned ``source``: a new one, or the caller's (the source itself for in place)."""
+    if given is None:
+        return torch.empty(source.shape, dtype=source.dtype, device=source.device)
+    if given.shape != source.shape or given.dtype != source.dtype or given.device != source.device:
+        raise RuntimeError(f"{name}: {label} must match its input in shape, dtype and device")
+    if given.stride(3) != 1 or any(size > 1 and stride <= 0 for size, stride in zip(given.shape, given.stride())):
+        raise RuntimeError(f"{name}: {label} needs a contiguous last dim and memory of its own for every element")
+    steps = sorted((stride, size) for size, stride in zip(given.shape, given.stride()) if size > 1)
+    if any(step < (size_before - 1) * step_before + 1 for (step_before, size_before), (step, _) in zip(steps, steps[1:])):
+        raise RuntimeError(f"{name}: {label} needs memory of its own for every element")
+    if given.data_ptr() == source.data_ptr() and given.stride() == source.stride():
+        return given  # in place; other inputs may be views of the same fused projection
+    if any(_overlap(given, other) for other in (source, *others)):
+        raise RuntimeError(f"{name}: {label} must be its input itself or lie outside the memory of the inputs")
+    return given
+
+
+def _rows(tensor: torch.Tensor) -> torch.Tensor:
+    return tensor if tensor.stride(3) == 1 else tensor.contiguous()
+
+
+def run_multi_axis_rotary(*, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, theta: float = 10000.0,
+                          sections: Sequence[int] | None = None, interleaved: bool = False, rotary_dim: int | None = None,
+                          inverse_frequencies: Sequence[float] | None = None, attention_scaling: float = 1.0,
+                          query_out: torch.Tensor | None = None,
+                          key_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Turned ``[B, Hq, T, D]`` queries and ``[B, Hkv, T, D]`` keys (any strides; new contiguous tensors unless ``query_out`` /
+    ``key_out`` are given, which may be the inputs themselves).
+
+    ``positions``: int64 ``[axes, B, T]``, or ``[B, T]`` for the same on every axis.  ``sections`` (pairs per axis; None: one
+    axis), ``interleaved``, ``theta`` and ``inverse_frequencies``: see the module.  ``attention_scaling`` multiplies cosine and
+    sine.  The first call with new parameters makes their tables and cannot be captured into a graph."""
+    name = "multi_axis_rotary"
+    _check_rows(name, query, key)
+    device = _require_cuda(name, query=query, key=key, positions=positions)
+    batch, heads, tokens, dim = (int(v) for v in query.shape)
+    width = dim if rotary_dim is None else int(rotary_dim)
+    if width > dim:
+        raise RuntimeError(f"{name}: rotary_dim {width} is larger than head_dim {dim}")
+    tables = rotary_tables(width, theta=theta, sections=sections, interleaved=interleaved,
+                           inverse_frequencies=inverse_frequencies, device=device)
+    strides = _check_positions(name, positions, tables.axis_count, batch, tokens)
+    query_to = _output(name, "query_out", query_out, query, [key])
+    key_to = _output(name, "key_out", key_out, key, [query])
+    if query_out is not None and key_out is not None:
+        in_place = query_to.data_ptr() == query.data_ptr() and key_to.data_ptr() == key.data_ptr()
+        if not in_place and _overlap(query_to, key_to):
+            raise RuntimeError(f"{name}: query_out and key_out must not overlap")
+    if query.numel() == 0 or key.numel() == 0:
+        if query.numel() or key.numel():
+            raise RuntimeError(f"{name}: query and key need at least one head each")
+        return query_to, key_to
+    query, key = _rows(query), _rows(key)
+    with on_device(device):
+        _lib.check(_lib.lib().anna_multi_axis_rotary(
+            ptr(query), *query.stride()[:3], ptr(query_to), *query_to.stride()[:3], ptr(key), *key.stride()[:3], ptr(key_to),
+            *key_to.stride()[:3], ptr(positions), *strides, ptr(tables.rates), ptr(tables.axes), float(attention_scaling), batch,
+            heads, int(key.shape[1]), tokens, dim, width, dtype_code(query.dtype), stream_ptr(device)), name)
+    return query_to, key_to
+
+
+def run_rotary_paged_kv_write(*, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
+                              value_pages: torch.Tensor, page_table: torch.Tensor, past_lengths: torch.Tensor,
+                              positions: torch.Tensor | None = None, rope_deltas: torch.Tensor | None = None,
+                              theta: float = 10000.0, sections: Sequence[int] | None = None, interleaved: bool = False,
+                              rotary_dim: int | None = None, inverse_frequencies: Sequence[float] | None = None,
+                              attention_scaling: float = 1.0, new_lengths: torch.Tensor | None = None,
+                              status: torch.Tensor | None = None) -> torch.Tensor:
+    """Turned queries ``[B, Hq, T, D]``; the turned keys and the values of ``[B, Hkv, T, D]`` go to their pages
+    ``[P, Hkv, S, D]`` at positions ``past_lengths[b] + t``, all in one launch.
+
+    ``positions``: as for ``run_multi_axis_rotary``; None: ``past_lengths[b] + t + rope_deltas[b]`` on every axis
+    (``rope_deltas`` int64 ``[B]`` or ``[B, 1]``, None: 0), the positions of text behind what the row holds.  ``new_lengths``
+    (int64 ``[B]``) receives ``past_lengths + T``; a token whose page id is invalid is not written and reported in ``status``
+    (int32 ``[1]``).  The page pools must be contiguous."""
+    name = "rotary_paged_kv_write"
+    _check_rows(name, query, key)
+    if value.shape != key.shape or value.dtype != key.dtype:
+        raise RuntimeError(f"{name}: key and value must share shape and dtype")
+    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape:
+        raise RuntimeError(f"{name}: key_pages and value_pages must be matching [pages, kv_heads, block_size, head_dim]")
+    if key_pages.shape[1] != key.shape[1] or key_pages.shape[3] != key.shape[3]:
+        raise RuntimeError(f"{name}: pages and keys disagree on kv_heads / head_dim")
+    if not (key_pages.dtype == value_pages.dtype == key.dtype):
+        raise RuntimeError(f"{name}: pages and keys must share the dtype")
+    if not key_pages.is_contiguous() or not value_pages.is_contiguous():
+        raise RuntimeError(f"{name}: page pools must be contiguous")
+    batch, heads, tokens, dim = (int(v) for v in query.shape)
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+        raise RuntimeError(f"{name}: page_table must be int32 [batch, max_blocks]")
+    for label, tensor in (("past_lengths", past_lengths), ("new_lengths", new_lengths)):
+        if tensor is not None and (tensor.dtype != torch.long or tuple(tensor.shape) != (batch,)):
+            raise RuntimeError(f"{name}: {label} must be int64 [batch]")
+    if new_lengths is not None and (not new_lengths.is_contiguous() or new_lengths.data_ptr() == past_lengths.data_ptr()):
+        raise RuntimeError(f"{name}: new_lengths must be contiguous and not past_lengths itself")
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise RuntimeError(f"{name}: status must be int32 [1]")
+    if rope_deltas is not None:
+        if positions is not None:
+            raise RuntimeError(f"{name}: rope_deltas belong to positions=None")
+        if rope_deltas.dtype != torch.long or tuple(rope_deltas.shape) not in ((batch,), (batch, 1)):
+            raise RuntimeError(f"{name}: rope_deltas must be int64 [batch] or [batch, 1]")
+    device = _require_cuda(name, query=query, key=key, value=value, key_pages=key_pages, value_pages=value_pages,
+                           page_table=page_table, past_lengths=past_lengths, positions=positions, rope_deltas=rope_deltas,
+                           new_lengths=new_lengths, status=status)
+    width = dim if rotary_dim is None else int(rotary_dim)
+    if width > dim:
+        raise RuntimeError(f"{name}: rotary_dim {width} is larger than head_dim {dim}")
+    tables = rotary_tables(width, theta=theta, sections=sections, interleaved=interleaved,
+                           inverse_frequencies=inverse_frequencies, device=device)
+    strides = (0, 0, 0) if positions is None else _check_positions(name, positions, tables.axis_count, batch, tokens)
+    out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    if query.numel() == 0 or key.numel() == 0:
+        if query.numel() or key.numel():
+            raise RuntimeError(f"{name}: query and key need at least one head each")
+        if new_lengths is not None:
+            new_lengths.copy_(past_lengths)
+        return out
+    if key_pages.shape[0] == 0 or page_table.shape[1] == 0:
+        raise RuntimeError(f"{name}: there are no pages to write to")
+    query, key, value = _rows(query), _rows(key), _rows(value)
+    page_table = page_table if page_table.stride(1) == 1 else page_table.contiguous()
+    past_lengths = past_lengths.contiguous()
+    with on_device(device):
+        _lib.check(_lib.lib().anna_rotary_paged_kv_write(
+            ptr(query), *query.stride()[:3], ptr(out), *out.stride()[:3], ptr(key), *key.stride()[:3], ptr(value),
+            *value.stride()[:3], ptr(key_pages), ptr(value_pages), ptr(page_table), page_table.stride(0), ptr(past_lengths),
+            ptr(new_lengths), ptr(positions), *strides, ptr(rope_deltas), 0 if rope_deltas is None else rope_deltas.stride(0),
+            ptr(tables.rates), ptr(tables.axes), float(attention_scaling), batch, heads, int(key.shape[1]), tokens, dim, width,
+            int(key_pages.shape[2]), int(key_pages.shape[0]), int(page_table.shape[1]), dtype_code(query.dtype), ptr(status),
+            stream_ptr(device)), name)
+    return out

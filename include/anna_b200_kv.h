@@ -151,6 +151,61 @@ int anna_paged_kv_write(const void* k_new, const void* v_new, int64_t kn_stride_
                         int64_t max_blocks, int dtype, int32_t* status, anna_stream_t stream);
 
 /*
+ * Rotary positions with several axes (time, height, width of images and video): pair i of a head is its dims
+ * (i, i + rotary_dim / 2), which a token turns by the angle 2 pi * rates[i] * positions[axes[i]]:
+ *   x1' = scale * (x1 cos - x2 sin),  x2' = scale * (x2 cos + x1 sin);  dims at or past rotary_dim stay as they are.
+ * Stands in for the rotary part of Qwen3Attention._forward_attention (src/anna/model/ops.py:1900-1914).
+ *   q, k       [B, Hq, T, D], [B, Hkv, T, D] with element strides per batch, head and token; last dim contiguous
+ *   q_out, k_out  the same; either the input itself with its strides (in place) or memory that does not overlap it
+ *   positions  int64, element strides per axis, batch and token (0: the same for all); magnitudes up to 2^31
+ *   rates      double [rotary_dim / 2], turns per position;  axes  int32 [rotary_dim / 2], all >= 0 and < the number of axes
+ * rotary_dim is even and at most D; no other limit on D below 4096.  Any alignment of whole elements; the widest that all tensors
+ * share is used.
+ */
+int anna_multi_axis_rotary(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, void* q_out,
+                           int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_t, const void* k, int64_t k_stride_b,
+                           int64_t k_stride_h, int64_t k_stride_t, void* k_out, int64_t ko_stride_b, int64_t ko_stride_h,
+                           int64_t ko_stride_t, const int64_t* positions, int64_t pos_stride_a, int64_t pos_stride_b,
+                           int64_t pos_stride_t, const double* rates, const int32_t* axes, float scale, int batch, int q_heads,
+                           int kv_heads, int tokens, int head_dim, int rotary_dim, int dtype, anna_stream_t stream);
+
+/*
+ * The same in front of anna_paged_kv_write, in one launch: queries are turned into q_out, keys are turned into their pages, values
+ * [B, Hkv, T, D] (strides of their own) go to theirs as they are.
+ *   positions    NULL: past_lengths[b] + t + rope_deltas[b * delta_stride] on every axis (rope_deltas may be NULL: 0)
+ *   page_table, past_lengths, new_lengths, status  as for anna_paged_kv_write; tokens without a valid page are not written
+ */
+int anna_rotary_paged_kv_write(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, void* q_out,
+                               int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_t, const void* k, int64_t k_stride_b,
+                               int64_t k_stride_h, int64_t k_stride_t, const void* v, int64_t v_stride_b, int64_t v_stride_h,
+                               int64_t v_stride_t, void* key_pages, void* value_pages, const int32_t* page_table,
+                               int64_t table_stride, const int64_t* past_lengths, int64_t* new_lengths, const int64_t* positions,
+                               int64_t pos_stride_a, int64_t pos_stride_b, int64_t pos_stride_t, const int64_t* rope_deltas,
+                               int64_t delta_stride, const double* rates, const int32_t* axes, float scale, int batch, int q_heads,
+                               int kv_heads, int tokens, int head_dim, int rotary_dim, int block_size, int64_t num_pages,
+                               int64_t max_blocks, int dtype, int32_t* status, anna_stream_t stream);
+
+/*
+ * Copies of whole pages, any number of pools at a time: pair i of pool g copies page pairs[2i] of src to page pairs[2i + 1] of dst.
+ * src and dst may be the same pool; then no target may be a source or another pair's target.  No counterpart in the reference,
+ * which copies page by page when it clones a cache (src/anna/model/ops.py:1323-1381).
+ *   pools          host array
+ *   pairs          host int32 [num_pairs, 2], for at most anna_page_copy_max_pairs() pairs (they travel in the launch) ...
+ *   device_pairs   ... or, for any number, the same in device memory (8-byte aligned); pairs is not read then
+ *   status         optional device int32: ANNA_DEV_BAD_PAGE is OR-ed in when an id is outside its pool (that copy is skipped)
+ */
+typedef struct anna_page_pool {
+  const void* src;
+  void* dst;
+  int64_t page_bytes;
+  int32_t src_pages, dst_pages; /* pages of each, for the check of the ids */
+  int32_t first_pair, count;    /* this pool's pairs; pools may share them */
+} anna_page_pool;
+int anna_page_copy_max_pairs(void);
+int anna_page_copy(const anna_page_pool* pools, int num_pools, const int32_t* pairs, int64_t num_pairs, const int32_t* device_pairs,
+                   int32_t* status, anna_stream_t stream);
+
+/*
  * Patch a device block table in place: entry i of `entries` is the int32 triple (row, column, page id); triples outside
  * [0, rows) x [0, cols) are ignored.  Replaces the per-row rebuild-and-upload of the table in
  * Qwen3DynamicCache._sync_page_table_layer_buffer (src/anna/model/ops.py:532-588) for the rows that took pages.
