@@ -17,6 +17,7 @@ from .fused_ops import (
     run_gqa_decode_splitkv_fused_out,
     run_gqa_decode_splitkv_turboquant_fused_out,
     run_paged_gqa_decode_fused,
+    run_tq_paged_multi_decode,
 )
 from .page_copy import run_page_copy, run_page_gather
 from .pools import Qwen3PagedLayerAllocator, TurboQuantLayerPool, resolve_value_group_size
@@ -33,4 +34,5 @@ __all__ = [
     "run_gqa_decode_fused", "run_gqa_decode_splitkv_fused", "run_gqa_decode_splitkv_fused_out",
     "run_gqa_decode_splitkv_turboquant_fused_out", "run_paged_gqa_decode_fused", "grouped_query_attention",
     "run_multi_axis_rotary", "run_rotary_paged_kv_write", "run_page_copy", "run_page_gather",
+    "run_tq_paged_multi_decode",
 ]

@@ -88,6 +88,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                            c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_i32, c_i32,
                                            c_ptr, c_ptr, c_size, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                            c_i64, c_i64, c_f32, c_i32, c_ptr, c_i32, c_ptr]),
+    "anna_tq_multi_decode_plan": (c_i32, [c_i32] * 4 + [c_i64, c_i32, c_i32, ctypes.POINTER(c_i32), ctypes.POINTER(c_i32)]),
+    "anna_tq_paged_multi_decode": (c_i32, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_i64] + [c_ptr] * 6 +
+                                   [c_ptr, c_i64, c_i64, c_i64] * 2 + [c_ptr, c_ptr, c_i32, c_ptr] + [c_i32] * 9 +
+                                   [c_i64, c_i64, c_f32, c_i32, c_ptr]),
     "anna_peer_signal_wait": (c_i32, [c_ptr, c_i32, c_i32, c_i64, c_i64, c_ptr, c_ptr]),
     "anna_kv_selftest_umma_tma": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, ctypes.POINTER(c_i32), c_ptr]),
     "anna_kv_selftest_umma_ts": (c_i32, [c_ptr, c_ptr, c_ptr, ctypes.POINTER(c_i32), c_ptr]),
@@ -192,6 +196,16 @@ def tq_decode_plan(batch: int, kv_heads: int, max_blocks: int, block_size: int, 
     check(lib().anna_tq_decode_plan(batch, kv_heads, max_blocks, block_size, residual_len, ctypes.byref(chunk),
                                     ctypes.byref(chunks)), "anna_tq_decode_plan")
     return int(chunk.value), int(chunks.value)
+
+
+def tq_multi_decode_plan(batch: int, heads: int, kv_heads: int, tokens: int, max_blocks: int, block_size: int,
+                         residual_len: int) -> tuple[int, int]:
+    """(chunks of the keys, arrival counters) of a multi-token decode."""
+    chunks = c_i32(0)
+    counters = c_i32(0)
+    check(lib().anna_tq_multi_decode_plan(batch, heads, kv_heads, tokens, max_blocks, block_size, residual_len,
+                                          ctypes.byref(chunks), ctypes.byref(counters)), "anna_tq_multi_decode_plan")
+    return int(chunks.value), int(counters.value)
 
 
 def tq_page_layout(head_dim: int, bits: int, block_size: int, dtype_code: int, value_group: int) -> dict[str, int]:

@@ -1,0 +1,341 @@
+// Attention of the newest T tokens of every sequence over [packed TurboQuant prefix | un-quantized window ring]: the CUDA-core
+// form and the entry points.
+//
+// Keys are scored in the basis of their codes, as in the single-token decode (tq_decode.cu):
+//   q . k_hat = norm / D * [ fwht(s1*q) . centroid[idx] + sqrt(pi/2)/sqrt(D) * rnorm * fwht(s2*fwht(s1*q)) . (2*sign-1) ]
+// so a CTA rotates its rows once and no key is taken back to the original basis.
+//
+// This form serves fp32 caches, head_dim 64 and pages that are no multiple of 16 tokens; everything in it is 32 bits.  A CTA of
+// 128 threads de-quantizes 32 tokens at a time into shared memory for its 8 rows.  Bound: FMA issue (3 D operations per row and
+// key, of which the shared-memory reads of the keys are shared by two rows).
+#include "tq_multi_params.cuh"
+
+namespace anna {
+
+constexpr int kMultiThreads = 128, kMultiWarps = 4;
+constexpr int kMultiRows = 8;    // of a CTA of this form
+constexpr int kMultiTokens = 32;  // de-quantized at a time: a lane's token
+
+template <int D>
+constexpr int kMultiSmemFloats = 3 * kMultiRows * D + 2 * kMultiTokens * (D + 1) + kMultiTokens * D + kMultiRows * kMultiTokens;
+
+template <typename T, int D, int BITS>
+__global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiParams p, int row_tiles) {
+  constexpr int E = D / 32;
+  constexpr int M = BITS - 1;
+  constexpr int VS = BITS == 2 ? 2 : 4;
+  extern __shared__ float smem[];
+  float* q_smem = smem;                                // [3][rows][D]: as it is, rotated, rotated twice; scaled
+  float* ka = q_smem + 3 * kMultiRows * D;             // [tokens][D + 1]: centroids, or the key itself
+  float* kb = ka + kMultiTokens * (D + 1);             // signs times the residual norm
+  float* vt = kb + kMultiTokens * (D + 1);             // [tokens][D]
+  float* weight = vt + kMultiTokens * D;               // [rows][tokens]
+  __shared__ float sm_cent[1 << M], sm_norm[kMultiTokens], sm_rescale[kMultiRows];
+  __shared__ bool sm_there[kMultiTokens];
+
+  const int chunk = blockIdx.x, kvh = blockIdx.y / row_tiles, tile = blockIdx.y % row_tiles;
+  const int64_t b = blockIdx.z;
+  const int row0 = tile * kMultiRows, count = min(kMultiRows, p.rows - row0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t len = max((int64_t)0, min(p.lengths[b], p.max_len));
+  const int64_t lq = len > p.residual_len ? len - p.residual_len : 0;
+  const int64_t t0 = (int64_t)chunk * p.chunk_tokens;
+  const int chunks = max(1, (int)((len + p.chunk_tokens - 1) / p.chunk_tokens));  // an empty row has one chunk, which writes zeros
+  if (chunk >= chunks) return;
+  const int64_t t1 = min(len, t0 + p.chunk_tokens);
+  const int64_t first_seen = len - p.tokens;  // newest key that query 0 sees
+
+  if (threadIdx.x < (1 << M)) sm_cent[threadIdx.x] = p.centroids[threadIdx.x];
+  const float f1 = p.scaling / (float)D;
+  const float f2 = f1 * 1.2533141373155001f * rsqrt_dim_const<D>();
+  for (int i = warp; i < kMultiRows; i += kMultiWarps) {
+    float w[E];
+    const int row = row0 + min(i, count - 1);
+    const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_stride_b + (int64_t)(kvh * p.groups + row % p.groups) * p.q_stride_h +
+                 (int64_t)(row / p.groups) * p.q_stride_t + lane * E;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      w[j] = ElemTraits<T>::to_float(q[j]);
+      q_smem[i * D + lane * E + j] = w[j] * p.scaling;
+      w[j] *= p.signs1[lane * E + j];
+    }
+    warp_fwht<E>(w, lane);
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      q_smem[(kMultiRows + i) * D + lane * E + j] = w[j] * f1;
+      w[j] *= p.signs2[lane * E + j];
+    }
+    warp_fwht<E>(w, lane);
+#pragma unroll
+    for (int j = 0; j < E; ++j) q_smem[(2 * kMultiRows + i) * D + lane * E + j] = w[j] * f2;
+  }
+
+  // rows warp and warp + 4 of this warp's softmax; the thread's dims of the output
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
+  constexpr int kDims = D >= kMultiThreads ? D / kMultiThreads : 1;
+  constexpr int kOutRows = D >= kMultiThreads ? kMultiRows : kMultiRows * D / kMultiThreads;
+  const int out_row0 = D >= kMultiThreads ? 0 : (int)threadIdx.x / D * kOutRows;
+  float acc[kOutRows][kDims];
+#pragma unroll
+  for (int r = 0; r < kOutRows; ++r)
+#pragma unroll
+    for (int j = 0; j < kDims; ++j) acc[r][j] = 0.0f;
+
+  const int64_t slot = len > lq ? p.window_slots[b] : 0;
+  const T* ring = reinterpret_cast<const T*>(p.window) + (slot * 2 * p.kv_heads + kvh) * p.residual_len * D;
+  const int64_t ring_values = (int64_t)p.kv_heads * p.residual_len * D;
+  for (int64_t base = t0; base < t1;) {
+    const bool packed = base < lq;
+    const int64_t stop = min(packed ? min(lq, t1) : t1, base + kMultiTokens);
+    const int n = (int)(stop - base);
+    __syncthreads();
+    // ---- 32 tokens into shared memory: a warp per token ------------------------------------------------------------------
+    for (int i = warp; i < n; i += kMultiWarps) {
+      const int64_t t = base + i;
+      if (!packed) {
+        const T* k = ring + (t % p.residual_len) * D;
+        for (int d = lane; d < D; d += 32) {
+          ka[i * (D + 1) + d] = ElemTraits<T>::to_float(k[d]);
+          vt[i * D + d] = ElemTraits<T>::to_float(k[ring_values + d]);
+        }
+        if (lane == 0) {
+          sm_there[i] = true;
+          sm_norm[i] = 1.0f;
+        }
+        continue;
+      }
+      const int64_t blk = t / p.block_size;
+      const int tok = (int)(t - blk * p.block_size);
+      const int32_t pid = blk < p.max_blocks ? p.block_table[b * p.table_stride + blk] : -1;
+      const bool there = pid >= 0 && pid < p.num_pages;
+      if (lane == 0) sm_there[i] = there;
+      const uint8_t* page = p.pages + (there ? ((int64_t)pid * p.kv_heads + kvh) * p.layout.chunk_bytes : 0);
+      const float rnorm = there ? reinterpret_cast<const float*>(page + p.layout.off_krnorm)[tok] : 0.0f;
+      if (lane == 0) sm_norm[i] = there ? reinterpret_cast<const float*>(page + p.layout.off_knorm)[tok] : 0.0f;
+      const uint8_t* keys = page + p.layout.off_kcodes + tok * p.layout.key_bytes;
+      const uint8_t* codes = page + p.layout.off_vdata + tok * p.layout.value_bytes;
+      const T* scales = reinterpret_cast<const T*>(page + p.layout.off_vscale) + tok * p.layout.groups;
+      const T* zeros = reinterpret_cast<const T*>(page + p.layout.off_vzero) + tok * p.layout.groups;
+      for (int d = lane; d < D; d += 32) {
+        uint32_t code = 0, sign = 0, value = 0;
+        float scale = 0.0f, zero = 0.0f;
+        if (there) {
+          if constexpr (BITS == 3) {
+            code = (keys[d >> 2] >> ((d & 3) * 2)) & 3u;
+            sign = (keys[D / 4 + (d >> 3)] >> (d & 7)) & 1u;
+          } else {
+            const uint32_t field = (keys[d * BITS >> 3] >> (d * BITS & 7)) & ((1u << BITS) - 1u);
+            code = field & ((1u << M) - 1u);
+            sign = field >> M;
+          }
+          value = (codes[d * VS >> 3] >> (d * VS & 7)) & ((1u << VS) - 1u);
+          scale = ElemTraits<T>::to_float(scales[d / p.value_group]);
+          zero = ElemTraits<T>::to_float(zeros[d / p.value_group]);
+        }
+        ka[i * (D + 1) + d] = sm_cent[code];
+        kb[i * (D + 1) + d] = sign != 0 ? rnorm : -rnorm;
+        vt[i * D + d] = fmaf((float)value, scale, zero);
+      }
+    }
+    __syncthreads();
+    // ---- scores: token `lane`, rows warp and warp + 4 ----------------------------------------------------------------------
+    float s[2] = {-INFINITY, -INFINITY};
+    if (lane < n) {
+      const float* x = ka + lane * (D + 1);
+      const float* y = kb + lane * (D + 1);
+      const float* q0 = q_smem + ((packed ? kMultiRows : 0) + warp) * D;
+      const float* q1 = q0 + kMultiWarps * D;
+      float a0 = 0.0f, a1 = 0.0f;
+      for (int d = 0; d < D; ++d) {
+        a0 = fmaf(q0[d], x[d], a0);
+        a1 = fmaf(q1[d], x[d], a1);
+      }
+      if (packed) {
+        q0 += kMultiRows * D;
+        q1 += kMultiRows * D;
+        float b0 = 0.0f, b1 = 0.0f;
+        for (int d = 0; d < D; ++d) {
+          b0 = fmaf(q0[d], y[d], b0);
+          b1 = fmaf(q1[d], y[d], b1);
+        }
+        a0 += b0;
+        a1 += b1;
+      }
+      const float a[2] = {a0 * sm_norm[lane], a1 * sm_norm[lane]};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = warp + k * kMultiWarps;
+        if (i < count && sm_there[lane] && base + lane <= first_seen + (row0 + i) / p.groups) s[k] = a[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float m_new = s[k];
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
+      m_new = fmaxf(m_run[k], m_new);
+      const float m_safe = m_new == -INFINITY ? 0.0f : m_new;
+      const float w = __expf(s[k] - m_safe), rescale = __expf(m_run[k] - m_safe);
+      l_run[k] = l_run[k] * rescale + w;  // a lane's share of the sum
+      m_run[k] = m_new;
+      weight[(warp + k * kMultiWarps) * kMultiTokens + lane] = w;
+      if (lane == 0) sm_rescale[warp + k * kMultiWarps] = rescale;
+    }
+    __syncthreads();
+    // ---- values -----------------------------------------------------------------------------------------------------------
+    const int d0 = D >= kMultiThreads ? (int)threadIdx.x : (int)threadIdx.x % D;
+#pragma unroll
+    for (int r = 0; r < kOutRows; ++r)
+#pragma unroll
+      for (int j = 0; j < kDims; ++j) acc[r][j] *= sm_rescale[out_row0 + r];
+    for (int i = 0; i < n; ++i) {
+      if (!sm_there[i]) continue;
+      float v[kDims];
+#pragma unroll
+      for (int j = 0; j < kDims; ++j) v[j] = vt[i * D + d0 + j * kMultiThreads];
+#pragma unroll
+      for (int r = 0; r < kOutRows; ++r) {
+        const float w = weight[(out_row0 + r) * kMultiTokens + i];
+        // a value that the row does not see may be infinite or NaN
+        if (w != 0.0f) {
+#pragma unroll
+          for (int j = 0; j < kDims; ++j) acc[r][j] = fmaf(w, v[j], acc[r][j]);
+        }
+      }
+    }
+    base = stop;
+  }
+
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) l_run[k] += __shfl_xor_sync(0xffffffffu, l_run[k], d);
+  }
+  __syncthreads();
+  const int d0 = D >= kMultiThreads ? (int)threadIdx.x : (int)threadIdx.x % D;
+  if (chunks == 1) {
+    float* den = weight;
+    if (lane == 0) {
+      den[warp] = l_run[0];
+      den[warp + kMultiWarps] = l_run[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kOutRows; ++r) {
+      if (out_row0 + r >= count) break;
+      const float l = den[out_row0 + r], inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int j = 0; j < kDims; ++j) {
+        const float o[1] = {acc[r][j] * inv};
+        multi_store<T, 1>(p, b, kvh, row0 + out_row0 + r, d0 + j * kMultiThreads, o);
+      }
+    }
+    return;
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = warp + k * kMultiWarps;
+      if (i < count)
+        reinterpret_cast<float2*>(p.stats)[multi_row_index(p, b, kvh, row0 + i) * p.num_chunks + chunk] = make_float2(m_run[k], l_run[k]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kOutRows; ++r) {
+    if (out_row0 + r >= count) break;
+    float* to = p.values + (multi_row_index(p, b, kvh, row0 + out_row0 + r) * p.num_chunks + chunk) * D;
+#pragma unroll
+    for (int j = 0; j < kDims; ++j) to[d0 + j * kMultiThreads] = acc[r][j];
+  }
+  multi_merge<T, D, kMultiWarps>(p, b, kvh, tile, row_tiles, row0, count, chunks);
+}
+
+// Chunks of the keys: two waves of four CTAs per SM, counting 16 rows to a row tile, in multiples of 128 tokens (two tiles of 16
+// for each of four warps).
+static void multi_plan(int batch, int kv_heads, int rows, int64_t max_len, int* chunk_tokens, int* num_chunks) {
+  const int64_t units = (int64_t)batch * kv_heads * ((rows + 15) / 16);
+  const int64_t wanted = (148 * 8 + units - 1) / units;
+  const int64_t len = max_len > 0 ? max_len : 1;
+  int64_t chunk = ((len + wanted - 1) / wanted + 127) / 128 * 128;
+  if (chunk > 4096) chunk = 4096;
+  while ((len + chunk - 1) / chunk > 512) chunk *= 2;
+  *chunk_tokens = (int)chunk;
+  *num_chunks = (int)((len + chunk - 1) / chunk);
+}
+
+}  // namespace anna
+
+using namespace anna;
+
+extern "C" int anna_tq_multi_decode_plan(int batch, int q_heads, int kv_heads, int tokens, int64_t max_blocks, int block_size,
+                                         int residual_len, int* num_chunks, int* counters) {
+  ANNA_REQUIRE(num_chunks != nullptr && counters != nullptr, "anna_tq_multi_decode_plan: null pointer argument");
+  ANNA_REQUIRE(batch > 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && tokens > 0 && max_blocks >= 0 && block_size > 0 &&
+                   residual_len > 0, "anna_tq_multi_decode_plan: bad sizes");
+  ANNA_REQUIRE((int64_t)tokens * q_heads < (1 << 20) && max_blocks < (1ll << 31) / block_size - residual_len,
+               "anna_tq_multi_decode_plan: too many queries or keys");
+  const int rows = tokens * (q_heads / kv_heads);
+  const int64_t tiles = (int64_t)batch * kv_heads * ((rows + kMultiRows - 1) / kMultiRows);
+  ANNA_REQUIRE(tiles < (1ll << 31), "anna_tq_multi_decode_plan: too many rows");
+  int chunk = 0;
+  multi_plan(batch, kv_heads, rows, max_blocks * block_size + residual_len, &chunk, num_chunks);
+  *counters = (int)tiles;
+  return ANNA_OK;
+}
+
+extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+                                          const uint8_t* packed_pages, const int32_t* block_table, int64_t table_stride,
+                                          const void* window, const int64_t* window_slots, const int64_t* lengths,
+                                          const float* signs1, const float* signs2, const float* centroids, const void* gate,
+                                          int64_t gate_stride_b, int64_t gate_stride_h, int64_t gate_stride_t, void* out,
+                                          int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t, float* partial_stats,
+                                          float* partial_values, int chunk_capacity, int32_t* counters, int batch, int q_heads,
+                                          int kv_heads, int tokens, int head_dim, int block_size, int residual_len, int bits,
+                                          int value_group, int64_t num_pages, int64_t max_blocks, float scaling, int dtype,
+                                          anna_stream_t stream) {
+  const char* what = "anna_tq_paged_multi_decode";
+  ANNA_REQUIRE(q && window && window_slots && lengths && signs1 && signs2 && centroids && out && counters, "%s: null pointer argument", what);
+  ANNA_REQUIRE(max_blocks == 0 || (packed_pages && block_table && num_pages > 0), "%s: a block table needs pages", what);
+  int num_chunks = 0, tiles = 0;
+  if (const int rc = anna_tq_multi_decode_plan(batch, q_heads, kv_heads, tokens, max_blocks, block_size, residual_len, &num_chunks, &tiles))
+    return rc;
+  ANNA_REQUIRE(batch <= 65535, "%s: at most 65535 sequences", what);
+  if (chunk_capacity < num_chunks || (num_chunks > 1 && (partial_stats == nullptr || partial_values == nullptr)))
+    return set_error(ANNA_ERR_WORKSPACE, "%s: scratch holds %d chunks, %d are needed", what, chunk_capacity, num_chunks);
+  TqMultiParams p{};
+  ANNA_REQUIRE(dtype == ANNA_DTYPE_F32 || dtype == ANNA_DTYPE_F16 || dtype == ANNA_DTYPE_BF16, "%s: unknown dtype %d", what, dtype);
+  if (!tq_make_layout(head_dim, bits, block_size, dtype_bytes_of(dtype), value_group, &p.layout))
+    return set_error(ANNA_ERR_UNSUPPORTED, "%s: unsupported page geometry (head_dim %d, bits %d, value group %d)", what, head_dim, bits,
+                     value_group);
+  ANNA_REQUIRE(aligned_to(packed_pages, 16) && aligned_to(window, 16), "%s: pages and window must be 16-byte aligned", what);
+  ANNA_REQUIRE(aligned_to(partial_stats, 8) && aligned_to(partial_values, 16), "%s: scratch must be 8- and 16-byte aligned", what);
+  p.q = q; p.q_stride_b = q_stride_b; p.q_stride_h = q_stride_h; p.q_stride_t = q_stride_t;
+  p.pages = packed_pages; p.block_table = block_table; p.table_stride = table_stride;
+  p.window = window; p.window_slots = window_slots; p.lengths = lengths;
+  p.signs1 = signs1; p.signs2 = signs2; p.centroids = centroids;
+  p.gate = gate; p.gate_stride_b = gate_stride_b; p.gate_stride_h = gate_stride_h; p.gate_stride_t = gate_stride_t;
+  p.out = out; p.out_stride_b = out_stride_b; p.out_stride_h = out_stride_h; p.out_stride_t = out_stride_t;
+  p.stats = partial_stats; p.values = partial_values; p.counters = counters;
+  p.q_heads = q_heads; p.kv_heads = kv_heads; p.groups = q_heads / kv_heads; p.tokens = tokens; p.rows = tokens * p.groups;
+  p.block_size = block_size; p.residual_len = residual_len; p.value_group = value_group;
+  p.block_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if ((1 << s) == block_size) p.block_shift = s;
+  p.num_pages = num_pages; p.max_blocks = max_blocks; p.max_len = max_blocks * block_size + residual_len;
+  p.scaling = scaling;
+  multi_plan(batch, kv_heads, p.rows, p.max_len, &p.chunk_tokens, &p.num_chunks);
+  const int row_tiles = (p.rows + kMultiRows - 1) / kMultiRows;
+  ANNA_REQUIRE((int64_t)kv_heads * row_tiles <= 65535, "%s: too many queries", what);
+  const dim3 grid((unsigned)p.num_chunks, (unsigned)(kv_heads * row_tiles), (unsigned)batch);
+  return ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+    return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
+      return ANNA_DISPATCH_TQ_BITS(bits, BITS, [&]() -> int {
+        constexpr int smem = kMultiSmemFloats<D> * 4;
+        auto kernel = tq_multi_kernel<T, D, BITS>;
+        ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        kernel<<<grid, kMultiThreads, smem, (cudaStream_t)stream>>>(p, row_tiles);
+        return check_launch("tq_multi_kernel");
+      });
+    });
+  });
+}

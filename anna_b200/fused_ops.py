@@ -57,6 +57,9 @@ NEW_SCHEMAS = {
     "tq_paged_decode":
         "(Tensor query, Tensor packed_pages, Tensor page_table, Tensor window, Tensor window_slots, Tensor lengths, "
         "float scaling, int bits, int residual_len, int block_size, int value_group_size, Tensor? gate=None) -> Tensor",
+    "tq_paged_multi_decode":
+        "(Tensor query, Tensor packed_pages, Tensor page_table, Tensor window, Tensor window_slots, Tensor lengths, "
+        "float scaling, int bits, int residual_len, int block_size, int value_group_size, Tensor? gate=None) -> Tensor",
 }
 
 
@@ -679,7 +682,83 @@ def _op_tq_paged_decode(query, packed_pages, page_table, window, window_slots, l
     return out
 
 
+def multi_scratch(device: torch.device, batch: int, heads: int, kv_heads: int, tokens: int, head_dim: int, max_blocks: int,
+                  block_size: int, residual_len: int):
+    """(partial_stats, partial_values, chunks, counters) of a multi-token decode.  Under a graph capture they are the graph's own:
+    graphs may be replayed side by side, and those of the stream are replaced when a larger call needs more."""
+    key = (batch, heads, kv_heads, tokens, max_blocks, block_size, residual_len)
+    plan = _MULTI_PLANS.get(key)
+    if plan is None:
+        if len(_MULTI_PLANS) > 4096:
+            _MULTI_PLANS.clear()
+        plan = _MULTI_PLANS[key] = _lib.tq_multi_decode_plan(*key)
+    chunks, arrivals = plan
+    rows = batch * heads * tokens * chunks if chunks > 1 else 0
+    floats = rows * (head_dim + 2)
+    with on_device(device):
+        if torch.cuda.is_current_stream_capturing():
+            buf = torch.empty(max(floats, 1), dtype=torch.float32, device=device)
+            return buf[rows * head_dim:], buf, chunks, torch.zeros(arrivals, dtype=torch.int32, device=device)
+    buf = _SCRATCH.get(device, floats)
+    return buf[rows * head_dim:], buf, chunks, _SCRATCH.counters(device, arrivals)
+
+
+_MULTI_PLANS: dict[tuple, tuple[int, int]] = {}
+
+
+def multi_decode(name, query, packed_pages, page_table, window, window_slots, lengths, tables, scaling, gate, *, kv_heads, bits,
+                 residual_len, block_size, value_group):
+    """Launch of the multi-token decode on arguments that have been checked; pages and table may be None."""
+    device = query.device
+    batch, heads, tokens, dim = (int(v) for v in query.shape)
+    query = _last_dim_contiguous(query)
+    gate = None if gate is None else _last_dim_contiguous(gate)
+    out = torch.empty((batch, heads, tokens, dim), dtype=query.dtype, device=device)
+    if out.numel() == 0:
+        return out
+    max_blocks = 0 if page_table is None else int(page_table.shape[1])
+    stats, values, chunks, counters = multi_scratch(device, batch, heads, kv_heads, tokens, dim, max_blocks, block_size, residual_len)
+    with on_device(device):
+        _lib.check(_lib.lib().anna_tq_paged_multi_decode(
+            ptr(query), *query.stride()[:3], ptr(packed_pages) if max_blocks else None, ptr(page_table) if max_blocks else None,
+            page_table.stride(0) if max_blocks else 0, ptr(window), ptr(window_slots), ptr(lengths), ptr(tables.signs1),
+            ptr(tables.signs2), ptr(tables.centroids), ptr(gate), *((0, 0, 0) if gate is None else gate.stride()[:3]), ptr(out),
+            *out.stride()[:3], ptr(stats), ptr(values), chunks, ptr(counters), batch, heads, kv_heads, tokens, dim, block_size,
+            residual_len, bits, value_group, int(packed_pages.shape[0]) if max_blocks else 0, max_blocks, float(scaling),
+            dtype_code(query.dtype), stream_ptr(device)), name)
+    return out
+
+
+def _op_tq_paged_multi_decode(query, packed_pages, page_table, window, window_slots, lengths, scaling, bits, residual_len,
+                              block_size, value_group_size, gate=None):
+    """Decode of the newest T tokens of B rows over [packed prefix | window ring]."""
+    from .tq_tables import key_tables
+
+    name = "tq_paged_multi_decode"
+    if query.dim() != 4:
+        raise RuntimeError(f"{name}: query must be [batch, heads, tokens, head_dim]")
+    batch, heads, _, dim = (int(v) for v in query.shape)
+    _check_tq_geometry(name, packed_pages, page_table, window, window_slots, lengths, batch, dim, bits, residual_len,
+                       block_size, value_group_size, query.dtype)
+    kv_heads = int(packed_pages.shape[1])
+    if kv_heads < 1 or heads % kv_heads != 0 or int(window.shape[2]) != kv_heads:
+        raise RuntimeError(f"{name}: query heads must be a multiple of the kv heads of the pages and the window")
+    if page_table.shape[1] > 0 and packed_pages.shape[0] == 0:
+        raise RuntimeError(f"{name}: a block table needs pages")
+    if gate is not None and (gate.shape != query.shape or gate.dtype != query.dtype):
+        raise RuntimeError(f"{name}: gate must match the query in shape and dtype")
+    device = _require_cuda(name, query=query, packed_pages=packed_pages, page_table=page_table, window=window,
+                           window_slots=window_slots, lengths=lengths, gate=gate)
+    if page_table.stride(1) != 1:
+        page_table = page_table.contiguous()
+    tables = key_tables(head_dim=dim, bits=bits, device=device)
+    return multi_decode(name, query, packed_pages, page_table, window, window_slots.contiguous(), lengths.contiguous(), tables, scaling,
+                        gate, kv_heads=kv_heads, bits=bits, residual_len=residual_len, block_size=block_size,
+                        value_group=value_group_size)
+
+
 _IMPLS = {
+    "tq_paged_multi_decode": _op_tq_paged_multi_decode,
     "paged_kv_write": _op_paged_kv_write,
     "tq_append": _op_tq_append,
     "tq_paged_decode": _op_tq_paged_decode,
@@ -717,6 +796,7 @@ _META = {
     "paged_kv_write": _meta_none,
     "tq_append": _meta_none,
     "tq_paged_decode": _meta_like_query,
+    "tq_paged_multi_decode": _meta_like_query,
 }
 
 
@@ -841,3 +921,15 @@ def run_paged_gqa_decode_fused(*, query, key_pages, value_pages, page_table, vis
     if gate is None:
         return op(query, key_pages, value_pages, page_table, visible_lengths, float(scaling))
     return op(query, key_pages, value_pages, page_table, visible_lengths, float(scaling), gate)
+
+
+def run_tq_paged_multi_decode(*, query, packed_pages, page_table, window, window_slots, lengths, scaling, bits, residual_len,
+                              block_size, value_group_size, gate=None):
+    """Attention of the newest T tokens of every row over a packed TurboQuant cache: ``query`` ``[B, Hq, T, D]`` (any strides),
+    ``lengths`` int64 ``[B]`` with the new tokens among them; query ``t`` sees the keys up to position ``lengths[b] - T + t``, one
+    that sees none gives zeros.  ``gate`` (shape and dtype of the query): the output is multiplied by its sigmoid.  The cache is
+    given as for ``torch.ops.anna.tq_paged_decode``."""
+    _resolve("tq_paged_multi_decode")
+    op = _op_tq_paged_multi_decode  # same function the dispatcher would reach for CUDA tensors
+    return op(query, packed_pages, page_table, window, window_slots, lengths, float(scaling), int(bits), int(residual_len),
+              int(block_size), int(value_group_size), gate)

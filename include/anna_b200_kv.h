@@ -393,6 +393,31 @@ int anna_tq_paged_decode_peers(const void* q, int64_t q_stride_b, int64_t q_stri
                                void* const* peer_outputs, int num_peers, anna_stream_t stream);
 
 /*
+ * Attention of the newest T tokens of every row over [packed prefix | window ring], for drafted tokens and short chunks: query t of
+ * a row with `lengths[b]` tokens (the new ones among them) sees the keys at positions up to lengths[b] - T + t, as the causal mask
+ * of grouped_query_attention (src/anna/model/ops.py:1552-1574) has it over the de-quantized view; a query that sees no key gives
+ * zeros.  One launch, no dense view.
+ *   q, gate, out   [B, Hq, T, D] with element strides per batch, head and token, last dim contiguous; gate may be NULL, else
+ *                  the output is multiplied by sigmoid(gate)
+ *   packed_pages, block_table, window, window_slots, lengths, signs1, signs2, centroids  as for anna_tq_paged_decode (pages and
+ *                  table may be NULL with max_blocks == 0); holes of the table (ids outside [0, num_pages)) are keys that nobody sees
+ *   partial_stats  float [B, Hq, T, chunk_capacity, 2], partial_values float [B, Hq, T, chunk_capacity, D] with chunk_capacity >=
+ *                  the num_chunks of anna_tq_multi_decode_plan (may be NULL where that is 1); 8- and 16-byte aligned
+ *   counters       int32, as many as the plan says, zero; left at zero
+ * dtype F32 / F16 / BF16, head_dim 64 / 128 / 256, any page size and any value group that divides head_dim.
+ */
+int anna_tq_multi_decode_plan(int batch, int q_heads, int kv_heads, int tokens, int64_t max_blocks, int block_size, int residual_len,
+                              int* num_chunks, int* counters);
+int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, const uint8_t* packed_pages,
+                               const int32_t* block_table, int64_t table_stride, const void* window, const int64_t* window_slots,
+                               const int64_t* lengths, const float* signs1, const float* signs2, const float* centroids,
+                               const void* gate, int64_t gate_stride_b, int64_t gate_stride_h, int64_t gate_stride_t, void* out,
+                               int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t, float* partial_stats,
+                               float* partial_values, int chunk_capacity, int32_t* counters, int batch, int q_heads, int kv_heads,
+                               int tokens, int head_dim, int block_size, int residual_len, int bits, int value_group,
+                               int64_t num_pages, int64_t max_blocks, float scaling, int dtype, anna_stream_t stream);
+
+/*
  * Arrival flags between the ranks of one box.  flag_arrays[r] (host array of `world` device pointers, 8-byte aligned)
  * is rank r's array of `world` uint64 flags in memory every rank can write; entry [rank] is the caller's own.  One warp
  * stores `step` into flag `rank` of every other rank (release, system scope: everything this stream wrote to peer
