@@ -324,6 +324,7 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
   p.num_pages = num_pages; p.max_blocks = max_blocks; p.max_len = max_blocks * block_size + residual_len;
   p.scaling = scaling;
   multi_plan(batch, kv_heads, p.rows, p.max_len, &p.chunk_tokens, &p.num_chunks);
+  if (tq_multi_mma_applicable(p, batch, head_dim, bits, dtype)) return launch_tq_multi_mma(p, batch, head_dim, bits, dtype, (cudaStream_t)stream);
   const int row_tiles = (p.rows + kMultiRows - 1) / kMultiRows;
   ANNA_REQUIRE((int64_t)kv_heads * row_tiles <= 65535, "%s: too many queries", what);
   const dim3 grid((unsigned)p.num_chunks, (unsigned)(kv_heads * row_tiles), (unsigned)batch);

@@ -323,6 +323,28 @@ def test_nans_reach_the_rows_that_see_them_and_no_others(cuda_device, dtype, dim
             case.check(got, rows=~bad & ~mask_of(case, what == 0))
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,bits", [("bf16", 128, 4), ("fp16", 256, 3), ("fp16", 128, 2), ("fp32", 128, 4)])
+def test_packed_infinities_behind_a_query(cuda_device, dtype, dim, bits):
+    """New tokens that have left the window: the scale of one of them is infinite or NaN in one group of dims."""
+    window, tokens, length = 2, 9, 70
+    case = Case(lengths=[length, 40], tokens=tokens, group=2, kv_heads=2, dim=dim, bits=bits, page=16, window=window, dtype=dtype,
+                device=cuda_device, seed=13)
+    at = length - 5  # queries 4 .. 8 see it
+    elem = 4 if dtype == "fp32" else 2
+    for value in (math.inf, math.nan):
+        offset = case.layout["off_vzero"] + (at % 16 * (dim // 32) + 1) * elem
+        where = (int(case.table[0, at // 16]), 1, slice(offset, offset + elem))
+        was = case.packed[where].clone()
+        case.packed[where] = torch.tensor([value], dtype=case.dtype).view(torch.uint8)
+        got = case.run()
+        case.packed[where] = was
+        bad = ~torch.isfinite(got)
+        assert bad[0, 2:, 4:, 32:64].all() and int(bad.sum()) == 2 * 5 * 32
+        assert bool((torch.isnan(got[bad]) if math.isnan(value) else got[bad] == value).all())
+        case.check(got, rows=~bad.any(-1))
+
+
+@pytest.mark.gpu
 def test_captured_calls_and_two_graphs_side_by_side(cuda_device):
     cases = [Case(lengths=[2000 + 300 * i, 100], tokens=4, group=4, kv_heads=2, dim=128, bits=4, page=16, window=16, dtype="bf16",
                   device=cuda_device, seed=i) for i in range(2)]
