@@ -88,9 +88,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                            c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_i32, c_i32,
                                            c_ptr, c_ptr, c_size, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                            c_i64, c_i64, c_f32, c_i32, c_ptr, c_i32, c_ptr]),
-    "anna_tq_multi_decode_plan": (c_i32, [c_i32] * 4 + [c_i64, c_i32, c_i32, ctypes.POINTER(c_i32), ctypes.POINTER(c_i32)]),
+    "anna_tq_multi_decode_plan": (c_i32, [c_i32] * 5 + [ctypes.POINTER(c_i64), ctypes.POINTER(c_i32)]),
     "anna_tq_paged_multi_decode": (c_i32, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_i64] + [c_ptr] * 6 +
-                                   [c_ptr, c_i64, c_i64, c_i64] * 2 + [c_ptr, c_ptr, c_i32, c_ptr] + [c_i32] * 9 +
+                                   [c_ptr, c_i64, c_i64, c_i64] * 2 + [c_ptr, c_i64, c_ptr] + [c_i32] * 9 +
                                    [c_i64, c_i64, c_f32, c_i32, c_ptr]),
     "anna_peer_signal_wait": (c_i32, [c_ptr, c_i32, c_i32, c_i64, c_i64, c_ptr, c_ptr]),
     "anna_kv_selftest_umma_tma": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, ctypes.POINTER(c_i32), c_ptr]),
@@ -198,14 +198,13 @@ def tq_decode_plan(batch: int, kv_heads: int, max_blocks: int, block_size: int, 
     return int(chunk.value), int(chunks.value)
 
 
-def tq_multi_decode_plan(batch: int, heads: int, kv_heads: int, tokens: int, max_blocks: int, block_size: int,
-                         residual_len: int) -> tuple[int, int]:
-    """(chunks of the keys, arrival counters) of a multi-token decode."""
-    chunks = c_i32(0)
+def tq_multi_decode_plan(batch: int, heads: int, kv_heads: int, tokens: int, head_dim: int) -> tuple[int, int]:
+    """(floats of scratch, arrival counters) of a multi-token decode."""
+    floats = c_i64(0)
     counters = c_i32(0)
-    check(lib().anna_tq_multi_decode_plan(batch, heads, kv_heads, tokens, max_blocks, block_size, residual_len,
-                                          ctypes.byref(chunks), ctypes.byref(counters)), "anna_tq_multi_decode_plan")
-    return int(chunks.value), int(counters.value)
+    check(lib().anna_tq_multi_decode_plan(batch, heads, kv_heads, tokens, head_dim, ctypes.byref(floats), ctypes.byref(counters)),
+          "anna_tq_multi_decode_plan")
+    return int(floats.value), int(counters.value)
 
 
 def tq_page_layout(head_dim: int, bits: int, block_size: int, dtype_code: int, value_group: int) -> dict[str, int]:

@@ -19,6 +19,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstring>
 #include <map>
 #include <mutex>
@@ -754,7 +755,388 @@ PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Py_RETURN_NONE;
 }
 
+// ---- several tokens at a time, and page copies ---------------------------------------------------------------------------------
+
+bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
+
+// Arrival counters of a stream: zero whenever no call is under way.  A call under graph capture gets its own, zeroed by the graph:
+// graphs may be replayed side by side.  The stream's device must be current.
+at::Tensor arrival_counters(c10::Device device, cudaStream_t stream, int64_t count) {
+  const auto options = at::TensorOptions().dtype(at::kInt).device(device);
+  if (capturing()) return at::zeros({count}, options);
+  static auto* kept = new std::map<std::pair<int64_t, int64_t>, at::Tensor>();  // never destroyed: see scratch_table
+  at::Tensor& counters = (*kept)[{device.index(), reinterpret_cast<int64_t>(stream)}];
+  if (!counters.defined() || counters.numel() < count) counters = at::zeros({count < 4096 ? 4096 : count}, options);
+  return counters;
+}
+
+// tq_multi_decode(query, gate | None, packed_pages, table, window, slots, lengths, signs1, signs2, centroids, scaling, bits,
+//                 residual_len, block_size, value_group) -> output | None
+PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 15) return PyErr_Format(PyExc_TypeError, "tq_multi_decode takes 15 arguments");
+  bool ok = true;
+  const at::Tensor* query = tensor(args[0]);
+  const at::Tensor* gate = optional_tensor(args[1], &ok);
+  const at::Tensor* t[8];  // pages, table, window, slots, lengths, signs1, signs2, centroids
+  for (int i = 0; i < 8; ++i) {
+    t[i] = tensor(args[2 + i]);
+    ok = ok && t[i] != nullptr;
+  }
+  const double scaling = PyFloat_AsDouble(args[10]);
+  if (scaling == -1.0 && PyErr_Occurred()) return nullptr;
+  int64_t n[4];  // bits, residual_len, block_size, value_group
+  if (!int_args(args + 11, 4, n)) return nullptr;
+  int code = 0;
+  if (!ok || query == nullptr || !query->is_cuda() || !plain(*query, query->device(), 4) || query->stride(3) != 1 || query->numel() == 0 ||
+      !dtype_code(query->scalar_type(), &code))
+    Py_RETURN_NONE;
+  const c10::Device device = query->device();
+  for (const at::Tensor* x : t)
+    if (x->device() != device || x->layout() != at::kStrided) Py_RETURN_NONE;
+  const at::Tensor &pages = *t[0], &table = *t[1], &window = *t[2], &slots = *t[3], &lengths = *t[4];
+  const int64_t batch = query->size(0), heads = query->size(1), tokens = query->size(2), dim = query->size(3);
+  anna_tq_layout layout;
+  if (n[1] <= 0 || n[2] <= 0 || n[1] > INT32_MAX || n[2] > INT32_MAX || n[3] > INT32_MAX || tokens > INT32_MAX ||
+      anna_tq_page_layout((int)dim, (int)n[0], (int)n[2], code, (int)n[3], &layout) != ANNA_OK)
+    Py_RETURN_NONE;
+  if (pages.dim() != 3 || pages.scalar_type() != at::kByte || !pages.is_contiguous() || pages.size(2) != layout.chunk_bytes ||
+      pages.size(0) == 0 || pages.size(1) == 0 || heads % pages.size(1) != 0 || table.dim() != 2 || table.scalar_type() != at::kInt ||
+      table.size(0) != batch || (table.size(1) > 1 && table.stride(1) != 1) || window.dim() != 5 ||
+      window.scalar_type() != query->scalar_type() || !window.is_contiguous() || window.size(1) != 2 || window.size(2) != pages.size(1) ||
+      window.size(3) != n[1] || window.size(4) != dim)
+    Py_RETURN_NONE;
+  for (const at::Tensor* x : {&slots, &lengths})
+    if (x->dim() != 1 || x->scalar_type() != at::kLong || x->size(0) != batch || !x->is_contiguous()) Py_RETURN_NONE;
+  if (gate != nullptr && (!plain(*gate, device, 4) || gate->stride(3) != 1 || gate->scalar_type() != query->scalar_type() ||
+                          gate->sizes() != query->sizes()))
+    Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(device);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  const int kv_heads = (int)pages.size(1);
+  const int64_t max_blocks = table.size(1);
+  int status;
+  if (tokens == 1) {
+    // One token is the single-token decode (one row of 4000 tokens, 32/8 heads: 11.5 us there, 22.5 here), in scratch of its own.
+    int chunk = 0, chunks = 0;
+    status = anna_tq_decode_plan((int)batch, kv_heads, max_blocks, (int)n[2], (int)n[1], &chunk, &chunks);
+    if (status != 0) return failed("tq_paged_multi_decode", status);
+    const int64_t groups = (heads / kv_heads + 7) / 8, stats = (batch * heads * chunks * 2 + 3) / 4 * 4;
+    const size_t frag_bytes = anna_tq_query_scratch_bytes((int)batch, (int)heads, kv_heads, (int)dim);
+    at::Tensor out = at::empty(query->sizes(), query->options());
+    at::Tensor partials = at::empty({stats + batch * heads * chunks * dim}, query->options().dtype(at::kFloat));
+    at::Tensor frags = at::empty({(int64_t)frag_bytes}, query->options().dtype(at::kByte));
+    at::Tensor counters = arrival_counters(device, stream, 2 * batch * kv_heads * groups);
+    {
+      pybind11::gil_scoped_release unlocked;
+      status = anna_tq_paged_decode(
+          query->data_ptr(), query->stride(0), query->stride(1), static_cast<const uint8_t*>(pages.data_ptr()),
+          static_cast<const int32_t*>(table.data_ptr()), table.stride(0), window.data_ptr(), static_cast<const int64_t*>(slots.data_ptr()),
+          static_cast<const int64_t*>(lengths.data_ptr()), floats(t[5]), floats(t[6]), floats(t[7]), address(gate),
+          gate == nullptr ? 0 : gate->stride(0), gate == nullptr ? 0 : gate->stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+          partials.data_ptr<float>(), partials.data_ptr<float>() + stats, chunks, 0, static_cast<int32_t*>(counters.data_ptr()),
+          frags.data_ptr(), frag_bytes, (int)batch, (int)heads, kv_heads, (int)dim, (int)n[2], (int)n[1], (int)n[0], (int)n[3],
+          pages.size(0), max_blocks, (float)scaling, code, stream);
+    }
+    if (status != 0) return failed("tq_paged_multi_decode", status);
+    return THPVariable_Wrap(std::move(out));
+  }
+  int64_t floats_needed = 0;
+  int arrivals = 0;
+  status = anna_tq_multi_decode_plan((int)batch, (int)heads, kv_heads, (int)tokens, (int)dim, &floats_needed, &arrivals);
+  if (status != 0) return failed("tq_paged_multi_decode", status);
+  at::Tensor out = at::empty(query->sizes(), query->options());
+  at::Tensor scratch = at::empty({floats_needed}, query->options().dtype(at::kFloat)), counters = arrival_counters(device, stream, arrivals);
+  {
+    pybind11::gil_scoped_release unlocked;
+    status = anna_tq_paged_multi_decode(
+        query->data_ptr(), query->stride(0), query->stride(1), query->stride(2), static_cast<const uint8_t*>(pages.data_ptr()),
+        static_cast<const int32_t*>(table.data_ptr()), table.stride(0), window.data_ptr(), static_cast<const int64_t*>(slots.data_ptr()),
+        static_cast<const int64_t*>(lengths.data_ptr()), floats(t[5]), floats(t[6]), floats(t[7]), address(gate),
+        gate == nullptr ? 0 : gate->stride(0), gate == nullptr ? 0 : gate->stride(1), gate == nullptr ? 0 : gate->stride(2), out.data_ptr(),
+        out.stride(0), out.stride(1), out.stride(2), scratch.data_ptr<float>(), floats_needed, static_cast<int32_t*>(counters.data_ptr()), (int)batch, (int)heads, kv_heads, (int)tokens, (int)dim, (int)n[2], (int)n[1], (int)n[0],
+        (int)n[3], pages.size(0), max_blocks, (float)scaling, code, stream);
+  }
+  if (status != 0) return failed("tq_paged_multi_decode", status);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// Strides per axis, batch and token of positions [axes, B, T] or [B, T]; false for others.
+bool position_strides(const at::Tensor& positions, c10::Device device, int64_t axes, int64_t batch, int64_t tokens, int64_t* strides) {
+  if (positions.device() != device || positions.layout() != at::kStrided || positions.scalar_type() != at::kLong) return false;
+  const int64_t d = positions.dim();
+  if ((d != 2 && d != 3) || positions.size(d - 2) != batch || positions.size(d - 1) != tokens) return false;
+  if (d == 3 && positions.size(0) != axes) return false;
+  strides[0] = d == 3 ? positions.stride(0) : 0;
+  strides[1] = positions.stride(d - 2);
+  strides[2] = positions.stride(d - 1);
+  return true;
+}
+// queries and keys as run_multi_axis_rotary takes them
+bool rotary_rows(const at::Tensor* query, const at::Tensor* key, int* code) {
+  if (query == nullptr || key == nullptr || !query->is_cuda() || !plain(*query, query->device(), 4) || !plain(*key, query->device(), 4))
+    return false;
+  return query->stride(3) == 1 && key->stride(3) == 1 && query->numel() != 0 && key->numel() != 0 && query->size(0) == key->size(0) &&
+         query->size(2) == key->size(2) && query->size(3) == key->size(3) && query->scalar_type() == key->scalar_type() &&
+         query->size(3) <= INT32_MAX && query->size(2) <= INT32_MAX && query->size(0) <= INT32_MAX && query->size(1) <= INT32_MAX &&
+         key->size(1) <= INT32_MAX && dtype_code(query->scalar_type(), code);
+}
+
+// rotary(query, key, positions, rates, axes, axis_count, rotary_dim, scale) -> (query, key) turned | None
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) return PyErr_Format(PyExc_TypeError, "rotary takes 8 arguments");
+  const at::Tensor *query = tensor(args[0]), *key = tensor(args[1]), *positions = tensor(args[2]), *rates = tensor(args[3]),
+                   *axes = tensor(args[4]);
+  int64_t n[2];  // axis_count, rotary_dim
+  if (!int_args(args + 5, 2, n)) return nullptr;
+  const double scale = PyFloat_AsDouble(args[7]);
+  if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+  int code = 0;
+  int64_t ps[3];
+  if (positions == nullptr || rates == nullptr || axes == nullptr || !rotary_rows(query, key, &code) ||
+      !position_strides(*positions, query->device(), n[0], query->size(0), query->size(2), ps))
+    Py_RETURN_NONE;
+  const c10::Device device = query->device();
+  const c10::cuda::CUDAGuard guard(device);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  at::Tensor q = at::empty(query->sizes(), query->options()), k = at::empty(key->sizes(), key->options());
+  const int status = anna_multi_axis_rotary(
+      query->data_ptr(), query->stride(0), query->stride(1), query->stride(2), q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
+      key->data_ptr(), key->stride(0), key->stride(1), key->stride(2), k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+      static_cast<const int64_t*>(positions->data_ptr()), ps[0], ps[1], ps[2], static_cast<const double*>(rates->data_ptr()),
+      static_cast<const int32_t*>(axes->data_ptr()), (float)scale, (int)query->size(0), (int)query->size(1), (int)key->size(1),
+      (int)query->size(2), (int)query->size(3), (int)n[1], code, stream);
+  if (status != 0) return failed("multi_axis_rotary", status);
+  PyObject* pair = PyTuple_New(2);
+  if (pair == nullptr) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(q)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(k)));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+// rotary_write(query, key, value, key_pages, value_pages, table, past, positions | None, deltas | None, new_lengths | None,
+//              status | None, rates, axes, axis_count, rotary_dim, scale) -> query turned | None
+PyObject* rotary_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 16) return PyErr_Format(PyExc_TypeError, "rotary_write takes 16 arguments");
+  bool ok = true;
+  const at::Tensor *query = tensor(args[0]), *key = tensor(args[1]), *value = tensor(args[2]), *kp = tensor(args[3]), *vp = tensor(args[4]),
+                   *table = tensor(args[5]), *past = tensor(args[6]);
+  const at::Tensor *positions = optional_tensor(args[7], &ok), *deltas = optional_tensor(args[8], &ok), *fresh = optional_tensor(args[9], &ok),
+                   *word = optional_tensor(args[10], &ok);
+  const at::Tensor *rates = tensor(args[11]), *axes = tensor(args[12]);
+  int64_t n[2];  // axis_count, rotary_dim
+  if (!int_args(args + 13, 2, n)) return nullptr;
+  const double scale = PyFloat_AsDouble(args[15]);
+  if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+  int code = 0;
+  if (!ok || value == nullptr || kp == nullptr || vp == nullptr || table == nullptr || past == nullptr || rates == nullptr ||
+      axes == nullptr || !rotary_rows(query, key, &code))
+    Py_RETURN_NONE;
+  const c10::Device device = query->device();
+  const int64_t batch = query->size(0), tokens = query->size(2);
+  const at::ScalarType type = query->scalar_type();
+  if (!plain(*value, device, 4) || value->sizes() != key->sizes() || value->stride(3) != 1 || value->scalar_type() != type ||
+      !plain(*kp, device, 4) || !plain(*vp, device, 4) || kp->sizes() != vp->sizes() || kp->scalar_type() != type || vp->scalar_type() != type ||
+      !kp->is_contiguous() || !vp->is_contiguous() || kp->size(0) == 0 || kp->size(1) != key->size(1) || kp->size(2) == 0 ||
+      kp->size(2) > INT32_MAX || kp->size(3) != key->size(3))
+    Py_RETURN_NONE;
+  if (!plain(*table, device, 2) || table->scalar_type() != at::kInt || table->size(0) != batch || table->size(1) == 0 ||
+      (table->size(1) > 1 && table->stride(1) != 1))
+    Py_RETURN_NONE;
+  for (const at::Tensor* x : {past, fresh})
+    if (x != nullptr && (!plain(*x, device, 1) || x->scalar_type() != at::kLong || x->size(0) != batch || !x->is_contiguous())) Py_RETURN_NONE;
+  if (fresh != nullptr && fresh->data_ptr() == past->data_ptr()) Py_RETURN_NONE;
+  if (word != nullptr && (word->device() != device || word->scalar_type() != at::kInt || word->numel() != 1)) Py_RETURN_NONE;
+  if (deltas != nullptr && (positions != nullptr || deltas->device() != device || deltas->scalar_type() != at::kLong ||
+                            (deltas->dim() != 1 && !(deltas->dim() == 2 && deltas->size(1) == 1)) || deltas->size(0) != batch))
+    Py_RETURN_NONE;
+  int64_t ps[3] = {0, 0, 0};
+  if (positions != nullptr && !position_strides(*positions, device, n[0], batch, tokens, ps)) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(device);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  at::Tensor q = at::empty(query->sizes(), query->options());
+  const int status = anna_rotary_paged_kv_write(
+      query->data_ptr(), query->stride(0), query->stride(1), query->stride(2), q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
+      key->data_ptr(), key->stride(0), key->stride(1), key->stride(2), value->data_ptr(), value->stride(0), value->stride(1),
+      value->stride(2), kp->data_ptr(), vp->data_ptr(), static_cast<const int32_t*>(table->data_ptr()), table->stride(0),
+      static_cast<const int64_t*>(past->data_ptr()), static_cast<int64_t*>(address(fresh)), static_cast<const int64_t*>(address(positions)),
+      ps[0], ps[1], ps[2], static_cast<const int64_t*>(address(deltas)), deltas == nullptr ? 0 : deltas->stride(0),
+      static_cast<const double*>(rates->data_ptr()), static_cast<const int32_t*>(axes->data_ptr()), (float)scale, (int)batch,
+      (int)query->size(1), (int)key->size(1), (int)tokens, (int)query->size(3), (int)n[1], (int)kp->size(2), kp->size(0), table->size(1),
+      code, static_cast<int32_t*>(address(word)), stream);
+  if (status != 0) return failed("rotary_paged_kv_write", status);
+  return THPVariable_Wrap(std::move(q));
+  END_HANDLE_TH_ERRORS
+}
+
+// A list or tuple of plain ints that are page ids; false for all others.
+struct PageIds {
+  PyObject *source, *target;  // the lists (borrowed)
+  int64_t first, count;       // in the call's pairs
+  int32_t highest_source, highest_target;
+};
+bool page_ids(PyObject* ids, std::vector<int32_t>* out, int32_t* highest) {
+  if (!PyList_CheckExact(ids) && !PyTuple_CheckExact(ids)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(ids);
+  out->resize((size_t)n);
+  *highest = -1;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* entry = PySequence_Fast_GET_ITEM(ids, i);
+    if (!PyLong_CheckExact(entry)) return false;
+    int overflow = 0;
+    const long id = PyLong_AsLongAndOverflow(entry, &overflow);
+    if (overflow != 0 || id < 0 || id >= INT32_MAX) return false;
+    (*out)[(size_t)i] = (int32_t)id;
+    if ((int32_t)id > *highest) *highest = (int32_t)id;
+  }
+  return true;
+}
+bool page_pool(const at::Tensor* pool, const at::Tensor* first) {
+  return pool != nullptr && pool->is_cuda() && pool->layout() == at::kStrided && pool->dim() >= 2 && pool->is_contiguous() &&
+         pool->size(0) > 0 && pool->size(0) < INT32_MAX && pool->device() == first->device();
+}
+
+int launch_page_copy(c10::Device device, const std::vector<anna_page_pool>& pools, const std::vector<int32_t>& pairs) {
+  const int64_t count = (int64_t)pairs.size() / 2;
+  if (count == 0 || pools.empty()) return ANNA_OK;
+  at::Tensor on_gpu;
+  if (count > anna_page_copy_max_pairs()) on_gpu = upload_bytes(device.index(), pairs.data(), (int64_t)pairs.size() * 4, {count * 2}, at::kInt);
+  return anna_page_copy(pools.data(), (int)pools.size(), pairs.data(), count,
+                        on_gpu.defined() ? static_cast<const int32_t*>(on_gpu.data_ptr()) : nullptr, nullptr,
+                        c10::cuda::getCurrentCUDAStream(device.index()).stream());
+}
+
+// page_copy([(pool, source ids, target ids), ...]) -> True | None
+PyObject* page_copy(PyObject*, PyObject* copies) {
+  HANDLE_TH_ERRORS
+  if (!PyList_CheckExact(copies) || PyList_GET_SIZE(copies) == 0) Py_RETURN_NONE;
+  const at::Tensor* first = nullptr;
+  std::vector<PageIds> lists;
+  std::vector<int32_t> pairs, source, target;
+  std::vector<anna_page_pool> pools;
+  std::vector<uint8_t> marks;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(copies); ++i) {
+    PyObject* entry = PyList_GET_ITEM(copies, i);
+    if (!PyTuple_CheckExact(entry) || PyTuple_GET_SIZE(entry) != 3) Py_RETURN_NONE;
+    const at::Tensor* pool = tensor(PyTuple_GET_ITEM(entry, 0));
+    if (first == nullptr) first = pool;
+    if (!page_pool(pool, first)) Py_RETURN_NONE;
+    PyObject *from = PyTuple_GET_ITEM(entry, 1), *to = PyTuple_GET_ITEM(entry, 2);
+    const PageIds* ids = nullptr;
+    for (size_t k = lists.size(); k-- > 0 && lists.size() - k <= 4;)  // pools of a layer name the same lists
+      if (lists[k].source == from && lists[k].target == to) ids = &lists[k];
+    if (ids == nullptr) {
+      PageIds made{from, to, (int64_t)pairs.size() / 2, 0, -1, -1};
+      if (!page_ids(from, &source, &made.highest_source) || !page_ids(to, &target, &made.highest_target) || source.size() != target.size())
+        Py_RETURN_NONE;
+      made.count = (int64_t)source.size();
+      if (made.first + made.count >= INT32_MAX) Py_RETURN_NONE;
+      marks.assign((size_t)std::max(made.highest_source, made.highest_target) + 1, 0);
+      for (const int32_t id : target)
+        if (marks[(size_t)id]++ != 0) Py_RETURN_NONE;  // a target twice
+      for (const int32_t id : source)
+        if (marks[(size_t)id] != 0) Py_RETURN_NONE;  // a source that is a target
+      for (size_t k = 0; k < source.size(); ++k) {
+        pairs.push_back(source[k]);
+        pairs.push_back(target[k]);
+      }
+      lists.push_back(made);
+      ids = &lists.back();
+    }
+    if (ids->highest_source >= pool->size(0) || ids->highest_target >= pool->size(0)) Py_RETURN_NONE;
+    const int64_t bytes = (int64_t)pool->nbytes() / pool->size(0);
+    if (ids->count == 0 || bytes == 0) continue;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(pool->data_ptr());
+    spans.emplace_back(at, at + pool->nbytes());
+    pools.push_back({pool->data_ptr(), pool->data_ptr(), bytes, (int32_t)pool->size(0), (int32_t)pool->size(0), (int32_t)ids->first,
+                     (int32_t)ids->count});
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t k = 1; k < spans.size(); ++k)
+    if (spans[k].first < spans[k - 1].second) Py_RETURN_NONE;  // one pool twice, or pools that overlap
+  const c10::cuda::CUDAGuard guard(first->device());
+  const int status = launch_page_copy(first->device(), pools, pairs);
+  if (status != 0) return failed("page_copy", status);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// page_gather([(pool, ids), ...], spare pages) -> [new pool, ...] | None
+PyObject* page_gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 2) return PyErr_Format(PyExc_TypeError, "page_gather(pools, spare pages)");
+  int64_t spare;
+  if (!int_args(args + 1, 1, &spare)) return nullptr;
+  PyObject* given = args[0];
+  if (!PyList_CheckExact(given) || PyList_GET_SIZE(given) == 0 || spare < 0 || spare >= INT32_MAX) Py_RETURN_NONE;
+  const at::Tensor* first = nullptr;
+  std::vector<PageIds> lists;
+  std::vector<int32_t> pairs, source;
+  std::vector<anna_page_pool> pools;
+  std::vector<int64_t> counts;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(given); ++i) {
+    PyObject* entry = PyList_GET_ITEM(given, i);
+    if (!PyTuple_CheckExact(entry) || PyTuple_GET_SIZE(entry) != 2) Py_RETURN_NONE;
+    const at::Tensor* pool = tensor(PyTuple_GET_ITEM(entry, 0));
+    if (first == nullptr) first = pool;
+    if (!page_pool(pool, first)) Py_RETURN_NONE;
+    PyObject* from = PyTuple_GET_ITEM(entry, 1);
+    const PageIds* ids = nullptr;
+    for (size_t k = lists.size(); k-- > 0 && lists.size() - k <= 4;)
+      if (lists[k].source == from) ids = &lists[k];
+    if (ids == nullptr) {
+      PageIds made{from, nullptr, (int64_t)pairs.size() / 2, 0, -1, -1};
+      if (!page_ids(from, &source, &made.highest_source)) Py_RETURN_NONE;
+      made.count = (int64_t)source.size();
+      if (made.first + made.count + spare >= INT32_MAX) Py_RETURN_NONE;
+      const size_t at = pairs.size();
+      pairs.resize(at + 2 * source.size());
+      for (size_t k = 0; k < source.size(); ++k) {
+        pairs[at + 2 * k] = source[k];
+        pairs[at + 2 * k + 1] = (int32_t)k;
+      }
+      lists.push_back(made);
+      ids = &lists.back();
+    }
+    if (ids->highest_source >= pool->size(0)) Py_RETURN_NONE;
+    counts.push_back(ids->count + spare);
+    pools.push_back({pool->data_ptr(), nullptr, (int64_t)pool->nbytes() / pool->size(0), (int32_t)pool->size(0), (int32_t)(ids->count + spare),
+                     (int32_t)ids->first, (int32_t)ids->count});
+  }
+  const c10::cuda::CUDAGuard guard(first->device());
+  PyObject* out = PyList_New(PyList_GET_SIZE(given));
+  if (out == nullptr) return nullptr;
+  struct Held {
+    PyObject* list;
+    ~Held() { Py_XDECREF(list); }
+  } held{out};
+  for (size_t i = 0; i < pools.size(); ++i) {
+    const at::Tensor& pool = *tensor(PyTuple_GET_ITEM(PyList_GET_ITEM(given, (Py_ssize_t)i), 0));
+    std::vector<int64_t> sizes = pool.sizes().vec();
+    sizes[0] = counts[i];
+    at::Tensor fresh = at::empty(sizes, pool.options());
+    pools[i].dst = fresh.data_ptr();
+    if (pools[i].page_bytes == 0) pools[i].count = 0;
+    PyList_SET_ITEM(out, (Py_ssize_t)i, THPVariable_Wrap(std::move(fresh)));
+  }
+  const int status = launch_page_copy(first->device(), pools, pairs);
+  if (status != 0) return failed("page_gather", status);
+  held.list = nullptr;
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"tq_multi_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tq_multi_decode)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
+    {"rotary_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary_write)), METH_FASTCALL, nullptr},
+    {"page_copy", page_copy, METH_O, nullptr},
+    {"page_gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(page_gather)), METH_FASTCALL, nullptr},
     {"take_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(take_pages)), METH_FASTCALL, nullptr},
     {"release_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(release_pages)), METH_FASTCALL, nullptr},
     {"copy_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(copy_pages)), METH_FASTCALL, nullptr},

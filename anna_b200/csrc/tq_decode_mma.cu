@@ -23,6 +23,7 @@
 #include "tq_common.cuh"
 #include "prefill_params.cuh"
 #include "tq_decode_params.cuh"
+#include "tq_multi_params.cuh"
 
 #include <cstdlib>
 
@@ -1599,12 +1600,13 @@ extern "C" int anna_kv_selftest_wait_expiry(int* expired, anna_stream_t stream) 
 // since the library was loaded (0 in a healthy run).  Synchronises the device.
 extern "C" int anna_kv_device_faults(int* count) {
   ANNA_REQUIRE(count != nullptr, "anna_kv_device_faults: null output pointer");
-  int mma = 0, umma = 0, prefill = 0;
+  int mma = 0, umma = 0, prefill = 0, multi = 0;
   int rc = anna::tq_decode_mma_faults(&mma);
   if (rc == ANNA_OK) rc = anna::tq_decode_umma_faults(&umma);
   if (rc == ANNA_OK) rc = anna::prefill_umma_faults(&prefill);
+  if (rc == ANNA_OK) rc = anna::tq_multi_mma_faults(&multi);
   if (rc != ANNA_OK) return rc;
-  *count = mma + umma + prefill;
+  *count = mma + umma + prefill + multi;
   return ANNA_OK;
 }
 

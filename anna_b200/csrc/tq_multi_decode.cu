@@ -33,19 +33,14 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
   __shared__ float sm_cent[1 << M], sm_norm[kMultiTokens], sm_rescale[kMultiRows];
   __shared__ bool sm_there[kMultiTokens];
 
-  const int chunk = blockIdx.x, kvh = blockIdx.y / row_tiles, tile = blockIdx.y % row_tiles;
-  const int64_t b = blockIdx.z;
-  const int row0 = tile * kMultiRows, count = min(kMultiRows, p.rows - row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < (1 << M)) sm_cent[threadIdx.x] = p.centroids[threadIdx.x];
+  multi_for_each_segment<T, D, kMultiThreads>(p, row_tiles, [&](int64_t b, int kvh, int tile, int64_t t0, int64_t t1, const MultiPartial& part) {
+  const int row0 = tile * kMultiRows, count = min(kMultiRows, p.rows - row0);
   const int64_t len = max((int64_t)0, min(p.lengths[b], p.max_len));
   const int64_t lq = len > p.residual_len ? len - p.residual_len : 0;
-  const int64_t t0 = (int64_t)chunk * p.chunk_tokens;
-  const int chunks = max(1, (int)((len + p.chunk_tokens - 1) / p.chunk_tokens));  // an empty row has one chunk, which writes zeros
-  if (chunk >= chunks) return;
-  const int64_t t1 = min(len, t0 + p.chunk_tokens);
   const int64_t first_seen = len - p.tokens;  // newest key that query 0 sees
 
-  if (threadIdx.x < (1 << M)) sm_cent[threadIdx.x] = p.centroids[threadIdx.x];
   const float f1 = p.scaling / (float)D;
   const float f2 = f1 * 1.2533141373155001f * rsqrt_dim_const<D>();
   for (int i = warp; i < kMultiRows; i += kMultiWarps) {
@@ -213,7 +208,7 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
   }
   __syncthreads();
   const int d0 = D >= kMultiThreads ? (int)threadIdx.x : (int)threadIdx.x % D;
-  if (chunks == 1) {
+  if (part.count == 1) {
     float* den = weight;
     if (lane == 0) {
       den[warp] = l_run[0];
@@ -230,55 +225,47 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
         multi_store<T, 1>(p, b, kvh, row0 + out_row0 + r, d0 + j * kMultiThreads, o);
       }
     }
+    __syncthreads();
     return;
   }
+  const int64_t at = multi_partial_row(part, part.mine, kMultiRows);
   if (lane == 0) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int i = warp + k * kMultiWarps;
       if (i < count)
-        reinterpret_cast<float2*>(p.stats)[multi_row_index(p, b, kvh, row0 + i) * p.num_chunks + chunk] = make_float2(m_run[k], l_run[k]);
+        reinterpret_cast<float2*>(p.stats)[at + i] = make_float2(m_run[k], l_run[k]);
     }
   }
 #pragma unroll
   for (int r = 0; r < kOutRows; ++r) {
     if (out_row0 + r >= count) break;
-    float* to = p.values + (multi_row_index(p, b, kvh, row0 + out_row0 + r) * p.num_chunks + chunk) * D;
+    float* to = p.values + (at + out_row0 + r) * D;
 #pragma unroll
     for (int j = 0; j < kDims; ++j) to[d0 + j * kMultiThreads] = acc[r][j];
   }
-  multi_merge<T, D, kMultiWarps>(p, b, kvh, tile, row_tiles, row0, count, chunks);
+  multi_merge<T, D, kMultiWarps, kMultiRows>(p, b, kvh, tile, row_tiles, count, part, smem);
+  __syncthreads();
+  });
 }
 
-// Chunks of the keys: two waves of four CTAs per SM, counting 16 rows to a row tile, in multiples of 128 tokens (two tiles of 16
-// for each of four warps).
-static void multi_plan(int batch, int kv_heads, int rows, int64_t max_len, int* chunk_tokens, int* num_chunks) {
-  const int64_t units = (int64_t)batch * kv_heads * ((rows + 15) / 16);
-  const int64_t wanted = (148 * 8 + units - 1) / units;
-  const int64_t len = max_len > 0 ? max_len : 1;
-  int64_t chunk = ((len + wanted - 1) / wanted + 127) / 128 * 128;
-  if (chunk > 4096) chunk = 4096;
-  while ((len + chunk - 1) / chunk > 512) chunk *= 2;
-  *chunk_tokens = (int)chunk;
-  *num_chunks = (int)((len + chunk - 1) / chunk);
-}
+// Rows of a row tile and CTAs per SM of this form: a wave of two holds the partials of 8 rows where the other's four hold 16.
+static_assert(148 * 2 <= kMultiMaxCtas && kMultiRows <= kMultiScratchRows);
 
 }  // namespace anna
 
 using namespace anna;
 
-extern "C" int anna_tq_multi_decode_plan(int batch, int q_heads, int kv_heads, int tokens, int64_t max_blocks, int block_size,
-                                         int residual_len, int* num_chunks, int* counters) {
-  ANNA_REQUIRE(num_chunks != nullptr && counters != nullptr, "anna_tq_multi_decode_plan: null pointer argument");
-  ANNA_REQUIRE(batch > 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && tokens > 0 && max_blocks >= 0 && block_size > 0 &&
-                   residual_len > 0, "anna_tq_multi_decode_plan: bad sizes");
-  ANNA_REQUIRE((int64_t)tokens * q_heads < (1 << 20) && max_blocks < (1ll << 31) / block_size - residual_len,
-               "anna_tq_multi_decode_plan: too many queries or keys");
-  const int rows = tokens * (q_heads / kv_heads);
-  const int64_t tiles = (int64_t)batch * kv_heads * ((rows + kMultiRows - 1) / kMultiRows);
-  ANNA_REQUIRE(tiles < (1ll << 31), "anna_tq_multi_decode_plan: too many rows");
-  int chunk = 0;
-  multi_plan(batch, kv_heads, rows, max_blocks * block_size + residual_len, &chunk, num_chunks);
+extern "C" int anna_tq_multi_decode_plan(int batch, int q_heads, int kv_heads, int tokens, int head_dim, int64_t* scratch_size,
+                                         int* counters) {
+  const char* what = "anna_tq_multi_decode_plan";
+  ANNA_REQUIRE(scratch_size != nullptr && counters != nullptr, "%s: null pointer argument", what);
+  ANNA_REQUIRE(batch > 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && tokens > 0 && head_dim > 0, "%s: bad sizes", what);
+  ANNA_REQUIRE((int64_t)tokens * q_heads < (1 << 20) && (int64_t)tokens * (q_heads / kv_heads) * (q_heads / kv_heads) < (1ll << 32),
+               "%s: too many queries", what);
+  const int64_t tiles = (int64_t)batch * kv_heads * ((tokens * (q_heads / kv_heads) + kMultiRows - 1) / kMultiRows);
+  ANNA_REQUIRE(tiles < (1ll << 31), "%s: too many queries", what);
+  *scratch_size = (int64_t)kMultiMaxCtas * 2 * kMultiScratchRows * (head_dim + 2);
   *counters = (int)tiles;
   return ANNA_OK;
 }
@@ -288,55 +275,74 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
                                           const void* window, const int64_t* window_slots, const int64_t* lengths,
                                           const float* signs1, const float* signs2, const float* centroids, const void* gate,
                                           int64_t gate_stride_b, int64_t gate_stride_h, int64_t gate_stride_t, void* out,
-                                          int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t, float* partial_stats,
-                                          float* partial_values, int chunk_capacity, int32_t* counters, int batch, int q_heads,
-                                          int kv_heads, int tokens, int head_dim, int block_size, int residual_len, int bits,
+                                          int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t, float* scratch,
+                                          int64_t scratch_size, int32_t* counters, int batch, int q_heads, int kv_heads,
+                                          int tokens, int head_dim, int block_size, int residual_len, int bits,
                                           int value_group, int64_t num_pages, int64_t max_blocks, float scaling, int dtype,
                                           anna_stream_t stream) {
   const char* what = "anna_tq_paged_multi_decode";
-  ANNA_REQUIRE(q && window && window_slots && lengths && signs1 && signs2 && centroids && out && counters, "%s: null pointer argument", what);
+  ANNA_REQUIRE(q && window && window_slots && lengths && signs1 && signs2 && centroids && out && counters && scratch,
+               "%s: null pointer argument", what);
+  ANNA_REQUIRE(max_blocks >= 0 && block_size > 0 && residual_len > 0, "%s: bad sizes", what);
   ANNA_REQUIRE(max_blocks == 0 || (packed_pages && block_table && num_pages > 0), "%s: a block table needs pages", what);
-  int num_chunks = 0, tiles = 0;
-  if (const int rc = anna_tq_multi_decode_plan(batch, q_heads, kv_heads, tokens, max_blocks, block_size, residual_len, &num_chunks, &tiles))
-    return rc;
-  ANNA_REQUIRE(batch <= 65535, "%s: at most 65535 sequences", what);
-  if (chunk_capacity < num_chunks || (num_chunks > 1 && (partial_stats == nullptr || partial_values == nullptr)))
-    return set_error(ANNA_ERR_WORKSPACE, "%s: scratch holds %d chunks, %d are needed", what, chunk_capacity, num_chunks);
+  int64_t needed = 0;
+  int tiles = 0;
+  if (const int rc = anna_tq_multi_decode_plan(batch, q_heads, kv_heads, tokens, head_dim, &needed, &tiles)) return rc;
+  if (scratch_size < needed)
+    return set_error(ANNA_ERR_WORKSPACE, "%s: scratch holds %lld floats, %lld are needed", what, (long long)scratch_size, (long long)needed);
+  ANNA_REQUIRE(max_blocks < ((1ll << 30) - residual_len) / block_size, "%s: too many keys", what);
   TqMultiParams p{};
   ANNA_REQUIRE(dtype == ANNA_DTYPE_F32 || dtype == ANNA_DTYPE_F16 || dtype == ANNA_DTYPE_BF16, "%s: unknown dtype %d", what, dtype);
   if (!tq_make_layout(head_dim, bits, block_size, dtype_bytes_of(dtype), value_group, &p.layout))
     return set_error(ANNA_ERR_UNSUPPORTED, "%s: unsupported page geometry (head_dim %d, bits %d, value group %d)", what, head_dim, bits,
                      value_group);
   ANNA_REQUIRE(aligned_to(packed_pages, 16) && aligned_to(window, 16), "%s: pages and window must be 16-byte aligned", what);
-  ANNA_REQUIRE(aligned_to(partial_stats, 8) && aligned_to(partial_values, 16), "%s: scratch must be 8- and 16-byte aligned", what);
+  ANNA_REQUIRE(aligned_to(scratch, 16), "%s: scratch must be 16-byte aligned", what);
   p.q = q; p.q_stride_b = q_stride_b; p.q_stride_h = q_stride_h; p.q_stride_t = q_stride_t;
   p.pages = packed_pages; p.block_table = block_table; p.table_stride = table_stride;
   p.window = window; p.window_slots = window_slots; p.lengths = lengths;
   p.signs1 = signs1; p.signs2 = signs2; p.centroids = centroids;
   p.gate = gate; p.gate_stride_b = gate_stride_b; p.gate_stride_h = gate_stride_h; p.gate_stride_t = gate_stride_t;
   p.out = out; p.out_stride_b = out_stride_b; p.out_stride_h = out_stride_h; p.out_stride_t = out_stride_t;
-  p.stats = partial_stats; p.values = partial_values; p.counters = counters;
+  p.values = scratch; p.stats = scratch + (int64_t)kMultiMaxCtas * 2 * kMultiScratchRows * head_dim; p.counters = counters;
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.groups = q_heads / kv_heads; p.tokens = tokens; p.rows = tokens * p.groups;
+  p.groups_inverse = (uint32_t)(((1ull << 32) + p.groups - 1) / p.groups);  // of one: not read
   p.block_size = block_size; p.residual_len = residual_len; p.value_group = value_group;
   p.block_shift = -1;
   for (int s = 0; s < 31; ++s)
     if ((1 << s) == block_size) p.block_shift = s;
   p.num_pages = num_pages; p.max_blocks = max_blocks; p.max_len = max_blocks * block_size + residual_len;
   p.scaling = scaling;
-  multi_plan(batch, kv_heads, p.rows, p.max_len, &p.chunk_tokens, &p.num_chunks);
-  if (tq_multi_mma_applicable(p, batch, head_dim, bits, dtype)) return launch_tq_multi_mma(p, batch, head_dim, bits, dtype, (cudaStream_t)stream);
+  p.stream_tiles = tq_multi_mma_applicable(p, head_dim, dtype) && head_dim == 128 && p.rows <= 16 ? 32 : 64;
   const int row_tiles = (p.rows + kMultiRows - 1) / kMultiRows;
-  ANNA_REQUIRE((int64_t)kv_heads * row_tiles <= 65535, "%s: too many queries", what);
-  const dim3 grid((unsigned)p.num_chunks, (unsigned)(kv_heads * row_tiles), (unsigned)batch);
-  return ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
-    return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
-      return ANNA_DISPATCH_TQ_BITS(bits, BITS, [&]() -> int {
-        constexpr int smem = kMultiSmemFloats<D> * 4;
-        auto kernel = tq_multi_kernel<T, D, BITS>;
-        ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        kernel<<<grid, kMultiThreads, smem, (cudaStream_t)stream>>>(p, row_tiles);
-        return check_launch("tq_multi_kernel");
+  const bool tensor_cores = tq_multi_mma_applicable(p, head_dim, dtype);
+  // The line of a launch has room for so many rows and positions: larger batches go in several, one behind the other.
+  const int64_t row_positions = (int64_t)kv_heads * row_tiles * ((p.max_len + kBalancedTileTokens - 1) / kBalancedTileTokens + p.stream_tiles);
+  ANNA_REQUIRE(row_positions < (1ll << 30), "%s: too many queries and keys of one sequence", what);
+  int most = (int)(((1ll << 30) - 1) / row_positions);
+  if (most > kBalancedMaxRows) most = kBalancedMaxRows;
+  for (int at = 0; at < batch; at += most) {
+    p.batch = batch - at < most ? batch - at : most;
+    const int rc = tensor_cores ? launch_tq_multi_mma(p, head_dim, bits, dtype, (cudaStream_t)stream)
+                                : ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+      return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
+        return ANNA_DISPATCH_TQ_BITS(bits, BITS, [&]() -> int {
+          constexpr int smem = kMultiSmemFloats<D> * 4;
+          auto kernel = tq_multi_kernel<T, D, BITS>;
+          ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+          kernel<<<multi_ctas(p, row_tiles, D == 256 ? 1 : 2), kMultiThreads, smem, (cudaStream_t)stream>>>(p, row_tiles);
+          return check_launch("tq_multi_kernel");
+        });
       });
     });
-  });
+    if (rc != ANNA_OK) return rc;
+    const int64_t elem = dtype_bytes_of(dtype);
+    p.q = static_cast<const uint8_t*>(p.q) + (int64_t)most * q_stride_b * elem;
+    p.out = static_cast<uint8_t*>(p.out) + (int64_t)most * out_stride_b * elem;
+    if (p.gate != nullptr) p.gate = static_cast<const uint8_t*>(p.gate) + (int64_t)most * gate_stride_b * elem;
+    if (p.block_table != nullptr) p.block_table += (int64_t)most * table_stride;
+    p.window_slots += most;
+    p.lengths += most;
+  }
+  return ANNA_OK;
 }

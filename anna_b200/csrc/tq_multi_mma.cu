@@ -9,14 +9,14 @@
 //       Q1 = fwht(s1*q), Q2 = sqrt(pi/2)/sqrt(D) * fwht(s2*Q1), each row scaled to a largest value of 1 and rounded to fp16
 //   score (log2 units) = f_row * norm_token * S,   f_row = largest value of the row * |scaling| * log2(e) / D
 //   online softmax in fp32 on the accumulators, P rounded to fp16
-//   O[rows x D] += P . (code * scale + zero)                       value codes as fp16 by exponent bits, one packed FMA a pair
+//   O[rows x D] += P . (code * scale + zero)                       value codes as fp16 by exponent bits
 //
 // The k-slots of the products and the columns of O are free to permute: a lane takes the coordinates whose codes it can unpack with
 // the fewest instructions, and 2 * D/8 neighbouring dims of an output row.
 //
 // What is rounded below 32 bits: the rotated queries, centroids and residual norms to fp16 (2^-12 of the row's largest value, of the
-// centroid and of the norm), probabilities and values to fp16 (2^-12 of themselves; bf16 caches fold 16 * scale into the zero,
-// up to 2^-8 of a quantization step).  Together they stay below the rounding of a bf16 output (2^-9 of the value).
+// centroid and of the norm), value scales and zeros, probabilities and values to fp16 (2^-12 of themselves).  Together they stay
+// below the rounding of a bf16 output (2^-9 of the value).
 #include "mbarrier_utils.cuh"
 #include "tq_multi_params.cuh"
 
@@ -24,7 +24,7 @@ namespace anna {
 
 __device__ int32_t g_tq_multi_faults;  // bumped when a bounded wait on a tile copy expires
 
-constexpr int kMultiMmaWarps = 4, kMultiMmaThreads = 32 * kMultiMmaWarps;
+constexpr int kMultiMmaWarps = 8, kMultiMmaThreads = 32 * kMultiMmaWarps;
 constexpr int kTile = 16;        // tokens
 constexpr int kStepTiles = 2;    // tiles of a step: one softmax update
 constexpr int kRingStages = 2;   // steps of a warp's ring
@@ -52,13 +52,15 @@ struct MultiCfg {
   static constexpr int kMergeStride = D + 8 * (D / 32) + 4;
   static constexpr int kMerge = kMultiMmaWarps * 16 * kMergeStride * 4;
   static constexpr int kWork = kRing + kQuery > kMerge ? kRing + kQuery : kMerge;
+  static_assert(kWork >= kRows * kMultiMaxPartials * 4, "the weights of the partials lie there, too");
   static constexpr int kOffBars = kWork;                                  // mbarriers [warps][stages]
   static constexpr int kOffValid = kOffBars + kMultiMmaWarps * kRingStages * 8;  // tokens per tile [warps][stages][tiles]
   static constexpr int kOffFactor = kOffValid + kMultiMmaWarps * kRingStages * kStepTiles * 4;  // f_row [rows]
-  static constexpr int kOffStats = kOffFactor + kRows * 4;                // m, l of the warps [warps][rows][2]
+  static constexpr int kOffLimit = kOffFactor + kRows * 4;                // newest key that the row sees [rows]
+  static constexpr int kOffStats = kOffLimit + kRows * 4;                 // m, l of the warps [warps][rows][2]
   static constexpr int kOffStrange = kOffStats + kMultiMmaWarps * kRows * 8;  // see strange_values
   static constexpr int kSmem = kOffStrange + 8;
-  static constexpr int kMinBlocks = D == 128 && MT == 1 ? 3 : 2;
+  static constexpr int kCtas = D == 128 && MT == 1 ? 2 : 1;  // per SM
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -86,6 +88,25 @@ __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   asm("sub.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+__device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 w, x, y, z;\n"
+      " mov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
 template <int LUT>
 __device__ __forceinline__ uint32_t lop3(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
@@ -110,8 +131,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// x << n, to the right for negative n
-__device__ __forceinline__ uint32_t shifted(uint32_t x, int n) { return n >= 0 ? x << n : x >> -n; }
+// x << n as a product: the multiply pipe has room, the logic pipe has not
+__device__ __forceinline__ uint32_t times_power(uint32_t x, int n) {
+  if (n == 0) return x;
+  uint32_t r;
+  asm("mul.lo.u32 %0, %1, %2;\n" : "=r"(r) : "r"(x), "r"(1u << n));
+  return r;
+}
 
 // A value that some rows see and others do not may be infinite or NaN, and zero times that is NaN: where a tile is cut by the rows'
 // limits, such values go into the product as zeros, and the rows that see them get them at the end (strange_values).
@@ -164,7 +190,7 @@ __device__ __forceinline__ FragSlot sign_slot(int c) {
 }
 
 template <typename T, int D, int BITS, int MT>
-__global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinBlocks)
+__global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas)
     tq_multi_mma_kernel(const TqMultiParams p, int row_tiles) {
   using Cfg = MultiCfg<D, BITS, MT>;
   constexpr int E = D / 32;
@@ -174,50 +200,93 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
   constexpr int kCols = 2 * kStepTiles;                     // 8-token columns of a step
   extern __shared__ __align__(1024) uint8_t smem[];
 
-  const int chunk = blockIdx.x, kvh = blockIdx.y / row_tiles, tile = blockIdx.y % row_tiles;
-  const int64_t b = blockIdx.z;
-  const int row0 = tile * Cfg::kRows, count = min(Cfg::kRows, p.rows - row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-  const int len = (int)max((int64_t)0, min(p.lengths[b], p.max_len));
-  const int lq = max(0, len - p.residual_len);
-  const int t0 = chunk * p.chunk_tokens;
-  const int chunks = max(1, (len + p.chunk_tokens - 1) / p.chunk_tokens);  // an empty row has one, which writes zeros
-  if (chunk >= chunks) return;
-  const int t1 = min(len, t0 + p.chunk_tokens);
-  const int q_end = min(t1, lq);
-  const int first_seen = len - p.tokens;  // newest key that query 0 sees
-
-  // ---- copies of the first steps ---------------------------------------------------------------------------------------------
   uint8_t* ring = smem + warp * Cfg::kWarpRing;
   const uint32_t bars = smem_u32(smem + Cfg::kOffBars) + warp * kRingStages * 8;
   volatile int* ring_valid = reinterpret_cast<volatile int*>(smem + Cfg::kOffValid) + warp * kRingStages * kStepTiles;
   int* strange = reinterpret_cast<int*>(smem + Cfg::kOffStrange);
-  if (threadIdx.x == 0) *strange = 0;
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < kRingStages; ++i) mbar_init(bars + 8 * i, 1);
     mbar_init_fence();
   }
+  // The centroids are rounded to fp16 at the scale, of 512 between 1 and 2, that leaves the smallest squared error over the codebook:
+  // as they are, their rounding was the largest error of an fp16 cache's output.
+  constexpr int kCentroids = 1 << (BITS - 1);
+  float cent[kCentroids];
+#pragma unroll
+  for (int e = 0; e < kCentroids; ++e) cent[e] = __ldg(p.centroids + e);
+  auto scale_of = [](uint32_t j) { return 1.0f + (float)j * (1.0f / 512.0f); };
+  uint32_t best = 0xffffffffu;  // error (its lowest bits left out), number of the scale
+#pragma unroll
+  for (int i = 0; i < 512 / kMultiMmaThreads; ++i) {
+    const uint32_t j = i * kMultiMmaThreads + threadIdx.x;
+    float error = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kCentroids; ++e) {
+      const float x = cent[e] * scale_of(j), d = x - __half2float(__float2half_rn(x));
+      error = fmaf(d, d, error);
+    }
+    error /= scale_of(j) * scale_of(j);
+    best = min(best, (__float_as_uint(error) & ~511u) | j);
+  }
+  best = __reduce_min_sync(0xffffffffu, best);
+  uint32_t* best_of = reinterpret_cast<uint32_t*>(smem + Cfg::kOffStats);
+  if (lane == 0) best_of[warp] = best;
   __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMultiMmaWarps; ++w) best = min(best, best_of[w]);
+  const float cent_scale = scale_of(best & 511u);
+  // tables of the centroids' low and high bytes
+  uint32_t lut_lo[2] = {0u, 0u}, lut_hi[2] = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < kCentroids; ++e) {
+    const uint32_t bits = __half_as_ushort(__float2half_rn(cent[e] * cent_scale));
+    lut_lo[e / 4] |= (bits & 0xffu) << (8 * (e % 4));
+    lut_hi[e / 4] |= (bits >> 8) << (8 * (e % 4));
+  }
+  uint32_t phase = 0;  // of the ring, which goes on from segment to segment
+  int stage = 0;
+  bool dead = false;  // a bounded wait expired: this warp consumes nothing any more
+
+  multi_for_each_segment<T, D, kMultiMmaThreads>(p, row_tiles, [&](int b, int kvh, int tile, int t0, int t1, const MultiPartial& part) {
+  const int row0 = tile * Cfg::kRows, count = min(Cfg::kRows, p.rows - row0);
+  const int len = (int)max((int64_t)0, min(p.lengths[b], p.max_len));
+  const int lq = max(0, len - p.residual_len);
+  const int q_end = min(t1, lq);
+  const int first_seen = len - p.tokens;  // newest key that query 0 sees
+  if (threadIdx.x == 0) *strange = 0;
+
+  // ---- copies of the first steps ---------------------------------------------------------------------------------------------
   const int tiles = q_end > t0 ? (q_end - t0 + kTile - 1) / kTile : 0;
   const int steps = (tiles + kStepTiles - 1) / kStepTiles;
-  const int my_steps = steps > warp ? (steps - warp + kMultiMmaWarps - 1) / kMultiMmaWarps : 0;
-  const int32_t* table = p.block_table + b * p.table_stride;
+  const int my_steps = steps > warp && !dead ? (steps - warp + kMultiMmaWarps - 1) / kMultiMmaWarps : 0;
+  const int32_t* table = p.block_table + (int64_t)b * p.table_stride;
+  // Page ids of the warp's next 16 steps, a tile a lane, and those of the 16 behind them: a step that looks up its own waits for the
+  // table before it can ask for the tile.
+  auto ids_of = [&](int group) {
+    const int ts = t0 + (((group * 16 + lane / 2) * kMultiMmaWarps + warp) * kStepTiles + (lane & 1)) * kTile;
+    if (ts >= q_end) return -1;
+    const int blk = p.block_shift >= 0 ? ts >> p.block_shift : ts / p.block_size;
+    return blk < p.max_blocks ? table[blk] : -1;
+  };
+  int32_t ids = ids_of(0), ids_next = ids_of(1);
   // A tile of a 16-token page is one run of bytes, of a larger page six (codes, norms, residual norms, value codes, scales, zeros).
-  // Lanes 0 and 1 look up and copy a tile each; lane 0 arms the barrier with the bytes of both.
+  // Lanes 0 and 1 copy a tile each; lane 0 arms the barrier with the bytes of both.
   auto issue = [&](int step, int stage) {
+    if (step % 16 == 0 && step > 0) {
+      ids = ids_next;
+      ids_next = ids_of(step / 16 + 1);
+    }
+    const int32_t pid = __shfl_sync(0xffffffffu, ids, 2 * (step % 16) + (lane & 1));
     int valid = 0, at = 0;
     const uint8_t* page = nullptr;
     if (lane < kStepTiles) {
       const int ts = t0 + ((step * kMultiMmaWarps + warp) * kStepTiles + lane) * kTile;
-      if (ts < q_end) {
-        const int blk = p.block_shift >= 0 ? ts >> p.block_shift : ts / p.block_size;
-        at = ts - blk * p.block_size;
-        const int32_t pid = blk < p.max_blocks ? table[blk] : -1;
-        if (pid >= 0 && pid < p.num_pages) {  // else a hole: nothing to copy
-          valid = min(kTile, q_end - ts);
-          page = p.pages + ((int64_t)pid * p.kv_heads + kvh) * p.layout.chunk_bytes;
-        }
+      if (pid >= 0 && pid < p.num_pages) {  // else a hole, or behind the end: nothing to copy
+        valid = min(kTile, q_end - ts);
+        at = p.block_size == kTile ? 0 : p.block_shift >= 0 ? ts & (p.block_size - 1) : ts % p.block_size;
+        page = p.pages + ((int64_t)pid * p.kv_heads + kvh) * p.layout.chunk_bytes;
       }
       ring_valid[stage * kStepTiles + lane] = valid;
     }
@@ -244,10 +313,11 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
   };
 #pragma unroll
   for (int i = 0; i < kRingStages - 1; ++i)
-    if (i < my_steps) issue(i, i);
+    if (i < my_steps) issue(i, (stage + i) % kRingStages);
 
   // ---- rotated queries as A fragments ----------------------------------------------------------------------------------------
   float* factor = reinterpret_cast<float*>(smem + Cfg::kOffFactor);
+  int* row_limit = reinterpret_cast<int*>(smem + Cfg::kOffLimit);
   __half* frags = reinterpret_cast<__half*>(smem + Cfg::kRing);
   {
     const float sign = p.scaling < 0.0f ? -1.0f : 1.0f;
@@ -260,8 +330,9 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
     }
     for (int i = warp; i < Cfg::kRows; i += kMultiMmaWarps) {
       const int row = row0 + min(i, count - 1);  // rows that are not there: the last one again, not stored
-      const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_stride_b + (int64_t)(kvh * p.groups + row % p.groups) * p.q_stride_h +
-                   (int64_t)(row / p.groups) * p.q_stride_t + lane * E;
+      const int t = multi_token_of(p, row);
+      const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_stride_b + (int64_t)(kvh * p.groups + row - t * p.groups) * p.q_stride_h +
+                   (int64_t)t * p.q_stride_t + lane * E;
       float w1[E], w2[E];
       lane_load<T, E>(q, w1);
 #pragma unroll
@@ -283,7 +354,8 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
       top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
       const float inv = top == 0.0f ? 0.0f : 1.0f / top;
       // a factor of zero (a zero query, no scaling) would make NaN of hidden scores
-      if (lane == 0) factor[i] = max_nan(top * fabsf(p.scaling) * (1.4426950408889634f / (float)D), 1e-30f);
+      if (lane == 0) row_limit[i] = first_seen + t;
+      if (lane == 0) factor[i] = max_nan(top * fabsf(p.scaling) * (1.4426950408889634f / (float)D) / cent_scale, 1e-30f);
       const int up = i % 16 / 8, m = i / 16;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -295,27 +367,15 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
       }
     }
   }
-  // tables of the centroids' low and high bytes
-  uint32_t lut_lo[2] = {0u, 0u}, lut_hi[2] = {0u, 0u};
-#pragma unroll
-  for (int e = 0; e < (1 << (BITS - 1)); ++e) {
-    const uint32_t bits = __half_as_ushort(__float2half_rn(__ldg(p.centroids + e)));
-    lut_lo[e / 4] |= (bits & 0xffu) << (8 * (e % 4));
-    lut_hi[e / 4] |= (bits >> 8) << (8 * (e % 4));
-  }
   __syncthreads();
 
   // rows gid and gid + 8 of every 16
-  float f_row[MT][2], m_run[MT][2], l_run[MT][2];
-  int limit[MT][2];  // newest key that the row sees
+  float m_run[MT][2], l_run[MT][2];
   float o[MT][D / 8][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int i = 16 * m + gid + 8 * k;
-      f_row[m][k] = factor[i];
-      limit[m][k] = first_seen + (row0 + min(i, count - 1)) / p.groups;
       m_run[m][k] = -INFINITY;
       l_run[m][k] = 0.0f;
     }
@@ -335,6 +395,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
     constexpr int N = decltype(cols)::value;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
+      const float f_row[2] = {factor[16 * m + gid], factor[16 * m + gid + 8]};
       float top[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -344,13 +405,13 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
         top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
         top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
       }
-      const bool moves = top[0] > m_run[m][0] && !(f_row[m][0] * (top[0] - m_run[m][0]) <= kMoveLimit);
-      const bool moves1 = top[1] > m_run[m][1] && !(f_row[m][1] * (top[1] - m_run[m][1]) <= kMoveLimit);
+      const bool moves = top[0] > m_run[m][0] && !(f_row[0] * (top[0] - m_run[m][0]) <= kMoveLimit);
+      const bool moves1 = top[1] > m_run[m][1] && !(f_row[1] * (top[1] - m_run[m][1]) <= kMoveLimit);
       if (__any_sync(0xffffffffu, moves || moves1)) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float next = fmaxf(m_run[m][k], top[k]);
-          const float by = next == -INFINITY ? 1.0f : exp2_approx(f_row[m][k] * (m_run[m][k] - next));
+          const float by = next == -INFINITY ? 1.0f : exp2_approx(f_row[k] * (m_run[m][k] - next));
           m_run[m][k] = next;
           l_run[m][k] *= by;
 #pragma unroll
@@ -362,23 +423,23 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float base = m_run[m][k] == -INFINITY ? 0.0f : f_row[m][k] * m_run[m][k];
-        float sum = 0.0f;
+        const float base = m_run[m][k] == -INFINITY ? 0.0f : f_row[k] * m_run[m][k];
+        float2 sum = make_float2(l_run[m][k], 0.0f);
 #pragma unroll
-        for (int c = 0; c < N; ++c)
-#pragma unroll
-          for (int i = 2 * k; i < 2 * k + 2; ++i) {
-            s[m][c][i] = exp2_approx(fmaf(f_row[m][k], s[m][c][i], -base));
-            sum += s[m][c][i];
-          }
-        l_run[m][k] += sum;
+        for (int c = 0; c < N; ++c) {
+          const float2 x = fma_f32x2(make_float2(f_row[k], f_row[k]), make_float2(s[m][c][2 * k], s[m][c][2 * k + 1]),
+                                     make_float2(-base, -base));
+          const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+          s[m][c][2 * k] = e.x;
+          s[m][c][2 * k + 1] = e.y;
+          sum = add_f32x2(sum, e);
+        }
+        l_run[m][k] = sum.x + sum.y;
       }
     }
   };
 
   // ---- packed prefix -----------------------------------------------------------------------------------------------------------
-  uint32_t phase = 0;
-  int stage = 0;
   for (int n = 0; n < my_steps; ++n) {
     __syncwarp();  // every lane is done with the stage that is re-armed next
     if (n + kRingStages - 1 < my_steps) issue(n + kRingStages - 1, (stage + kRingStages - 1) % kRingStages);
@@ -387,6 +448,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
       // wait (bounded) for the copies still in flight before the merge reuses the ring, then give this chunk up
       for (int k = 1; k < kRingStages && n + k < my_steps; ++k)
         (void)mbar_wait(bars + 8 * ((stage + k) % kRingStages), stage + k >= kRingStages ? phase ^ 1u : phase);
+      dead = true;
       break;
     }
     const uint8_t* st = ring + stage * kStepTiles * Cfg::kTileStride;
@@ -409,62 +471,65 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[m][c][r] = 0.0f;
     {
-      uint32_t words[kCols][kKeyWords], flips[kCols];  // flips: the residual norm, negative, twice in fp16
+      // a lane's words of a token are loaded in two halves, which keeps the registers of four CTAs per SM (head_dim 128)
+      constexpr int kHalfWords = kKeyWords / 2;
+      uint32_t words[kCols][kHalfWords], flips[kCols];  // flips: the residual norm at the centroids' scale, negative, twice in fp16
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         const uint8_t* at = st + c / 2 * Cfg::kTileStride;
         const int t = tok + 8 * (c & 1);
-        load_words<kKeyWords>(at + t * Cfg::kKeyBytes + tig * (4 * kKeyWords), words[c]);
-        const uint32_t r = __half_as_ushort(__float2half_rn(-*reinterpret_cast<const float*>(at + Cfg::kOffRnorm + 4 * t)));
+        const uint32_t r = __half_as_ushort(__float2half_rn(-cent_scale * *reinterpret_cast<const float*>(at + Cfg::kOffRnorm + 4 * t)));
         flips[c] = r | r << 16;
       }
       constexpr int kNibbleWords = D / 32;
 #pragma unroll
       for (int w = 0; w < kNibbleWords; ++w) {
-        uint4 a[MT][2];
+        if (w % (kNibbleWords / 2) == 0) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+          for (int c = 0; c < kCols; ++c)
+            load_words<kHalfWords>(st + c / 2 * Cfg::kTileStride + (tok + 8 * (c & 1)) * Cfg::kKeyBytes + tig * (4 * kKeyWords) +
+                                       w / (kNibbleWords / 2) * (4 * kHalfWords), words[c]);
+        }
+        const int at = BITS == 4 ? w % kHalfWords : w / 2 % kHalfWords;  // the nibble word's word
+        // a k-step at a time, the columns' products side by side: those of one column wait for one another
 #pragma unroll
-          for (int i = 0; i < 2; ++i) a[m][i] = frag[(m * 2 * Cfg::kSteps + 2 * w + i) * 32];
+        for (int i = 0; i < 2; ++i) {
+          uint4 a[MT];
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          uint32_t codes;
-          if constexpr (BITS == 4) codes = words[c][w] & 0x77777777u;
-          else codes = (words[c][w / 2] >> (2 * (w & 1))) & (BITS == 3 ? 0x33333333u : 0x11111111u);
-          uint32_t k[4];
+          for (int m = 0; m < MT; ++m) a[m] = frag[(m * 2 * Cfg::kSteps + 2 * w + i) * 32];
+          uint32_t k[kCols][2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t sel = i == 0 ? codes : codes >> 16;
+          for (int c = 0; c < kCols; ++c) {
+            uint32_t sel = (BITS == 2 || BITS == 3) && (w & 1) != 0 ? words[c][at] >> (i == 0 ? 2 : 18) : i == 0 ? words[c][at] : words[c][at] >> 16;
+            sel &= BITS == 4 ? 0x7777u : BITS == 3 ? 0x3333u : 0x1111u;
             const uint32_t lo = permute(lut_lo[0], lut_lo[1], sel), hi = permute(lut_hi[0], lut_hi[1], sel);
-            k[2 * i] = permute(lo, hi, 0x5140);
-            k[2 * i + 1] = permute(lo, hi, 0x7362);
+            k[c][0] = permute(lo, hi, 0x5140);
+            k[c][1] = permute(lo, hi, 0x7362);
           }
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            mma_f16(s[m][c], a[m][0], k[0], k[1]);
-            mma_f16(s[m][c], a[m][1], k[2], k[3]);
-          }
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) mma_f16(s[m][c], a[m], k[c][0], k[c][1]);
         }
         if constexpr (BITS != 3) {
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
+          for (int i = 0; i < 2; ++i) {
+            uint4 a[MT];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) a[m][i] = frag[(m * 2 * Cfg::kSteps + Cfg::kSteps + 2 * w + i) * 32];
+            for (int m = 0; m < MT; ++m) a[m] = frag[(m * 2 * Cfg::kSteps + Cfg::kSteps + 2 * w + i) * 32];
+            uint32_t k[kCols][2];
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            uint32_t k[4];
+            for (int c = 0; c < kCols; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              // the sign of nibble i is its top bit; of a 2-bit field, the upper bit of the even or the odd ones
-              const uint32_t word = BITS == 4 ? words[c][w] : words[c][w / 2];
-              const int up = 12 - 4 * i + (BITS == 2 && (w & 1) == 0 ? 2 : 0);
-              k[i] = lop3<kAndXor>(shifted(word, up), 0x80008000u, flips[c]);
-            }
+              for (int r = 0; r < 2; ++r) {
+                // the sign of nibble n is its top bit; of a 2-bit field, the upper bit of the even or the odd ones
+                const int up = 12 - 4 * (2 * i + r) + (BITS == 2 && (w & 1) == 0 ? 2 : 0);
+                k[c][r] = lop3<kAndXor>(times_power(words[c][at], up), 0x80008000u, flips[c]);
+              }
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              mma_f16(s[m][c], a[m][0], k[0], k[1]);
-              mma_f16(s[m][c], a[m][1], k[2], k[3]);
-            }
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+              for (int m = 0; m < MT; ++m) mma_f16(s[m][c], a[m], k[c][0], k[c][1]);
           }
         }
       }
@@ -483,8 +548,8 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
           for (int c = 0; c < kCols; ++c) {
             const uint32_t word = signs[c][x / 8];
             const int up = 15 - 2 * (x % 8);
-            const uint32_t k0 = lop3<kAndXor>(word << up, 0x80008000u, flips[c]);
-            const uint32_t k1 = lop3<kAndXor>(word << (up - 1), 0x80008000u, flips[c]);
+            const uint32_t k0 = lop3<kAndXor>(times_power(word, up), 0x80008000u, flips[c]);
+            const uint32_t k1 = lop3<kAndXor>(times_power(word, up - 1), 0x80008000u, flips[c]);
 #pragma unroll
             for (int m = 0; m < MT; ++m) mma_f16(s[m][c], a[m], k0, k1);
           }
@@ -498,7 +563,11 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[m][c][r] *= norm[r & 1];
+        for (int k = 0; k < 2; ++k) {
+          const float2 x = mul_f32x2(make_float2(s[m][c][2 * k], s[m][c][2 * k + 1]), make_float2(norm[0], norm[1]));
+          s[m][c][2 * k] = x.x;
+          s[m][c][2 * k + 1] = x.y;
+        }
     }
     const bool full = total == kStepTiles * kTile;
     const bool cut = ts + kStepTiles * kTile - 1 > first_seen;
@@ -510,7 +579,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int in_tile = 8 * (c & 1) + ((r & 1) ? tok_b : tok_a);
-            if (in_tile >= valid[c / 2] || ts + c / 2 * kTile + in_tile > limit[m][r / 2]) s[m][c][r] = -INFINITY;
+            if (in_tile >= valid[c / 2] || ts + c / 2 * kTile + in_tile > row_limit[16 * m + gid + 8 * (r / 2)]) s[m][c][r] = -INFINITY;
           }
     }
     softmax(s, std::integral_constant<int, kCols>{});
@@ -525,7 +594,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
         pa[m] = make_uint4(pack2<__half>(s[m][2 * u][0], s[m][2 * u][1]), pack2<__half>(s[m][2 * u][2], s[m][2 * u][3]),
                            pack2<__half>(s[m][2 * u + 1][0], s[m][2 * u + 1][1]), pack2<__half>(s[m][2 * u + 1][2], s[m][2 * u + 1][3]));
       uint32_t scale[2], zero[2], words[2][2][kValWords];
-      constexpr float kBase = BITS == 2 ? 4.0f : 16.0f;  // what the exponent bits add to a code
+      constexpr float kBase = BITS == 2 ? 4.0f : 16.0f;  // above all codes
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int ta = tok_a + 8 * i, tb = tok_b + 8 * i;
@@ -542,37 +611,41 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
           if (!finite_f16(fabsf(za) + kBase * fabsf(sa))) { sa = za = 0.0f; *strange = 1; }
           if (!finite_f16(fabsf(zb) + kBase * fabsf(sb))) { sb = zb = 0.0f; *strange = 1; }
         }
-        // bf16 caches: the base goes into the zero, whose rounding the output's hides; fp16 caches take it off the code
-        if constexpr (sizeof(T) == 2 && !std::is_same_v<T, __half>) {
-          za = fmaf(-kBase, sa, za);
-          zb = fmaf(-kBase, sb, zb);
-        }
         scale[i] = pack2<__half>(sa, sb);
         zero[i] = pack2<__half>(za, zb);
         load_words<kValWords>(at + Cfg::kOffVal + ta * Cfg::kValBytes + gid * (4 * kValWords), words[i][0]);
         load_words<kValWords>(at + Cfg::kOffVal + tb * Cfg::kValBytes + gid * (4 * kValWords), words[i][1]);
       }
-      constexpr int kPerHalf = BITS == 2 ? 8 : 4;  // codes of 16 bits
+      // A code in the lowest bits under the exponent of 1024 reads as 1024 + code in fp16, one a field higher under the exponent of 64
+      // (2-bit codes: 256) as 64 + code, and taking that off is exact.  So one shift serves the two fields of a byte: the logic pipe,
+      // which binds this kernel, has one operation per register of two values and a shift per four, instead of two.
+      constexpr int kWidth = BITS == 2 ? 2 : 4, kPerWord = 32 / kWidth;
+      constexpr uint32_t kField = (1u << kWidth) - 1u;
 #pragma unroll
       for (int w = 0; w < kValWords; ++w)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t x0 = permute(words[0][0][w], words[0][1][w], h == 0 ? 0x5410 : 0x7632);
-          const uint32_t x1 = permute(words[1][0][w], words[1][1][w], h == 0 ? 0x5410 : 0x7632);
+          uint32_t x[2];
 #pragma unroll
-          for (int i = 0; i < kPerHalf; ++i) {
-            const int up = BITS == 2 ? 8 - 2 * i : 6 - 4 * i;
-            constexpr uint32_t kMask = BITS == 2 ? 0x03000300u : 0x03C003C0u, kBits = BITS == 2 ? 0x44004400u : 0x4C004C00u;
-            uint32_t v0 = lop3<kAndOr>(shifted(x0, up), kMask, kBits), v1 = lop3<kAndOr>(shifted(x1, up), kMask, kBits);
-            if constexpr (std::is_same_v<T, __half>) {
-              v0 = sub_f16x2(v0, kBits);
-              v1 = sub_f16x2(v1, kBits);
+          for (int i = 0; i < 2; ++i) x[i] = permute(words[i][0][w], words[i][1][w], h == 0 ? 0x5410 : 0x7632);
+#pragma unroll
+          for (int f = 0; f < kPerWord / 2; f += 2) {
+#pragma unroll
+            for (int up = 0; up < 2; ++up) {
+              uint32_t v[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t mask = kField << (kWidth * up) | kField << (kWidth * up + 16);
+                const uint32_t base = up == 0 ? 0x64006400u : BITS == 2 ? 0x5C005C00u : 0x54005400u;
+                v[i] = sub_f16x2(lop3<kAndOr>(x[i], mask, base), base);
+                v[i] = fma_f16x2(v[i], scale[i], zero[i]);
+              }
+              const int j = w * kPerWord + h * (kPerWord / 2) + f + up;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) mma_f16(o[m][j], pa[m], v[0], v[1]);
             }
-            v0 = fma_f16x2(v0, scale[0], zero[0]);
-            v1 = fma_f16x2(v1, scale[1], zero[1]);
-            const int j = (2 * w + h) * kPerHalf + i;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) mma_f16(o[m][j], pa[m], v0, v1);
+            for (int i = 0; i < 2; ++i) x[i] >>= 2 * kWidth;
           }
         }
     }
@@ -583,7 +656,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
   for (int ts = w0 + warp * kTile; ts < t1; ts += kMultiMmaWarps * kTile) {
     const int valid = min(kTile, t1 - ts);
     const int R = p.residual_len;
-    const T* keys = reinterpret_cast<const T*>(p.window) + (p.window_slots[b] * 2 * p.kv_heads + kvh) * (int64_t)R * D;
+    const T* keys = reinterpret_cast<const T*>(p.window) + (p.window_slots[b] * 2 * p.kv_heads + kvh) * R * D;
     const T* values = keys + (int64_t)p.kv_heads * R * D;
     auto ring_row = [&](int t) { return (int64_t)((ts + min(t, valid - 1)) % R) * D; };
     float s[MT][2][4];
@@ -602,8 +675,9 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int row = row0 + min(16 * m + gid + 8 * k, count - 1);
-          q[m][k] = reinterpret_cast<const T*>(p.q) + b * p.q_stride_b + (int64_t)(kvh * p.groups + row % p.groups) * p.q_stride_h +
-                    (int64_t)(row / p.groups) * p.q_stride_t + tig * (D / 4);
+          const int t = multi_token_of(p, row);
+          q[m][k] = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_stride_b + (int64_t)(kvh * p.groups + row - t * p.groups) * p.q_stride_h +
+                    (int64_t)t * p.q_stride_t + tig * (D / 4);
         }
       // 8 coordinates of this lane are two k-steps
 #pragma unroll
@@ -628,8 +702,8 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
         for (int r = 0; r < 4; ++r) {
           const int in_tile = 8 * c + ((r & 1) ? tok_b : tok_a);
           // to the units of the row's factor
-          const float x = s[m][c][r] * (p.scaling * 1.4426950408889634f / f_row[m][r / 2]);
-          s[m][c][r] = in_tile >= valid || ts + in_tile > limit[m][r / 2] ? -INFINITY : x;
+          const float x = s[m][c][r] * (p.scaling * 1.4426950408889634f / factor[16 * m + gid + 8 * (r / 2)]);
+          s[m][c][r] = in_tile >= valid || ts + in_tile > row_limit[16 * m + gid + 8 * (r / 2)] ? -INFINITY : x;
         }
     softmax(s, std::integral_constant<int, 2>{});
     // bf16 probabilities as a sum of two, so that they keep 16 bits
@@ -685,7 +759,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
 
   // Adds the infinite and NaN values that the products left out, at the row's dims d .. d + 3.
   auto strange_values = [&](int row, int d, float4& sum) {
-    const int seen = min(t1 - 1, first_seen + row / p.groups);
+    const int seen = min(t1 - 1, first_seen + multi_token_of(p, row));
     for (int t = max(t0, first_seen - kStepTiles * kTile); t <= seen; ++t) {
       float v[4];
       bool fine = true;
@@ -732,16 +806,36 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
       if (tig == 0) stats[warp * Cfg::kRows + 16 * m + gid + 8 * k] = make_float2(m_run[m][k], l_run[m][k]);
     }
   __syncthreads();  // and nobody reads the ring or the queries any more
+  // a thread per row: what each warp's sums count, in place of its maximum; the row's maximum and denominator in place of its factor
+  // and its limit
+  if (threadIdx.x < Cfg::kRows) {
+    const int i = threadIdx.x;
+    const float f = factor[i];
+    float top = -INFINITY, den = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kMultiMmaWarps; ++w) top = fmaxf(top, stats[w * Cfg::kRows + i].x);
+#pragma unroll
+    for (int w = 0; w < kMultiMmaWarps; ++w) {
+      const float2 x = stats[w * Cfg::kRows + i];
+      // a warp without a key for the row has no sums; where none has, a NaN may be in them
+      const float by = top == -INFINITY ? 1.0f : x.x == -INFINITY ? 0.0f : exp2_approx(f * (x.x - top));
+      stats[w * Cfg::kRows + i].x = by;
+      den = fmaf(x.y, by, den);
+    }
+    const bool alone = part.count == 1;
+    // a NaN among the scores has to stay one, so only a row without a key is zero
+    factor[i] = alone ? (den == 0.0f ? 0.0f : 1.0f / den) : 1.0f;
+    if (!alone && i < count)
+      reinterpret_cast<float2*>(p.stats)[multi_partial_row(part, part.mine, Cfg::kRows) + i] =
+          make_float2(top * f * 0.6931471805599453f, den);  // natural units
+  }
+  __syncthreads();
   float* merged = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int i = 16 * m + gid + 8 * k;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kMultiMmaWarps; ++w) top = fmaxf(top, stats[w * Cfg::kRows + i].x);
-      const float by = m_run[m][k] == -INFINITY && top != -INFINITY ? 0.0f : top == -INFINITY ? 1.0f : exp2_approx(f_row[m][k] * (m_run[m][k] - top));
+      const float by = stats[warp * Cfg::kRows + 16 * m + gid + 8 * k].x;
       float* to = merged + (warp * 16 + gid + 8 * k) * Cfg::kMergeStride;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -756,63 +850,65 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kMinB
     const int rows = min(16, count - 16 * m);
     for (int item = threadIdx.x; item < rows * (D / 4); item += kMultiMmaThreads) {
       const int i = item / (D / 4), d = 4 * (item % (D / 4));
+      const float* from = merged + i * Cfg::kMergeStride + d + 8 * (d / 32);
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float top = -INFINITY, den = 0.0f;
 #pragma unroll
       for (int w = 0; w < kMultiMmaWarps; ++w) {
-        const float4 x = *reinterpret_cast<const float4*>(merged + (w * 16 + i) * Cfg::kMergeStride + d + 8 * (d / 32));
+        const float4 x = *reinterpret_cast<const float4*>(from + w * 16 * Cfg::kMergeStride);
         sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-        top = fmaxf(top, stats[w * Cfg::kRows + 16 * m + i].x);
-      }
-      const float f = factor[16 * m + i];
-#pragma unroll
-      for (int w = 0; w < kMultiMmaWarps; ++w) {
-        const float2 x = stats[w * Cfg::kRows + 16 * m + i];
-        den += x.y * (x.x == -INFINITY ? (top == -INFINITY ? 1.0f : 0.0f) : exp2_approx(f * (x.x - top)));
       }
       const int row = row0 + 16 * m + i;
       if (*strange != 0) strange_values(row, d, sum);
-      if (chunks == 1) {
-        const float inv = den == 0.0f ? 0.0f : 1.0f / den;  // a NaN among the scores has to stay one
+      if (part.count == 1) {
+        const float inv = factor[16 * m + i];
         const float out[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
         multi_store<T, 4>(p, b, kvh, row, d, out);
       } else {
-        const int64_t at = multi_row_index(p, b, kvh, row) * p.num_chunks + chunk;
-        *reinterpret_cast<float4*>(p.values + at * D + d) = sum;
-        if (d == 0) reinterpret_cast<float2*>(p.stats)[at] = make_float2(top * f * 0.6931471805599453f, den);  // natural units
+        *reinterpret_cast<float4*>(p.values + (multi_partial_row(part, part.mine, Cfg::kRows) + 16 * m + i) * D + d) = sum;
       }
     }
     __syncthreads();
   }
-  if (chunks > 1) multi_merge<T, D, kMultiMmaWarps>(p, b, kvh, tile, row_tiles, row0, count, chunks);
+  if (part.count > 1) multi_merge<T, D, kMultiMmaWarps, Cfg::kRows>(p, b, kvh, tile, row_tiles, count, part, merged);
+  // the next segment's copies land where the merge and the queries were
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  __syncthreads();
+  });
 }
 
-bool tq_multi_mma_applicable(const TqMultiParams& p, int batch, int head_dim, int bits, int dtype) {
+bool tq_multi_mma_applicable(const TqMultiParams& p, int head_dim, int dtype) {
   if (dtype == ANNA_DTYPE_F32 || (head_dim != 128 && head_dim != 256) || p.value_group != 32 || p.block_size % kTile != 0) return false;
   // the window product reads queries 16 bytes at a time
   return aligned_to(p.q, 16) && p.q_stride_b % 8 == 0 && p.q_stride_h % 8 == 0 && p.q_stride_t % 8 == 0 && p.max_len < (1ll << 30);
 }
 
 template <typename T, int D, int BITS, int MT>
-static int launch(const TqMultiParams& p, int batch, cudaStream_t stream) {
+static int launch(const TqMultiParams& p, cudaStream_t stream) {
   using Cfg = MultiCfg<D, BITS, MT>;
+  static_assert(148 * Cfg::kCtas <= kMultiMaxCtas && Cfg::kCtas * Cfg::kRows <= 2 * kMultiScratchRows, "partials of more rows than there is room for");
   const int row_tiles = (p.rows + Cfg::kRows - 1) / Cfg::kRows;
   auto kernel = tq_multi_mma_kernel<T, D, BITS, MT>;
   ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
-  const dim3 grid((unsigned)p.num_chunks, (unsigned)(p.kv_heads * row_tiles), (unsigned)batch);
-  kernel<<<grid, kMultiMmaThreads, Cfg::kSmem, stream>>>(p, row_tiles);
+  kernel<<<multi_ctas(p, row_tiles, Cfg::kCtas), kMultiMmaThreads, Cfg::kSmem, stream>>>(p, row_tiles);
   return check_launch("tq_multi_mma_kernel");
 }
 
-int launch_tq_multi_mma(const TqMultiParams& p, int batch, int head_dim, int bits, int dtype, cudaStream_t stream) {
+int launch_tq_multi_mma(const TqMultiParams& p, int head_dim, int bits, int dtype, cudaStream_t stream) {
   auto pick = [&](auto elem) -> int {
     using T = decltype(elem);
     return ANNA_DISPATCH_TQ_BITS(bits, BITS, [&]() -> int {
-      if (head_dim == 128) return p.rows > 16 ? launch<T, 128, BITS, 2>(p, batch, stream) : launch<T, 128, BITS, 1>(p, batch, stream);
-      return launch<T, 256, BITS, 1>(p, batch, stream);
+      if (head_dim == 128) return p.rows > 16 ? launch<T, 128, BITS, 2>(p, stream) : launch<T, 128, BITS, 1>(p, stream);
+      return launch<T, 256, BITS, 1>(p, stream);
     });
   };
   return dtype == ANNA_DTYPE_F16 ? pick(__half{}) : pick(__nv_bfloat16{});
+}
+
+int tq_multi_mma_faults(int* count) {
+  int32_t value = 0;
+  ANNA_CUDA_CHECK(cudaMemcpyFromSymbol(&value, g_tq_multi_faults, sizeof(value)));
+  *count = value;
+  return ANNA_OK;
 }
 
 }  // namespace anna

@@ -682,28 +682,15 @@ def _op_tq_paged_decode(query, packed_pages, page_table, window, window_slots, l
     return out
 
 
-def multi_scratch(device: torch.device, batch: int, heads: int, kv_heads: int, tokens: int, head_dim: int, max_blocks: int,
-                  block_size: int, residual_len: int):
-    """(partial_stats, partial_values, chunks, counters) of a multi-token decode.  Under a graph capture they are the graph's own:
-    graphs may be replayed side by side, and those of the stream are replaced when a larger call needs more."""
-    key = (batch, heads, kv_heads, tokens, max_blocks, block_size, residual_len)
-    plan = _MULTI_PLANS.get(key)
-    if plan is None:
-        if len(_MULTI_PLANS) > 4096:
-            _MULTI_PLANS.clear()
-        plan = _MULTI_PLANS[key] = _lib.tq_multi_decode_plan(*key)
-    chunks, arrivals = plan
-    rows = batch * heads * tokens * chunks if chunks > 1 else 0
-    floats = rows * (head_dim + 2)
+def multi_scratch(device: torch.device, batch: int, heads: int, kv_heads: int, tokens: int, head_dim: int):
+    """(scratch, counters) of a multi-token decode.  The scratch is the call's own; the counters, zero between calls, are the
+    stream's, or under a graph capture the graph's (graphs may be replayed side by side)."""
+    floats, arrivals = _lib.tq_multi_decode_plan(batch, heads, kv_heads, tokens, head_dim)
+    scratch = torch.empty(floats, dtype=torch.float32, device=device)
     with on_device(device):
         if torch.cuda.is_current_stream_capturing():
-            buf = torch.empty(max(floats, 1), dtype=torch.float32, device=device)
-            return buf[rows * head_dim:], buf, chunks, torch.zeros(arrivals, dtype=torch.int32, device=device)
-    buf = _SCRATCH.get(device, floats)
-    return buf[rows * head_dim:], buf, chunks, _SCRATCH.counters(device, arrivals)
-
-
-_MULTI_PLANS: dict[tuple, tuple[int, int]] = {}
+            return scratch, torch.zeros(arrivals, dtype=torch.int32, device=device)
+    return scratch, _SCRATCH.counters(device, arrivals)
 
 
 def multi_decode(name, query, packed_pages, page_table, window, window_slots, lengths, tables, scaling, gate, *, kv_heads, bits,
@@ -717,13 +704,13 @@ def multi_decode(name, query, packed_pages, page_table, window, window_slots, le
     if out.numel() == 0:
         return out
     max_blocks = 0 if page_table is None else int(page_table.shape[1])
-    stats, values, chunks, counters = multi_scratch(device, batch, heads, kv_heads, tokens, dim, max_blocks, block_size, residual_len)
+    scratch, counters = multi_scratch(device, batch, heads, kv_heads, tokens, dim)
     with on_device(device):
         _lib.check(_lib.lib().anna_tq_paged_multi_decode(
             ptr(query), *query.stride()[:3], ptr(packed_pages) if max_blocks else None, ptr(page_table) if max_blocks else None,
             page_table.stride(0) if max_blocks else 0, ptr(window), ptr(window_slots), ptr(lengths), ptr(tables.signs1),
             ptr(tables.signs2), ptr(tables.centroids), ptr(gate), *((0, 0, 0) if gate is None else gate.stride()[:3]), ptr(out),
-            *out.stride()[:3], ptr(stats), ptr(values), chunks, ptr(counters), batch, heads, kv_heads, tokens, dim, block_size,
+            *out.stride()[:3], ptr(scratch), scratch.numel(), ptr(counters), batch, heads, kv_heads, tokens, dim, block_size,
             residual_len, bits, value_group, int(packed_pages.shape[0]) if max_blocks else 0, max_blocks, float(scaling),
             dtype_code(query.dtype), stream_ptr(device)), name)
     return out
@@ -735,6 +722,14 @@ def _op_tq_paged_multi_decode(query, packed_pages, page_table, window, window_sl
     from .tq_tables import key_tables
 
     name = "tq_paged_multi_decode"
+    if query.is_cuda and bits in (2, 3, 4) and query.shape[-1] in (64, 128, 256):
+        tables = key_tables(head_dim=query.shape[-1], bits=bits, device=query.device)
+        out = (_LAUNCH or launch_module()).tq_multi_decode(query, gate, packed_pages, page_table, window, window_slots, lengths,
+                                                           tables.signs1, tables.signs2, tables.centroids, scaling, bits, residual_len,
+                                                           block_size, value_group_size)
+        if out is not None:
+            return out
+    # not the ordinary call: arguments to be checked, or copied into the layout that the kernels read
     if query.dim() != 4:
         raise RuntimeError(f"{name}: query must be [batch, heads, tokens, head_dim]")
     batch, heads, _, dim = (int(v) for v in query.shape)

@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .fused_ops import MetadataUploader, on_device, stream_ptr
+from .fused_ops import MetadataUploader, launch_module, on_device, stream_ptr
 
 
 def _ids(name: str, values) -> np.ndarray:
@@ -85,9 +85,12 @@ def run_page_copy(*, copies: Sequence[tuple[torch.Tensor, Sequence[int], Sequenc
     ``target[i]``, in place.  A source may have several targets; no page may be a target twice, or a target and a source (the
     copies of a call have no order)."""
     name = "page_copy"
+    copies = list(copies)
+    if launch_module().page_copy(copies):
+        return
+    # not the ordinary call: arguments to be converted or refused, or a pool that is named twice
     device = None
     pairs, entries = _Pairs(), []
-    copies = list(copies)  # holds the lists that are known by their addresses below
     known: dict[tuple[int, int], tuple[np.ndarray, np.ndarray, int]] = {}
     of_pool: dict[int, tuple[int, list[np.ndarray], list[np.ndarray]]] = {}
     for pool, source, target in copies:
@@ -136,9 +139,12 @@ def run_page_gather(*, pools: Sequence[tuple[torch.Tensor, Sequence[int]]], spar
     name = "page_gather"
     if spare_pages < 0:
         raise ValueError(f"{name}: spare_pages must not be negative")
+    pools = list(pools)
+    new_pools = launch_module().page_gather(pools, spare_pages)
+    if new_pools is not None:
+        return new_pools
     device = None
     pairs, entries, out = _Pairs(), [], []
-    pools = list(pools)  # holds the lists that are known by their addresses below
     known: dict[int, tuple[np.ndarray, int]] = {}
     for pool, ids in pools:
         device = _check_pool(name, pool, device)

@@ -17,7 +17,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .fused_ops import _require_cuda, dtype_code, on_device, ptr, stream_ptr
+from .fused_ops import _require_cuda, dtype_code, launch_module, on_device, ptr, stream_ptr
 
 
 @dataclass(frozen=True)
@@ -145,6 +145,14 @@ def run_multi_axis_rotary(*, query: torch.Tensor, key: torch.Tensor, positions: 
     axis), ``interleaved``, ``theta`` and ``inverse_frequencies``: see the module.  ``attention_scaling`` multiplies cosine and
     sine.  The first call with new parameters makes their tables and cannot be captured into a graph."""
     name = "multi_axis_rotary"
+    if query_out is None and key_out is None and query.is_cuda and (rotary_dim or 0) <= query.shape[-1]:
+        width = query.shape[-1] if rotary_dim is None else rotary_dim
+        tables = rotary_tables(width, theta=theta, sections=sections, interleaved=interleaved,
+                               inverse_frequencies=inverse_frequencies, device=query.device)
+        turned = launch_module().rotary(query, key, positions, tables.rates, tables.axes, tables.axis_count, width, attention_scaling)
+        if turned is not None:
+            return turned
+    # not the ordinary call: arguments to be checked or converted
     _check_rows(name, query, key)
     device = _require_cuda(name, query=query, key=key, positions=positions)
     batch, heads, tokens, dim = (int(v) for v in query.shape)
@@ -188,6 +196,16 @@ def run_rotary_paged_kv_write(*, query: torch.Tensor, key: torch.Tensor, value: 
     (int64 ``[B]``) receives ``past_lengths + T``; a token whose page id is invalid is not written and reported in ``status``
     (int32 ``[1]``).  The page pools must be contiguous."""
     name = "rotary_paged_kv_write"
+    if query.is_cuda and (rotary_dim or 0) <= query.shape[-1]:
+        width = query.shape[-1] if rotary_dim is None else rotary_dim
+        tables = rotary_tables(width, theta=theta, sections=sections, interleaved=interleaved,
+                               inverse_frequencies=inverse_frequencies, device=query.device)
+        turned = launch_module().rotary_write(query, key, value, key_pages, value_pages, page_table, past_lengths, positions, rope_deltas,
+                                              new_lengths, status, tables.rates, tables.axes, tables.axis_count, width,
+                                              attention_scaling)
+        if turned is not None:
+            return turned
+    # not the ordinary call: arguments to be checked or converted
     _check_rows(name, query, key)
     if value.shape != key.shape or value.dtype != key.dtype:
         raise RuntimeError(f"{name}: key and value must share shape and dtype")

@@ -401,19 +401,17 @@ int anna_tq_paged_decode_peers(const void* q, int64_t q_stride_b, int64_t q_stri
  *                  the output is multiplied by sigmoid(gate)
  *   packed_pages, block_table, window, window_slots, lengths, signs1, signs2, centroids  as for anna_tq_paged_decode (pages and
  *                  table may be NULL with max_blocks == 0); holes of the table (ids outside [0, num_pages)) are keys that nobody sees
- *   partial_stats  float [B, Hq, T, chunk_capacity, 2], partial_values float [B, Hq, T, chunk_capacity, D] with chunk_capacity >=
- *                  the num_chunks of anna_tq_multi_decode_plan (may be NULL where that is 1); 8- and 16-byte aligned
+ *   scratch        scratch_size floats, as many as anna_tq_multi_decode_plan says, 16-byte aligned, of any content
  *   counters       int32, as many as the plan says, zero; left at zero
  * dtype F32 / F16 / BF16, head_dim 64 / 128 / 256, any page size and any value group that divides head_dim.
  */
-int anna_tq_multi_decode_plan(int batch, int q_heads, int kv_heads, int tokens, int64_t max_blocks, int block_size, int residual_len,
-                              int* num_chunks, int* counters);
+int anna_tq_multi_decode_plan(int batch, int q_heads, int kv_heads, int tokens, int head_dim, int64_t* scratch_size, int* counters);
 int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, const uint8_t* packed_pages,
                                const int32_t* block_table, int64_t table_stride, const void* window, const int64_t* window_slots,
                                const int64_t* lengths, const float* signs1, const float* signs2, const float* centroids,
                                const void* gate, int64_t gate_stride_b, int64_t gate_stride_h, int64_t gate_stride_t, void* out,
-                               int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t, float* partial_stats,
-                               float* partial_values, int chunk_capacity, int32_t* counters, int batch, int q_heads, int kv_heads,
+                               int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_t, float* scratch,
+                               int64_t scratch_size, int32_t* counters, int batch, int q_heads, int kv_heads,
                                int tokens, int head_dim, int block_size, int residual_len, int bits, int value_group,
                                int64_t num_pages, int64_t max_blocks, float scaling, int dtype, anna_stream_t stream);
 

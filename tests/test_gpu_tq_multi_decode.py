@@ -196,16 +196,35 @@ def test_against_the_dense_keys_and_values(cuda_device, dtype, bits, shape, toke
 @pytest.mark.parametrize("dtype,dim,page,bits", [("bf16", 128, 16, 4), ("fp16", 128, 32, 3), ("bf16", 256, 16, 2), ("fp32", 128, 16, 4),
                                                   ("bf16", 64, 16, 4)])
 @pytest.mark.parametrize("tokens,group", [(4, 4), (9, 2), (40, 1)])
-def test_long_rows_in_many_chunks(cuda_device, dtype, dim, page, bits, tokens, group):
+def test_long_rows_that_several_ctas_share(cuda_device, dtype, dim, page, bits, tokens, group):
     lengths = [3001, 129, 1024, 2047]
     case = Case(lengths=lengths, tokens=tokens, group=group, kv_heads=1, dim=dim, bits=bits, page=page, window=33, dtype=dtype,
                 device=cuda_device, seed=5)
-    chunks, _ = _lib.tq_multi_decode_plan(4, group, 1, tokens, int(case.table.shape[1]), page, 33)
-    assert chunks > 1
     first = case.run()
     case.check(first)
     for _ in range(3):
         assert torch.equal(case.run(), first)  # the merge has an order of its own
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,page", [("bf16", 128, 16), ("fp16", 256, 32), ("fp32", 128, 16)])
+@pytest.mark.parametrize("tokens,group", [(3, 4), (6, 4)])
+def test_many_rows_of_all_lengths(cuda_device, dtype, dim, page, tokens, group):
+    """Shares that hold several streams, end inside one, or hold none; empty rows among them."""
+    rng = np.random.default_rng(3)
+    lengths = [int(n) for n in rng.integers(0, 400, 70)] + [0, 0, 2500, 1, 16, 0]
+    case = Case(lengths=lengths, tokens=tokens, group=group, kv_heads=2, dim=dim, bits=4, page=page, window=20, dtype=dtype,
+                device=cuda_device, seed=15)
+    first = case.run(gate=True)
+    case.check(first, gate=True)
+    assert torch.equal(case.run(gate=True), first)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_lines_up(cuda_device):
+    lengths = [(37 * i) % 23 for i in range(1100)]
+    case = Case(lengths=lengths, tokens=2, group=2, kv_heads=1, dim=128, bits=4, page=16, window=4, dtype="bf16", device=cuda_device)
+    case.check(case.run(gate=True), gate=True)
 
 
 @pytest.mark.gpu
@@ -429,28 +448,28 @@ def test_calls_that_cannot_be_are_refused():
 def test_entry_points_refuse_what_they_cannot_run():
     library, ok = _lib.lib(), 0x10000
 
-    def call(q=ok, pages=ok, table=ok, window=ok, out=ok, stats=ok, values=ok, capacity=512, counters=ok, batch=1, heads=4, kv=2, tokens=3,
+    def call(q=ok, pages=ok, table=ok, window=ok, out=ok, scratch=ok, floats=1 << 24, counters=ok, batch=1, heads=4, kv=2, tokens=3,
              dim=128, page=16, window_len=16, bits=4, group=32, num_pages=4, blocks=300, dtype=2):
         return library.anna_tq_paged_multi_decode(q, 1536, 384, 128, pages, table, blocks, window, ok, ok, ok, ok, ok, None, 0, 0, 0, out,
-                                                  1536, 384, 128, stats, values, capacity, counters, batch, heads, kv, tokens, dim, page,
+                                                  1536, 384, 128, scratch, floats, counters, batch, heads, kv, tokens, dim, page,
                                                   window_len, bits, group, num_pages, blocks, 0.1, dtype, None)
 
     for bad, status in ((dict(q=None), 1), (dict(window=None), 1), (dict(out=None), 1), (dict(counters=None), 1), (dict(pages=None), 1),
                         (dict(num_pages=0), 1), (dict(batch=0), 1), (dict(heads=3), 1), (dict(tokens=0), 1), (dict(dtype=7), 1),
-                        (dict(bits=5), 2), (dict(group=0), 2), (dict(group=7), 2), (dict(dim=96), 2), (dict(capacity=1), 4), (dict(stats=None), 4),
-                        (dict(pages=ok + 8), 1), (dict(window=ok + 8), 1), (dict(stats=ok + 4), 1), (dict(values=ok + 8), 1),
-                        (dict(blocks=1 << 40), 1), (dict(tokens=1 << 20), 1), (dict(batch=1 << 17), 1)):
+                        (dict(bits=5), 2), (dict(group=0), 2), (dict(group=7), 2), (dict(dim=96), 2), (dict(floats=1), 4), (dict(scratch=None), 1),
+                        (dict(pages=ok + 8), 1), (dict(window=ok + 8), 1), (dict(scratch=ok + 8), 1),
+                        (dict(blocks=1 << 40), 1), (dict(blocks=-1), 1), (dict(page=0), 1), (dict(window_len=0), 1), (dict(tokens=1 << 20), 1),
+                        (dict(tokens=60000, blocks=1 << 22), 1)):
         assert call(**bad) == status, bad
         assert "multi_decode" in _lib.last_error() or "head_dim" in _lib.last_error()
 
 
-def test_plan_covers_the_keys():
-    for batch, heads, kv_heads, tokens, blocks, page, window in itertools.product((1, 7, 64), (8, 32), (8,), (1, 4, 33), (0, 1, 100, 4096),
-                                                                                  (16, 24), (1, 128)):
-        chunks, counters = _lib.tq_multi_decode_plan(batch, heads, kv_heads, tokens, blocks, page, window)
-        assert 1 <= chunks <= 512 and counters >= batch * kv_heads
+def test_plan_needs_no_lengths():
+    for batch, (heads, kv_heads), tokens, dim in itertools.product((1, 7, 4096), ((8, 8), (32, 8), (12, 1)), (1, 4, 33), (64, 128, 256)):
+        floats, counters = _lib.tq_multi_decode_plan(batch, heads, kv_heads, tokens, dim)
+        assert floats == 296 * 2 * 16 * (dim + 2) and counters == batch * kv_heads * -(-tokens * (heads // kv_heads) // 8)
     with pytest.raises(RuntimeError, match="multi_decode_plan"):
-        _lib.tq_multi_decode_plan(1, 3, 2, 1, 1, 16, 16)
+        _lib.tq_multi_decode_plan(1, 3, 2, 1, 128)
 
 
 def test_meta_kernel_gives_the_shape():
