@@ -54,7 +54,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "anna_decode_plan": (c_i32, [c_i32, c_i32, c_i64, ctypes.POINTER(c_i32), ctypes.POINTER(c_i32)]),
     "anna_paged_kv_write": (c_i32, [c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_i32,
                                     c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_i32, c_ptr, c_ptr]),
-    "anna_multi_axis_rotary": (c_i32, [c_ptr, c_i64, c_i64, c_i64] * 4 + [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_f32] +
+    "anna_multi_axis_rotary": (c_i32, [c_ptr, c_i64, c_i64, c_i64] * 5 + [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_f32] +
                                [c_i32] * 7 + [c_ptr]),
     "anna_rotary_paged_kv_write": (c_i32, [c_ptr, c_i64, c_i64, c_i64] * 4 + [c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr] +
                                    [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_f32] + [c_i32] * 7 +

@@ -26,10 +26,12 @@ import torch
 
 from . import _lib
 from .fused_ops import MetadataUploader, dtype_code, on_device, ptr, stream_ptr
+from .page_copy import run_page_copy, run_page_gather
 from .pools import Qwen3PagedLayerAllocator, TurboQuantLayerPool, native_page_ids
 from .prefix_block_cache import PrefixBlockPool
+from .rotary import run_multi_axis_rotary, run_rotary_paged_kv_write
 from .turboquant import (VALID_KV_CACHE_QUANT_BITS, TurboQuantKVRow, launch_tq_append, launch_tq_decode,
-                         launch_tq_gather_dense)
+                         launch_tq_gather_dense, launch_tq_multi_decode)
 
 
 @dataclass
@@ -111,6 +113,58 @@ class Qwen3PageAllocator:
         self.prefix_block_pool.clear()
         self.packed_prefix_block_pool.clear()
         return released
+
+    def compact(self, caches, *, spare_pages: int = 0) -> int:
+        """Move the pages in use to the front of pools that hold no others (plus ``spare_pages`` free ones per layer) and give the
+        old pools back; window rings likewise.  The reference gives pages back only when a pool has none in use (``trim``).
+
+        ``caches`` are all caches that map pages of this allocator: their block tables are rewritten, the pages of a row next to
+        each other.  A page with an owner outside of them is an error, before anything has changed.  Pools and block tables move,
+        so captured graphs that read them are not valid any more, and other streams must be done with them.  A layer is copied at
+        a time, in one launch; returns the number of pages given back."""
+        caches = list({id(cache): cache for cache in caches}.values())
+        if spare_pages < 0:
+            raise ValueError("spare_pages must not be negative")
+        for cache in caches:
+            if cache.allocator is not self:
+                raise ValueError("compact: a cache belongs to another allocator")
+        plans = []
+        for layer_idx, (layer, pool) in enumerate(zip(self.layers, self.turboquant_layers)):
+            rows = {id(row): row for cache in caches for row in cache.turboquant_rows[layer_idx] if row is not None and row.initialized}
+            plain = [table for cache in caches if not cache.uses_turboquant_for_layer(layer_idx)
+                     for table in cache.page_tables[layer_idx]]
+            packed = [row._blocks for row in rows.values()]
+            plans.append((self._renumbered(layer._book, plain, "layer", layer_idx),
+                          self._renumbered(pool._book, packed, "packed layer", layer_idx), plain, list(rows.values())))
+            slots = [row.slot for row in rows.values()]
+            if len(set(slots)) != len(slots) or len(slots) + len(pool.free_slots) != pool.slot_capacity():
+                raise RuntimeError(f"compact: window rings of layer {layer_idx} belong to rows that are not in the given caches")
+        released = 0
+        for layer_idx, (plain_ids, packed_ids, plain, rows) in enumerate(plans):
+            layer, pool = self.layers[layer_idx], self.turboquant_layers[layer_idx]
+            released += layer.compact(plain_ids, spare_pages)
+            released += pool.compact(packed_ids, rows, spare_pages)
+            self.prefix_block_pool.move_pages(layer_idx, plain_ids)
+            self.packed_prefix_block_pool.move_pages(layer_idx, packed_ids)
+            for table in plain:
+                table[:] = [plain_ids[page_id] for page_id in table]
+            for cache in caches:
+                cache._forget_device_tables(layer_idx)
+        return released
+
+    @staticmethod
+    def _renumbered(book, tables: list[list[int]], what: str, layer_idx: int) -> dict[int, int]:
+        """New ids of the pages of ``tables``, in their order; every page must have as many owners as tables map it."""
+        found: dict[int, int] = {}
+        for table in tables:
+            for page_id in table:
+                found[page_id] = found.get(page_id, 0) + 1
+        owners = book.refcount
+        if owners != found:
+            differ = next(page_id for page_id in {**owners, **found} if owners.get(page_id) != found.get(page_id))
+            raise RuntimeError(f"compact: page {differ} of {what} {layer_idx} has {owners.get(differ, 0)} owners, the given caches map "
+                               f"it {found.get(differ, 0)} times")
+        return {page_id: new for new, page_id in enumerate(found)}
 
     def to(self, *, device: torch.device | None = None, dtype: torch.dtype | None = None) -> "Qwen3PageAllocator":
         for layer in self.layers:
@@ -221,6 +275,27 @@ class _QuantizedStep:
     def holds(self, pool: TurboQuantLayerPool, rows: list, device: torch.device) -> bool:
         return (self.pool is pool and self.version == pool.version and self.slots_dev.device == device
                 and self.rows == rows)
+
+
+class _PendingRotary:
+    """The rotary positions that an append gives its keys, and the queries that go with them."""
+
+    __slots__ = ("query", "positions", "deltas", "how")
+
+    def __init__(self, query: torch.Tensor, positions: torch.Tensor | None, deltas: torch.Tensor | None, how: dict) -> None:
+        self.query, self.positions, self.deltas, self.how = query, positions, deltas, how
+
+    def turn(self, key: torch.Tensor, past_lengths: torch.Tensor) -> torch.Tensor:
+        self.query, key = run_multi_axis_rotary(
+            query=self.query, key=key, positions=self.positions, past_lengths=past_lengths if self.positions is None else None,
+            rope_deltas=self.deltas, **self.how)
+        return key
+
+    def write(self, key: torch.Tensor, value: torch.Tensor, layer: Qwen3PagedLayerAllocator, table: torch.Tensor,
+              past_lengths: torch.Tensor, new_lengths: torch.Tensor | None) -> None:
+        self.query = run_rotary_paged_kv_write(
+            query=self.query, key=key, value=value, key_pages=layer.key_pages, value_pages=layer.value_pages, page_table=table,
+            past_lengths=past_lengths, positions=self.positions, rope_deltas=self.deltas, new_lengths=new_lengths, **self.how)
 
 
 class Qwen3DynamicCache:
@@ -436,6 +511,45 @@ class Qwen3DynamicCache:
         if self.uses_turboquant_for_layer(layer_idx):
             return self._update_turboquant_layer(key_states, value_states, layer_idx,
                                                  require_dense_cache=require_dense_cache)
+        return self._update_paged_layer(key_states, value_states, layer_idx, require_dense_cache, None)
+
+    def update_rotary(self, query_states: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, *,
+                      positions: torch.Tensor | None = None, require_dense_cache: bool = True, **rotary):
+        """``update`` of keys that get their rotary positions on the way; returns ``(query, K | None, V | None, past_lengths)``
+        with the turned queries ``[B, Hq, T, D]``.
+
+        ``positions`` (int64 ``[axes, B, T]`` or ``[B, T]``): None counts on from each row's length, plus the cache's
+        ``rope_deltas`` where it has some (text behind images, ops.py:1900-1914).  ``rotary``: ``theta``, ``sections``,
+        ``interleaved``, ``rotary_dim``, ``inverse_frequencies``, ``attention_scaling`` of ``run_multi_axis_rotary``.
+        Un-quantized layers turn and write in one launch."""
+        if key_states.shape != value_states.shape or key_states.dim() != 4:
+            raise ValueError("update_rotary expects matching [batch, kv_heads, tokens, head_dim] key and value tensors")
+        if (query_states.dim() != 4 or query_states.shape[0] != key_states.shape[0] or query_states.shape[2:] != key_states.shape[2:]
+                or query_states.dtype != key_states.dtype):
+            raise ValueError("update_rotary expects [batch, heads, tokens, head_dim] queries that match the keys")
+        if query_states.device.type != "cuda":
+            raise RuntimeError("anna_b200 caches live on a CUDA device; there is no CPU fallback for update_rotary().")
+        batch_size = int(key_states.shape[0])
+        deltas = None
+        if positions is None and self.rope_deltas is not None:
+            deltas = self.rope_deltas.to(device=key_states.device, dtype=torch.long).reshape(batch_size)
+        pending = _PendingRotary(query_states, positions, deltas, rotary)
+        if self.uses_turboquant_for_layer(layer_idx):
+            self._ensure_batch_size(batch_size)
+            key_states = pending.turn(key_states, self._past_lengths_on_device(layer_idx, key_states.device))
+            dense = self._update_turboquant_layer(key_states, value_states, layer_idx, require_dense_cache=require_dense_cache)
+        else:
+            dense = self._update_paged_layer(key_states, value_states, layer_idx, require_dense_cache, pending)
+        return (pending.query, *dense)
+
+    def _past_lengths_on_device(self, layer_idx: int, device: torch.device) -> torch.Tensor:
+        past = list(self.layer_lengths[layer_idx])
+        state = self._dev_lengths[layer_idx]
+        current = state.current(past) if state is not None and state.device == device else None
+        return MetadataUploader.for_device(device).upload([past])[0] if current is None else current
+
+    def _update_paged_layer(self, key_states, value_states, layer_idx: int, require_dense_cache: bool,
+                            rotary: "_PendingRotary | None"):
         batch_size, kv_heads, append_length, head_dim = (int(v) for v in key_states.shape)
         self._ensure_batch_size(batch_size)
         device = key_states.device
@@ -491,11 +605,16 @@ class Qwen3DynamicCache:
         layer = self.allocator.layers[layer_idx]
         if table_dev is not None and append_length > 0:
             if segments == [(0, append_length)]:
-                self._launch_page_write(layer, key_states, value_states, table_dev, past, past_dev=past_lengths,
-                                        new_lengths_dev=new_lengths)
+                if rotary is not None:
+                    rotary.write(key_states, value_states, layer, table_dev, past_lengths, new_lengths)
+                else:
+                    self._launch_page_write(layer, key_states, value_states, table_dev, past, past_dev=past_lengths,
+                                            new_lengths_dev=new_lengths)
                 if state is not None:
                     state.after_append(lengths)
             else:
+                if rotary is not None:  # some of the tokens' pages are another sequence's
+                    key_states = rotary.turn(key_states, past_lengths)
                 for start, end in segments:
                     if end > start:
                         self._launch_page_write(layer, key_states[:, :, start:end, :],
@@ -812,8 +931,15 @@ class Qwen3DynamicCache:
         if int(query_states.shape[1]) != pool.kv_heads * num_key_value_groups:
             raise ValueError(
                 f"Expected {pool.kv_heads * num_key_value_groups} query heads, got {int(query_states.shape[1])}.")
-        device = query_states.device
-        table_dev = self._sync_page_table_layer_buffer(layer_idx, batch_size=batch, device=device)
+        table_dev, slots, lengths, slots_dev, lengths_dev = self._quantized_state(layer_idx, query_states.device)
+        return launch_tq_decode(pool, query_states, table_dev, slots, lengths, scaling, gate, slots_dev=slots_dev,
+                                lengths_dev=lengths_dev, output=output, peer_outputs=peer_outputs)
+
+    def _quantized_state(self, layer_idx: int, device: torch.device):
+        """(device table, slots, lengths, slots and lengths on the device or None) of a quantized layer's rows, derived from the
+        rows and kept for later calls where that holds."""
+        pool, rows = self._tq_pool(layer_idx), self.turboquant_rows[layer_idx]
+        table_dev = self._sync_page_table_layer_buffer(layer_idx, batch_size=len(rows), device=device)
         lengths = [0 if row is None else row.length for row in rows]
         slots = [0 if row is None else row.slot for row in rows]
         state = self._dev_lengths[layer_idx]
@@ -832,8 +958,38 @@ class Qwen3DynamicCache:
             # no headroom: the next append derives its step from the rows
             self._tq_step[layer_idx] = _QuantizedStep(pool, rows, table_dev, lengths, lengths_dev, slots, slots_dev, -1,
                                                       uploaded_on)
-        return launch_tq_decode(pool, query_states, table_dev, slots, lengths, scaling, gate, slots_dev=slots_dev,
-                                lengths_dev=lengths_dev, output=output, peer_outputs=peer_outputs)
+        return table_dev, slots, lengths, slots_dev, lengths_dev
+
+    def turboquant_multi_token_decode_attention(self, layer_idx: int, query_states: torch.Tensor, *, scaling: float,
+                                                num_key_value_groups: int, gate: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the newest T tokens of every row, ``query_states`` ``[B, Hq, T, D]``, after ``update`` has appended them:
+        drafted tokens, or a short chunk of a prompt, without the dense view of the cache.  Query ``t`` sees the keys up to its
+        own position, keys of the same chunk among them (de-quantized where they have left the window); in a row of fewer than T
+        tokens the queries that see none give zeros.  One launch for the whole batch."""
+        if not self.uses_turboquant_for_layer(layer_idx):
+            raise ValueError(f"Layer {layer_idx} does not use TurboQuant-backed KV storage.")
+        if query_states.ndim != 4:
+            raise ValueError("TurboQuant decode attention expects query_states shaped [batch, query_heads, tokens, head_dim].")
+        if gate is not None and (gate.shape != query_states.shape or gate.dtype != query_states.dtype):
+            raise ValueError(
+                f"TurboQuant decode gate expects query layout {tuple(query_states.shape)}, got {tuple(gate.shape)}.")
+        batch, heads = int(query_states.shape[0]), int(query_states.shape[1])
+        rows = self.turboquant_rows[layer_idx]
+        if batch != len(rows):
+            raise ValueError(f"Cache batch size mismatch: expected {len(rows)}, got {batch}")
+        pool = self._tq_pool(layer_idx)
+        if query_states.numel() == 0 or not pool.configured or all(row is None or row.length <= 0 for row in rows):
+            return query_states.new_zeros(query_states.shape)
+        if heads != pool.kv_heads * num_key_value_groups:
+            raise ValueError(f"Expected {pool.kv_heads * num_key_value_groups} query heads, got {heads}.")
+        if int(query_states.shape[3]) != pool.head_dim:
+            raise ValueError(f"Expected head_dim {pool.head_dim}, got {int(query_states.shape[3])}.")
+        step = self._tq_step[layer_idx]
+        if (step is not None and step.holds(pool, rows, query_states.device)
+                and step.readable(query_states.device, self._captured)):
+            return launch_tq_multi_decode(pool, query_states, step.table, step.slots_dev, step.lengths_dev, float(scaling), gate)
+        table_dev, _, _, slots_dev, lengths_dev = self._quantized_state(layer_idx, query_states.device)
+        return launch_tq_multi_decode(pool, query_states, table_dev, slots_dev, lengths_dev, float(scaling), gate)
 
     # -- dense views -------------------------------------------------------------------------------------------------------
 
@@ -1096,6 +1252,87 @@ class Qwen3DynamicCache:
         if self._prompt_token_ids is not None:
             cloned._prompt_token_ids = list(self._prompt_token_ids)
         return cloned
+
+    def fork_rows(self, row_indices) -> "Qwen3DynamicCache":
+        """A cache whose row ``i`` goes on from row ``row_indices[i]`` of this one, which stays as it is; a row may be forked any
+        number of times (candidates of one prompt, drafts that may be dropped).  Full pages are shared; partly filled pages and
+        window rings, which either side writes next, are copied, those of all layers in one launch.  ``clone`` copies a partly
+        filled page at the first append instead, a launch or two per row and layer."""
+        batch_size = self.get_batch_size()
+        rows = [int(idx) for idx in row_indices]
+        if any(idx < 0 or idx >= batch_size for idx in rows):
+            raise IndexError(f"fork_rows row indices out of range for batch size {batch_size}: {rows}")
+        forked = self._new_like(len(rows))
+        forked.reserved_seq_capacity = self.reserved_seq_capacity
+        forked._prefix_kv_share = self._prefix_kv_share
+        if self.rope_deltas is not None:
+            index = torch.tensor(rows, device=self.rope_deltas.device, dtype=torch.long)
+            forked.rope_deltas = self.rope_deltas.index_select(0, index)
+        copies: list[tuple[int, str, list[int], list[int]]] = []  # (layer, which pool, sources, targets)
+        for layer_idx in range(self.config.num_hidden_layers):
+            forked.layer_lengths[layer_idx] = [self.layer_lengths[layer_idx][idx] for idx in rows]
+            for name in ("conv_states", "recurrent_states"):
+                state = getattr(self, name)[layer_idx]
+                if state is not None:
+                    index = torch.tensor(rows, device=state.device, dtype=torch.long)
+                    getattr(forked, name)[layer_idx] = state.index_select(0, index)
+            sources: list[int] = []
+            targets: list[int] = []
+            if self.uses_turboquant_for_layer(layer_idx):
+                old_slots: list[int] = []
+                new_slots: list[int] = []
+                for new_idx, old_idx in enumerate(rows):
+                    row = self.turboquant_rows[layer_idx][old_idx]
+                    if row is None:
+                        continue
+                    fork, pages = row._fork()
+                    forked.turboquant_rows[layer_idx][new_idx] = fork
+                    if pages is not None:
+                        sources.append(pages[0])
+                        targets.append(pages[1])
+                    if fork.initialized and row.length > 0:
+                        old_slots.append(row.slot)
+                        new_slots.append(fork.slot)
+                copies.append((layer_idx, "window", old_slots, new_slots))
+                copies.append((layer_idx, "packed_pages", sources, targets))
+                continue
+            layer = self.allocator.layers[layer_idx]
+            for new_idx, old_idx in enumerate(rows):
+                length = self.layer_lengths[layer_idx][old_idx]
+                table = self.page_tables[layer_idx][old_idx]
+                full = length // self.block_size
+                own = list(table[:full])
+                for page_id in own:
+                    self.allocator.retain_shared_page(layer_idx, page_id)
+                if length % self.block_size:
+                    private = self.allocator.allocate(layer_idx, 1, key_template=layer.key_pages, value_template=layer.value_pages)[0]
+                    sources.append(table[full])
+                    targets.append(private)
+                    own.append(private)
+                forked.page_tables[layer_idx][new_idx] = own
+            # this cache's rows may share pages now, and the pools may have moved
+            copies.append((layer_idx, "key_pages", sources, targets))
+            copies.append((layer_idx, "value_pages", sources, targets))
+        forked.seen_tokens = max((forked._request_seq_length(idx) for idx in range(len(rows))), default=0)
+        work = []
+        for layer_idx, name, sources, targets in copies:  # pools may have grown meanwhile
+            if sources:
+                owner = self.allocator.turboquant_layers if name in ("window", "packed_pages") else self.allocator.layers
+                work.append((getattr(owner[layer_idx], name), sources, targets))
+        if work:
+            run_page_copy(copies=work)
+        return forked
+
+    def _forget_device_tables(self, layer_idx: int) -> None:
+        """The layer's pages have other ids: tables are built and uploaded again."""
+        self.page_table_caches[layer_idx] = None
+        self.page_table_capacities[layer_idx] = 0
+        self._table_rows_synced[layer_idx] = None
+        self._table_host[layer_idx] = None
+        self._table_blocks_total[layer_idx] = -1
+        self._page_headroom[layer_idx] = None
+        self._table_view[layer_idx] = None
+        self._tq_step[layer_idx] = None
 
     def release(self) -> None:
         """Give every page and window ring of this cache back to the allocator (ops.py:1383-1410)."""

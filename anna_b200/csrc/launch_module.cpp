@@ -770,7 +770,7 @@ at::Tensor arrival_counters(c10::Device device, cudaStream_t stream, int64_t cou
   return counters;
 }
 
-// tq_multi_decode(query, gate | None, packed_pages, table, window, slots, lengths, signs1, signs2, centroids, scaling, bits,
+// tq_multi_decode(query, gate | None, packed_pages | None, table | None, window, slots, lengths, signs1, signs2, centroids, scaling, bits,
 //                 residual_len, block_size, value_group) -> output | None
 PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -778,9 +778,10 @@ PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   bool ok = true;
   const at::Tensor* query = tensor(args[0]);
   const at::Tensor* gate = optional_tensor(args[1], &ok);
-  const at::Tensor* t[8];  // pages, table, window, slots, lengths, signs1, signs2, centroids
-  for (int i = 0; i < 8; ++i) {
-    t[i] = tensor(args[2 + i]);
+  const at::Tensor *pages = optional_tensor(args[2], &ok), *table = optional_tensor(args[3], &ok);
+  const at::Tensor* t[6];  // window, slots, lengths, signs1, signs2, centroids
+  for (int i = 0; i < 6; ++i) {
+    t[i] = tensor(args[4 + i]);
     ok = ok && t[i] != nullptr;
   }
   const double scaling = PyFloat_AsDouble(args[10]);
@@ -794,17 +795,21 @@ PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const c10::Device device = query->device();
   for (const at::Tensor* x : t)
     if (x->device() != device || x->layout() != at::kStrided) Py_RETURN_NONE;
-  const at::Tensor &pages = *t[0], &table = *t[1], &window = *t[2], &slots = *t[3], &lengths = *t[4];
+  const at::Tensor &window = *t[0], &slots = *t[1], &lengths = *t[2];
   const int64_t batch = query->size(0), heads = query->size(1), tokens = query->size(2), dim = query->size(3);
   anna_tq_layout layout;
   if (n[1] <= 0 || n[2] <= 0 || n[1] > INT32_MAX || n[2] > INT32_MAX || n[3] > INT32_MAX || tokens > INT32_MAX ||
       anna_tq_page_layout((int)dim, (int)n[0], (int)n[2], code, (int)n[3], &layout) != ANNA_OK)
     Py_RETURN_NONE;
-  if (pages.dim() != 3 || pages.scalar_type() != at::kByte || !pages.is_contiguous() || pages.size(2) != layout.chunk_bytes ||
-      pages.size(0) == 0 || pages.size(1) == 0 || heads % pages.size(1) != 0 || table.dim() != 2 || table.scalar_type() != at::kInt ||
-      table.size(0) != batch || (table.size(1) > 1 && table.stride(1) != 1) || window.dim() != 5 ||
-      window.scalar_type() != query->scalar_type() || !window.is_contiguous() || window.size(1) != 2 || window.size(2) != pages.size(1) ||
-      window.size(3) != n[1] || window.size(4) != dim)
+  if (window.dim() != 5 || window.scalar_type() != query->scalar_type() || !window.is_contiguous() || window.size(1) != 2 ||
+      window.size(2) == 0 || heads % window.size(2) != 0 || window.size(3) != n[1] || window.size(4) != dim)
+    Py_RETURN_NONE;
+  if (table != nullptr && (!plain(*table, device, 2) || table->scalar_type() != at::kInt || table->size(0) != batch ||
+                           (table->size(1) > 1 && table->stride(1) != 1)))
+    Py_RETURN_NONE;
+  const int64_t max_blocks = table == nullptr ? 0 : table->size(1);
+  if (max_blocks > 0 && (pages == nullptr || !plain(*pages, device, 3) || pages->scalar_type() != at::kByte || !pages->is_contiguous() ||
+                         pages->size(2) != layout.chunk_bytes || pages->size(0) == 0 || pages->size(1) != window.size(2)))
     Py_RETURN_NONE;
   for (const at::Tensor* x : {&slots, &lengths})
     if (x->dim() != 1 || x->scalar_type() != at::kLong || x->size(0) != batch || !x->is_contiguous()) Py_RETURN_NONE;
@@ -813,8 +818,10 @@ PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard(device);
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-  const int kv_heads = (int)pages.size(1);
-  const int64_t max_blocks = table.size(1);
+  const int kv_heads = (int)window.size(2);
+  const int64_t num_pages = max_blocks > 0 ? pages->size(0) : 0, table_stride = max_blocks > 0 ? table->stride(0) : 0;
+  const uint8_t* page_ptr = max_blocks > 0 ? static_cast<const uint8_t*>(pages->data_ptr()) : nullptr;
+  const int32_t* table_ptr = max_blocks > 0 ? static_cast<const int32_t*>(table->data_ptr()) : nullptr;
   int status;
   if (tokens == 1) {
     // One token is the single-token decode (one row of 4000 tokens, 32/8 heads: 11.5 us there, 22.5 here), in scratch of its own.
@@ -830,13 +837,12 @@ PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     {
       pybind11::gil_scoped_release unlocked;
       status = anna_tq_paged_decode(
-          query->data_ptr(), query->stride(0), query->stride(1), static_cast<const uint8_t*>(pages.data_ptr()),
-          static_cast<const int32_t*>(table.data_ptr()), table.stride(0), window.data_ptr(), static_cast<const int64_t*>(slots.data_ptr()),
-          static_cast<const int64_t*>(lengths.data_ptr()), floats(t[5]), floats(t[6]), floats(t[7]), address(gate),
+          query->data_ptr(), query->stride(0), query->stride(1), page_ptr, table_ptr, table_stride, window.data_ptr(), static_cast<const int64_t*>(slots.data_ptr()),
+          static_cast<const int64_t*>(lengths.data_ptr()), floats(t[3]), floats(t[4]), floats(t[5]), address(gate),
           gate == nullptr ? 0 : gate->stride(0), gate == nullptr ? 0 : gate->stride(1), out.data_ptr(), out.stride(0), out.stride(1),
           partials.data_ptr<float>(), partials.data_ptr<float>() + stats, chunks, 0, static_cast<int32_t*>(counters.data_ptr()),
           frags.data_ptr(), frag_bytes, (int)batch, (int)heads, kv_heads, (int)dim, (int)n[2], (int)n[1], (int)n[0], (int)n[3],
-          pages.size(0), max_blocks, (float)scaling, code, stream);
+          num_pages, max_blocks, (float)scaling, code, stream);
     }
     if (status != 0) return failed("tq_paged_multi_decode", status);
     return THPVariable_Wrap(std::move(out));
@@ -850,12 +856,11 @@ PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   {
     pybind11::gil_scoped_release unlocked;
     status = anna_tq_paged_multi_decode(
-        query->data_ptr(), query->stride(0), query->stride(1), query->stride(2), static_cast<const uint8_t*>(pages.data_ptr()),
-        static_cast<const int32_t*>(table.data_ptr()), table.stride(0), window.data_ptr(), static_cast<const int64_t*>(slots.data_ptr()),
-        static_cast<const int64_t*>(lengths.data_ptr()), floats(t[5]), floats(t[6]), floats(t[7]), address(gate),
+        query->data_ptr(), query->stride(0), query->stride(1), query->stride(2), page_ptr, table_ptr, table_stride, window.data_ptr(), static_cast<const int64_t*>(slots.data_ptr()),
+        static_cast<const int64_t*>(lengths.data_ptr()), floats(t[3]), floats(t[4]), floats(t[5]), address(gate),
         gate == nullptr ? 0 : gate->stride(0), gate == nullptr ? 0 : gate->stride(1), gate == nullptr ? 0 : gate->stride(2), out.data_ptr(),
         out.stride(0), out.stride(1), out.stride(2), scratch.data_ptr<float>(), floats_needed, static_cast<int32_t*>(counters.data_ptr()), (int)batch, (int)heads, kv_heads, (int)tokens, (int)dim, (int)n[2], (int)n[1], (int)n[0],
-        (int)n[3], pages.size(0), max_blocks, (float)scaling, code, stream);
+        (int)n[3], num_pages, max_blocks, (float)scaling, code, stream);
   }
   if (status != 0) return failed("tq_paged_multi_decode", status);
   return THPVariable_Wrap(std::move(out));
@@ -883,20 +888,32 @@ bool rotary_rows(const at::Tensor* query, const at::Tensor* key, int* code) {
          key->size(1) <= INT32_MAX && dtype_code(query->scalar_type(), code);
 }
 
-// rotary(query, key, positions, rates, axes, axis_count, rotary_dim, scale) -> (query, key) turned | None
+// Positions, or what they are derived from.
+bool row_starts(const at::Tensor* positions, const at::Tensor* past, const at::Tensor* deltas, c10::Device device, int64_t batch) {
+  if (positions == nullptr && past == nullptr) return false;
+  if (past != nullptr && (!plain(*past, device, 1) || past->scalar_type() != at::kLong || past->size(0) != batch || !past->is_contiguous()))
+    return false;
+  return deltas == nullptr || (positions == nullptr && deltas->device() == device && deltas->layout() == at::kStrided &&
+                               deltas->scalar_type() == at::kLong && deltas->size(0) == batch &&
+                               (deltas->dim() == 1 || (deltas->dim() == 2 && deltas->size(1) == 1)));
+}
+
+// rotary(query, key, positions | None, past | None, deltas | None, rates, axes, axis_count, rotary_dim, scale) -> (query, key) turned | None
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 8) return PyErr_Format(PyExc_TypeError, "rotary takes 8 arguments");
-  const at::Tensor *query = tensor(args[0]), *key = tensor(args[1]), *positions = tensor(args[2]), *rates = tensor(args[3]),
-                   *axes = tensor(args[4]);
+  if (nargs != 10) return PyErr_Format(PyExc_TypeError, "rotary takes 10 arguments");
+  bool ok = true;
+  const at::Tensor *query = tensor(args[0]), *key = tensor(args[1]), *rates = tensor(args[5]), *axes = tensor(args[6]);
+  const at::Tensor *positions = optional_tensor(args[2], &ok), *past = optional_tensor(args[3], &ok), *deltas = optional_tensor(args[4], &ok);
   int64_t n[2];  // axis_count, rotary_dim
-  if (!int_args(args + 5, 2, n)) return nullptr;
-  const double scale = PyFloat_AsDouble(args[7]);
+  if (!int_args(args + 7, 2, n)) return nullptr;
+  const double scale = PyFloat_AsDouble(args[9]);
   if (scale == -1.0 && PyErr_Occurred()) return nullptr;
   int code = 0;
-  int64_t ps[3];
-  if (positions == nullptr || rates == nullptr || axes == nullptr || !rotary_rows(query, key, &code) ||
-      !position_strides(*positions, query->device(), n[0], query->size(0), query->size(2), ps))
+  int64_t ps[3] = {0, 0, 0};
+  if (!ok || rates == nullptr || axes == nullptr || !rotary_rows(query, key, &code) ||
+      !row_starts(positions, past, deltas, query->device(), query->size(0)) ||
+      (positions != nullptr && !position_strides(*positions, query->device(), n[0], query->size(0), query->size(2), ps)))
     Py_RETURN_NONE;
   const c10::Device device = query->device();
   const c10::cuda::CUDAGuard guard(device);
@@ -905,7 +922,8 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int status = anna_multi_axis_rotary(
       query->data_ptr(), query->stride(0), query->stride(1), query->stride(2), q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
       key->data_ptr(), key->stride(0), key->stride(1), key->stride(2), k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-      static_cast<const int64_t*>(positions->data_ptr()), ps[0], ps[1], ps[2], static_cast<const double*>(rates->data_ptr()),
+      static_cast<const int64_t*>(address(positions)), ps[0], ps[1], ps[2], static_cast<const int64_t*>(address(past)),
+      static_cast<const int64_t*>(address(deltas)), deltas == nullptr ? 0 : deltas->stride(0), static_cast<const double*>(rates->data_ptr()),
       static_cast<const int32_t*>(axes->data_ptr()), (float)scale, (int)query->size(0), (int)query->size(1), (int)key->size(1),
       (int)query->size(2), (int)query->size(3), (int)n[1], code, stream);
   if (status != 0) return failed("multi_axis_rotary", status);
@@ -947,13 +965,11 @@ PyObject* rotary_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!plain(*table, device, 2) || table->scalar_type() != at::kInt || table->size(0) != batch || table->size(1) == 0 ||
       (table->size(1) > 1 && table->stride(1) != 1))
     Py_RETURN_NONE;
-  for (const at::Tensor* x : {past, fresh})
-    if (x != nullptr && (!plain(*x, device, 1) || x->scalar_type() != at::kLong || x->size(0) != batch || !x->is_contiguous())) Py_RETURN_NONE;
+  if (!row_starts(positions, past, deltas, device, batch)) Py_RETURN_NONE;
+  if (fresh != nullptr && (!plain(*fresh, device, 1) || fresh->scalar_type() != at::kLong || fresh->size(0) != batch || !fresh->is_contiguous()))
+    Py_RETURN_NONE;
   if (fresh != nullptr && fresh->data_ptr() == past->data_ptr()) Py_RETURN_NONE;
   if (word != nullptr && (word->device() != device || word->scalar_type() != at::kInt || word->numel() != 1)) Py_RETURN_NONE;
-  if (deltas != nullptr && (positions != nullptr || deltas->device() != device || deltas->scalar_type() != at::kLong ||
-                            (deltas->dim() != 1 && !(deltas->dim() == 2 && deltas->size(1) == 1)) || deltas->size(0) != batch))
-    Py_RETURN_NONE;
   int64_t ps[3] = {0, 0, 0};
   if (positions != nullptr && !position_strides(*positions, device, n[0], batch, tokens, ps)) Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard(device);

@@ -61,9 +61,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
   const int t = (int)(blockIdx.x % p.tokens);
 
   int64_t page_row = -1;  // of head 0, in elements
-  int64_t past = 0;
+  const int64_t past = kPaged || p.positions == nullptr ? p.past_lengths[b] : 0;
   if constexpr (kPaged) {
-    past = p.past_lengths[b];
     const int64_t at = past + t;
     const int64_t blk = at / p.block_size;
     int32_t pid = -1;
@@ -145,7 +144,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
   }
   for (int i = threadIdx.x; i < p.half; i += kRotaryThreads) {
     int64_t position;
-    if (!kPaged || p.positions != nullptr) {
+    if (p.positions != nullptr) {
       position = p.positions[p.axes[i] * p.pos_stride_a + b * p.pos_stride_b + t * p.pos_stride_t];
     } else {
       position = past + t + (p.rope_deltas != nullptr ? p.rope_deltas[b * p.delta_stride] : 0);
@@ -241,11 +240,13 @@ extern "C" int anna_multi_axis_rotary(const void* q, int64_t q_stride_b, int64_t
                                       int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_t, const void* k,
                                       int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t, void* k_out,
                                       int64_t ko_stride_b, int64_t ko_stride_h, int64_t ko_stride_t, const int64_t* positions,
-                                      int64_t pos_stride_a, int64_t pos_stride_b, int64_t pos_stride_t, const double* rates,
-                                      const int32_t* axes, float scale, int batch, int q_heads, int kv_heads, int tokens,
+                                      int64_t pos_stride_a, int64_t pos_stride_b, int64_t pos_stride_t,
+                                      const int64_t* past_lengths, const int64_t* rope_deltas, int64_t delta_stride,
+                                      const double* rates, const int32_t* axes, float scale, int batch, int q_heads, int kv_heads, int tokens,
                                       int head_dim, int rotary_dim, int dtype, anna_stream_t stream) {
-  ANNA_REQUIRE(positions != nullptr && k_out != nullptr, "anna_multi_axis_rotary: null pointer argument");
+  ANNA_REQUIRE((positions != nullptr || past_lengths != nullptr) && k_out != nullptr, "anna_multi_axis_rotary: null pointer argument");
   RotaryParams p{};
+  p.past_lengths = past_lengths; p.rope_deltas = rope_deltas; p.delta_stride = delta_stride;
   p.q = {q, q_stride_b, q_stride_h, q_stride_t};
   p.q_out = {q_out, qo_stride_b, qo_stride_h, qo_stride_t};
   p.k = {k, k_stride_b, k_stride_h, k_stride_t};

@@ -157,6 +157,15 @@ class _PageBook:
             unshared += left == 1
         return freed, unshared
 
+    def renumber(self, new_ids: dict[int, int], capacity: int) -> None:
+        """Pages are now ``new_ids[old id]`` of a pool of ``capacity`` pages; the others are free, lowest ids handed out first."""
+        counts = array("i", bytes(self._counts.itemsize * capacity))
+        for old, new in new_ids.items():
+            counts[new] = self.owners(old)
+        self._counts = counts
+        self._strays = None
+        self.free_pages[:] = [page_id for page_id in range(capacity - 1, -1, -1) if counts[page_id] == 0]
+
     def clear(self) -> None:
         self.free_pages.clear()
         self._counts = array("i")
@@ -244,6 +253,25 @@ class Qwen3PagedLayerAllocator:
         self.key_pages = None
         self.value_pages = None
         return capacity
+
+    def compact(self, new_ids: dict[int, int], spare_pages: int) -> int:
+        """Keep the pages ``new_ids`` (old id -> new id, 0 .. n - 1) in a pool of n + ``spare_pages`` pages; pages given back."""
+        before = self.capacity()
+        after = len(new_ids) + spare_pages if new_ids else 0
+        if before == 0 or after >= before:
+            # nothing to give back: the pages stay where they are, so that ids can
+            new_ids.update({page_id: page_id for page_id in new_ids})
+            return 0
+        if new_ids:
+            from .page_copy import run_page_gather
+
+            ids = list(new_ids)
+            self.key_pages, self.value_pages = run_page_gather(pools=[(self.key_pages, ids), (self.value_pages, ids)],
+                                                               spare_pages=spare_pages)
+        else:
+            self.key_pages = self.value_pages = None
+        self._book.renumber(new_ids, after)
+        return before - after
 
     def to(self, *, device: torch.device | None = None, dtype: torch.dtype | None = None) -> None:
         for name in ("key_pages", "value_pages"):
@@ -382,6 +410,40 @@ class TurboQuantLayerPool:
     def release_slot(self, slot: int) -> None:
         self.version += 1
         self.free_slots.append(int(slot))
+
+    def compact(self, new_ids: dict[int, int], rows: list, spare_pages: int) -> int:
+        """Keep the pages ``new_ids`` (old id -> new id, 0 .. n - 1) and the window rings of ``rows`` in pools that hold no more than
+        ``spare_pages`` others; rewrites the rows' block tables and slots.  Pages given back."""
+        from .page_copy import run_page_gather
+
+        before, slots_before = self.capacity(), self.slot_capacity()
+        after = len(new_ids) + spare_pages if new_ids else 0
+        moves_pages, moves_slots = 0 <= after < before, len(rows) < slots_before
+        if not moves_pages:
+            new_ids.update({page_id: page_id for page_id in new_ids})
+        if not moves_pages and not moves_slots:
+            return 0
+        work = []
+        if moves_pages and new_ids:
+            work.append((self.packed_pages, list(new_ids)))
+        if moves_slots and rows:
+            work.append((self.window, [row.slot for row in rows]))
+        moved = []
+        for pool, ids in work:  # spare pages are the page pool's
+            moved += run_page_gather(pools=[(pool, ids)], spare_pages=spare_pages if pool is self.packed_pages else 0)
+        if moves_pages:
+            self.packed_pages = moved.pop(0) if new_ids else None
+            self._book.renumber(new_ids, after)
+            for row in rows:
+                row.block_table = [new_ids[page_id] for page_id in row._blocks]
+                row._table_np_valid = 0
+        if moves_slots:
+            self.window = moved.pop(0) if rows else None
+            for slot, row in enumerate(rows):
+                row.slot = slot
+            self.free_slots.clear()
+        self.version += 1
+        return before - after if moves_pages else 0
 
     def trim(self) -> int:
         capacity = self.capacity()

@@ -44,6 +44,17 @@ class PrefixBlockPool:
             page_id = self._page_of.pop(key)
             self._keys_of.pop((layer_idx, page_id), None)
 
+    def move_pages(self, layer_idx: int, new_ids: dict[int, int]) -> None:
+        """The layer's pages have other ids now; keys of pages that are not among them are dropped."""
+        for key in [k for k in self._page_of if k[0] == layer_idx]:
+            page_id = self._page_of.pop(key)
+            self._keys_of.pop((layer_idx, page_id), None)
+            if page_id in new_ids:
+                self._page_of[key] = new_ids[page_id]
+        for key, page_id in self._page_of.items():
+            if key[0] == layer_idx:
+                self._keys_of.setdefault((layer_idx, page_id), set()).add(key)
+
     def clear(self) -> None:
         self._page_of.clear()
         self._keys_of.clear()

@@ -133,7 +133,19 @@ def _rows(tensor: torch.Tensor) -> torch.Tensor:
     return tensor if tensor.stride(3) == 1 else tensor.contiguous()
 
 
-def run_multi_axis_rotary(*, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, theta: float = 10000.0,
+def _check_row_starts(name: str, batch: int, positions, past_lengths, rope_deltas) -> None:
+    """Positions, or what they are derived from: lengths before the call and offsets of text behind images."""
+    if past_lengths is not None and (past_lengths.dtype != torch.long or tuple(past_lengths.shape) != (batch,)):
+        raise RuntimeError(f"{name}: past_lengths must be int64 [batch]")
+    if rope_deltas is not None:
+        if positions is not None:
+            raise RuntimeError(f"{name}: rope_deltas belong to positions=None")
+        if rope_deltas.dtype != torch.long or tuple(rope_deltas.shape) not in ((batch,), (batch, 1)):
+            raise RuntimeError(f"{name}: rope_deltas must be int64 [batch] or [batch, 1]")
+
+
+def run_multi_axis_rotary(*, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor | None = None,
+                          past_lengths: torch.Tensor | None = None, rope_deltas: torch.Tensor | None = None, theta: float = 10000.0,
                           sections: Sequence[int] | None = None, interleaved: bool = False, rotary_dim: int | None = None,
                           inverse_frequencies: Sequence[float] | None = None, attention_scaling: float = 1.0,
                           query_out: torch.Tensor | None = None,
@@ -141,7 +153,8 @@ def run_multi_axis_rotary(*, query: torch.Tensor, key: torch.Tensor, positions: 
     """Turned ``[B, Hq, T, D]`` queries and ``[B, Hkv, T, D]`` keys (any strides; new contiguous tensors unless ``query_out`` /
     ``key_out`` are given, which may be the inputs themselves).
 
-    ``positions``: int64 ``[axes, B, T]``, or ``[B, T]`` for the same on every axis.  ``sections`` (pairs per axis; None: one
+    ``positions``: int64 ``[axes, B, T]``, or ``[B, T]`` for the same on every axis; None: ``past_lengths[b] + t + rope_deltas[b]``
+    on every axis (``past_lengths`` int64 ``[B]``, ``rope_deltas`` int64 ``[B]`` or ``[B, 1]``, None: 0).  ``sections`` (pairs per axis; None: one
     axis), ``interleaved``, ``theta`` and ``inverse_frequencies``: see the module.  ``attention_scaling`` multiplies cosine and
     sine.  The first call with new parameters makes their tables and cannot be captured into a graph."""
     name = "multi_axis_rotary"
@@ -149,19 +162,23 @@ def run_multi_axis_rotary(*, query: torch.Tensor, key: torch.Tensor, positions: 
         width = query.shape[-1] if rotary_dim is None else rotary_dim
         tables = rotary_tables(width, theta=theta, sections=sections, interleaved=interleaved,
                                inverse_frequencies=inverse_frequencies, device=query.device)
-        turned = launch_module().rotary(query, key, positions, tables.rates, tables.axes, tables.axis_count, width, attention_scaling)
+        turned = launch_module().rotary(query, key, positions, past_lengths, rope_deltas, tables.rates, tables.axes, tables.axis_count, width, attention_scaling)
         if turned is not None:
             return turned
     # not the ordinary call: arguments to be checked or converted
     _check_rows(name, query, key)
-    device = _require_cuda(name, query=query, key=key, positions=positions)
+    if positions is None and past_lengths is None:
+        raise RuntimeError(f"{name}: positions or past_lengths must be given")
+    _check_row_starts(name, int(query.shape[0]), positions, past_lengths, rope_deltas)
+    device = _require_cuda(name, query=query, key=key, positions=positions, past_lengths=past_lengths, rope_deltas=rope_deltas)
     batch, heads, tokens, dim = (int(v) for v in query.shape)
     width = dim if rotary_dim is None else int(rotary_dim)
     if width > dim:
         raise RuntimeError(f"{name}: rotary_dim {width} is larger than head_dim {dim}")
     tables = rotary_tables(width, theta=theta, sections=sections, interleaved=interleaved,
                            inverse_frequencies=inverse_frequencies, device=device)
-    strides = _check_positions(name, positions, tables.axis_count, batch, tokens)
+    strides = (0, 0, 0) if positions is None else _check_positions(name, positions, tables.axis_count, batch, tokens)
+    past_lengths = None if past_lengths is None else past_lengths.contiguous()
     query_to = _output(name, "query_out", query_out, query, [key])
     key_to = _output(name, "key_out", key_out, key, [query])
     if query_out is not None and key_out is not None:
@@ -176,7 +193,8 @@ def run_multi_axis_rotary(*, query: torch.Tensor, key: torch.Tensor, positions: 
     with on_device(device):
         _lib.check(_lib.lib().anna_multi_axis_rotary(
             ptr(query), *query.stride()[:3], ptr(query_to), *query_to.stride()[:3], ptr(key), *key.stride()[:3], ptr(key_to),
-            *key_to.stride()[:3], ptr(positions), *strides, ptr(tables.rates), ptr(tables.axes), float(attention_scaling), batch,
+            *key_to.stride()[:3], ptr(positions), *strides, ptr(past_lengths), ptr(rope_deltas),
+            0 if rope_deltas is None else rope_deltas.stride(0), ptr(tables.rates), ptr(tables.axes), float(attention_scaling), batch,
             heads, int(key.shape[1]), tokens, dim, width, dtype_code(query.dtype), stream_ptr(device)), name)
     return query_to, key_to
 
@@ -191,8 +209,7 @@ def run_rotary_paged_kv_write(*, query: torch.Tensor, key: torch.Tensor, value: 
     """Turned queries ``[B, Hq, T, D]``; the turned keys and the values of ``[B, Hkv, T, D]`` go to their pages
     ``[P, Hkv, S, D]`` at positions ``past_lengths[b] + t``, all in one launch.
 
-    ``positions``: as for ``run_multi_axis_rotary``; None: ``past_lengths[b] + t + rope_deltas[b]`` on every axis
-    (``rope_deltas`` int64 ``[B]`` or ``[B, 1]``, None: 0), the positions of text behind what the row holds.  ``new_lengths``
+    ``positions`` and ``rope_deltas``: as for ``run_multi_axis_rotary``.  ``new_lengths``
     (int64 ``[B]``) receives ``past_lengths + T``; a token whose page id is invalid is not written and reported in ``status``
     (int32 ``[1]``).  The page pools must be contiguous."""
     name = "rotary_paged_kv_write"
@@ -220,18 +237,12 @@ def run_rotary_paged_kv_write(*, query: torch.Tensor, key: torch.Tensor, value: 
     batch, heads, tokens, dim = (int(v) for v in query.shape)
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
         raise RuntimeError(f"{name}: page_table must be int32 [batch, max_blocks]")
-    for label, tensor in (("past_lengths", past_lengths), ("new_lengths", new_lengths)):
-        if tensor is not None and (tensor.dtype != torch.long or tuple(tensor.shape) != (batch,)):
-            raise RuntimeError(f"{name}: {label} must be int64 [batch]")
-    if new_lengths is not None and (not new_lengths.is_contiguous() or new_lengths.data_ptr() == past_lengths.data_ptr()):
-        raise RuntimeError(f"{name}: new_lengths must be contiguous and not past_lengths itself")
+    _check_row_starts(name, batch, positions, past_lengths, rope_deltas)
+    if new_lengths is not None and (new_lengths.dtype != torch.long or tuple(new_lengths.shape) != (batch,)
+                                    or not new_lengths.is_contiguous() or new_lengths.data_ptr() == past_lengths.data_ptr()):
+        raise RuntimeError(f"{name}: new_lengths must be contiguous int64 [batch] and not past_lengths itself")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise RuntimeError(f"{name}: status must be int32 [1]")
-    if rope_deltas is not None:
-        if positions is not None:
-            raise RuntimeError(f"{name}: rope_deltas belong to positions=None")
-        if rope_deltas.dtype != torch.long or tuple(rope_deltas.shape) not in ((batch,), (batch, 1)):
-            raise RuntimeError(f"{name}: rope_deltas must be int64 [batch] or [batch, 1]")
     device = _require_cuda(name, query=query, key=key, value=value, key_pages=key_pages, value_pages=value_pages,
                            page_table=page_table, past_lengths=past_lengths, positions=positions, rope_deltas=rope_deltas,
                            new_lengths=new_lengths, status=status)

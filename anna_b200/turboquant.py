@@ -13,7 +13,7 @@ from array import array
 import torch
 
 from . import _lib
-from .fused_ops import (MetadataUploader, dtype_code, launch_module, on_device, ptr, query_scratch, split_scratch,
+from .fused_ops import (MetadataUploader, dtype_code, launch_module, multi_decode, on_device, ptr, query_scratch, split_scratch,
                         stream_ptr)
 from .pools import TurboQuantLayerPool, native_page_ids, resolve_value_group_size
 from .tq_tables import key_tables
@@ -153,6 +153,24 @@ def launch_tq_decode(pool: TurboQuantLayerPool, query_states: torch.Tensor, tabl
         else:
             _lib.check(_lib.lib().anna_tq_paged_decode(*common, stream_ptr(device)), "anna_tq_paged_decode")
     return out
+
+
+def launch_tq_multi_decode(pool: TurboQuantLayerPool, query_states: torch.Tensor, table_dev: torch.Tensor | None,
+                           slots_dev: torch.Tensor, lengths_dev: torch.Tensor, scaling: float,
+                           gate: torch.Tensor | None) -> torch.Tensor:
+    """Attention of ``[B, Hq, T, D]`` queries, the newest T tokens of B rows of one layer, over packed prefix + window ring."""
+    _require_cuda(query_states, "TurboQuant decode")
+    if query_states.dtype != pool.dtype:
+        raise RuntimeError(f"query dtype {query_states.dtype} must match the cache dtype {pool.dtype}")
+    tables = pool.tables
+    out = launch_module().tq_multi_decode(query_states, gate, pool.packed_pages, table_dev, pool.window, slots_dev, lengths_dev,
+                                          tables.signs1, tables.signs2, tables.centroids, scaling, pool.bits, pool.residual_len,
+                                          pool.block_size, pool.value_group)
+    if out is not None:
+        return out
+    return multi_decode("TurboQuant decode", query_states, pool.packed_pages, table_dev, pool.window, slots_dev, lengths_dev, tables,
+                        scaling, gate, kv_heads=pool.kv_heads, bits=pool.bits, residual_len=pool.residual_len,
+                        block_size=pool.block_size, value_group=pool.value_group)
 
 
 def launch_tq_materialize(pool: TurboQuantLayerPool, table_dev: torch.Tensor, quantized_lengths: list[int],
@@ -569,6 +587,28 @@ class TurboQuantKVRow:
         cloned.block_table = list(self.block_table)
         self.pool.window[cloned.slot].copy_(self.pool.window[self.slot])
         return cloned
+
+    def _fork(self) -> tuple["TurboQuantKVRow", tuple[int, int] | None]:
+        """A row that goes on from this one with a ring slot of its own, whose contents the caller has to copy: full pages are
+        shared, and of a partly filled last page the (source, target) ids come back for the caller to copy."""
+        fork = TurboQuantKVRow(bits=self.bits, residual_len=self.residual_len, value_group_size=self.value_group_size)
+        if not self.initialized:
+            return fork, None
+        pool = self.pool
+        assert pool is not None
+        fork._attach(pool)
+        full = self.quantized_length // pool.block_size
+        blocks = list(self._blocks[:full])
+        for page_id in blocks:
+            pool.retain_page(page_id)
+        pages = None
+        if self.quantized_length % pool.block_size:
+            private = pool.allocate(1)[0]
+            pages = (self._blocks[full], private)
+            blocks.append(private)
+        fork.block_table = blocks
+        fork._length = self._length
+        return fork, pages
 
     def release(self) -> None:
         """Give the pages and the ring slot back to the pool; the row is empty afterwards."""

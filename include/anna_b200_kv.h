@@ -157,7 +157,8 @@ int anna_paged_kv_write(const void* k_new, const void* v_new, int64_t kn_stride_
  * Stands in for the rotary part of Qwen3Attention._forward_attention (src/anna/model/ops.py:1900-1914).
  *   q, k       [B, Hq, T, D], [B, Hkv, T, D] with element strides per batch, head and token; last dim contiguous
  *   q_out, k_out  the same; either the input itself with its strides (in place) or memory that does not overlap it
- *   positions  int64, element strides per axis, batch and token (0: the same for all); magnitudes up to 2^31
+ *   positions  int64, element strides per axis, batch and token (0: the same for all); magnitudes up to 2^31.  NULL:
+ *              past_lengths[b] + t + rope_deltas[b * delta_stride] on every axis (rope_deltas may be NULL: 0)
  *   rates      double [rotary_dim / 2], turns per position;  axes  int32 [rotary_dim / 2], all >= 0 and < the number of axes
  * rotary_dim is even and at most D; no other limit on D below 4096.  Any alignment of whole elements; the widest that all tensors
  * share is used.
@@ -166,13 +167,13 @@ int anna_multi_axis_rotary(const void* q, int64_t q_stride_b, int64_t q_stride_h
                            int64_t qo_stride_b, int64_t qo_stride_h, int64_t qo_stride_t, const void* k, int64_t k_stride_b,
                            int64_t k_stride_h, int64_t k_stride_t, void* k_out, int64_t ko_stride_b, int64_t ko_stride_h,
                            int64_t ko_stride_t, const int64_t* positions, int64_t pos_stride_a, int64_t pos_stride_b,
-                           int64_t pos_stride_t, const double* rates, const int32_t* axes, float scale, int batch, int q_heads,
+                           int64_t pos_stride_t, const int64_t* past_lengths, const int64_t* rope_deltas, int64_t delta_stride,
+                           const double* rates, const int32_t* axes, float scale, int batch, int q_heads,
                            int kv_heads, int tokens, int head_dim, int rotary_dim, int dtype, anna_stream_t stream);
 
 /*
  * The same in front of anna_paged_kv_write, in one launch: queries are turned into q_out, keys are turned into their pages, values
  * [B, Hkv, T, D] (strides of their own) go to theirs as they are.
- *   positions    NULL: past_lengths[b] + t + rope_deltas[b * delta_stride] on every axis (rope_deltas may be NULL: 0)
  *   page_table, past_lengths, new_lengths, status  as for anna_paged_kv_write; tokens without a valid page are not written
  */
 int anna_rotary_paged_kv_write(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, void* q_out,

@@ -108,6 +108,10 @@ def test_far_positions_negative_ones_and_scaling(cuda_device):
     for x, out in zip((q, k), got):
         want, bound = turned(x, positions, 64, frequencies=frequencies, scale=1.25)
         assert_close(out, want, 3 * bound)
+    past, deltas = torch.tensor([70000]), torch.tensor([[-200]])
+    want = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=(past[:, None] + deltas + torch.arange(6)).to(cuda_device))
+    got = anna_b200.run_multi_axis_rotary(query=q, key=k, past_lengths=past.to(cuda_device), rope_deltas=deltas.to(cuda_device))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     exact_zero = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=torch.zeros(1, 6, dtype=torch.long, device=cuda_device))
     assert torch.equal(exact_zero[0], q) and torch.equal(exact_zero[1], k)  # no turn changes no bit
 
@@ -242,6 +246,11 @@ def test_calls_that_cannot_be_are_refused():
         call(query=q, key=k[:, :, :2], positions=positions)
     with pytest.raises(RuntimeError, match="dtype"):
         call(query=q, key=k.half(), positions=positions)
+    for change, match in ((dict(positions=None), "past_lengths"), (dict(positions=None, past_lengths=positions), "past_lengths"),
+                          (dict(rope_deltas=positions[:, 0]), "rope_deltas"),
+                          (dict(positions=None, past_lengths=positions[:, 0], rope_deltas=positions), "rope_deltas")):
+        with pytest.raises(RuntimeError, match=match):
+            call(**{**dict(query=q, key=k, positions=positions), **change})
     with pytest.raises(RuntimeError, match="batch, heads"):
         call(query=q[0], key=k, positions=positions)
     with pytest.raises(RuntimeError, match="float16, bfloat16"):
@@ -263,8 +272,8 @@ def test_entry_points_refuse_what_they_cannot_run():
     library, ok = _lib.lib(), 0x10000
 
     def rotary_call(q=ok, out=ok, k=ok, positions=ok, rates=ok, batch=1, heads=2, kv=1, tokens=1, dim=64, width=64, dtype=2):
-        return library.anna_multi_axis_rotary(q, 64, 64, 64, out, 64, 64, 64, k, 64, 64, 64, out, 64, 64, 64, positions, 0, 1, 1,
-                                              rates, ok, 1.0, batch, heads, kv, tokens, dim, width, dtype, None)
+        return library.anna_multi_axis_rotary(q, 64, 64, 64, out, 64, 64, 64, k, 64, 64, 64, out, 64, 64, 64, positions, 0, 1, 1, None,
+                                              None, 0, rates, ok, 1.0, batch, heads, kv, tokens, dim, width, dtype, None)
 
     for bad in (dict(q=None), dict(out=None), dict(k=None), dict(positions=None), dict(rates=None), dict(batch=0), dict(heads=0),
                 dict(tokens=0), dict(width=0), dict(width=63), dict(width=66), dict(dim=8192, width=64), dict(dtype=3), dict(q=ok + 1),
