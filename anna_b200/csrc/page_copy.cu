@@ -5,7 +5,7 @@
 // operations are 32 gathers, 32 scatters and the upload of the ids.  What a launch has to know travels in its parameters where it
 // fits (128 pools and 2816 pairs of ids, 29 KB), so that an ordinary fork uploads nothing.
 //
-// The work is cut into units of kUnitBytes of one page, whatever the pages' sizes; a CTA finds the pool of a unit by bisection
+// The work is cut into units of at most kUnitBytes of one page, whatever the pages' sizes; a CTA finds the pool of a unit by bisection
 // over the pools' first units, which it keeps in shared memory.
 #include "common.cuh"
 
@@ -25,8 +25,8 @@ struct CopyPool {
   int32_t src_pages, dst_pages;
   int32_t first_pair;
   int32_t units_per_page;
-  int32_t access;  // bytes
-  int32_t unused;
+  int32_t access;      // bytes
+  int32_t unit_bytes;  // the page's bytes dealt evenly, in whole 512
 };
 
 template <int POOLS, int PAIRS>
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
     const CopyPool& pool = t.pools[lo];
     const int64_t mine = unit - pool.first_unit;
     const int64_t copy = mine / pool.units_per_page;
-    const int64_t at = (mine - copy * pool.units_per_page) * kUnitBytes;
+    const int64_t at = (mine - copy * pool.units_per_page) * pool.unit_bytes;
     const int2 pair = PAIRS > 0 ? t.pairs[PAIRS > 0 ? pool.first_pair + copy : 0] : device_pairs[pool.first_pair + copy];
     if (pair.x < 0 || pair.x >= pool.src_pages || pair.y < 0 || pair.y >= pool.dst_pages) {
       if (status != nullptr && threadIdx.x == 0) atomicOr(status, (int)ANNA_DEV_BAD_PAGE);
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
     }
     const uint8_t* src = pool.src + pair.x * pool.page_bytes + at;
     uint8_t* dst = pool.dst + pair.y * pool.page_bytes + at;
-    const int64_t bytes = min((int64_t)kUnitBytes, pool.page_bytes - at);
+    const int64_t bytes = min((int64_t)pool.unit_bytes, pool.page_bytes - at);
     if (pool.access == 16) copy_unit<uint4>(src, dst, bytes);
     else if (pool.access >= 4) copy_unit<uint32_t>(src, dst, bytes);
     else copy_unit<uint8_t>(src, dst, bytes);
@@ -88,9 +88,9 @@ static int launch_copies(const CopyPool* pools, int num_pools, const int2* pairs
   CopyTables<POOLS, PAIRS> t;
   memcpy(t.pools, pools, sizeof(CopyPool) * num_pools);
   if (PAIRS > 0) memcpy(t.pairs, pairs, sizeof(int2) * num_pairs);
-  const int64_t most = 148 * 8;
-  page_copy_kernel<POOLS, PAIRS><<<(unsigned)(units < most ? units : most), kCopyThreads, 0, stream>>>(t, num_pools, units, device_pairs,
-                                                                                                       status);
+  // a CTA per unit: 300 window rings of four layers 201 us (6.2 TB/s), 228 with eight CTAs per SM that go on from unit to unit
+  const int64_t ctas = units < INT32_MAX ? units : INT32_MAX;
+  page_copy_kernel<POOLS, PAIRS><<<(unsigned)ctas, kCopyThreads, 0, stream>>>(t, num_pools, units, device_pairs, status);
   return check_launch("page_copy_kernel");
 }
 
@@ -135,6 +135,7 @@ extern "C" int anna_page_copy(const anna_page_pool* pools, int num_pools, const 
       c.dst_pages = g.dst_pages;
       c.first_pair = g.first_pair;
       c.units_per_page = (int32_t)((g.page_bytes + kUnitBytes - 1) / kUnitBytes);
+      c.unit_bytes = (int32_t)(((g.page_bytes + c.units_per_page - 1) / c.units_per_page + 511) / 512 * 512);
       c.access = 16;
       while (reinterpret_cast<uintptr_t>(g.src) % c.access || reinterpret_cast<uintptr_t>(g.dst) % c.access || g.page_bytes % c.access)
         c.access /= 2;

@@ -98,6 +98,42 @@ def test_turned_queries_and_keys(cuda_device, case, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(3, 4, 1, 4001, 64, 32, (4, 6, 6), True, 16), (2, 1, 1, 12007, 24, 24, (5, 7), False, 24),
+                                  (7, 3, 3, 900, 128, 128, None, False, 8), (1, 9, 2, 3001, 256, 64, (11, 11, 10), True, 32),
+                                  (1, 33, 1, 2600, 32, 16, (3, 5), False, 16), (2, 2, 1, 1700, 16, 16, None, False, 16)], ids=str)
+def test_many_tokens(cuda_device, case, dtype):
+    """Several tokens a CTA, the last of them fewer, rows of the batch inside a CTA."""
+    batch, q_heads, kv_heads, tokens, dim, width, sections, interleaved, page = case
+    q, k = states(batch, q_heads, kv_heads, tokens, dim, dtype, cuda_device)
+    v = states(batch, 1, kv_heads, tokens, dim, dtype, cuda_device, seed=2)[1]
+    axes = 1 if sections is None else len(sections)
+    positions = torch.randint(0, 1 << 18, (axes, batch, tokens), generator=torch.Generator().manual_seed(1))
+    how = dict(theta=1e6, sections=sections, interleaved=interleaved, rotary_dim=width)
+    got = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions.to(cuda_device), **how)
+    for x, out in zip((q, k), got):
+        assert_close(out, *turned(x, positions, width, theta=1e6, sections=sections, interleaved=interleaved))
+    past = torch.arange(batch) * 5 + 2
+    blocks = (int(past.max()) + tokens + page - 1) // page
+    order = torch.randperm(batch * blocks, generator=torch.Generator().manual_seed(3)).view(batch, blocks)
+    pools = [torch.zeros(batch * blocks, kv_heads, page, dim, device=cuda_device, dtype=dtype) for _ in range(2)]
+    new = torch.zeros(batch, dtype=torch.long, device=cuda_device)
+    out = anna_b200.run_rotary_paged_kv_write(query=q, key=k, value=v, key_pages=pools[0], value_pages=pools[1],
+                                              page_table=order.int().to(cuda_device), past_lengths=past.to(cuda_device),
+                                              positions=positions.to(cuda_device), new_lengths=new, **how)
+    assert torch.equal(out, got[0]) and new.tolist() == (past + tokens).tolist()
+    want = [torch.zeros_like(pool) for pool in pools]
+    at = past[:, None] + torch.arange(tokens)
+    pages = order.gather(1, at // page).to(cuda_device)
+    for pool, x in zip(want, (got[1], v)):
+        pool[pages, :, (at % page).to(cuda_device)] = x.transpose(1, 2)
+    assert torch.equal(pools[0], want[0]) and torch.equal(pools[1], want[1])
+    qi, ki = q.clone(), k.clone()
+    anna_b200.run_multi_axis_rotary(query=qi, key=ki, positions=positions.to(cuda_device), query_out=qi, key_out=ki, **how)
+    assert torch.equal(qi, got[0]) and torch.equal(ki, got[1])
+
+
+@pytest.mark.gpu
 def test_far_positions_negative_ones_and_scaling(cuda_device):
     q, k = states(1, 2, 1, 6, 64, torch.float32, cuda_device)
     positions = torch.tensor([[0, 1, -5, 262143, (1 << 31) - 1, -(1 << 31)]])
