@@ -15,6 +15,7 @@ namespace anna {
 constexpr int kMultiThreads = 128, kMultiWarps = 4;
 constexpr int kMultiRows = 8;    // of a CTA of this form
 constexpr int kMultiTokens = 32;  // de-quantized at a time: a lane's token
+constexpr int kMultiAhead = 4;    // tokens of a warp whose codes are on their way together
 
 template <int D>
 constexpr int kMultiSmemFloats = 3 * kMultiRows * D + 2 * kMultiTokens * (D + 1) + kMultiTokens * D + kMultiRows * kMultiTokens;
@@ -84,52 +85,94 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
     const int64_t stop = min(packed ? min(lq, t1) : t1, base + kMultiTokens);
     const int n = (int)(stop - base);
     __syncthreads();
-    // ---- 32 tokens into shared memory: a warp per token ------------------------------------------------------------------
-    for (int i = warp; i < n; i += kMultiWarps) {
-      const int64_t t = base + i;
+    // ---- 32 tokens into shared memory -----------------------------------------------------------------------------------------
+    // A lane finds the page of its token; then a warp takes a token at a time, whose codes are on their way for several at once.
+    int64_t chunk = -1;  // of this lane's token, in bytes
+    int in_page = 0;
+    if (packed && lane < n) {
+      const int64_t t = base + lane, blk = t / p.block_size;
+      in_page = (int)(t - blk * p.block_size);
+      const int32_t pid = blk < p.max_blocks ? p.block_table[b * p.table_stride + blk] : -1;
+      if (pid >= 0 && pid < p.num_pages) chunk = ((int64_t)pid * p.kv_heads + kvh) * p.layout.chunk_bytes;
+      if (warp == 0) {
+        sm_there[lane] = chunk >= 0;
+        sm_norm[lane] = chunk >= 0 ? reinterpret_cast<const float*>(p.pages + chunk + p.layout.off_knorm)[in_page] : 0.0f;
+      }
+    }
+    if (!packed && warp == 0 && lane < n) {
+      sm_there[lane] = true;
+      sm_norm[lane] = 1.0f;
+    }
+    for (int i = warp; i < n; i += kMultiWarps * kMultiAhead) {
       if (!packed) {
-        const T* k = ring + (t % p.residual_len) * D;
-        for (int d = lane; d < D; d += 32) {
-          ka[i * (D + 1) + d] = ElemTraits<T>::to_float(k[d]);
-          vt[i * D + d] = ElemTraits<T>::to_float(k[ring_values + d]);
+        float k[kMultiAhead][E], v[kMultiAhead][E];
+#pragma unroll
+        for (int u = 0; u < kMultiAhead; ++u) {
+          const T* key = ring + ((base + min(i + u * kMultiWarps, n - 1)) % p.residual_len) * D;
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            k[u][j] = ElemTraits<T>::to_float(key[lane + 32 * j]);
+            v[u][j] = ElemTraits<T>::to_float(key[ring_values + lane + 32 * j]);
+          }
         }
-        if (lane == 0) {
-          sm_there[i] = true;
-          sm_norm[i] = 1.0f;
+#pragma unroll
+        for (int u = 0; u < kMultiAhead; ++u) {
+          const int at = i + u * kMultiWarps;
+          if (at >= n) break;
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            ka[at * (D + 1) + lane + 32 * j] = k[u][j];
+            vt[at * D + lane + 32 * j] = v[u][j];
+          }
         }
         continue;
       }
-      const int64_t blk = t / p.block_size;
-      const int tok = (int)(t - blk * p.block_size);
-      const int32_t pid = blk < p.max_blocks ? p.block_table[b * p.table_stride + blk] : -1;
-      const bool there = pid >= 0 && pid < p.num_pages;
-      if (lane == 0) sm_there[i] = there;
-      const uint8_t* page = p.pages + (there ? ((int64_t)pid * p.kv_heads + kvh) * p.layout.chunk_bytes : 0);
-      const float rnorm = there ? reinterpret_cast<const float*>(page + p.layout.off_krnorm)[tok] : 0.0f;
-      if (lane == 0) sm_norm[i] = there ? reinterpret_cast<const float*>(page + p.layout.off_knorm)[tok] : 0.0f;
-      const uint8_t* keys = page + p.layout.off_kcodes + tok * p.layout.key_bytes;
-      const uint8_t* codes = page + p.layout.off_vdata + tok * p.layout.value_bytes;
-      const T* scales = reinterpret_cast<const T*>(page + p.layout.off_vscale) + tok * p.layout.groups;
-      const T* zeros = reinterpret_cast<const T*>(page + p.layout.off_vzero) + tok * p.layout.groups;
-      for (int d = lane; d < D; d += 32) {
-        uint32_t code = 0, sign = 0, value = 0;
-        float scale = 0.0f, zero = 0.0f;
-        if (there) {
-          if constexpr (BITS == 3) {
-            code = (keys[d >> 2] >> ((d & 3) * 2)) & 3u;
-            sign = (keys[D / 4 + (d >> 3)] >> (d & 7)) & 1u;
-          } else {
-            const uint32_t field = (keys[d * BITS >> 3] >> (d * BITS & 7)) & ((1u << BITS) - 1u);
-            code = field & ((1u << M) - 1u);
-            sign = field >> M;
-          }
-          value = (codes[d * VS >> 3] >> (d * VS & 7)) & ((1u << VS) - 1u);
-          scale = ElemTraits<T>::to_float(scales[d / p.value_group]);
-          zero = ElemTraits<T>::to_float(zeros[d / p.value_group]);
+      uint8_t code[kMultiAhead][E], sign[kMultiAhead][E], value[kMultiAhead][E];
+      T scale[kMultiAhead][E], zero[kMultiAhead][E];
+      float rnorm[kMultiAhead];
+#pragma unroll
+      for (int u = 0; u < kMultiAhead; ++u) {
+        const int at = min(i + u * kMultiWarps, n - 1);
+        const int64_t where = __shfl_sync(0xffffffffu, chunk, at);
+        const int tok = __shfl_sync(0xffffffffu, in_page, at);
+        const bool there = where >= 0;
+        const uint8_t* page = p.pages + (there ? where : 0);
+        const uint8_t* keys = page + p.layout.off_kcodes + tok * p.layout.key_bytes;
+        const uint8_t* codes = page + p.layout.off_vdata + tok * p.layout.value_bytes;
+        const T* scales = reinterpret_cast<const T*>(page + p.layout.off_vscale) + tok * p.layout.groups;
+        const T* zeros = reinterpret_cast<const T*>(page + p.layout.off_vzero) + tok * p.layout.groups;
+        rnorm[u] = there ? reinterpret_cast<const float*>(page + p.layout.off_krnorm)[tok] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int d = lane + 32 * j;
+          code[u][j] = there ? keys[BITS == 3 ? d >> 2 : d * BITS >> 3] : 0;
+          sign[u][j] = BITS == 3 && there ? keys[D / 4 + (d >> 3)] : 0;
+          value[u][j] = there ? codes[d * VS >> 3] : 0;
+          scale[u][j] = there ? scales[d / p.value_group] : T(0.0f);
+          zero[u][j] = there ? zeros[d / p.value_group] : T(0.0f);
         }
-        ka[i * (D + 1) + d] = sm_cent[code];
-        kb[i * (D + 1) + d] = sign != 0 ? rnorm : -rnorm;
-        vt[i * D + d] = fmaf((float)value, scale, zero);
+      }
+#pragma unroll
+      for (int u = 0; u < kMultiAhead; ++u) {
+        const int at = i + u * kMultiWarps;
+        if (at >= n) break;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int d = lane + 32 * j;
+          uint32_t index, negative;
+          if constexpr (BITS == 3) {
+            index = (code[u][j] >> ((d & 3) * 2)) & 3u;
+            negative = ((sign[u][j] >> (d & 7)) & 1u) ^ 1u;
+          } else {
+            const uint32_t field = (code[u][j] >> (d * BITS & 7)) & ((1u << BITS) - 1u);
+            index = field & ((1u << M) - 1u);
+            negative = (field >> M) ^ 1u;
+          }
+          ka[at * (D + 1) + d] = sm_cent[index];
+          kb[at * (D + 1) + d] = negative != 0 ? -rnorm[u] : rnorm[u];
+          vt[at * D + d] = fmaf((float)((value[u][j] >> (d * VS & 7)) & ((1u << VS) - 1u)), ElemTraits<T>::to_float(scale[u][j]),
+                                ElemTraits<T>::to_float(zero[u][j]));
+        }
       }
     }
     __syncthreads();
@@ -141,6 +184,7 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
       const float* q0 = q_smem + ((packed ? kMultiRows : 0) + warp) * D;
       const float* q1 = q0 + kMultiWarps * D;
       float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll 16
       for (int d = 0; d < D; ++d) {
         a0 = fmaf(q0[d], x[d], a0);
         a1 = fmaf(q1[d], x[d], a1);
@@ -149,6 +193,7 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
         q0 += kMultiRows * D;
         q1 += kMultiRows * D;
         float b0 = 0.0f, b1 = 0.0f;
+#pragma unroll 16
         for (int d = 0; d < D; ++d) {
           b0 = fmaf(q0[d], y[d], b0);
           b1 = fmaf(q1[d], y[d], b1);
@@ -183,8 +228,8 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
     for (int r = 0; r < kOutRows; ++r)
 #pragma unroll
       for (int j = 0; j < kDims; ++j) acc[r][j] *= sm_rescale[out_row0 + r];
+#pragma unroll 4
     for (int i = 0; i < n; ++i) {
-      if (!sm_there[i]) continue;
       float v[kDims];
 #pragma unroll
       for (int j = 0; j < kDims; ++j) v[j] = vt[i * D + d0 + j * kMultiThreads];
@@ -298,7 +343,8 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
                      value_group);
   ANNA_REQUIRE(aligned_to(packed_pages, 16) && aligned_to(window, 16), "%s: pages and window must be 16-byte aligned", what);
   ANNA_REQUIRE(aligned_to(scratch, 16), "%s: scratch must be 16-byte aligned", what);
-  p.q = q; p.q_stride_b = q_stride_b; p.q_stride_h = q_stride_h; p.q_stride_t = q_stride_t;
+  // the stride of a dim of one entry may be anything
+  p.q = q; p.q_stride_b = batch > 1 ? q_stride_b : 0; p.q_stride_h = q_heads > 1 ? q_stride_h : 0; p.q_stride_t = tokens > 1 ? q_stride_t : 0;
   p.pages = packed_pages; p.block_table = block_table; p.table_stride = table_stride;
   p.window = window; p.window_slots = window_slots; p.lengths = lengths;
   p.signs1 = signs1; p.signs2 = signs2; p.centroids = centroids;
@@ -313,9 +359,10 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
     if ((1 << s) == block_size) p.block_shift = s;
   p.num_pages = num_pages; p.max_blocks = max_blocks; p.max_len = max_blocks * block_size + residual_len;
   p.scaling = scaling;
-  p.stream_tiles = tq_multi_mma_applicable(p, head_dim, dtype) && head_dim == 128 && p.rows <= 16 ? 32 : 64;
   const int row_tiles = (p.rows + kMultiRows - 1) / kMultiRows;
   const bool tensor_cores = tq_multi_mma_applicable(p, head_dim, dtype);
+  p.stream_tiles = !tensor_cores ? 4 : head_dim == 128 && p.rows <= 16 ? 32 : 64;
+  p.min_share = tensor_cores ? 32 : 4;
   // The line of a launch has room for so many rows and positions: larger batches go in several, one behind the other.
   const int64_t row_positions = (int64_t)kv_heads * row_tiles * ((p.max_len + kBalancedTileTokens - 1) / kBalancedTileTokens + p.stream_tiles);
   ANNA_REQUIRE(row_positions < (1ll << 30), "%s: too many queries and keys of one sequence", what);
@@ -337,7 +384,7 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
     });
     if (rc != ANNA_OK) return rc;
     const int64_t elem = dtype_bytes_of(dtype);
-    p.q = static_cast<const uint8_t*>(p.q) + (int64_t)most * q_stride_b * elem;
+    p.q = static_cast<const uint8_t*>(p.q) + (int64_t)most * p.q_stride_b * elem;
     p.out = static_cast<uint8_t*>(p.out) + (int64_t)most * out_stride_b * elem;
     if (p.gate != nullptr) p.gate = static_cast<const uint8_t*>(p.gate) + (int64_t)most * gate_stride_b * elem;
     if (p.block_table != nullptr) p.block_table += (int64_t)most * table_stride;

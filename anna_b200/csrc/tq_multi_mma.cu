@@ -491,25 +491,21 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
                                        w / (kNibbleWords / 2) * (4 * kHalfWords), words[c]);
         }
         const int at = BITS == 4 ? w % kHalfWords : w / 2 % kHalfWords;  // the nibble word's word
-        // a k-step at a time, the columns' products side by side: those of one column wait for one another
+        // a k-step at a time, column by column: a product runs while the next column is unpacked, and one column's products are four apart
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint4 a[MT];
 #pragma unroll
           for (int m = 0; m < MT; ++m) a[m] = frag[(m * 2 * Cfg::kSteps + 2 * w + i) * 32];
-          uint32_t k[kCols][2];
 #pragma unroll
           for (int c = 0; c < kCols; ++c) {
             uint32_t sel = (BITS == 2 || BITS == 3) && (w & 1) != 0 ? words[c][at] >> (i == 0 ? 2 : 18) : i == 0 ? words[c][at] : words[c][at] >> 16;
             sel &= BITS == 4 ? 0x7777u : BITS == 3 ? 0x3333u : 0x1111u;
             const uint32_t lo = permute(lut_lo[0], lut_lo[1], sel), hi = permute(lut_hi[0], lut_hi[1], sel);
-            k[c][0] = permute(lo, hi, 0x5140);
-            k[c][1] = permute(lo, hi, 0x7362);
+            const uint32_t k0 = permute(lo, hi, 0x5140), k1 = permute(lo, hi, 0x7362);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) mma_f16(s[m][c], a[m], k0, k1);
           }
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) mma_f16(s[m][c], a[m], k[c][0], k[c][1]);
         }
         if constexpr (BITS != 3) {
 #pragma unroll
@@ -517,19 +513,18 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
             uint4 a[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) a[m] = frag[(m * 2 * Cfg::kSteps + Cfg::kSteps + 2 * w + i) * 32];
-            uint32_t k[kCols][2];
 #pragma unroll
-            for (int c = 0; c < kCols; ++c)
+            for (int c = 0; c < kCols; ++c) {
+              uint32_t k[2];
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 // the sign of nibble n is its top bit; of a 2-bit field, the upper bit of the even or the odd ones
                 const int up = 12 - 4 * (2 * i + r) + (BITS == 2 && (w & 1) == 0 ? 2 : 0);
-                k[c][r] = lop3<kAndXor>(times_power(words[c][at], up), 0x80008000u, flips[c]);
+                k[r] = lop3<kAndXor>(times_power(words[c][at], up), 0x80008000u, flips[c]);
               }
 #pragma unroll
-            for (int c = 0; c < kCols; ++c)
-#pragma unroll
-              for (int m = 0; m < MT; ++m) mma_f16(s[m][c], a[m], k[c][0], k[c][1]);
+              for (int m = 0; m < MT; ++m) mma_f16(s[m][c], a[m], k[0], k[1]);
+            }
           }
         }
       }

@@ -42,6 +42,7 @@ struct TqMultiParams {
   // What a stream costs a CTA beside its tiles (queries, first copies, merge), in tiles: 10 to 15 us.  By this number, 32 ragged rows of
   // 0.5-16 K tokens, 20 queries to a KV head: 16 182 us, 32 141, 64 135, 96 139; 16 rows of 0.4-4 K of 256 dims 100, 84, 76, 82.
   int stream_tiles;
+  int min_share;  // positions of the line that a CTA takes at least
   anna_tq_layout layout;
 };
 
@@ -73,8 +74,6 @@ __device__ __forceinline__ int64_t multi_partial_row(const MultiPartial& part, i
 }
 
 constexpr int kMultiMaxPartials = 256;  // of a stream
-constexpr int kMultiMinShare = 32;  // positions of the line
-
 // Writes the zeros of this CTA's sequences without a key and calls segment(b, kvh, tile, t0, t1, partial) for each part of its share.
 // All threads call it; `segment` ends with the CTA synchronised.
 template <typename T, int D, int THREADS, typename Fn>
@@ -93,7 +92,7 @@ __device__ __forceinline__ void multi_for_each_segment(const TqMultiParams& p, i
       multi_store<T, 4>(p, b, row / p.rows, row % p.rows, item % (D / 4) * 4, zeros);
     }
   }
-  const int share = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, kMultiMinShare),
+  const int share = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_share),
                         (max_tiles + kMultiMaxPartials - 3) / (kMultiMaxPartials - 2));
   int pos = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
   const int end = min(pos + share, total);
@@ -200,7 +199,7 @@ int tq_multi_mma_faults(int* count);  // bounded copy waits that expired on the 
 constexpr int kMultiMaxCtas = 148 * 2, kMultiScratchRows = 16;  // or half the CTAs and twice the rows
 inline int multi_ctas(const TqMultiParams& p, int row_tiles, int per_sm) {
   const int64_t line = (int64_t)p.batch * p.kv_heads * row_tiles * ((p.max_len + kBalancedTileTokens - 1) / kBalancedTileTokens + p.stream_tiles);
-  const int64_t shares = (line + kMultiMinShare - 1) / kMultiMinShare;
+  const int64_t shares = (line + p.min_share - 1) / p.min_share;
   return (int)(shares < 148 * per_sm ? shares : 148 * per_sm);
 }
 
