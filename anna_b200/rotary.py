@@ -70,8 +70,13 @@ def rotary_tables(rotary_dim: int, *, theta: float = 10000.0, sections: Sequence
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first call with new rotary parameters uploads their tables: make it outside graph capture")
     with _LOCK:
-        if len(_TABLES) >= 1024:  # parameters that change from call to call are not a model's
-            _TABLES.clear()
+        found = _TABLES.get(key)
+        if found is not None:  # another thread's
+            return found
+        # Graphs and other streams may read tables at any time, so none is given back.
+        if len(_TABLES) >= 4096:
+            raise RuntimeError("more than 4096 sets of rotary parameters: their tables stay on the device, so they are for parameters of "
+                               "models, not for some that change from call to call")
         tables = RotaryTables(axis_count=1 if sections is None else len(sections),
                               rates=torch.tensor([f / (2.0 * math.pi) for f in frequencies], dtype=torch.float64, device=device),
                               axes=torch.tensor(axes, dtype=torch.int32, device=device))
@@ -111,6 +116,27 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return begin < other_end and other_begin < end
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether ``[B, H, T, D]`` tensors of the same B and T share no element: they lie apart, or they are parts of one fused
+    projection, next to each other in every row or in every token."""
+    if not _overlap(a, b):
+        return True
+    offset, rest = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+    if rest:
+        return False
+    for outer in ((0,), (0, 2)):
+        if any(a.shape[d] > 1 and a.stride(d) != b.stride(d) for d in outer):
+            continue
+        steps = sorted((a.stride(d), a.shape[d]) for d in outer if a.shape[d] > 1)
+        if not steps or steps[0][0] <= 0 or any(step < before * size for (before, size), (step, _) in zip(steps, steps[1:])):
+            continue
+        window = steps[0][0]  # elements of one row or token, a's and b's parts among them
+        span_a, span_b = (1 + sum((x.shape[d] - 1) * x.stride(d) for d in range(4) if d not in outer) for x in (a, b))
+        if (offset >= span_a and offset + span_b <= window) or (-offset >= span_b and -offset + span_a <= window):
+            return True
+    return False
+
+
 def _output(name: str, label: str, given: torch.Tensor | None, source: torch.Tensor, others: list[torch.Tensor]) -> torch.Tensor:
     """The tensor that receives the turned ``source``: a new one, or the caller's (the source itself for in place)."""
     if given is None:
@@ -119,11 +145,15 @@ def _output(name: str, label: str, given: torch.Tensor | None, source: torch.Ten
         raise RuntimeError(f"{name}: {label} must match its input in shape, dtype and device")
     if given.stride(3) != 1 or any(size > 1 and stride <= 0 for size, stride in zip(given.shape, given.stride())):
         raise RuntimeError(f"{name}: {label} needs a contiguous last dim and memory of its own for every element")
-    steps = sorted((stride, size) for size, stride in zip(given.shape, given.stride()) if size > 1)
-    if any(step < (size_before - 1) * step_before + 1 for (step_before, size_before), (step, _) in zip(steps, steps[1:])):
-        raise RuntimeError(f"{name}: {label} needs memory of its own for every element")
-    if given.data_ptr() == source.data_ptr() and given.stride() == source.stride():
-        return given  # in place; other inputs may be views of the same fused projection
+    reach = 0  # of the dims with smaller strides
+    for stride, size in sorted((stride, size) for size, stride in zip(given.shape, given.stride()) if size > 1):
+        if stride <= reach:
+            raise RuntimeError(f"{name}: {label} needs memory of its own for every element")
+        reach += (size - 1) * stride
+    if given.data_ptr() == source.data_ptr() and given.stride() == source.stride():  # in place
+        if not all(_apart(given, other) for other in others):
+            raise RuntimeError(f"{name}: {label} is written in place and overlaps another input")
+        return given
     if any(_overlap(given, other) for other in (source, *others)):
         raise RuntimeError(f"{name}: {label} must be its input itself or lie outside the memory of the inputs")
     return given
@@ -142,6 +172,29 @@ def _check_row_starts(name: str, batch: int, positions, past_lengths, rope_delta
             raise RuntimeError(f"{name}: rope_deltas belong to positions=None")
         if rope_deltas.dtype != torch.long or tuple(rope_deltas.shape) not in ((batch,), (batch, 1)):
             raise RuntimeError(f"{name}: rope_deltas must be int64 [batch] or [batch, 1]")
+
+
+def check_rotary_arguments(name: str, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor | None,
+                           rope_deltas: torch.Tensor | None, *, theta: float = 10000.0, sections: Sequence[int] | None = None,
+                           interleaved: bool = False, rotary_dim: int | None = None,
+                           inverse_frequencies: Sequence[float] | None = None, attention_scaling: float = 1.0) -> None:
+    """Refuses what ``run_multi_axis_rotary`` and ``run_rotary_paged_kv_write`` would, and makes the tables: for callers that count
+    tokens before they launch."""
+    _check_rows(name, query, key)
+    batch, _, tokens, dim = (int(v) for v in query.shape)
+    if positions is not None or rope_deltas is not None:
+        _check_row_starts(name, batch, positions, None, rope_deltas)
+    device = _require_cuda(name, query=query, key=key, positions=positions, rope_deltas=rope_deltas)
+    width = dim if rotary_dim is None else int(rotary_dim)
+    if width > dim:
+        raise RuntimeError(f"{name}: rotary_dim {width} is larger than head_dim {dim}")
+    float(attention_scaling)
+    tables = rotary_tables(width, theta=theta, sections=sections, interleaved=interleaved, inverse_frequencies=inverse_frequencies,
+                           device=device)
+    if positions is not None:
+        _check_positions(name, positions, tables.axis_count, batch, tokens)
+    if (query.shape[1] == 0) != (key.shape[1] == 0):
+        raise RuntimeError(f"{name}: query and key need at least one head each")
 
 
 def run_multi_axis_rotary(*, query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor | None = None,
@@ -238,9 +291,12 @@ def run_rotary_paged_kv_write(*, query: torch.Tensor, key: torch.Tensor, value: 
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
         raise RuntimeError(f"{name}: page_table must be int32 [batch, max_blocks]")
     _check_row_starts(name, batch, positions, past_lengths, rope_deltas)
-    if new_lengths is not None and (new_lengths.dtype != torch.long or tuple(new_lengths.shape) != (batch,)
-                                    or not new_lengths.is_contiguous() or new_lengths.data_ptr() == past_lengths.data_ptr()):
-        raise RuntimeError(f"{name}: new_lengths must be contiguous int64 [batch] and not past_lengths itself")
+    if new_lengths is not None:
+        if new_lengths.dtype != torch.long or tuple(new_lengths.shape) != (batch,) or not new_lengths.is_contiguous():
+            raise RuntimeError(f"{name}: new_lengths must be contiguous int64 [batch]")
+        read = [x for x in (past_lengths, positions, rope_deltas) if x is not None and x.numel() > 0]
+        if batch > 0 and any(_overlap(new_lengths, x) for x in read):
+            raise RuntimeError(f"{name}: new_lengths must lie outside the memory of past_lengths, positions and rope_deltas")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise RuntimeError(f"{name}: status must be int32 [1]")
     device = _require_cuda(name, query=query, key=key, value=value, key_pages=key_pages, value_pages=value_pages,

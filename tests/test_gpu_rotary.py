@@ -263,6 +263,58 @@ def test_outputs_that_overlap_are_refused(cuda_device):
         anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions, query_out=shared, key_out=shared)
 
 
+@pytest.mark.gpu
+def test_in_place_on_parts_of_one_projection_and_on_shared_memory(cuda_device):
+    gen = torch.Generator(device=cuda_device).manual_seed(0)
+    positions = torch.arange(5, device=cuda_device)[None].expand(2, 5)
+    tokens = torch.randn(2, 5, 7 * 64, device=cuda_device, generator=gen)  # heads of a token next to each other
+    rows = torch.randn(2, 7, 5, 64, device=cuda_device, generator=gen)     # heads of a row next to each other
+    by_token = tokens.view(2, 5, 7, 64).transpose(1, 2)
+    for q, k in ((by_token[:, :4], by_token[:, 4:6]), (by_token[:, 3:], by_token[:, :2]), (rows[:, :4], rows[:, 4:6]),
+                 (rows[:, 3:], rows[:, 1:3])):
+        want = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions)
+        got = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions, query_out=q, key_out=k)
+        assert got[0] is q and got[1] is k and torch.equal(q, want[0]) and torch.equal(k, want[1])
+    for q, k in ((rows, rows), (rows[:, :4], rows[:, 3:]), (by_token[:, :4], by_token[:, 3:]), (rows[:, :, :4], rows[:, :, 1:])):
+        where = positions[:, :q.shape[2]]
+        for outs in (dict(query_out=q), dict(key_out=k), dict(query_out=q, key_out=k)):
+            with pytest.raises(RuntimeError, match="in place"):
+                anna_b200.run_multi_axis_rotary(query=q, key=k, positions=where, **outs)
+    # 2 x 2 rows of 64 dims, 64 and 65 elements apart: two of them share elements
+    woven = torch.zeros(256, device=cuda_device).as_strided((1, 2, 2, 64), (256, 65, 64, 1))
+    with pytest.raises(RuntimeError, match="query_out"):
+        anna_b200.run_multi_axis_rotary(query=woven, key=rows[:1, :1, :2], positions=positions[:1, :2], query_out=woven)
+
+
+@pytest.mark.gpu
+def test_new_lengths_that_are_read_are_refused(cuda_device):
+    q, k = torch.randn(3, 2, 1, 64, device=cuda_device), torch.randn(3, 1, 1, 64, device=cuda_device)
+    pages = [torch.zeros(4, 1, 8, 64, device=cuda_device) for _ in range(2)]
+    table = torch.arange(3, device=cuda_device, dtype=torch.int32)[:, None]
+    memory = torch.zeros(9, device=cuda_device, dtype=torch.long)
+
+    def run(**more):
+        return anna_b200.run_rotary_paged_kv_write(query=q, key=k, value=k, key_pages=pages[0], value_pages=pages[1], page_table=table,
+                                                   **more)
+
+    for more in (dict(past_lengths=memory[:3], new_lengths=memory[:3]), dict(past_lengths=memory[:3], new_lengths=memory[1:4]),
+                 dict(past_lengths=memory[:3], new_lengths=memory[4:7], positions=memory[3:6, None]),
+                 dict(past_lengths=memory[:3], new_lengths=memory[4:7], rope_deltas=memory[6:])):
+        with pytest.raises(RuntimeError, match="new_lengths"):
+            run(**more)
+    run(past_lengths=memory[:3], new_lengths=memory[3:6], positions=memory[6:, None])
+    assert memory.tolist() == [0, 0, 0, 1, 1, 1, 0, 0, 0]
+
+
+@pytest.mark.gpu
+def test_tables_are_kept_and_counted(cuda_device, monkeypatch):
+    first = rotary.rotary_tables(64, theta=123.0, device=cuda_device)
+    assert rotary.rotary_tables(64, theta=123.0, device=cuda_device) is first
+    monkeypatch.setattr(rotary, "_TABLES", {i: first for i in range(4096)})
+    with pytest.raises(RuntimeError, match="rotary parameters"):
+        rotary.rotary_tables(64, theta=124.0, device=cuda_device)
+
+
 def test_pairs_to_axes():
     for width, sections, interleaved in ((128, (16, 24, 24), False), (128, (24, 20, 20), True), (64, (11, 11, 10), True),
                                          (64, (32,), True), (8, (0, 0, 4), True), (8, (0, 4), False), (64, None, True)):
