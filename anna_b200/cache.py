@@ -29,7 +29,7 @@ from .fused_ops import MetadataUploader, dtype_code, on_device, ptr, stream_ptr
 from .page_copy import run_page_copy, run_page_gather
 from .pools import Qwen3PagedLayerAllocator, TurboQuantLayerPool, native_page_ids
 from .prefix_block_cache import PrefixBlockPool
-from .rotary import run_multi_axis_rotary, run_rotary_paged_kv_write
+from .rotary import check_rotary_arguments, run_multi_axis_rotary, run_rotary_paged_kv_write
 from .turboquant import (VALID_KV_CACHE_QUANT_BITS, TurboQuantKVRow, launch_tq_append, launch_tq_decode,
                          launch_tq_gather_dense, launch_tq_multi_decode)
 
@@ -142,12 +142,15 @@ class Qwen3PageAllocator:
         released = 0
         for layer_idx, (plain_ids, packed_ids, plain, rows) in enumerate(plans):
             layer, pool = self.layers[layer_idx], self.turboquant_layers[layer_idx]
+            # a pool that cannot be copied (memory) leaves everything as it is then: ids change right behind their pool
             released += layer.compact(plain_ids, spare_pages)
-            released += pool.compact(packed_ids, rows, spare_pages)
-            self.prefix_block_pool.move_pages(layer_idx, plain_ids)
-            self.packed_prefix_block_pool.move_pages(layer_idx, packed_ids)
             for table in plain:
                 table[:] = [plain_ids[page_id] for page_id in table]
+            self.prefix_block_pool.move_pages(layer_idx, plain_ids)
+            for cache in caches:
+                cache._forget_device_tables(layer_idx)
+            released += pool.compact(packed_ids, rows, spare_pages)
+            self.packed_prefix_block_pool.move_pages(layer_idx, packed_ids)
             for cache in caches:
                 cache._forget_device_tables(layer_idx)
         return released
@@ -533,6 +536,9 @@ class Qwen3DynamicCache:
         deltas = None
         if positions is None and self.rope_deltas is not None:
             deltas = self.rope_deltas.to(device=key_states.device, dtype=torch.long).reshape(batch_size)
+        # before tokens are counted and pages taken for them
+        check_rotary_arguments("update_rotary", query_states, key_states, positions, deltas, **rotary)
+        self._check_pool_geometry(key_states, value_states, layer_idx)
         pending = _PendingRotary(query_states, positions, deltas, rotary)
         if self.uses_turboquant_for_layer(layer_idx):
             self._ensure_batch_size(batch_size)
@@ -541,6 +547,18 @@ class Qwen3DynamicCache:
         else:
             dense = self._update_paged_layer(key_states, value_states, layer_idx, require_dense_cache, pending)
         return (pending.query, *dense)
+
+    def _check_pool_geometry(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
+        """Keys and values that the layer's pages, where it has some, can take."""
+        if value_states.dtype != key_states.dtype or value_states.device != key_states.device:
+            raise ValueError("keys and values must share dtype and device")
+        if self.uses_turboquant_for_layer(layer_idx):
+            return  # the append compares before it counts
+        pages = self.allocator.layers[layer_idx].key_pages
+        if pages is not None and (pages.shape[1] != key_states.shape[1] or pages.shape[3] != key_states.shape[3]
+                                  or pages.dtype != key_states.dtype or pages.device != key_states.device):
+            raise ValueError(f"the pages of layer {layer_idx} are {list(pages.shape)} {pages.dtype} on {pages.device}, the keys "
+                             f"{list(key_states.shape)} {key_states.dtype} on {key_states.device}")
 
     def _past_lengths_on_device(self, layer_idx: int, device: torch.device) -> torch.Tensor:
         past = list(self.layer_lengths[layer_idx])
@@ -1268,7 +1286,19 @@ class Qwen3DynamicCache:
         if self.rope_deltas is not None:
             index = torch.tensor(rows, device=self.rope_deltas.device, dtype=torch.long)
             forked.rope_deltas = self.rope_deltas.index_select(0, index)
-        copies: list[tuple[int, str, list[int], list[int]]] = []  # (layer, which pool, sources, targets)
+        try:
+            copies = self._fork_into(forked, rows)
+            if copies:
+                run_page_copy(copies=copies)
+        except BaseException:
+            forked.release()  # pages taken so far
+            raise
+        forked.seen_tokens = max((forked._request_seq_length(idx) for idx in range(len(rows))), default=0)
+        return forked
+
+    def _fork_into(self, forked: "Qwen3DynamicCache", rows: list[int]) -> list[tuple[torch.Tensor, list[int], list[int]]]:
+        """Gives the rows of ``forked`` their pages and rings; the (pool, sources, targets) that are to be copied."""
+        work: list[tuple[object, str, list[int], list[int]]] = []  # (owner of the pool, its name, sources, targets)
         for layer_idx in range(self.config.num_hidden_layers):
             forked.layer_lengths[layer_idx] = [self.layer_lengths[layer_idx][idx] for idx in rows]
             for name in ("conv_states", "recurrent_states"):
@@ -1279,6 +1309,7 @@ class Qwen3DynamicCache:
             sources: list[int] = []
             targets: list[int] = []
             if self.uses_turboquant_for_layer(layer_idx):
+                pool = self.allocator.turboquant_layers[layer_idx]
                 old_slots: list[int] = []
                 new_slots: list[int] = []
                 for new_idx, old_idx in enumerate(rows):
@@ -1293,35 +1324,24 @@ class Qwen3DynamicCache:
                     if fork.initialized and row.length > 0:
                         old_slots.append(row.slot)
                         new_slots.append(fork.slot)
-                copies.append((layer_idx, "window", old_slots, new_slots))
-                copies.append((layer_idx, "packed_pages", sources, targets))
+                work += [(pool, "window", old_slots, new_slots), (pool, "packed_pages", sources, targets)]
                 continue
             layer = self.allocator.layers[layer_idx]
             for new_idx, old_idx in enumerate(rows):
                 length = self.layer_lengths[layer_idx][old_idx]
                 table = self.page_tables[layer_idx][old_idx]
+                own = forked.page_tables[layer_idx][new_idx]
                 full = length // self.block_size
-                own = list(table[:full])
-                for page_id in own:
+                for page_id in table[:full]:
                     self.allocator.retain_shared_page(layer_idx, page_id)
+                    own.append(page_id)
                 if length % self.block_size:
-                    private = self.allocator.allocate(layer_idx, 1, key_template=layer.key_pages, value_template=layer.value_pages)[0]
+                    own += self.allocator.allocate(layer_idx, 1, key_template=layer.key_pages, value_template=layer.value_pages)
                     sources.append(table[full])
-                    targets.append(private)
-                    own.append(private)
-                forked.page_tables[layer_idx][new_idx] = own
-            # this cache's rows may share pages now, and the pools may have moved
-            copies.append((layer_idx, "key_pages", sources, targets))
-            copies.append((layer_idx, "value_pages", sources, targets))
-        forked.seen_tokens = max((forked._request_seq_length(idx) for idx in range(len(rows))), default=0)
-        work = []
-        for layer_idx, name, sources, targets in copies:  # pools may have grown meanwhile
-            if sources:
-                owner = self.allocator.turboquant_layers if name in ("window", "packed_pages") else self.allocator.layers
-                work.append((getattr(owner[layer_idx], name), sources, targets))
-        if work:
-            run_page_copy(copies=work)
-        return forked
+                    targets.append(own[-1])
+            work += [(layer, "key_pages", sources, targets), (layer, "value_pages", sources, targets)]
+        # allocations may have moved the pools
+        return [(getattr(owner, name), sources, targets) for owner, name, sources, targets in work if sources]
 
     def _forget_device_tables(self, layer_idx: int) -> None:
         """The layer's pages have other ids: tables are built and uploaded again."""

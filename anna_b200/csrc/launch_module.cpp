@@ -968,7 +968,13 @@ PyObject* rotary_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!row_starts(positions, past, deltas, device, batch)) Py_RETURN_NONE;
   if (fresh != nullptr && (!plain(*fresh, device, 1) || fresh->scalar_type() != at::kLong || fresh->size(0) != batch || !fresh->is_contiguous()))
     Py_RETURN_NONE;
-  if (fresh != nullptr && fresh->data_ptr() == past->data_ptr()) Py_RETURN_NONE;
+  if (fresh != nullptr) {  // memory that the call reads and writes
+    const uintptr_t to = reinterpret_cast<uintptr_t>(fresh->data_ptr()), from = reinterpret_cast<uintptr_t>(past->data_ptr());
+    const uintptr_t bytes = (uintptr_t)batch * 8;
+    if (to < from + bytes && from < to + bytes) Py_RETURN_NONE;
+    for (const at::Tensor* x : {positions, deltas})
+      if (x != nullptr && x->storage().data_ptr().get() == fresh->storage().data_ptr().get()) Py_RETURN_NONE;
+  }
   if (word != nullptr && (word->device() != device || word->scalar_type() != at::kInt || word->numel() != 1)) Py_RETURN_NONE;
   int64_t ps[3] = {0, 0, 0};
   if (positions != nullptr && !position_strides(*positions, device, n[0], batch, tokens, ps)) Py_RETURN_NONE;
@@ -1052,6 +1058,7 @@ PyObject* page_copy(PyObject*, PyObject* copies) {
         Py_RETURN_NONE;
       made.count = (int64_t)source.size();
       if (made.first + made.count >= INT32_MAX) Py_RETURN_NONE;
+      if (made.highest_source >= pool->size(0) || made.highest_target >= pool->size(0)) Py_RETURN_NONE;
       marks.assign((size_t)std::max(made.highest_source, made.highest_target) + 1, 0);
       for (const int32_t id : target)
         if (marks[(size_t)id]++ != 0) Py_RETURN_NONE;  // a target twice

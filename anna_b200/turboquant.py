@@ -162,6 +162,8 @@ def launch_tq_multi_decode(pool: TurboQuantLayerPool, query_states: torch.Tensor
     _require_cuda(query_states, "TurboQuant decode")
     if query_states.dtype != pool.dtype:
         raise RuntimeError(f"query dtype {query_states.dtype} must match the cache dtype {pool.dtype}")
+    if query_states.device != pool.device or (gate is not None and gate.device != pool.device):
+        raise RuntimeError(f"TurboQuant decode: query and gate must be on the cache's device {pool.device}")
     tables = pool.tables
     out = launch_module().tq_multi_decode(query_states, gate, pool.packed_pages, table_dev, pool.window, slots_dev, lengths_dev,
                                           tables.signs1, tables.signs2, tables.centroids, scaling, pool.bits, pool.residual_len,
@@ -598,15 +600,17 @@ class TurboQuantKVRow:
         assert pool is not None
         fork._attach(pool)
         full = self.quantized_length // pool.block_size
-        blocks = list(self._blocks[:full])
-        for page_id in blocks:
-            pool.retain_page(page_id)
-        pages = None
+        pages, private = None, []
         if self.quantized_length % pool.block_size:
-            private = pool.allocate(1)[0]
-            pages = (self._blocks[full], private)
-            blocks.append(private)
-        fork.block_table = blocks
+            try:
+                private = pool.allocate(1)
+            except BaseException:
+                fork.release()
+                raise
+            pages = (self._blocks[full], private[0])
+        for page_id in self._blocks[:full]:
+            pool.retain_page(page_id)
+        fork.block_table = list(self._blocks[:full]) + private
         fork._length = self._length
         return fork, pages
 

@@ -124,6 +124,27 @@ def test_forks_of_forks_of_clones_and_empty_rows(cuda_device, mode):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("mode", ["none", "turboquant"])
+def test_a_fork_that_fails_keeps_no_pages(cuda_device, mode, monkeypatch):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    cache = new_cache(2, mode)
+    append(cache, states(gen, 2, 61, KV_HEADS), states(gen, 2, 61, KV_HEADS))
+    before, held = views(cache), pages_in_use(cache)
+
+    def fails(**_):
+        raise RuntimeError("no copy")
+
+    with monkeypatch.context() as patch:
+        patch.setattr("anna_b200.cache.run_page_copy", fails)
+        with pytest.raises(RuntimeError, match="no copy"):
+            cache.fork_rows([0, 1, 1])
+    assert pages_in_use(cache) == held
+    assert_same(views(cache), before)
+    cache.fork_rows([1, 0]).release()
+    assert pages_in_use(cache) == held
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["none", "turboquant"])
 @pytest.mark.parametrize("spare", [0, 5])
 def test_compaction_keeps_every_row(cuda_device, mode, spare):
     gen = torch.Generator(device="cuda").manual_seed(6)
@@ -288,6 +309,69 @@ def test_a_request_with_images_drafts_and_candidates(cuda_device, dtype, page):
             assert_same(views(cache), after)
     cache.release()
     assert pages_in_use(cache) == [0] * 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["none", "turboquant"])
+def test_a_refused_append_leaves_the_cache_alone(cuda_device, mode):
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    cache = new_cache(2, mode)
+    append(cache, states(gen, 2, 31, KV_HEADS), states(gen, 2, 31, KV_HEADS))
+    before, held = views(cache), pages_in_use(cache)
+    q, k = states(gen, 2, 5, HEADS), states(gen, 2, 5, KV_HEADS)
+    positions = torch.zeros(3, 2, 5, dtype=torch.long, device="cuda")
+    for bad in (dict(positions=positions[:, :, :4]), dict(positions=positions.int()), dict(positions=positions[:2]),
+                dict(rotary_dim=DIM + 2), dict(rotary_dim=31, sections=None), dict(sections=(1, 2, 3)), dict(theta=-1.0),
+                dict(positions=positions.cpu())):
+        with pytest.raises((RuntimeError, ValueError)):
+            cache.update_rotary(q, k, k, 0, **{**ROTARY, **bad})
+    for k2 in (k[:, :1], k[..., :64], k.float()):
+        q2 = q[..., :k2.shape[-1]].to(k2.dtype)
+        with pytest.raises((RuntimeError, ValueError)):
+            cache.update_rotary(q2, k2, k2, 0)
+    with pytest.raises((RuntimeError, ValueError)):
+        cache.update_rotary(q, k, k.half(), 0, **ROTARY)
+    assert cache.layer_lengths == [[31, 31], [31, 31]] and pages_in_use(cache) == held
+    assert_same(views(cache), before)
+    cache.update_rotary(q, k, k, 0, **ROTARY)
+    assert cache.layer_lengths[0] == [36, 36]
+
+
+@pytest.mark.gpu
+def test_a_compaction_that_runs_out_of_memory_keeps_every_row(cuda_device, monkeypatch):
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    allocator = Qwen3PageAllocator(KVCacheConfig(num_hidden_layers=2, cache_block_size=16))
+    caches = [new_cache(2, mode, allocator=allocator) for mode in ("none", "turboquant", "none", "turboquant")]
+    for cache in caches:
+        append(cache, states(gen, 2, 77, KV_HEADS), states(gen, 2, 77, KV_HEADS))
+    for cache in caches[:2]:
+        cache.release()
+    caches = caches[2:]
+    before, gather = [views(cache) for cache in caches], anna_b200.page_copy.run_page_gather
+    for works in range(6):  # two layers, each with un-quantized pages, packed pages and rings
+        left = [works]
+
+        def some(**arguments):
+            if left[0] == 0:
+                raise torch.cuda.OutOfMemoryError("no room")
+            left[0] -= 1
+            return gather(**arguments)
+
+        with monkeypatch.context() as patch:
+            patch.setattr("anna_b200.page_copy.run_page_gather", some)
+            try:
+                allocator.compact(caches)
+            except torch.cuda.OutOfMemoryError:
+                pass
+        for cache, want in zip(caches, before):
+            assert_same(views(cache), want)
+    for cache in caches:
+        append(cache, states(gen, 2, 40, KV_HEADS), states(gen, 2, 40, KV_HEADS))
+    for cache, want in zip(caches, before):
+        for new, old in zip(views(cache), want, strict=True):
+            for (k, v), (k0, v0) in zip(new, old, strict=True):
+                if cache.kv_cache_quantization == "none":
+                    assert torch.equal(k[:, :77], k0) and torch.equal(v[:, :77], v0)
 
 
 @pytest.mark.gpu

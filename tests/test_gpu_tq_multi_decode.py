@@ -285,6 +285,9 @@ def test_strides_alignment_and_types_of_query_and_gate(cuda_device, dtype, dim):
     last = torch.zeros(*q.shape, 2, device=cuda_device, dtype=q.dtype)
     last[..., 0] = q
     assert torch.equal(case.run(query=last[..., 0]), want)
+    one = Case(lengths=[99], tokens=2, group=1, kv_heads=1, dim=dim, bits=4, page=16, window=16, dtype=dtype, device=cuda_device, seed=3)
+    q1, want1 = one.query.to(cuda_device), one.run()
+    assert torch.equal(one.run(query=q1.as_strided(q1.shape, (3, 5, dim, 1))), want1)  # dims of one entry have any stride
     stretched = q[:1, :1].expand(q.shape)
     got = case.run(query=stretched)
     assert torch.equal(got, case.run(query=stretched.contiguous()))
