@@ -363,6 +363,7 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
   const bool tensor_cores = tq_multi_mma_applicable(p, head_dim, dtype);
   p.stream_tiles = !tensor_cores ? 4 : head_dim == 128 && p.rows <= 16 ? 32 : 64;
   p.min_share = tensor_cores ? 32 : 4;
+  p.whole_tiles = tensor_cores ? 48 : 0;
   // The line of a launch has room for so many rows and positions: larger batches go in several, one behind the other.
   const int64_t row_positions = (int64_t)kv_heads * row_tiles * ((p.max_len + kBalancedTileTokens - 1) / kBalancedTileTokens + p.stream_tiles);
   ANNA_REQUIRE(row_positions < (1ll << 30), "%s: too many queries and keys of one sequence", what);

@@ -210,33 +210,37 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
     for (int i = 0; i < kRingStages; ++i) mbar_init(bars + 8 * i, 1);
     mbar_init_fence();
   }
-  // The centroids are rounded to fp16 at the scale, of 512 between 1 and 2, that leaves the smallest squared error over the codebook:
-  // as they are, their rounding was the largest error of an fp16 cache's output.
+  // The centroids are rounded to fp16; for an fp16 cache at the scale, of 512 between 1 and 2, that leaves the smallest squared error
+  // over the codebook: as they are, their rounding was the largest error of its output.  A bf16 output hides it, and the search costs
+  // 2 % of a long call (verification of 4 tokens over 16 rows of 32768: 259 -> 256 us without it).
   constexpr int kCentroids = 1 << (BITS - 1);
   float cent[kCentroids];
 #pragma unroll
   for (int e = 0; e < kCentroids; ++e) cent[e] = __ldg(p.centroids + e);
-  auto scale_of = [](uint32_t j) { return 1.0f + (float)j * (1.0f / 512.0f); };
-  uint32_t best = 0xffffffffu;  // error (its lowest bits left out), number of the scale
+  float cent_scale = 1.0f;
+  if constexpr (std::is_same_v<T, __half>) {
+    auto scale_of = [](uint32_t j) { return 1.0f + (float)j * (1.0f / 512.0f); };
+    uint32_t best = 0xffffffffu;  // error (its lowest bits left out), number of the scale
 #pragma unroll
-  for (int i = 0; i < 512 / kMultiMmaThreads; ++i) {
-    const uint32_t j = i * kMultiMmaThreads + threadIdx.x;
-    float error = 0.0f;
+    for (int i = 0; i < 512 / kMultiMmaThreads; ++i) {
+      const uint32_t j = i * kMultiMmaThreads + threadIdx.x;
+      float error = 0.0f;
 #pragma unroll
-    for (int e = 0; e < kCentroids; ++e) {
-      const float x = cent[e] * scale_of(j), d = x - __half2float(__float2half_rn(x));
-      error = fmaf(d, d, error);
+      for (int e = 0; e < kCentroids; ++e) {
+        const float x = cent[e] * scale_of(j), d = x - __half2float(__float2half_rn(x));
+        error = fmaf(d, d, error);
+      }
+      error /= scale_of(j) * scale_of(j);
+      best = min(best, (__float_as_uint(error) & ~511u) | j);
     }
-    error /= scale_of(j) * scale_of(j);
-    best = min(best, (__float_as_uint(error) & ~511u) | j);
-  }
-  best = __reduce_min_sync(0xffffffffu, best);
-  uint32_t* best_of = reinterpret_cast<uint32_t*>(smem + Cfg::kOffStats);
-  if (lane == 0) best_of[warp] = best;
-  __syncthreads();
+    best = __reduce_min_sync(0xffffffffu, best);
+    uint32_t* best_of = reinterpret_cast<uint32_t*>(smem + Cfg::kOffStats);
+    if (lane == 0) best_of[warp] = best;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kMultiMmaWarps; ++w) best = min(best, best_of[w]);
-  const float cent_scale = scale_of(best & 511u);
+    for (int w = 0; w < kMultiMmaWarps; ++w) best = min(best, best_of[w]);
+    cent_scale = scale_of(best & 511u);
+  }
   // tables of the centroids' low and high bytes
   uint32_t lut_lo[2] = {0u, 0u}, lut_hi[2] = {0u, 0u};
 #pragma unroll

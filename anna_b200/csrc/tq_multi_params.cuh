@@ -43,6 +43,7 @@ struct TqMultiParams {
   // 0.5-16 K tokens, 20 queries to a KV head: 16 182 us, 32 141, 64 135, 96 139; 16 rows of 0.4-4 K of 256 dims 100, 84, 76, 82.
   int stream_tiles;
   int min_share;  // positions of the line that a CTA takes at least
+  int whole_tiles;  // streams of no more tiles, a CTA for each, are not cut: see multi_for_each_segment
   anna_tq_layout layout;
 };
 
@@ -92,29 +93,34 @@ __device__ __forceinline__ void multi_for_each_segment(const TqMultiParams& p, i
       multi_store<T, 4>(p, b, row / p.rows, row % p.rows, item % (D / 4) * 4, zeros);
     }
   }
-  const int share = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_share),
-                        (max_tiles + kMultiMaxPartials - 3) / (kMultiMaxPartials - 2));
-  int pos = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
-  const int end = min(pos + share, total);
+  // Streams of few tiles with a CTA for each are not cut: what a CTA less has to do does not pay for the merge (16 rows of 300-500
+  // tokens of 256 dims, 64 queries to a KV head: 41 us, 26 so).
+  const bool whole = max_tiles <= p.whole_tiles && p.batch * streams_per_row <= (int)gridDim.x;
+  const int share = whole ? 0 : max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_share),
+                                    (max_tiles + kMultiMaxPartials - 3) / (kMultiMaxPartials - 2));
+  int pos = whole ? 0 : (int)min((int64_t)blockIdx.x * share, (int64_t)total);
+  const int end = whole ? (int)blockIdx.x < p.batch * streams_per_row ? 1 : 0 : min(pos + share, total);
   if (pos >= end) return;
   int b = 0, hi = p.batch;  // s_prefix[b] <= pos < s_prefix[hi]
-  while (hi - b > 1) {
+  if (whole) b = blockIdx.x / streams_per_row;
+  while (!whole && hi - b > 1) {
     const int mid = (b + hi) >> 1;
     if (s_prefix[mid] <= pos) b = mid;
     else hi = mid;
   }
   while (pos < end) {
-    while (s_prefix[b + 1] <= pos) ++b;
+    while (share != 0 && s_prefix[b + 1] <= pos) ++b;
     const int len = (int)max((int64_t)0, min(p.lengths[b], p.max_len));
     const int n = (len + kBalancedTileTokens - 1) / kBalancedTileTokens + p.stream_tiles;
-    const int stream = (pos - s_prefix[b]) / n, at = (pos - s_prefix[b]) - stream * n;
-    const int stop = min(n, at + end - pos);
+    const int stream = share == 0 ? (int)blockIdx.x - b * streams_per_row : (pos - s_prefix[b]) / n;
+    const int at = share == 0 ? 0 : pos - s_prefix[b] - stream * n;
+    const int stop = share == 0 ? n : min(n, at + end - pos);
     if (stop > p.stream_tiles) {
       const int begin = s_prefix[b] + stream * n;
-      const int first = (begin + p.stream_tiles) / share;
+      const int first = share == 0 ? 0 : (begin + p.stream_tiles) / share;
       segment(b, stream / row_tiles, stream % row_tiles, max(0, at - p.stream_tiles) * kBalancedTileTokens,
               min(len, (stop - p.stream_tiles) * kBalancedTileTokens),
-              MultiPartial{first, (begin + n - 1) / share - first + 1, (int)blockIdx.x - first});
+              MultiPartial{first, share == 0 ? 1 : (begin + n - 1) / share - first + 1, (int)blockIdx.x - first});
     }
     pos += stop - at;
   }
