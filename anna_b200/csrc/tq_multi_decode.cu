@@ -5,7 +5,8 @@
 //   q . k_hat = norm / D * [ fwht(s1*q) . centroid[idx] + sqrt(pi/2)/sqrt(D) * rnorm * fwht(s2*fwht(s1*q)) . (2*sign-1) ]
 // so a CTA rotates its rows once and no key is taken back to the original basis.
 //
-// This form serves fp32 caches, head_dim 64 and pages that are no multiple of 16 tokens; everything in it is 32 bits.  A CTA of
+// This form serves fp32 caches, head_dim 64, pages that are no multiple of 8 tokens and value groups other than 32; everything in it
+// is 32 bits.  A CTA of
 // 128 threads de-quantizes 32 tokens at a time into shared memory for its 8 rows.  Bound: FMA issue (3 D operations per row and
 // key, of which the shared-memory reads of the keys are shared by two rows).
 #include "tq_multi_params.cuh"

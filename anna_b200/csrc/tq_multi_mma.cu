@@ -54,8 +54,8 @@ struct MultiCfg {
   static constexpr int kWork = kRing + kQuery > kMerge ? kRing + kQuery : kMerge;
   static_assert(kWork >= kRows * kMultiMaxPartials * 4, "the weights of the partials lie there, too");
   static constexpr int kOffBars = kWork;                                  // mbarriers [warps][stages]
-  static constexpr int kOffValid = kOffBars + kMultiMmaWarps * kRingStages * 8;  // tokens per tile [warps][stages][tiles]
-  static constexpr int kOffFactor = kOffValid + kMultiMmaWarps * kRingStages * kStepTiles * 4;  // f_row [rows]
+  static constexpr int kOffValid = kOffBars + kMultiMmaWarps * kRingStages * 8;  // tokens of the pieces [warps][stages][tiles or halves]
+  static constexpr int kOffFactor = kOffValid + kMultiMmaWarps * kRingStages * kStepTiles * 8;  // f_row [rows]
   static constexpr int kOffLimit = kOffFactor + kRows * 4;                // newest key that the row sees [rows]
   static constexpr int kOffStats = kOffLimit + kRows * 4;                 // m, l of the warps [warps][rows][2]
   static constexpr int kOffStrange = kOffStats + kMultiMmaWarps * kRows * 8;  // see strange_values
@@ -189,7 +189,7 @@ __device__ __forceinline__ FragSlot sign_slot(int c) {
   return {2 * word + i % 4 / 2, tig, i % 2, i / 4};
 }
 
-template <typename T, int D, int BITS, int MT>
+template <typename T, int D, int BITS, int MT, bool HALVED>
 __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas)
     tq_multi_mma_kernel(const TqMultiParams p, int row_tiles) {
   using Cfg = MultiCfg<D, BITS, MT>;
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   uint8_t* ring = smem + warp * Cfg::kWarpRing;
   const uint32_t bars = smem_u32(smem + Cfg::kOffBars) + warp * kRingStages * 8;
-  volatile int* ring_valid = reinterpret_cast<volatile int*>(smem + Cfg::kOffValid) + warp * kRingStages * kStepTiles;
+  volatile int* ring_valid = reinterpret_cast<volatile int*>(smem + Cfg::kOffValid) + warp * kRingStages * kStepTiles * 2;
   int* strange = reinterpret_cast<int*>(smem + Cfg::kOffStrange);
   if (lane == 0) {
 #pragma unroll
@@ -266,52 +266,63 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
   const int steps = (tiles + kStepTiles - 1) / kStepTiles;
   const int my_steps = steps > warp && !dead ? (steps - warp + kMultiMmaWarps - 1) / kMultiMmaWarps : 0;
   const int32_t* table = p.block_table + (int64_t)b * p.table_stride;
-  // Page ids of the warp's next 16 steps, a tile a lane, and those of the 16 behind them: a step that looks up its own waits for the
-  // table before it can ask for the tile.
+  // A piece is a run of tokens of one page: a tile, or half a tile where a page is no multiple of 16 tokens.
+  // (Decided at run time, 16 rows of 32768 tokens took 264 us instead of 261.)
+  constexpr int halved = HALVED ? 1 : 0, piece_tokens = kTile >> halved, group_steps = 16 >> halved;  // steps whose pieces are 32
+  const int piece = lane & ((kStepTiles << halved) - 1);                                               // the lane's piece of a step
+  // Page ids of the warp's next 32 pieces, one a lane, and those of the 32 behind them: a step that looks up its own waits for the table
+  // before it can ask for the tokens.
   auto ids_of = [&](int group) {
-    const int ts = t0 + (((group * 16 + lane / 2) * kMultiMmaWarps + warp) * kStepTiles + (lane & 1)) * kTile;
+    const int step = group * group_steps + (lane >> (1 + halved));
+    const int ts = t0 + (step * kMultiMmaWarps + warp) * kStepTiles * kTile + piece * piece_tokens;
     if (ts >= q_end) return -1;
     const int blk = p.block_shift >= 0 ? ts >> p.block_shift : ts / p.block_size;
     return blk < p.max_blocks ? table[blk] : -1;
   };
   int32_t ids = ids_of(0), ids_next = ids_of(1);
-  // A tile of a 16-token page is one run of bytes, of a larger page six (codes, norms, residual norms, value codes, scales, zeros).
-  // Lanes 0 and 1 copy a tile each; lane 0 arms the barrier with the bytes of both.
+  // A tile of a 16-token page is one run of bytes, other pieces are six (codes, norms, residual norms, value codes, scales, zeros).
+  // The first lanes copy a piece each; lane 0 arms the barrier with the bytes of all.
   auto issue = [&](int step, int stage) {
-    if (step % 16 == 0 && step > 0) {
+    const int in_group = step & (group_steps - 1);
+    if (in_group == 0 && step > 0) {
       ids = ids_next;
-      ids_next = ids_of(step / 16 + 1);
+      ids_next = ids_of(step / group_steps + 1);
     }
-    const int32_t pid = __shfl_sync(0xffffffffu, ids, 2 * (step % 16) + (lane & 1));
+    const int32_t pid = __shfl_sync(0xffffffffu, ids, (in_group << (1 + halved)) + piece);
     int valid = 0, at = 0;
     const uint8_t* page = nullptr;
-    if (lane < kStepTiles) {
-      const int ts = t0 + ((step * kMultiMmaWarps + warp) * kStepTiles + lane) * kTile;
+    const bool copies = lane < kStepTiles << halved;
+    if (copies) {
+      const int ts = t0 + (step * kMultiMmaWarps + warp) * kStepTiles * kTile + piece * piece_tokens;
       if (pid >= 0 && pid < p.num_pages) {  // else a hole, or behind the end: nothing to copy
-        valid = min(kTile, q_end - ts);
+        valid = min(piece_tokens, q_end - ts);
         at = p.block_size == kTile ? 0 : p.block_shift >= 0 ? ts & (p.block_size - 1) : ts % p.block_size;
         page = p.pages + ((int64_t)pid * p.kv_heads + kvh) * p.layout.chunk_bytes;
       }
-      ring_valid[stage * kStepTiles + lane] = valid;
+      ring_valid[stage * (kStepTiles << halved) + lane] = valid;
     }
     const uint32_t bar = bars + 8 * stage;
     const unsigned have = __ballot_sync(0xffffffffu, valid > 0);
     if (lane == 0) {
-      if (have != 0u) mbar_expect_tx(bar, (uint32_t)__popc(have) * Cfg::kTileBytes);
+      if (have != 0u) mbar_expect_tx(bar, (uint32_t)__popc(have) * (Cfg::kTileBytes >> halved));
       else mbar_arrive(bar);  // the phase completes at once
     }
     __syncwarp();
     if (valid > 0) {
-      const uint32_t dst = smem_u32(ring + (stage * kStepTiles + lane) * Cfg::kTileStride);
+      const uint32_t dst = smem_u32(ring + (stage * kStepTiles + (lane >> halved)) * Cfg::kTileStride);
       if (p.block_size == kTile) {
         bulk_copy_g2s(dst, page, Cfg::kTileBytes, bar);
       } else {
-        bulk_copy_g2s(dst, page + p.layout.off_kcodes + at * Cfg::kKeyBytes, kTile * Cfg::kKeyBytes, bar);
-        bulk_copy_g2s(dst + Cfg::kOffNorm, page + p.layout.off_knorm + 4 * at, 4 * kTile, bar);
-        bulk_copy_g2s(dst + Cfg::kOffRnorm, page + p.layout.off_krnorm + 4 * at, 4 * kTile, bar);
-        bulk_copy_g2s(dst + Cfg::kOffVal, page + p.layout.off_vdata + at * Cfg::kValBytes, kTile * Cfg::kValBytes, bar);
-        bulk_copy_g2s(dst + Cfg::kOffScale, page + p.layout.off_vscale + at * Cfg::kGroups * 2, kTile * Cfg::kGroups * 2, bar);
-        bulk_copy_g2s(dst + Cfg::kOffZero, page + p.layout.off_vzero + at * Cfg::kGroups * 2, kTile * Cfg::kGroups * 2, bar);
+        const int to = (lane & halved) * piece_tokens;
+        bulk_copy_g2s(dst + to * Cfg::kKeyBytes, page + p.layout.off_kcodes + at * Cfg::kKeyBytes, piece_tokens * Cfg::kKeyBytes, bar);
+        bulk_copy_g2s(dst + Cfg::kOffNorm + 4 * to, page + p.layout.off_knorm + 4 * at, 4 * piece_tokens, bar);
+        bulk_copy_g2s(dst + Cfg::kOffRnorm + 4 * to, page + p.layout.off_krnorm + 4 * at, 4 * piece_tokens, bar);
+        bulk_copy_g2s(dst + Cfg::kOffVal + to * Cfg::kValBytes, page + p.layout.off_vdata + at * Cfg::kValBytes,
+                      piece_tokens * Cfg::kValBytes, bar);
+        bulk_copy_g2s(dst + Cfg::kOffScale + to * Cfg::kGroups * 2, page + p.layout.off_vscale + at * Cfg::kGroups * 2,
+                      piece_tokens * Cfg::kGroups * 2, bar);
+        bulk_copy_g2s(dst + Cfg::kOffZero + to * Cfg::kGroups * 2, page + p.layout.off_vzero + at * Cfg::kGroups * 2,
+                      piece_tokens * Cfg::kGroups * 2, bar);
       }
     }
   };
@@ -456,12 +467,15 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
       break;
     }
     const uint8_t* st = ring + stage * kStepTiles * Cfg::kTileStride;
-    int valid[kStepTiles], total = 0;
+    constexpr int kPieces = kStepTiles << halved;
+    int valid[kPieces], total = 0;
 #pragma unroll
-    for (int u = 0; u < kStepTiles; ++u) {
-      valid[u] = ring_valid[stage * kStepTiles + u];
-      total += valid[u];
+    for (int i = 0; i < kPieces; ++i) {
+      valid[i] = ring_valid[stage * kPieces + i];
+      total += valid[i];
     }
+    // tokens of column c, eight of a tile, that are there
+    auto there = [&](int c) { return HALVED ? valid[c % kPieces] : valid[c / 2] - 8 * (c & 1); };
     if (++stage == kRingStages) { stage = 0; phase ^= 1u; }
     if (total == 0) continue;  // holes only
     const int ts = t0 + (n * kMultiMmaWarps + warp) * kStepTiles * kTile;
@@ -577,8 +591,8 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int in_tile = 8 * (c & 1) + ((r & 1) ? tok_b : tok_a);
-            if (in_tile >= valid[c / 2] || ts + c / 2 * kTile + in_tile > row_limit[16 * m + gid + 8 * (r / 2)]) s[m][c][r] = -INFINITY;
+            const int t = (r & 1) ? tok_b : tok_a;
+            if (t >= there(c) || ts + 8 * c + t > row_limit[16 * m + gid + 8 * (r / 2)]) s[m][c][r] = -INFINITY;
           }
     }
     softmax(s, std::integral_constant<int, kCols>{});
@@ -603,8 +617,8 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
         float sa = ElemTraits<T>::to_float(scales[ta * Cfg::kGroups]), sb = ElemTraits<T>::to_float(scales[tb * Cfg::kGroups]);
         float za = ElemTraits<T>::to_float(zeros[ta * Cfg::kGroups]), zb = ElemTraits<T>::to_float(zeros[tb * Cfg::kGroups]);
         if (!full) {  // the bytes of tokens that are not there may be anything
-          if (ta >= valid[u]) sa = za = 0.0f;
-          if (tb >= valid[u]) sb = zb = 0.0f;
+          if (tok_a >= there(2 * u + i)) sa = za = 0.0f;
+          if (tok_b >= there(2 * u + i)) sb = zb = 0.0f;
         }
         if (cut) {
           if (!finite_f16(fabsf(za) + kBase * fabsf(sa))) { sa = za = 0.0f; *strange = 1; }
@@ -876,31 +890,37 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
 }
 
 bool tq_multi_mma_applicable(const TqMultiParams& p, int head_dim, int dtype) {
-  if (dtype == ANNA_DTYPE_F32 || (head_dim != 128 && head_dim != 256) || p.value_group != 32 || p.block_size % kTile != 0) return false;
+  if (dtype == ANNA_DTYPE_F32 || (head_dim != 128 && head_dim != 256) || p.value_group != 32 || p.block_size % 8 != 0) return false;
   // the window product reads queries 16 bytes at a time
   return aligned_to(p.q, 16) && p.q_stride_b % 8 == 0 && p.q_stride_h % 8 == 0 && p.q_stride_t % 8 == 0 && p.max_len < (1ll << 30);
 }
 
-template <typename T, int D, int BITS, int MT>
+template <typename T, int D, int BITS, int MT, bool HALVED>
 static int launch(const TqMultiParams& p, cudaStream_t stream) {
   using Cfg = MultiCfg<D, BITS, MT>;
   static_assert(148 * Cfg::kCtas <= kMultiMaxCtas && Cfg::kCtas * Cfg::kRows <= 2 * kMultiScratchRows, "partials of more rows than there is room for");
   const int row_tiles = (p.rows + Cfg::kRows - 1) / Cfg::kRows;
-  auto kernel = tq_multi_mma_kernel<T, D, BITS, MT>;
+  auto kernel = tq_multi_mma_kernel<T, D, BITS, MT, HALVED>;
   ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
   kernel<<<multi_ctas(p, row_tiles, Cfg::kCtas), kMultiMmaThreads, Cfg::kSmem, stream>>>(p, row_tiles);
   return check_launch("tq_multi_mma_kernel");
 }
 
-int launch_tq_multi_mma(const TqMultiParams& p, int head_dim, int bits, int dtype, cudaStream_t stream) {
+template <bool HALVED>
+static int launch_pages_of(const TqMultiParams& p, int head_dim, int bits, int dtype, cudaStream_t stream) {
   auto pick = [&](auto elem) -> int {
     using T = decltype(elem);
     return ANNA_DISPATCH_TQ_BITS(bits, BITS, [&]() -> int {
-      if (head_dim == 128) return p.rows > 16 ? launch<T, 128, BITS, 2>(p, stream) : launch<T, 128, BITS, 1>(p, stream);
-      return launch<T, 256, BITS, 1>(p, stream);
+      if (head_dim == 128) return p.rows > 16 ? launch<T, 128, BITS, 2, HALVED>(p, stream) : launch<T, 128, BITS, 1, HALVED>(p, stream);
+      return launch<T, 256, BITS, 1, HALVED>(p, stream);
     });
   };
   return dtype == ANNA_DTYPE_F16 ? pick(__half{}) : pick(__nv_bfloat16{});
+}
+
+int launch_tq_multi_mma(const TqMultiParams& p, int head_dim, int bits, int dtype, cudaStream_t stream) {
+  return p.block_size % kTile == 0 ? launch_pages_of<false>(p, head_dim, bits, dtype, stream)
+                                   : launch_pages_of<true>(p, head_dim, bits, dtype, stream);
 }
 
 int tq_multi_mma_faults(int* count) {

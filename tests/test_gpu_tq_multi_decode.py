@@ -236,7 +236,20 @@ def test_holes_of_the_block_table_are_keys_that_nobody_sees(cuda_device, dtype, 
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim,page", [("bf16", 128, 16), ("fp32", 128, 16), ("fp16", 256, 32)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("bits", [2, 3, 4])
+@pytest.mark.parametrize("dim,page", [(128, 8), (128, 24), (256, 40), (128, 136), (128, 12)])
+@pytest.mark.parametrize("holes", [False, True])
+def test_pages_that_end_inside_a_tile(cuda_device, dtype, bits, dim, page, holes):
+    case = Case(lengths=[1500, 733, 30, 0, 8 * 33 + 5], tokens=6, group=3, kv_heads=2, dim=dim, bits=bits, page=page, window=9, dtype=dtype,
+                device=cuda_device, holes=holes, seed=page)
+    got = case.run(gate=True)
+    case.check(got, gate=True)
+    assert torch.equal(case.run(gate=True), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,page", [("bf16", 128, 16), ("fp32", 128, 16), ("fp16", 256, 32), ("bf16", 128, 24), ("fp16", 256, 8)])
 def test_bytes_behind_the_last_token_do_not_count(cuda_device, dtype, dim, page):
     """The last page's free slots, the ring's free slots and the pages of nobody hold NaNs and infinities."""
     case = Case(lengths=[307, 61, 9], tokens=4, group=2, kv_heads=2, dim=dim, bits=4, page=page, window=40, dtype=dtype,
