@@ -5,9 +5,8 @@
 //   q . k_hat = norm / D * [ fwht(s1*q) . centroid[idx] + sqrt(pi/2)/sqrt(D) * rnorm * fwht(s2*fwht(s1*q)) . (2*sign-1) ]
 // so a CTA rotates its rows once and no key is taken back to the original basis.
 //
-// This form serves fp32 caches, head_dim 64, pages that are no multiple of 8 tokens and value groups other than 32; everything in it
-// is 32 bits.  A CTA of
-// 128 threads de-quantizes 32 tokens at a time into shared memory for its 8 rows.  Bound: FMA issue (3 D operations per row and
+// This form serves fp32 caches, pages that are no multiple of 8 tokens and value groups other than 32; everything in it is 32 bits.  A
+// CTA of 128 threads de-quantizes 32 tokens at a time into shared memory for its 8 rows.  Bound: FMA issue (3 D operations per row and
 // key, of which the shared-memory reads of the keys are shared by two rows).
 #include "tq_multi_params.cuh"
 
@@ -362,7 +361,7 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
   p.scaling = scaling;
   const int row_tiles = (p.rows + kMultiRows - 1) / kMultiRows;
   const bool tensor_cores = tq_multi_mma_applicable(p, head_dim, dtype);
-  p.stream_tiles = !tensor_cores ? 4 : head_dim == 128 && p.rows <= 16 ? 32 : 64;
+  p.stream_tiles = !tensor_cores ? 4 : head_dim <= 128 && p.rows <= 16 ? 32 : 64;
   p.min_share = tensor_cores ? 32 : 4;
   p.whole_tiles = tensor_cores ? 48 : 0;
   // The line of a launch has room for so many rows and positions: larger batches go in several, one behind the other.

@@ -196,7 +196,7 @@ __device__ __forceinline__ void multi_merge(const TqMultiParams& p, int64_t b, i
   }
 }
 
-// Tensor-core form (tq_multi_mma.cu): 16-bit caches, head_dim 128 / 256, value groups of 32, pages of a multiple of 8 tokens.
+// Tensor-core form (tq_multi_mma.cu): 16-bit caches, head_dim 64, 128 and 256, value groups of 32, pages of a multiple of 8 tokens.
 bool tq_multi_mma_applicable(const TqMultiParams& p, int head_dim, int dtype);
 int launch_tq_multi_mma(const TqMultiParams& p, int head_dim, int bits, int dtype, cudaStream_t stream);
 int tq_multi_mma_faults(int* count);  // bounded copy waits that expired on the current device

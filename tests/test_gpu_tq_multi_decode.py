@@ -193,7 +193,7 @@ def test_against_the_dense_keys_and_values(cuda_device, dtype, bits, shape, toke
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim,page,bits", [("bf16", 128, 16, 4), ("fp16", 128, 32, 3), ("bf16", 256, 16, 2), ("fp32", 128, 16, 4),
+@pytest.mark.parametrize("dtype,dim,page,bits", [("bf16", 128, 16, 4), ("fp16", 128, 32, 3), ("bf16", 256, 16, 2), ("fp32", 128, 16, 4), ("bf16", 64, 16, 3), ("fp16", 64, 24, 2), ("fp32", 64, 16, 4),
                                                   ("bf16", 64, 16, 4)])
 @pytest.mark.parametrize("tokens,group", [(4, 4), (9, 2), (40, 1)])
 def test_long_rows_that_several_ctas_share(cuda_device, dtype, dim, page, bits, tokens, group):
@@ -238,7 +238,7 @@ def test_holes_of_the_block_table_are_keys_that_nobody_sees(cuda_device, dtype, 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("bits", [2, 3, 4])
-@pytest.mark.parametrize("dim,page", [(128, 8), (128, 24), (256, 40), (128, 136), (128, 12)])
+@pytest.mark.parametrize("dim,page", [(128, 8), (128, 24), (256, 40), (128, 136), (128, 12), (64, 16), (64, 8), (64, 72)])
 @pytest.mark.parametrize("holes", [False, True])
 def test_pages_that_end_inside_a_tile(cuda_device, dtype, bits, dim, page, holes):
     case = Case(lengths=[1500, 733, 30, 0, 8 * 33 + 5], tokens=6, group=3, kv_heads=2, dim=dim, bits=bits, page=page, window=9, dtype=dtype,
@@ -249,7 +249,7 @@ def test_pages_that_end_inside_a_tile(cuda_device, dtype, bits, dim, page, holes
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim,page", [("bf16", 128, 16), ("fp32", 128, 16), ("fp16", 256, 32), ("bf16", 128, 24), ("fp16", 256, 8)])
+@pytest.mark.parametrize("dtype,dim,page", [("bf16", 128, 16), ("fp32", 128, 16), ("fp16", 256, 32), ("bf16", 128, 24), ("fp16", 256, 8), ("fp16", 64, 16)])
 def test_bytes_behind_the_last_token_do_not_count(cuda_device, dtype, dim, page):
     """The last page's free slots, the ring's free slots and the pages of nobody hold NaNs and infinities."""
     case = Case(lengths=[307, 61, 9], tokens=4, group=2, kv_heads=2, dim=dim, bits=4, page=page, window=40, dtype=dtype,
@@ -331,7 +331,7 @@ def mask_of(case, newest):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("fp16", 256), ("fp32", 128)])
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("fp16", 256), ("fp32", 128), ("fp16", 64)])
 def test_nans_reach_the_rows_that_see_them_and_no_others(cuda_device, dtype, dim):
     case = Case(lengths=[150, 90], tokens=4, group=2, kv_heads=2, dim=dim, bits=4, page=16, window=16, dtype=dtype, device=cuda_device, seed=6)
     case.check(case.run())
@@ -358,7 +358,7 @@ def test_nans_reach_the_rows_that_see_them_and_no_others(cuda_device, dtype, dim
             case.check(got, rows=~bad & ~mask_of(case, what == 0))
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim,bits", [("bf16", 128, 4), ("fp16", 256, 3), ("fp16", 128, 2), ("fp32", 128, 4)])
+@pytest.mark.parametrize("dtype,dim,bits", [("bf16", 128, 4), ("fp16", 256, 3), ("fp16", 128, 2), ("fp32", 128, 4), ("bf16", 64, 2), ("fp16", 64, 4)])
 def test_packed_infinities_behind_a_query(cuda_device, dtype, dim, bits):
     """New tokens that have left the window: the scale of one of them is infinite or NaN in one group of dims."""
     window, tokens, length = 2, 9, 70
