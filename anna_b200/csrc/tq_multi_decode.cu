@@ -45,8 +45,9 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
   const float f1 = p.scaling / (float)D;
   const float f2 = f1 * 1.2533141373155001f * rsqrt_dim_const<D>();
   for (int i = warp; i < kMultiRows; i += kMultiWarps) {
+    if (i >= count) break;  // rows that are not there: their scores are not looked at
     float w[E];
-    const int row = row0 + min(i, count - 1);
+    const int row = row0 + i;
     const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_stride_b + (int64_t)(kvh * p.groups + row % p.groups) * p.q_stride_h +
                  (int64_t)(row / p.groups) * p.q_stride_t + lane * E;
 #pragma unroll
@@ -294,8 +295,11 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
   });
 }
 
-// Rows of a row tile and CTAs per SM of this form: a wave of two holds the partials of 8 rows where the other's four hold 16.
-static_assert(148 * 2 <= kMultiMaxCtas && kMultiRows <= kMultiScratchRows);
+// CTAs per SM: what shared memory holds, and there is room for the partials of.  (8 fp32 rows of 20-3000 tokens, 20 queries to a KV head,
+// 64 dims: two per SM 135 us, four 96; 24 rows of 3-31 tokens, 160 queries, 128 dims: two 68, three 50.)
+template <int D>
+constexpr int kMultiCtas = D == 64 ? 4 : D == 128 ? 3 : 1;
+static_assert(148 * kMultiCtas<64> * kMultiRows <= kMultiMaxCtas * kMultiScratchRows, "partials of more rows than there is room for");
 
 }  // namespace anna
 
@@ -378,7 +382,7 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
           constexpr int smem = kMultiSmemFloats<D> * 4;
           auto kernel = tq_multi_kernel<T, D, BITS>;
           ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-          kernel<<<multi_ctas(p, row_tiles, D == 256 ? 1 : 2), kMultiThreads, smem, (cudaStream_t)stream>>>(p, row_tiles);
+          kernel<<<multi_ctas(p, row_tiles, kMultiCtas<D>), kMultiThreads, smem, (cudaStream_t)stream>>>(p, row_tiles);
           return check_launch("tq_multi_kernel");
         });
       });

@@ -347,7 +347,19 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
       s2[j] = p.signs2[lane * E + j];
     }
     for (int i = warp; i < Cfg::kRows; i += kMultiMmaWarps) {
-      const int row = row0 + min(i, count - 1);  // rows that are not there: the last one again, not stored
+      const int up = i % 16 / 8, m = i / 16, row_lane = 4 * (i % 8);
+      if (i >= count) {  // a row that is not there: zeros, which see no key
+        if (lane == 0) {
+          row_limit[i] = -1;
+          factor[i] = 1e-30f;
+        }
+        for (int k = lane; k < 2 * Cfg::kSteps * 4; k += 32) {
+          uint32_t* words = reinterpret_cast<uint32_t*>(frags) + ((m * 2 * Cfg::kSteps + k / 4) * 32 + row_lane + k % 4) * 4 + up;
+          words[0] = words[2] = 0u;
+        }
+        continue;
+      }
+      const int row = row0 + i;
       const int t = multi_token_of(p, row);
       const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_stride_b + (int64_t)(kvh * p.groups + row - t * p.groups) * p.q_stride_h +
                    (int64_t)t * p.q_stride_t + lane * E;
@@ -374,11 +386,9 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
       // a factor of zero (a zero query, no scaling) would make NaN of hidden scores
       if (lane == 0) row_limit[i] = first_seen + t;
       if (lane == 0) factor[i] = max_nan(top * fabsf(p.scaling) * (1.4426950408889634f / (float)D) / cent_scale, 1e-30f);
-      const int up = i % 16 / 8, m = i / 16;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const FragSlot a = index_slot<D, BITS>(lane * E + j), c = sign_slot<D, BITS>(lane * E + j);
-        const int row_lane = 4 * (i % 8);
         frags[(((m * 2 * Cfg::kSteps + a.step) * 32 + row_lane + a.tig) * 4 + 2 * a.reg + up) * 2 + a.half] = __float2half_rn(w1[j] * inv);
         frags[(((m * 2 * Cfg::kSteps + Cfg::kSteps + c.step) * 32 + row_lane + c.tig) * 4 + 2 * c.reg + up) * 2 + c.half] =
             __float2half_rn(w2[j] * inv);

@@ -202,7 +202,7 @@ int launch_tq_multi_mma(const TqMultiParams& p, int head_dim, int bits, int dtyp
 int tq_multi_mma_faults(int* count);  // bounded copy waits that expired on the current device
 
 // CTAs of a call: one resident wave, or fewer where that would leave shares below the smallest.
-constexpr int kMultiMaxCtas = 148 * 2, kMultiScratchRows = 16;  // or half the CTAs and twice the rows
+constexpr int kMultiMaxCtas = 148 * 2, kMultiScratchRows = 16;  // or other numbers with the same product
 inline int multi_ctas(const TqMultiParams& p, int row_tiles, int per_sm) {
   const int64_t line = (int64_t)p.batch * p.kv_heads * row_tiles * ((p.max_len + kBalancedTileTokens - 1) / kBalancedTileTokens + p.stream_tiles);
   const int64_t shares = (line + p.min_share - 1) / p.min_share;
