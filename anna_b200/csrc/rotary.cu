@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
 // The same for many tokens, where a vector is 4, 8, 16 or 32 pieces of 16 bytes: a lane holds a piece, and the other half of its pairs
 // comes from another lane, so that a vector is one load and one store of neighbouring lanes and its addresses are worked out once.
 // A CTA takes several tokens, and a lane has kRowsAhead vectors on their way.  (With the kernel above, 222 instructions per 32 pieces:
-// 16383 tokens of 20 heads of 256 dims, 64 turned, 156 us; 70 us so,
-// 4.8 TB/s.)
+// 16383 tokens of 20 heads of 256 dims, 64 turned, 156 us; 66 us so,
+// 5.1 TB/s.  Two or eight vectors ahead, four or sixteen tokens a CTA: as fast or slower.)
 constexpr int kManyTokens = 8, kRowsAhead = 4;
 
 struct RotaryToken {

@@ -7,7 +7,8 @@
 //
 // This form serves fp32 caches, pages that are no multiple of 8 tokens and value groups other than 32; everything in it is 32 bits.  A
 // CTA of 128 threads de-quantizes 32 tokens at a time into shared memory for its 8 rows.  Bound: FMA issue (3 D operations per row and
-// key, of which the shared-memory reads of the keys are shared by two rows).
+// key, of which the shared-memory reads of the keys are shared by two rows).  8 fp32 rows of 20-3000 tokens, 20 queries to a KV head of
+// 64 dims: 96 us; a pair of rows of 854-1709 tokens, 8 new tokens: 37 us (250 with one token's codes on their way at a time).
 #include "tq_multi_params.cuh"
 
 namespace anna {

@@ -14,9 +14,16 @@
 // The k-slots of the products and the columns of O are free to permute: a lane takes the coordinates whose codes it can unpack with
 // the fewest instructions, and 2 * D/8 neighbouring dims of an output row.
 //
+// Bound: the packed bytes of a sequence from HBM, once for 16 or 32 of its queries; today the issue of instructions.  4 new tokens of 16 rows
+// of 32768, 32/8 heads of 128, 4 bits: 260 us, 2.5 TB/s, 542 instructions per tile and warp (56 % of the issue slots, logic pipe 50 %,
+// products 35 % of their pipe).  A CTA of eight warps splits a share's steps among them, so that a share of 32 tiles is two steps of each
+// warp and the merge of their rows is one per share; two CTAs per SM (16 rows, up to 128 dims) is what the 128 registers of a thread
+// leave.  32 rows a CTA (two row tiles) unpack a key once for both, with half the warps: 8 new tokens 395 us, twice 260 as two calls.
+//
 // What is rounded below 32 bits: the rotated queries, centroids and residual norms to fp16 (2^-12 of the row's largest value, of the
 // centroid and of the norm), value scales and zeros, probabilities and values to fp16 (2^-12 of themselves).  Together they stay
-// below the rounding of a bf16 output (2^-9 of the value).
+// below the rounding of a bf16 output (2^-9 of the value); an fp16 output of unit size is off by 4e-4 in all, half of it its own rounding.
+// Values beyond 65504 become infinite.
 #pragma once
 
 #include "mbarrier_utils.cuh"
@@ -50,7 +57,7 @@ struct MultiCfg {
   static constexpr int kWarpRing = kRingStages * kStepTiles * kTileStride;
   static constexpr int kRing = kMultiMmaWarps * kWarpRing;
   static constexpr int kQuery = MT * 2 * kSteps * 32 * 16;  // A fragments of Q1, then of Q2
-  // the merge of the four warps: a row of O with its quarters 8 floats apart, so that the lanes that store together hit other banks
+  // the merge of the warps: a row of O with its quarters 8 floats apart, so that the lanes that store together hit other banks
   static constexpr int kMergeStride = D + 8 * (D / 32) + 4;
   static constexpr int kMerge = kMultiMmaWarps * 16 * kMergeStride * 4;
   static constexpr int kWork = kRing + kQuery > kMerge ? kRing + kQuery : kMerge;
@@ -833,7 +840,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
     }
   };
 
-  // ---- the four warps' rows together ---------------------------------------------------------------------------------------------
+  // ---- the warps' rows together ---------------------------------------------------------------------------------------------
   float2* stats = reinterpret_cast<float2*>(smem + Cfg::kOffStats);
 #pragma unroll
   for (int m = 0; m < MT; ++m)
