@@ -49,8 +49,10 @@ def rotary_tables(rotary_dim: int, *, theta: float = 10000.0, sections: Sequence
                   inverse_frequencies: Sequence[float] | None = None, device: torch.device) -> RotaryTables:
     """Rates and axes of the pairs on the device, made once for each set of parameters.  ``inverse_frequencies`` (radians per
     position, one for each pair) stands in for the powers of ``theta``."""
-    key = (rotary_dim, theta, None if sections is None else tuple(sections), bool(interleaved),
-           None if inverse_frequencies is None else tuple(inverse_frequencies), device)
+    if inverse_frequencies is not None:  # values, whatever holds them
+        inverse_frequencies = tuple(float(f) for f in inverse_frequencies)
+    sections = None if sections is None else tuple(int(s) for s in sections)
+    key = (rotary_dim, theta, sections, bool(interleaved), inverse_frequencies, device)
     found = _TABLES.get(key)
     if found is not None:
         return found
@@ -63,9 +65,9 @@ def rotary_tables(rotary_dim: int, *, theta: float = 10000.0, sections: Sequence
             raise ValueError(f"theta must be positive, got {theta}")
         frequencies = [float(theta) ** (-i / pairs) for i in range(pairs)]
     else:
-        frequencies = [float(f) for f in inverse_frequencies]
-        if len(frequencies) != pairs:
-            raise ValueError(f"inverse_frequencies must hold rotary_dim / 2 = {pairs} values, got {len(frequencies)}")
+        frequencies = list(inverse_frequencies)
+        if len(frequencies) != pairs or not all(map(math.isfinite, frequencies)):
+            raise ValueError(f"inverse_frequencies must hold rotary_dim / 2 = {pairs} finite values")
     with on_device(device):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first call with new rotary parameters uploads their tables: make it outside graph capture")

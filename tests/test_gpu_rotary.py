@@ -7,6 +7,7 @@ from __future__ import annotations
 import itertools
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -310,6 +311,12 @@ def test_new_lengths_that_are_read_are_refused(cuda_device):
 def test_tables_are_kept_and_counted(cuda_device, monkeypatch):
     first = rotary.rotary_tables(64, theta=123.0, device=cuda_device)
     assert rotary.rotary_tables(64, theta=123.0, device=cuda_device) is first
+    given = [rotary.rotary_tables(64, sections=s, inverse_frequencies=f, device=cuda_device)
+             for s, f in (((20, 12), [0.5] * 32), (torch.tensor([20, 12]), torch.full((32,), 0.5)), ([20, 12], np.full(32, 0.5)))]
+    assert given[1] is given[0] and given[2] is given[0]
+    for bad in ([0.5] * 31, [math.inf] * 32, [math.nan] * 32):
+        with pytest.raises(ValueError, match="inverse_frequencies"):
+            rotary.rotary_tables(64, inverse_frequencies=bad, device=cuda_device)
     monkeypatch.setattr(rotary, "_TABLES", {i: first for i in range(4096)})
     with pytest.raises(RuntimeError, match="rotary parameters"):
         rotary.rotary_tables(64, theta=124.0, device=cuda_device)

@@ -358,17 +358,18 @@ def test_nans_reach_the_rows_that_see_them_and_no_others(cuda_device, dtype, dim
             case.check(got, rows=~bad & ~mask_of(case, what == 0))
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,dim,bits", [("bf16", 128, 4), ("fp16", 256, 3), ("fp16", 128, 2), ("fp32", 128, 4), ("bf16", 64, 2), ("fp16", 64, 4)])
-def test_packed_infinities_behind_a_query(cuda_device, dtype, dim, bits):
+@pytest.mark.parametrize("dtype,dim,bits,page", [("bf16", 128, 4, 16), ("fp16", 256, 3, 16), ("fp16", 128, 2, 16), ("fp32", 128, 4, 16),
+                                                 ("bf16", 64, 2, 16), ("fp16", 64, 4, 16), ("bf16", 128, 4, 24), ("fp16", 64, 3, 8)])
+def test_packed_infinities_behind_a_query(cuda_device, dtype, dim, bits, page):
     """New tokens that have left the window: the scale of one of them is infinite or NaN in one group of dims."""
     window, tokens, length = 2, 9, 70
-    case = Case(lengths=[length, 40], tokens=tokens, group=2, kv_heads=2, dim=dim, bits=bits, page=16, window=window, dtype=dtype,
+    case = Case(lengths=[length, 40], tokens=tokens, group=2, kv_heads=2, dim=dim, bits=bits, page=page, window=window, dtype=dtype,
                 device=cuda_device, seed=13)
     at = length - 5  # queries 4 .. 8 see it
     elem = 4 if dtype == "fp32" else 2
     for value in (math.inf, math.nan):
-        offset = case.layout["off_vzero"] + (at % 16 * (dim // 32) + 1) * elem
-        where = (int(case.table[0, at // 16]), 1, slice(offset, offset + elem))
+        offset = case.layout["off_vzero"] + (at % page * (dim // 32) + 1) * elem
+        where = (int(case.table[0, at // page]), 1, slice(offset, offset + elem))
         was = case.packed[where].clone()
         case.packed[where] = torch.tensor([value], dtype=case.dtype).view(torch.uint8)
         got = case.run()
