@@ -6,27 +6,40 @@
 // so a CTA rotates its rows once and no key is taken back to the original basis.
 //
 // This form serves fp32 caches, pages that are no multiple of 8 tokens and value groups other than 32; everything in it is 32 bits.  A
-// CTA of 128 threads de-quantizes 32 tokens at a time into shared memory for its 8 rows.  Bound: FMA issue (3 D operations per row and
-// key, of which the shared-memory reads of the keys are shared by two rows).  8 fp32 rows of 20-3000 tokens, 20 queries to a KV head of
-// 64 dims: 96 us; a pair of rows of 854-1709 tokens, 8 new tokens: 37 us (250 with one token's codes on their way at a time).
+// CTA de-quantizes 32 tokens at a time into shared memory for its 8 rows; a warp scores two rows (256 dims: one) with a token a lane.
+// Bound: issue, of which the reads of shared memory are as many as the FMAs.  A lane takes neighbouring dims, so that its codes are one
+// load instead of one a dim: 8 fp32 rows of 20-3000 tokens, 20 queries to a KV head of 128 dims 181 -> 106 us, 256 dims (with 256 threads
+// instead of 128, too) 727 -> 240, 64 dims 96 -> 72.
 #include "tq_multi_params.cuh"
 
 namespace anna {
 
-constexpr int kMultiThreads = 128, kMultiWarps = 4;
+template <int D>
+constexpr int kMultiThreads = D == 256 ? 256 : 128;  // shared memory holds one CTA of 256 dims per SM
 constexpr int kMultiRows = 8;    // of a CTA of this form
 constexpr int kMultiTokens = 32;  // de-quantized at a time: a lane's token
 constexpr int kMultiAhead = 4;    // tokens of a warp whose codes are on their way together
+
+// This lane's NB bits of a run of codes.
+template <int NB>
+__device__ __forceinline__ uint32_t lane_bits(const uint8_t* codes, int lane) {
+  if constexpr (NB == 32) return reinterpret_cast<const uint32_t*>(codes)[lane];
+  else if constexpr (NB == 16) return reinterpret_cast<const uint16_t*>(codes)[lane];
+  else if constexpr (NB == 8) return codes[lane];
+  else return (uint32_t)codes[lane * NB / 8] >> (lane * NB % 8);
+}
 
 template <int D>
 constexpr int kMultiSmemFloats = 3 * kMultiRows * D + 2 * kMultiTokens * (D + 1) + kMultiTokens * D + kMultiRows * kMultiTokens;
 
 template <typename T, int D, int BITS>
-__global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiParams p, int row_tiles) {
-  constexpr int E = D / 32;
+__global__ void __launch_bounds__(kMultiThreads<D>) tq_multi_kernel(const TqMultiParams p, int row_tiles) {
+  constexpr int E = D / 32, kThreads = kMultiThreads<D>, kMultiWarps = kThreads / 32, kWarpRows = kMultiRows / kMultiWarps;
   constexpr int M = BITS - 1;
   constexpr int VS = BITS == 2 ? 2 : 4;
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
+  // Rows of D are held in an order of their own, dim lane * E + j at j * 32 + lane: a lane takes neighbouring dims, whose codes are one
+  // access, and neighbouring lanes write neighbouring floats.
   float* q_smem = smem;                                // [3][rows][D]: as it is, rotated, rotated twice; scaled
   float* ka = q_smem + 3 * kMultiRows * D;             // [tokens][D + 1]: centroids, or the key itself
   float* kb = ka + kMultiTokens * (D + 1);             // signs times the residual norm
@@ -37,7 +50,7 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < (1 << M)) sm_cent[threadIdx.x] = p.centroids[threadIdx.x];
-  multi_for_each_segment<T, D, kMultiThreads>(p, row_tiles, [&](int64_t b, int kvh, int tile, int64_t t0, int64_t t1, const MultiPartial& part) {
+  multi_for_each_segment<T, D, kThreads>(p, row_tiles, [&](int64_t b, int kvh, int tile, int64_t t0, int64_t t1, const MultiPartial& part) {
   const int row0 = tile * kMultiRows, count = min(kMultiRows, p.rows - row0);
   const int64_t len = max((int64_t)0, min(p.lengths[b], p.max_len));
   const int64_t lq = len > p.residual_len ? len - p.residual_len : 0;
@@ -54,30 +67,37 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       w[j] = ElemTraits<T>::to_float(q[j]);
-      q_smem[i * D + lane * E + j] = w[j] * p.scaling;
+      q_smem[i * D + j * 32 + lane] = w[j] * p.scaling;
       w[j] *= p.signs1[lane * E + j];
     }
     warp_fwht<E>(w, lane);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      q_smem[(kMultiRows + i) * D + lane * E + j] = w[j] * f1;
+      q_smem[(kMultiRows + i) * D + j * 32 + lane] = w[j] * f1;
       w[j] *= p.signs2[lane * E + j];
     }
     warp_fwht<E>(w, lane);
 #pragma unroll
-    for (int j = 0; j < E; ++j) q_smem[(2 * kMultiRows + i) * D + lane * E + j] = w[j] * f2;
+    for (int j = 0; j < E; ++j) q_smem[(2 * kMultiRows + i) * D + j * 32 + lane] = w[j] * f2;
   }
 
-  // rows warp and warp + 4 of this warp's softmax; the thread's dims of the output
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
-  constexpr int kDims = D >= kMultiThreads ? D / kMultiThreads : 1;
-  constexpr int kOutRows = D >= kMultiThreads ? kMultiRows : kMultiRows * D / kMultiThreads;
-  const int out_row0 = D >= kMultiThreads ? 0 : (int)threadIdx.x / D * kOutRows;
-  float acc[kOutRows][kDims];
+  // every kMultiWarps-th row from `warp` on is of this warp's softmax; the thread's rows of one dim of the output
+  float m_run[kWarpRows], l_run[kWarpRows];
 #pragma unroll
-  for (int r = 0; r < kOutRows; ++r)
+  for (int k = 0; k < kWarpRows; ++k) {
+    m_run[k] = -INFINITY;
+    l_run[k] = 0.0f;
+  }
+  static_assert(D <= kThreads && kThreads % D == 0, "a thread has one dim");
+  constexpr int kOutRows = kMultiRows * D / kThreads;
+  const int out_row0 = (int)threadIdx.x / D * kOutRows, place = (int)threadIdx.x % D, out_dim = place % 32 * E + place / 32;
+  float acc[kOutRows];
 #pragma unroll
-    for (int j = 0; j < kDims; ++j) acc[r][j] = 0.0f;
+  for (int r = 0; r < kOutRows; ++r) acc[r] = 0.0f;
+  int group[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) group[j] = (lane * E + j) / p.value_group;
+  const bool one_group = p.value_group % E == 0;
 
   const int64_t slot = len > lq ? p.window_slots[b] : 0;
   const T* ring = reinterpret_cast<const T*>(p.window) + (slot * 2 * p.kv_heads + kvh) * p.residual_len * D;
@@ -110,12 +130,9 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
         float k[kMultiAhead][E], v[kMultiAhead][E];
 #pragma unroll
         for (int u = 0; u < kMultiAhead; ++u) {
-          const T* key = ring + ((base + min(i + u * kMultiWarps, n - 1)) % p.residual_len) * D;
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            k[u][j] = ElemTraits<T>::to_float(key[lane + 32 * j]);
-            v[u][j] = ElemTraits<T>::to_float(key[ring_values + lane + 32 * j]);
-          }
+          const T* key = ring + ((base + min(i + u * kMultiWarps, n - 1)) % p.residual_len) * D + lane * E;
+          lane_load<T, E>(key, k[u]);
+          lane_load<T, E>(key + ring_values, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < kMultiAhead; ++u) {
@@ -123,13 +140,14 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
           if (at >= n) break;
 #pragma unroll
           for (int j = 0; j < E; ++j) {
-            ka[at * (D + 1) + lane + 32 * j] = k[u][j];
-            vt[at * D + lane + 32 * j] = v[u][j];
+            ka[at * (D + 1) + j * 32 + lane] = k[u][j];
+            vt[at * D + j * 32 + lane] = v[u][j];
           }
         }
         continue;
       }
-      uint8_t code[kMultiAhead][E], sign[kMultiAhead][E], value[kMultiAhead][E];
+      constexpr int kIndexBits = BITS == 3 ? 2 * E : BITS * E;
+      uint32_t code[kMultiAhead], sign[kMultiAhead], value[kMultiAhead];
       T scale[kMultiAhead][E], zero[kMultiAhead][E];
       float rnorm[kMultiAhead];
 #pragma unroll
@@ -144,14 +162,18 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
         const T* scales = reinterpret_cast<const T*>(page + p.layout.off_vscale) + tok * p.layout.groups;
         const T* zeros = reinterpret_cast<const T*>(page + p.layout.off_vzero) + tok * p.layout.groups;
         rnorm[u] = there ? reinterpret_cast<const float*>(page + p.layout.off_krnorm)[tok] : 0.0f;
+        code[u] = there ? lane_bits<kIndexBits>(keys, lane) : 0u;
+        sign[u] = BITS == 3 && there ? lane_bits<E>(keys + D / 4, lane) : 0u;
+        value[u] = there ? lane_bits<VS * E>(codes, lane) : 0u;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const int d = lane + 32 * j;
-          code[u][j] = there ? keys[BITS == 3 ? d >> 2 : d * BITS >> 3] : 0;
-          sign[u][j] = BITS == 3 && there ? keys[D / 4 + (d >> 3)] : 0;
-          value[u][j] = there ? codes[d * VS >> 3] : 0;
-          scale[u][j] = there ? scales[d / p.value_group] : T(0.0f);
-          zero[u][j] = there ? zeros[d / p.value_group] : T(0.0f);
+          if (j > 0 && one_group) {
+            scale[u][j] = scale[u][0];
+            zero[u][j] = zero[u][0];
+          } else {
+            scale[u][j] = there ? scales[group[j]] : T(0.0f);
+            zero[u][j] = there ? zeros[group[j]] : T(0.0f);
+          }
         }
       }
 #pragma unroll
@@ -160,58 +182,52 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
         if (at >= n) break;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const int d = lane + 32 * j;
           uint32_t index, negative;
           if constexpr (BITS == 3) {
-            index = (code[u][j] >> ((d & 3) * 2)) & 3u;
-            negative = ((sign[u][j] >> (d & 7)) & 1u) ^ 1u;
+            index = (code[u] >> (2 * j)) & 3u;
+            negative = ((sign[u] >> j) & 1u) ^ 1u;
           } else {
-            const uint32_t field = (code[u][j] >> (d * BITS & 7)) & ((1u << BITS) - 1u);
+            const uint32_t field = (code[u] >> (BITS * j)) & ((1u << BITS) - 1u);
             index = field & ((1u << M) - 1u);
             negative = (field >> M) ^ 1u;
           }
-          ka[at * (D + 1) + d] = sm_cent[index];
-          kb[at * (D + 1) + d] = negative != 0 ? -rnorm[u] : rnorm[u];
-          vt[at * D + d] = fmaf((float)((value[u][j] >> (d * VS & 7)) & ((1u << VS) - 1u)), ElemTraits<T>::to_float(scale[u][j]),
-                                ElemTraits<T>::to_float(zero[u][j]));
+          ka[at * (D + 1) + j * 32 + lane] = sm_cent[index];
+          kb[at * (D + 1) + j * 32 + lane] = negative != 0 ? -rnorm[u] : rnorm[u];
+          vt[at * D + j * 32 + lane] = fmaf((float)((value[u] >> (VS * j)) & ((1u << VS) - 1u)), ElemTraits<T>::to_float(scale[u][j]),
+                                            ElemTraits<T>::to_float(zero[u][j]));
         }
       }
     }
     __syncthreads();
-    // ---- scores: token `lane`, rows warp and warp + 4 ----------------------------------------------------------------------
-    float s[2] = {-INFINITY, -INFINITY};
-    if (lane < n) {
-      const float* x = ka + lane * (D + 1);
-      const float* y = kb + lane * (D + 1);
-      const float* q0 = q_smem + ((packed ? kMultiRows : 0) + warp) * D;
-      const float* q1 = q0 + kMultiWarps * D;
-      float a0 = 0.0f, a1 = 0.0f;
-#pragma unroll 16
-      for (int d = 0; d < D; ++d) {
-        a0 = fmaf(q0[d], x[d], a0);
-        a1 = fmaf(q1[d], x[d], a1);
-      }
-      if (packed) {
-        q0 += kMultiRows * D;
-        q1 += kMultiRows * D;
-        float b0 = 0.0f, b1 = 0.0f;
-#pragma unroll 16
-        for (int d = 0; d < D; ++d) {
-          b0 = fmaf(q0[d], y[d], b0);
-          b1 = fmaf(q1[d], y[d], b1);
-        }
-        a0 += b0;
-        a1 += b1;
-      }
-      const float a[2] = {a0 * sm_norm[lane], a1 * sm_norm[lane]};
+    // ---- scores: token `lane` --------------------------------------------------------------------------------------------------
+    float s[kWarpRows];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kWarpRows; ++k) s[k] = -INFINITY;
+    if (lane < n) {
+      float a[kWarpRows];
+      auto product = [&](const float* q, const float* x) {
+        float sum[kWarpRows];
+#pragma unroll
+        for (int k = 0; k < kWarpRows; ++k) sum[k] = 0.0f;
+#pragma unroll 16
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+          for (int k = 0; k < kWarpRows; ++k) sum[k] = fmaf(q[k * kMultiWarps * D + d], x[d], sum[k]);
+#pragma unroll
+        for (int k = 0; k < kWarpRows; ++k) a[k] += sum[k];
+      };
+#pragma unroll
+      for (int k = 0; k < kWarpRows; ++k) a[k] = 0.0f;
+      product(q_smem + ((packed ? kMultiRows : 0) + warp) * D, ka + lane * (D + 1));
+      if (packed) product(q_smem + (2 * kMultiRows + warp) * D, kb + lane * (D + 1));
+#pragma unroll
+      for (int k = 0; k < kWarpRows; ++k) {
         const int i = warp + k * kMultiWarps;
-        if (i < count && sm_there[lane] && base + lane <= first_seen + (row0 + i) / p.groups) s[k] = a[k];
+        if (i < count && sm_there[lane] && base + lane <= first_seen + (row0 + i) / p.groups) s[k] = a[k] * sm_norm[lane];
       }
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kWarpRows; ++k) {
       float m_new = s[k];
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
@@ -225,52 +241,51 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
     }
     __syncthreads();
     // ---- values -----------------------------------------------------------------------------------------------------------
-    const int d0 = D >= kMultiThreads ? (int)threadIdx.x : (int)threadIdx.x % D;
 #pragma unroll
-    for (int r = 0; r < kOutRows; ++r)
+    for (int r = 0; r < kOutRows; ++r) acc[r] *= sm_rescale[out_row0 + r];
+    int i = 0;
+    if (base + n - 1 <= first_seen) {  // every row sees every token
+      for (; i + 4 <= n; i += 4) {
+        float v[4];
 #pragma unroll
-      for (int j = 0; j < kDims; ++j) acc[r][j] *= sm_rescale[out_row0 + r];
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      float v[kDims];
+        for (int u = 0; u < 4; ++u) v[u] = vt[(i + u) * D + place];
 #pragma unroll
-      for (int j = 0; j < kDims; ++j) v[j] = vt[i * D + d0 + j * kMultiThreads];
+        for (int r = 0; r < kOutRows; ++r) {
+          const float4 w = *reinterpret_cast<const float4*>(weight + (out_row0 + r) * kMultiTokens + i);
+          acc[r] = fmaf(w.w, v[3], fmaf(w.z, v[2], fmaf(w.y, v[1], fmaf(w.x, v[0], acc[r]))));
+        }
+      }
+    }
+    for (; i < n; ++i) {
+      const float v = vt[i * D + place];
 #pragma unroll
       for (int r = 0; r < kOutRows; ++r) {
         const float w = weight[(out_row0 + r) * kMultiTokens + i];
-        // a value that the row does not see may be infinite or NaN
-        if (w != 0.0f) {
-#pragma unroll
-          for (int j = 0; j < kDims; ++j) acc[r][j] = fmaf(w, v[j], acc[r][j]);
-        }
+        if (w != 0.0f) acc[r] = fmaf(w, v, acc[r]);  // a value that the row does not see may be infinite or NaN
       }
     }
     base = stop;
   }
 
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < kWarpRows; ++k) {
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) l_run[k] += __shfl_xor_sync(0xffffffffu, l_run[k], d);
   }
   __syncthreads();
-  const int d0 = D >= kMultiThreads ? (int)threadIdx.x : (int)threadIdx.x % D;
   if (part.count == 1) {
     float* den = weight;
     if (lane == 0) {
-      den[warp] = l_run[0];
-      den[warp + kMultiWarps] = l_run[1];
+#pragma unroll
+      for (int k = 0; k < kWarpRows; ++k) den[warp + k * kMultiWarps] = l_run[k];
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kOutRows; ++r) {
       if (out_row0 + r >= count) break;
       const float l = den[out_row0 + r], inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-      for (int j = 0; j < kDims; ++j) {
-        const float o[1] = {acc[r][j] * inv};
-        multi_store<T, 1>(p, b, kvh, row0 + out_row0 + r, d0 + j * kMultiThreads, o);
-      }
+      const float o[1] = {acc[r] * inv};
+      multi_store<T, 1>(p, b, kvh, row0 + out_row0 + r, out_dim, o);
     }
     __syncthreads();
     return;
@@ -278,7 +293,7 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
   const int64_t at = multi_partial_row(part, part.mine, kMultiRows);
   if (lane == 0) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kWarpRows; ++k) {
       const int i = warp + k * kMultiWarps;
       if (i < count)
         reinterpret_cast<float2*>(p.stats)[at + i] = make_float2(m_run[k], l_run[k]);
@@ -287,9 +302,7 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
 #pragma unroll
   for (int r = 0; r < kOutRows; ++r) {
     if (out_row0 + r >= count) break;
-    float* to = p.values + (at + out_row0 + r) * D;
-#pragma unroll
-    for (int j = 0; j < kDims; ++j) to[d0 + j * kMultiThreads] = acc[r][j];
+    p.values[(at + out_row0 + r) * D + out_dim] = acc[r];
   }
   multi_merge<T, D, kMultiWarps, kMultiRows>(p, b, kvh, tile, row_tiles, count, part, smem);
   __syncthreads();
@@ -297,7 +310,7 @@ __global__ void __launch_bounds__(kMultiThreads) tq_multi_kernel(const TqMultiPa
 }
 
 // CTAs per SM: what shared memory holds, and there is room for the partials of.  (8 fp32 rows of 20-3000 tokens, 20 queries to a KV head,
-// 64 dims: two per SM 135 us, four 96; 24 rows of 3-31 tokens, 160 queries, 128 dims: two 68, three 50.)
+// 64 dims, with a load per dim: two per SM 135 us, four 96; 24 rows of 3-31 tokens, 160 queries, 128 dims: two 68, three 50.)
 template <int D>
 constexpr int kMultiCtas = D == 64 ? 4 : D == 128 ? 3 : 1;
 static_assert(148 * kMultiCtas<64> * kMultiRows <= kMultiMaxCtas * kMultiScratchRows, "partials of more rows than there is room for");
@@ -383,7 +396,7 @@ extern "C" int anna_tq_paged_multi_decode(const void* q, int64_t q_stride_b, int
           constexpr int smem = kMultiSmemFloats<D> * 4;
           auto kernel = tq_multi_kernel<T, D, BITS>;
           ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-          kernel<<<multi_ctas(p, row_tiles, kMultiCtas<D>), kMultiThreads, smem, (cudaStream_t)stream>>>(p, row_tiles);
+          kernel<<<multi_ctas(p, row_tiles, kMultiCtas<D>), kMultiThreads<D>, smem, (cudaStream_t)stream>>>(p, row_tiles);
           return check_launch("tq_multi_kernel");
         });
       });
