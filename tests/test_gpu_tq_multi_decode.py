@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import itertools
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -425,9 +426,64 @@ def test_another_stream_and_the_dispatcher(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,page", [("bf16", 16), ("fp32", 16), ("fp16", 24)])
+def test_threads_that_call_at_once(cuda_device, dtype, page):
+    """Two host threads on one stream and two on streams of their own: every call has scratch of its own, and the counters of a stream
+    are zero again when the next call on it begins."""
+    cases = [Case(lengths=[700 + 200 * i, 130, 0], tokens=1 + 2 * i, group=4, kv_heads=2, dim=128, bits=4, page=page, window=16, dtype=dtype,
+                  device=cuda_device, seed=i) for i in range(4)]
+    put = lambda x: x.to(cuda_device)  # noqa: E731
+    args = [dict(query=put(c.query), packed_pages=put(c.packed), page_table=put(c.table), window=put(c.window_ring), window_slots=put(c.slots),
+                 lengths=put(torch.tensor(c.lengths)), scaling=c.scaling, bits=4, residual_len=16, block_size=page, value_group_size=32)
+            for c in cases]
+    want = [anna_b200.run_tq_paged_multi_decode(**a) for a in args]
+    streams = [torch.cuda.current_stream(), torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def calls(i):
+        with torch.cuda.stream(streams[i]):
+            outs = [anna_b200.run_tq_paged_multi_decode(**args[i]) for _ in range(40)]
+            streams[i].synchronize()
+            wrong.extend(i for out in outs if not torch.equal(out, want[i]))
+
+    threads = [threading.Thread(target=calls, args=(i,)) for i in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("bf16", 64), ("fp32", 64)])
+def test_many_queries_of_a_sequence(cuda_device, dtype, dim):
+    case = Case(lengths=[330, 150], tokens=300, group=3, kv_heads=1, dim=dim, bits=4, page=16, window=40, dtype=dtype, device=cuda_device, seed=4)
+    case.check(case.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,page", [("bf16", 16), ("bf16", 24), ("fp32", 16)])
+def test_lengths_that_the_table_cannot_hold_are_cut(cuda_device, dtype, page):
+    """What a table of whole pages and the window hold is all there is: longer lengths read nothing else, negative ones are empty rows."""
+    full = 4 * page + 16
+    case = Case(lengths=[full, full], tokens=3, group=2, kv_heads=2, dim=128, bits=4, page=page, window=16, dtype=dtype, device=cuda_device, seed=6)
+    want = case.run()
+    case.check(want)
+    case.table = case.table[:, :4].contiguous()  # the fixture's tables have room for more
+    got = case.run(lengths=[2 ** 40, full + 1])
+    assert torch.equal(got, want)
+    got = case.run(lengths=[-5, full])
+    assert bool((got[0] == 0).all())
+    second = torch.zeros(got.shape[:3], dtype=torch.bool)
+    second[1] = True
+    case.check(got, rows=second)  # other shares than of two rows, so other roundings
+
+
+@pytest.mark.gpu
 def test_value_groups_and_empty_calls(cuda_device):
-    for group in (8, 16, 64):
-        case = Case(lengths=[90, 3], tokens=2, group=2, kv_heads=1, dim=128, bits=4, page=16, window=8, dtype="bf16", device=cuda_device,
+    for dim, group in ((128, 8), (128, 16), (128, 64), (128, 2), (256, 4), (256, 256), (64, 64)):
+        case = Case(lengths=[90, 3], tokens=2, group=2, kv_heads=1, dim=dim, bits=4, page=16, window=8, dtype="bf16", device=cuda_device,
                     value_group=group)
         case.check(case.run())
     q = torch.zeros(2, 4, 0, 128, device=cuda_device, dtype=torch.bfloat16)
