@@ -22,7 +22,7 @@
 //
 // What is rounded below 32 bits: the rotated queries, centroids and residual norms to fp16 (2^-12 of the row's largest value, of the
 // centroid and of the norm), value scales and zeros, probabilities and values to fp16 (2^-12 of themselves).  Together they stay
-// below the rounding of a bf16 output (2^-9 of the value); an fp16 output of unit size is off by 4e-4 in all, half of it its own rounding.
+// below the rounding of a bf16 output (2^-9 of the value); for fp16 see kSplit.
 // Values beyond 65504 become infinite.
 #pragma once
 
@@ -39,8 +39,13 @@ constexpr int kStepTiles = 2;    // tiles of a step: one softmax update
 constexpr int kRingStages = 2;   // steps of a warp's ring
 constexpr float kMoveLimit = 8.0f;  // log2 units by which a running maximum may be exceeded: probabilities stay below 2^8
 
-template <int D, int BITS, int MT>
+template <typename T, int D, int BITS, int MT>
 struct MultiCfg {
+  // An fp16 output shows what Q1 and P lose as one fp16 each, so that they are sums of two there, with a product for either part: 16 rows
+  // of 0.4-4 K tokens, 256 dims, 64 queries to a KV head, off by 2.9e-4 of the output instead of 3.9e-4 (2.1e-4 is its own rounding), 80 us
+  // instead of 70; 16 rows of 32768 tokens, 128 dims, 318 instead of 260.  A bf16 output hides it.
+  static constexpr bool kSplit = std::is_same_v<T, __half>;
+  static constexpr int kPlanes = kSplit ? 3 : 2;
   static constexpr int kRows = 16 * MT;
   static constexpr int kSteps = D / 16;  // k-steps of one product
   static constexpr int kGroups = D / 32;
@@ -56,7 +61,7 @@ struct MultiCfg {
   static constexpr int kTileStride = (kTileBytes + 127) / 128 * 128;
   static constexpr int kWarpRing = kRingStages * kStepTiles * kTileStride;
   static constexpr int kRing = kMultiMmaWarps * kWarpRing;
-  static constexpr int kQuery = MT * 2 * kSteps * 32 * 16;  // A fragments of Q1, then of Q2
+  static constexpr int kQuery = MT * kPlanes * kSteps * 32 * 16;  // A fragments of Q1, of Q2, of what is left of Q1
   // the merge of the warps: a row of O with its quarters 8 floats apart, so that the lanes that store together hit other banks
   static constexpr int kMergeStride = D + 8 * (D / 32) + 4;
   static constexpr int kMerge = kMultiMmaWarps * 16 * kMergeStride * 4;
@@ -200,9 +205,9 @@ __device__ __forceinline__ FragSlot sign_slot(int c) {
 }
 
 template <typename T, int D, int BITS, int MT, bool HALVED>
-__global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas)
+__global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kCtas)
     tq_multi_mma_kernel(const TqMultiParams p, int row_tiles) {
-  using Cfg = MultiCfg<D, BITS, MT>;
+  using Cfg = MultiCfg<T, D, BITS, MT>;
   constexpr int E = D / 32;
   constexpr int kKeyWords = BITS == 4 ? D / 32 : D / 64;  // of a lane's D/4 coordinates of a token: codes or indices
   constexpr int kSignWords = BITS == 3 && D > 64 ? D / 128 : 1;
@@ -360,8 +365,8 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
           row_limit[i] = -1;
           factor[i] = 1e-30f;
         }
-        for (int k = lane; k < 2 * Cfg::kSteps * 4; k += 32) {
-          uint32_t* words = reinterpret_cast<uint32_t*>(frags) + ((m * 2 * Cfg::kSteps + k / 4) * 32 + row_lane + k % 4) * 4 + up;
+        for (int k = lane; k < Cfg::kPlanes * Cfg::kSteps * 4; k += 32) {
+          uint32_t* words = reinterpret_cast<uint32_t*>(frags) + ((m * Cfg::kPlanes * Cfg::kSteps + k / 4) * 32 + row_lane + k % 4) * 4 + up;
           words[0] = words[2] = 0u;
         }
         continue;
@@ -396,8 +401,11 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const FragSlot a = index_slot<D, BITS>(lane * E + j), c = sign_slot<D, BITS>(lane * E + j);
-        frags[(((m * 2 * Cfg::kSteps + a.step) * 32 + row_lane + a.tig) * 4 + 2 * a.reg + up) * 2 + a.half] = __float2half_rn(w1[j] * inv);
-        frags[(((m * 2 * Cfg::kSteps + Cfg::kSteps + c.step) * 32 + row_lane + c.tig) * 4 + 2 * c.reg + up) * 2 + c.half] =
+        const __half most = __float2half_rn(w1[j] * inv);
+        __half* to = frags + (((m * Cfg::kPlanes * Cfg::kSteps + a.step) * 32 + row_lane + a.tig) * 4 + 2 * a.reg + up) * 2 + a.half;
+        to[0] = most;
+        if constexpr (Cfg::kSplit) to[2 * Cfg::kSteps * 32 * 8] = __float2half_rn(fmaf(w1[j], inv, -__half2float(most)));
+        frags[(((m * Cfg::kPlanes * Cfg::kSteps + Cfg::kSteps + c.step) * 32 + row_lane + c.tig) * 4 + 2 * c.reg + up) * 2 + c.half] =
             __float2half_rn(w2[j] * inv);
       }
     }
@@ -534,7 +542,12 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
         for (int i = 0; i < 2; ++i) {
           uint4 a[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) a[m] = frag[(m * 2 * Cfg::kSteps + 2 * w + i) * 32];
+          for (int m = 0; m < MT; ++m) a[m] = frag[(m * Cfg::kPlanes * Cfg::kSteps + 2 * w + i) * 32];
+          uint4 rest[MT];
+          if constexpr (Cfg::kSplit) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) rest[m] = frag[((m * Cfg::kPlanes + 2) * Cfg::kSteps + 2 * w + i) * 32];
+          }
 #pragma unroll
           for (int c = 0; c < kCols; ++c) {
             uint32_t sel = (BITS == 2 || BITS == 3) && (w & 1) != 0 ? words[c][at] >> (i == 0 ? 2 : 18) : i == 0 ? words[c][at] : words[c][at] >> 16;
@@ -542,7 +555,10 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
             const uint32_t lo = permute(lut_lo[0], lut_lo[1], sel), hi = permute(lut_hi[0], lut_hi[1], sel);
             const uint32_t k0 = permute(lo, hi, 0x5140), k1 = permute(lo, hi, 0x7362);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) mma_f16(s[m][c], a[m], k0, k1);
+            for (int m = 0; m < MT; ++m) {
+              mma_f16(s[m][c], a[m], k0, k1);
+              if constexpr (Cfg::kSplit) mma_f16(s[m][c], rest[m], k0, k1);
+            }
           }
         }
         if constexpr (BITS != 3) {
@@ -550,7 +566,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
           for (int i = 0; i < 2; ++i) {
             uint4 a[MT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) a[m] = frag[(m * 2 * Cfg::kSteps + Cfg::kSteps + 2 * w + i) * 32];
+            for (int m = 0; m < MT; ++m) a[m] = frag[(m * Cfg::kPlanes * Cfg::kSteps + Cfg::kSteps + 2 * w + i) * 32];
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
               uint32_t k[2];
@@ -582,7 +598,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
         for (int x = 0; x < Cfg::kSteps; ++x) {
           uint4 a[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) a[m] = frag[(m * 2 * Cfg::kSteps + Cfg::kSteps + x) * 32];
+          for (int m = 0; m < MT; ++m) a[m] = frag[(m * Cfg::kPlanes * Cfg::kSteps + Cfg::kSteps + x) * 32];
 #pragma unroll
           for (int c = 0; c < kCols; ++c) {
             const uint32_t word = signs[c][x / 8];
@@ -627,11 +643,22 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
 #pragma unroll
     for (int u = 0; u < kStepTiles; ++u) {
       const uint8_t* at = st + u * Cfg::kTileStride;
-      uint4 pa[MT];
+      uint4 pa[MT], rest[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m) {
         pa[m] = make_uint4(pack2<__half>(s[m][2 * u][0], s[m][2 * u][1]), pack2<__half>(s[m][2 * u][2], s[m][2 * u][3]),
                            pack2<__half>(s[m][2 * u + 1][0], s[m][2 * u + 1][1]), pack2<__half>(s[m][2 * u + 1][2], s[m][2 * u + 1][3]));
+        if constexpr (Cfg::kSplit) {
+          const uint32_t most[4] = {pa[m].x, pa[m].y, pa[m].z, pa[m].w};
+          uint32_t left[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&most[i]));
+            left[i] = pack2<__half>(s[m][2 * u + i / 2][2 * (i % 2)] - x.x, s[m][2 * u + i / 2][2 * (i % 2) + 1] - x.y);
+          }
+          rest[m] = make_uint4(left[0], left[1], left[2], left[3]);
+        }
+      }
       uint32_t scale[2], zero[2], words[2][2][kValWords];
       constexpr float kBase = BITS == 2 ? 4.0f : 16.0f;  // above all codes
 #pragma unroll
@@ -687,7 +714,10 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
               }
               const int j = w * kPerWord + h * (kPerWord / 2) + f + up;
 #pragma unroll
-              for (int m = 0; m < MT; ++m) mma_f16(o[m][j], pa[m], v[0], v[1]);
+              for (int m = 0; m < MT; ++m) {
+                mma_f16(o[m][j], pa[m], v[0], v[1]);
+                if constexpr (Cfg::kSplit) mma_f16(o[m][j], rest[m], v[0], v[1]);
+              }
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) x[i] >>= 2 * kWidth;
@@ -923,7 +953,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<D, BITS, MT>::kCtas
 
 template <typename T, int D, int BITS, int MT, bool HALVED>
 static int launch(const TqMultiParams& p, cudaStream_t stream) {
-  using Cfg = MultiCfg<D, BITS, MT>;
+  using Cfg = MultiCfg<T, D, BITS, MT>;
   static_assert(148 * Cfg::kCtas <= kMultiMaxCtas && Cfg::kCtas * Cfg::kRows <= 2 * kMultiScratchRows, "partials of more rows than there is room for");
   const int row_tiles = (p.rows + Cfg::kRows - 1) / Cfg::kRows;
   auto kernel = tq_multi_mma_kernel<T, D, BITS, MT, HALVED>;
