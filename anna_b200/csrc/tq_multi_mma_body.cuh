@@ -23,7 +23,7 @@
 // What is rounded below 32 bits: the rotated queries, centroids and residual norms to fp16 (2^-12 of the row's largest value, of the
 // centroid and of the norm), value scales and zeros, probabilities and values to fp16 (2^-12 of themselves).  Together they stay
 // below the rounding of a bf16 output (2^-9 of the value); for fp16 see kSplit.
-// Values beyond 65504 become infinite.
+// Below 2^-14 fp16 has fewer bits, down to 2^-24.  Values beyond its range keep to it by powers of two: see `lift`.
 #pragma once
 
 #include "mbarrier_utils.cuh"
@@ -153,14 +153,22 @@ __device__ __forceinline__ uint32_t times_power(uint32_t x, int n) {
   return r;
 }
 
-// A value that some rows see and others do not may be infinite or NaN, and zero times that is NaN: where a tile is cut by the rows'
-// limits, such values go into the product as zeros, and the rows that see them get them at the end (strange_values).
-__device__ __forceinline__ bool finite_f16(float v) { return fabsf(v) < 65520.0f; }  // rounded to fp16
+// A value of the window that some rows see and others do not may be infinite or NaN, and zero times that is NaN: where a tile is cut by
+// the rows' limits, such values go into the product as zeros, and the rows that see them get them at the end (strange_values).
 template <typename T>
 __device__ __forceinline__ uint32_t finite_halves(uint32_t pair) {  // all ones in the halves that are finite
   constexpr uint32_t kExp = std::is_same_v<T, __half> ? 0x7C007C00u : 0x7F807F80u, kOne = std::is_same_v<T, __half> ? 0x04000400u : 0x00800080u;
   const uint32_t over = ((pair & kExp) + kOne) & 0x80008000u;  // the exponent's carry
   return ~((over >> 15) * 0xffffu);
+}
+
+// Of either half, the larger magnitude, NaN if either is (its sign is of no use).
+template <typename T>
+__device__ __forceinline__ uint32_t max_magnitudes(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __half>) asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 template <int N>
@@ -482,6 +490,60 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
     }
   };
 
+  // Values are fp16 in the product, where those of a finite group may not fit.  So a column of O (a lane's column as B operand: dims of
+  // one group) has its values at a power of two, which falls when one could pass 2^15.  A step that the rows' limits cut is another
+  // matter: what is infinite or NaN there, or takes the power below 1, must not touch the rows that do not see it, and zero times it
+  // would.  From such a tile on the values are added in 32 bits, each to the rows that give it a weight.
+  constexpr float kCodes = BITS == 2 ? 4.0f : 16.0f;  // above all codes
+  float lift = 1.0f;
+  bool exact = false, lifted = false;  // lifted: not every column at 1, or exact
+  // Steps whose scales and zeros stay below 2^14 (over the codes) look no further as long as no column is lifted: 2^14 in the type's bits,
+  // each half with a bit on top that a larger magnitude, infinity and NaN take away.
+  constexpr uint32_t kOne = std::is_same_v<T, __half> ? 15 << 10 : 127 << 7, kPower = std::is_same_v<T, __half> ? 1 << 10 : 1 << 7;
+  constexpr uint32_t kMostZero = (0x8000u + kOne + 14 * kPower) * 0x10001u, kMostScale = (0x8000u + kOne + (BITS == 2 ? 12 : 10) * kPower) * 0x10001u;
+  auto lift_columns = [&](float by) {  // the columns of O that this lane holds, by the factors of their lanes
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float of_column = __shfl_sync(0xffffffffu, by, 4 * (2 * tig + h));
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          o[m][j][h] *= of_column;
+          o[m][j][2 + h] *= of_column;
+        }
+    }
+  };
+  // Four tokens of the eight from `base` on of the tile at `at`: those that the lanes of a quad hold in their column `r`.
+  auto exact_tokens = [&](auto&& weight, const uint8_t* at, int base, int r) {
+    constexpr int kWidth = BITS == 2 ? 2 : 4;
+#pragma unroll 1
+    for (int from = 0; from < 4; ++from) {
+      const int t = base + 2 * from + ((from ^ r) & 1);
+      float p_of[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) p_of[m][k] = __shfl_sync(0xffffffffu, weight(m, k), (lane & ~3) + from);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int column = 2 * tig + h, group = column * (D / 8) / 32;
+        const float scale = ElemTraits<T>::to_float(reinterpret_cast<const T*>(at + Cfg::kOffScale)[t * Cfg::kGroups + group]);
+        const float zero = ElemTraits<T>::to_float(reinterpret_cast<const T*>(at + Cfg::kOffZero)[t * Cfg::kGroups + group]);
+        const uint8_t* codes = at + Cfg::kOffVal + t * Cfg::kValBytes + column * (Cfg::kValBytes / 8);
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          const float v = fmaf((float)((codes[j * kWidth / 8] >> (j * kWidth % 8)) & ((1 << kWidth) - 1)), scale, zero);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (p_of[m][k] != 0.0f) o[m][j][2 * k + h] = fmaf(p_of[m][k], v, o[m][j][2 * k + h]);
+        }
+      }
+    }
+  };
+
   // ---- packed prefix -----------------------------------------------------------------------------------------------------------
   for (int n = 0; n < my_steps; ++n) {
     __syncwarp();  // every lane is done with the stage that is re-armed next
@@ -640,91 +702,146 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
     softmax(s, std::integral_constant<int, kCols>{});
 
     // ---- values ----
+    // In two forms, so that what a column's power takes costs the ordinary one nothing (in one, 16 rows of 32768 tokens took 280 us instead of 267).
+    bool careful = lifted;
+    if (!careful) {  // scales and zeros of two tokens of the step a lane
+      uint32_t words[Cfg::kGroups];
+      load_words<Cfg::kGroups>(st + (lane >> 4) * Cfg::kTileStride + Cfg::kOffScale + (lane & 15) * (4 * Cfg::kGroups), words);
 #pragma unroll
-    for (int u = 0; u < kStepTiles; ++u) {
-      const uint8_t* at = st + u * Cfg::kTileStride;
-      uint4 pa[MT], rest[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        pa[m] = make_uint4(pack2<__half>(s[m][2 * u][0], s[m][2 * u][1]), pack2<__half>(s[m][2 * u][2], s[m][2 * u][3]),
-                           pack2<__half>(s[m][2 * u + 1][0], s[m][2 * u + 1][1]), pack2<__half>(s[m][2 * u + 1][2], s[m][2 * u + 1][3]));
-        if constexpr (Cfg::kSplit) {
-          const uint32_t most[4] = {pa[m].x, pa[m].y, pa[m].z, pa[m].w};
-          uint32_t left[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&most[i]));
-            left[i] = pack2<__half>(s[m][2 * u + i / 2][2 * (i % 2)] - x.x, s[m][2 * u + i / 2][2 * (i % 2) + 1] - x.y);
-          }
-          rest[m] = make_uint4(left[0], left[1], left[2], left[3]);
-        }
-      }
-      uint32_t scale[2], zero[2], words[2][2][kValWords];
-      constexpr float kBase = BITS == 2 ? 4.0f : 16.0f;  // above all codes
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int ta = tok_a + 8 * i, tb = tok_b + 8 * i;
-        const int group = gid * (D / 8) / 32;
-        const T* scales = reinterpret_cast<const T*>(at + Cfg::kOffScale) + group;
-        const T* zeros = reinterpret_cast<const T*>(at + Cfg::kOffZero) + group;
-        float sa = ElemTraits<T>::to_float(scales[ta * Cfg::kGroups]), sb = ElemTraits<T>::to_float(scales[tb * Cfg::kGroups]);
-        float za = ElemTraits<T>::to_float(zeros[ta * Cfg::kGroups]), zb = ElemTraits<T>::to_float(zeros[tb * Cfg::kGroups]);
-        if (!full) {  // the bytes of tokens that are not there may be anything
-          if (tok_a >= there(2 * u + i)) sa = za = 0.0f;
-          if (tok_b >= there(2 * u + i)) sb = zb = 0.0f;
-        }
-        if (cut) {
-          if (!finite_f16(fabsf(za) + kBase * fabsf(sa))) { sa = za = 0.0f; *strange = 1; }
-          if (!finite_f16(fabsf(zb) + kBase * fabsf(sb))) { sb = zb = 0.0f; *strange = 1; }
-        }
-        scale[i] = pack2<__half>(sa, sb);
-        zero[i] = pack2<__half>(za, zb);
-        const uint8_t* codes = at + Cfg::kOffVal + gid * (Cfg::kValBytes / 8);
-        if constexpr (BITS == 2 && D == 64) {
-          words[i][0][0] = *reinterpret_cast<const uint16_t*>(codes + ta * Cfg::kValBytes);
-          words[i][1][0] = *reinterpret_cast<const uint16_t*>(codes + tb * Cfg::kValBytes);
-        } else {
-          load_words<kValWords>(codes + ta * Cfg::kValBytes, words[i][0]);
-          load_words<kValWords>(codes + tb * Cfg::kValBytes, words[i][1]);
-        }
-      }
-      // A code in the lowest bits under the exponent of 1024 reads as 1024 + code in fp16, one a field higher under the exponent of 64
-      // (2-bit codes: 256) as 64 + code, and taking that off is exact.  So one shift serves the two fields of a byte: the logic pipe,
-      // which binds this kernel, has one operation per register of two values and a shift per four, instead of two.
-      constexpr int kWidth = BITS == 2 ? 2 : 4, kPerWord = 32 / kWidth;
-      constexpr uint32_t kField = (1u << kWidth) - 1u;
-#pragma unroll
-      for (int w = 0; w < kValWords; ++w)
-#pragma unroll
-        for (int h = 0; h < (BITS == 2 && D == 64 ? 1 : 2); ++h) {
-          uint32_t x[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) x[i] = permute(words[i][0][w], words[i][1][w], h == 0 ? 0x5410 : 0x7632);
-#pragma unroll
-          for (int f = 0; f < kPerWord / 2; f += 2) {
-#pragma unroll
-            for (int up = 0; up < 2; ++up) {
-              uint32_t v[2];
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t mask = kField << (kWidth * up) | kField << (kWidth * up + 16);
-                const uint32_t base = up == 0 ? 0x64006400u : BITS == 2 ? 0x5C005C00u : 0x54005400u;
-                v[i] = sub_f16x2(lop3<kAndOr>(x[i], mask, base), base);
-                v[i] = fma_f16x2(v[i], scale[i], zero[i]);
-              }
-              const int j = w * kPerWord + h * (kPerWord / 2) + f + up;
-#pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                mma_f16(o[m][j], pa[m], v[0], v[1]);
-                if constexpr (Cfg::kSplit) mma_f16(o[m][j], rest[m], v[0], v[1]);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) x[i] >>= 2 * kWidth;
-          }
-        }
+      for (int i = 1; i < Cfg::kGroups; ++i) words[0] = max_magnitudes<T>(words[0], words[i]);
+      const uint32_t room = ((lane & 8) != 0 ? kMostZero : kMostScale) - (words[0] & 0x7fff7fffu);
+      careful = __any_sync(0xffffffffu, (room & 0x80008000u) != 0x80008000u) != 0;
     }
+    auto values = [&](auto careful_way) {
+      constexpr bool kCareful = decltype(careful_way)::value;
+#pragma unroll
+      for (int u = 0; u < kStepTiles; ++u) {
+        const uint8_t* at = st + u * Cfg::kTileStride;
+        uint4 pa[MT], rest[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          pa[m] = make_uint4(pack2<__half>(s[m][2 * u][0], s[m][2 * u][1]), pack2<__half>(s[m][2 * u][2], s[m][2 * u][3]),
+                             pack2<__half>(s[m][2 * u + 1][0], s[m][2 * u + 1][1]), pack2<__half>(s[m][2 * u + 1][2], s[m][2 * u + 1][3]));
+          if constexpr (Cfg::kSplit) {
+            const uint32_t most[4] = {pa[m].x, pa[m].y, pa[m].z, pa[m].w};
+            uint32_t left[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&most[i]));
+              left[i] = pack2<__half>(s[m][2 * u + i / 2][2 * (i % 2)] - x.x, s[m][2 * u + i / 2][2 * (i % 2) + 1] - x.y);
+            }
+            rest[m] = make_uint4(left[0], left[1], left[2], left[3]);
+          }
+        }
+        uint32_t scale[2], zero[2], words[2][2][kValWords];
+        float sc[2][2], ze[2][2];  // of tokens tok_a and tok_b, of the tile's first and second eight
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int ta = tok_a + 8 * i, tb = tok_b + 8 * i;
+          const int group = gid * (D / 8) / 32;
+          const T* scales = reinterpret_cast<const T*>(at + Cfg::kOffScale) + group;
+          const T* zeros = reinterpret_cast<const T*>(at + Cfg::kOffZero) + group;
+          sc[i][0] = ElemTraits<T>::to_float(scales[ta * Cfg::kGroups]); sc[i][1] = ElemTraits<T>::to_float(scales[tb * Cfg::kGroups]);
+          ze[i][0] = ElemTraits<T>::to_float(zeros[ta * Cfg::kGroups]); ze[i][1] = ElemTraits<T>::to_float(zeros[tb * Cfg::kGroups]);
+          if (!full) {  // the bytes of tokens that are not there may be anything
+            if (tok_a >= there(2 * u + i)) sc[i][0] = ze[i][0] = 0.0f;
+            if (tok_b >= there(2 * u + i)) sc[i][1] = ze[i][1] = 0.0f;
+          }
+          const uint8_t* codes = at + Cfg::kOffVal + gid * (Cfg::kValBytes / 8);
+          if constexpr (BITS == 2 && D == 64) {
+            words[i][0][0] = *reinterpret_cast<const uint16_t*>(codes + ta * Cfg::kValBytes);
+            words[i][1][0] = *reinterpret_cast<const uint16_t*>(codes + tb * Cfg::kValBytes);
+          } else {
+            load_words<kValWords>(codes + ta * Cfg::kValBytes, words[i][0]);
+            load_words<kValWords>(codes + tb * Cfg::kValBytes, words[i][1]);
+          }
+        }
+        if constexpr (kCareful) {
+          const float most_scale = max_nan(max_nan(fabsf(sc[0][0]), fabsf(sc[0][1])), max_nan(fabsf(sc[1][0]), fabsf(sc[1][1])));
+          const float most_zero = max_nan(max_nan(fabsf(ze[0][0]), fabsf(ze[0][1])), max_nan(fabsf(ze[1][0]), fabsf(ze[1][1])));
+          if (__any_sync(0xffffffffu, !exact && !(fmaf(most_zero, 1.0f / kCodes, most_scale) * lift <= 32768.0f / kCodes))) {
+            float reach = 0.0f;  // the column's largest value, in codes
+            bool fine = true;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float a = fabsf(sc[i / 2][i % 2]), z = fabsf(ze[i / 2][i % 2]);
+              if (a < INFINITY && z < INFINITY) reach = fmaxf(reach, fminf(fmaf(z, 1.0f / kCodes, a), 3.0e38f));
+              else fine = false;
+            }
+            reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 1));
+            reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 2));
+            float next = lift;
+            if (reach * lift > 32768.0f / kCodes)  // to between 2^11 and 2^12
+              next = __uint_as_float((uint32_t)(127 + 11 + 127 - (BITS == 2 ? 2 : 4)) * (1u << 23) - (__float_as_uint(reach) & 0x7f800000u));
+            exact = __any_sync(0xffffffffu, cut && (!fine || (next != lift && next < 1.0f))) != 0;
+            if (exact) next = 1.0f;
+            lift_columns(next / lift);
+            lift = next;
+            lifted = exact || __any_sync(0xffffffffu, lift != 1.0f) != 0;
+          }
+          if (exact) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) exact_tokens([&](int m, int k) { return s[m][2 * u + i][2 * k + r]; }, at, 8 * i, r);
+            }
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              sc[i][k] *= lift;
+              ze[i][k] *= lift;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          scale[i] = pack2<__half>(sc[i][0], sc[i][1]);
+          zero[i] = pack2<__half>(ze[i][0], ze[i][1]);
+        }
+        // A code in the lowest bits under the exponent of 1024 reads as 1024 + code in fp16, one a field higher under the exponent of 64
+        // (2-bit codes: 256) as 64 + code, and taking that off is exact.  So one shift serves the two fields of a byte: the logic pipe,
+        // which binds this kernel, has one operation per register of two values and a shift per four, instead of two.
+        constexpr int kWidth = BITS == 2 ? 2 : 4, kPerWord = 32 / kWidth;
+        constexpr uint32_t kField = (1u << kWidth) - 1u;
+#pragma unroll
+        for (int w = 0; w < kValWords; ++w)
+#pragma unroll
+          for (int h = 0; h < (BITS == 2 && D == 64 ? 1 : 2); ++h) {
+            uint32_t x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[i] = permute(words[i][0][w], words[i][1][w], h == 0 ? 0x5410 : 0x7632);
+#pragma unroll
+            for (int f = 0; f < kPerWord / 2; f += 2) {
+#pragma unroll
+              for (int up = 0; up < 2; ++up) {
+                uint32_t v[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const uint32_t mask = kField << (kWidth * up) | kField << (kWidth * up + 16);
+                  const uint32_t base = up == 0 ? 0x64006400u : BITS == 2 ? 0x5C005C00u : 0x54005400u;
+                  v[i] = sub_f16x2(lop3<kAndOr>(x[i], mask, base), base);
+                  v[i] = fma_f16x2(v[i], scale[i], zero[i]);
+                }
+                const int j = w * kPerWord + h * (kPerWord / 2) + f + up;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                  mma_f16(o[m][j], pa[m], v[0], v[1]);
+                  if constexpr (Cfg::kSplit) mma_f16(o[m][j], rest[m], v[0], v[1]);
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 2; ++i) x[i] >>= 2 * kWidth;
+            }
+          }
+      }
+    };
+    if (careful) values(std::true_type{});
+    else values(std::false_type{});
   }
+
+  if (lifted) lift_columns(1.0f / lift);
 
   // ---- un-quantized window ring ------------------------------------------------------------------------------------------------
   const int w0 = max(t0, lq);
@@ -832,41 +949,20 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
     }
   }
 
-  // Adds the infinite and NaN values that the products left out, at the row's dims d .. d + 3.
+  // Adds the infinite and NaN values of the window that its products left out, at the row's dims d .. d + 3.
   auto strange_values = [&](int row, int d, float4& sum) {
-    const int seen = min(t1 - 1, first_seen + multi_token_of(p, row));
-    for (int t = max(t0, first_seen - kStepTiles * kTile); t <= seen; ++t) {
+    const int seen = min(t1 - 1, first_seen + multi_token_of(p, row)), w0 = max(t0, lq);
+    for (int t = max(w0, first_seen - kTile); t <= seen; ++t) {
+      if (w0 + (t - w0) / kTile * kTile + kTile - 1 <= first_seen) continue;  // of a tile that was not cut
+      const T* value = reinterpret_cast<const T*>(p.window) +
+                       (((p.window_slots[b] * 2 + 1) * p.kv_heads + kvh) * p.residual_len + t % p.residual_len) * D + d;
       float v[4];
-      bool fine = true;
-      if (t < lq) {
-        if (t0 + (t - t0) / (kStepTiles * kTile) * (kStepTiles * kTile) + kStepTiles * kTile - 1 <= first_seen) continue;
-        const int blk = t / p.block_size, at = t - blk * p.block_size;
-        const int32_t pid = blk < p.max_blocks ? table[blk] : -1;
-        if (pid < 0 || pid >= p.num_pages) continue;
-        const uint8_t* page = p.pages + ((int64_t)pid * p.kv_heads + kvh) * p.layout.chunk_bytes;
-        const float scale = ElemTraits<T>::to_float(reinterpret_cast<const T*>(page + p.layout.off_vscale)[at * Cfg::kGroups + d / 32]);
-        const float zero = ElemTraits<T>::to_float(reinterpret_cast<const T*>(page + p.layout.off_vzero)[at * Cfg::kGroups + d / 32]);
-        fine = finite_f16(fabsf(zero) + (BITS == 2 ? 4.0f : 16.0f) * fabsf(scale));
-        constexpr int kWidth = BITS == 2 ? 2 : 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int bit = (d + i) * kWidth;
-          const uint32_t code = (page[p.layout.off_vdata + at * Cfg::kValBytes + bit / 8] >> (bit % 8)) & ((1u << kWidth) - 1u);
-          v[i] = __half2float(__float2half_rn(fmaf((float)code, scale, zero)));
-        }
-      } else {
-        const int w0 = max(t0, lq);
-        if (w0 + (t - w0) / kTile * kTile + kTile - 1 <= first_seen) continue;
-        const T* value = reinterpret_cast<const T*>(p.window) +
-                         (((p.window_slots[b] * 2 + 1) * p.kv_heads + kvh) * p.residual_len + t % p.residual_len) * D + d;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = ElemTraits<T>::to_float(value[i]);
-          if (isfinite(v[i])) v[i] = 0.0f;  // is in the product
-          else fine = false;
-        }
+      for (int i = 0; i < 4; ++i) {
+        v[i] = ElemTraits<T>::to_float(value[i]);
+        if (isfinite(v[i])) v[i] = 0.0f;  // is in the product
       }
-      if (!fine) { sum.x += v[0]; sum.y += v[1]; sum.z += v[2]; sum.w += v[3]; }
+      sum.x += v[0]; sum.y += v[1]; sum.z += v[2]; sum.w += v[3];
     }
   };
 
