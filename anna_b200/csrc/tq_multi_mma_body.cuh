@@ -21,7 +21,8 @@
 // leave.  32 rows a CTA (two row tiles) unpack a key once for both, with half the warps: 8 new tokens 395 us, twice 260 as two calls.
 //
 // What is rounded below 32 bits: the rotated queries, centroids and residual norms to fp16 (2^-12 of the row's largest value, of the
-// centroid and of the norm), value scales and zeros, probabilities and values to fp16 (2^-12 of themselves).  Together they stay
+// centroid and of the norm), value scales and zeros, probabilities and values to fp16 (2^-12 of themselves; for small ones see
+// kTopLog2).  Together they stay
 // below the rounding of a bf16 output (2^-9 of the value); for fp16 see kSplit.
 // Below 2^-14 fp16 has fewer bits, down to 2^-24.  Values beyond its range keep to it by powers of two: see `lift`.
 #pragma once
@@ -37,7 +38,11 @@ constexpr int kMultiMmaWarps = 8, kMultiMmaThreads = 32 * kMultiMmaWarps;
 constexpr int kTile = 16;        // tokens
 constexpr int kStepTiles = 2;    // tiles of a step: one softmax update
 constexpr int kRingStages = 2;   // steps of a warp's ring
-constexpr float kMoveLimit = 8.0f;  // log2 units by which a running maximum may be exceeded: probabilities stay below 2^8
+// Probabilities are fp16 in the value product, whose range goes from 2^15 down to 2^-24: the running maximum stands at 2^7, and may be
+// exceeded by 2^8 before it moves.  So a weight has all its bits down to 2^-21 of the largest, and what is rounded below is at most
+// 2^-32 of it: of n such keys together, n * 2^-32.  (With the maximum at 1, 2^-25 of it: beside one key of 99 % of the weight the others
+// of 32768 were off by 2.5e-4 of the output, those of 99.9 % by 2.6e-2.)
+constexpr float kMoveLimit = 8.0f, kTopLog2 = 7.0f;
 
 template <typename T, int D, int BITS, int MT>
 struct MultiCfg {
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float base = m_run[m][k] == -INFINITY ? 0.0f : f_row[k] * m_run[m][k];
+        const float base = m_run[m][k] == -INFINITY ? 0.0f : fmaf(f_row[k], m_run[m][k], -kTopLog2);
         float2 sum = make_float2(l_run[m][k], 0.0f);
 #pragma unroll
         for (int c = 0; c < N; ++c) {

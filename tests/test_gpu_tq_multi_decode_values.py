@@ -3,6 +3,8 @@
 Limits beside those of test_gpu_tq_multi_decode.py are derived at each test."""
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -82,3 +84,48 @@ def test_values_beyond_fp16(cuda_device, dim, bits, page, tokens, group):
     put_values(case, 1, 20, 0, 0, scale=1e30, zero=-1e30)
     put_values(case, 1, 35, 0, 1, scale=1e20, zero=0.0)
     check_each(case, case.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,kv_heads,group", [(128, 8, 2), (256, 4, 2), (64, 8, 2), (128, 4, 12)])
+@pytest.mark.parametrize("sink", [0, 33, -1])
+def test_small_weights_beside_one_that_is_large(cuda_device, dtype, dim, kv_heads, group, sink):
+    """One key has the weight 2^26 times that of each of the 4111 others, and a value of zero: the output is what the others hold together.
+    A stream is one CTA's, whose warp with that key has an eighth of the others.
+
+    Small weights are off by 2^-32 of the large one, 2^-6 of themselves here; the large key's score by what Case.check allows of it (the sum
+    of the others is off by as much of itself), all other roundings by 2 * 2^-12 of the output and half a step of it."""
+    length, window = 4112, 16
+    case = Case(lengths=[length], tokens=2, group=group, kv_heads=kv_heads, dim=dim, bits=4, page=16, window=window, dtype=dtype,
+                device=cuda_device, seed=21)
+    at = sink % (length - window)
+    layout, pages, page, groups = case.layout, case.packed.shape[0], case.page, dim // 32
+
+    def put(name, values, width):
+        case.packed[:, :, layout[name]:layout[name] + page * width] = values.contiguous().view(torch.uint8).reshape(pages, kv_heads, -1)
+
+    small = 2.0 ** -20
+    key = case.dense[0][0][:, at]  # of each KV head
+    old = case.packed[int(case.table[0, at // page]), :, layout["off_knorm"]:layout["off_knorm"] + 4 * page].contiguous().view(torch.float32)
+    unit = key / old[:, at % page].double().numpy()[:, None]
+    query = torch.from_numpy(unit / np.linalg.norm(unit, axis=1, keepdims=True) * math.sqrt(dim)).to(case.dtype)
+    norm = torch.full((pages, kv_heads, page), small)
+    score = 26 * math.log(2.0)
+    norm[int(case.table[0, at // page]), :, at % page] = torch.from_numpy(score / ((query.double().numpy() * unit).sum(1) * case.scaling)).float()
+    put("off_knorm", norm, 4)
+    put("off_vscale", torch.zeros(pages, kv_heads, page, groups, dtype=case.dtype), 2 * groups)
+    zero = torch.ones(pages, kv_heads, page, groups, dtype=case.dtype)
+    zero[int(case.table[0, at // page]), :, at % page] = 0
+    put("off_vzero", zero, 2 * groups)
+    case.window_ring[:, 0] = 0
+    case.window_ring[:, 1] = 1
+    batch = 37
+    case.query = query[:, None, None].expand(kv_heads, group, 2, dim).reshape(1, -1, 2, dim).repeat(batch, 1, 1, 1)
+    case.table, case.slots, case.lengths = case.table.repeat(batch, 1), case.slots.repeat(batch), [length] * batch
+    got = case.run().cpu().double()
+    others = torch.tensor([length - 2.0, length - 1.0]).double() * math.exp(-score)  # all keys but the large one, and those behind the query
+    want = (others / (1 + others))[None, None, :, None].expand(got.shape)
+    largest = math.sqrt(math.pi / 2) * score * (2.0 ** -12 * (2.0 * math.sqrt(2 * math.log(2 * dim)) + 2) + 2 * dim * 2.0 ** -24)
+    limit = want * (2.0 ** -6 + math.expm1(largest) + 2 * 2.0 ** -12 + torch.finfo(case.dtype).eps / 2 + 1e-3)
+    assert float(((got - want).abs() / limit).max()) <= 1.0
