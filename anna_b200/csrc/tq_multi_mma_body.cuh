@@ -903,7 +903,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
           s[m][c][r] = in_tile >= valid || ts + in_tile > row_limit[16 * m + gid + 8 * (r / 2)] ? -INFINITY : x;
         }
     softmax(s, std::integral_constant<int, 2>{});
-    // bf16 probabilities as a sum of two, so that they keep 16 bits
+    // probabilities as a sum of two of the type, so that they keep 16 bits and more
     uint4 pa[MT], pb[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -913,8 +913,12 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
       for (int i = 0; i < 4; ++i) {
         const float x = s[m][i / 2][2 * (i % 2)], y = s[m][i / 2][2 * (i % 2) + 1];
         hi[i] = pack2<T>(x, y);
-        if constexpr (!std::is_same_v<T, __half>)
+        if constexpr (std::is_same_v<T, __half>) {
+          const float2 most = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+          lo[i] = pack2<T>(x - most.x, y - most.y);
+        } else {
           lo[i] = pack2<T>(x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u));
+        }
       }
     }
     const T* v[4] = {values + ring_row(tok_a) + gid * (D / 8), values + ring_row(tok_b) + gid * (D / 8),
@@ -948,7 +952,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           mma_elem<T>(o[m][8 * x + i], pa[m], v0, v1);
-          if constexpr (!std::is_same_v<T, __half>) mma_elem<T>(o[m][8 * x + i], pb[m], v0, v1);
+          mma_elem<T>(o[m][8 * x + i], pb[m], v0, v1);
         }
       }
     }

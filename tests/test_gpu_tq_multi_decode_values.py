@@ -3,12 +3,15 @@
 Limits beside those of test_gpu_tq_multi_decode.py are derived at each test."""
 from __future__ import annotations
 
+import itertools
 import math
 
 import numpy as np
 import pytest
 import torch
-from test_gpu_tq_multi_decode import Case
+from test_gpu_tq_multi_decode import Case, hadamard
+
+from anna_b200.tq_tables import key_tables
 
 
 def value_parts(case, name, pid, head, slot, group):
@@ -129,3 +132,82 @@ def test_small_weights_beside_one_that_is_large(cuda_device, dtype, dim, kv_head
     largest = math.sqrt(math.pi / 2) * score * (2.0 ** -12 * (2.0 * math.sqrt(2 * math.log(2 * dim)) + 2) + 2 * dim * 2.0 ** -24)
     limit = want * (2.0 ** -6 + math.expm1(largest) + 2 * 2.0 ** -12 + torch.finfo(case.dtype).eps / 2 + 1e-3)
     assert float(((got - want).abs() / limit).max()) <= 1.0
+
+
+def packed_parts(case):
+    """(centroid numbers, signs, norms, residual norms) of the codes in a 4-bit case's pages."""
+    pages, heads, page, dim, layout = case.packed.shape[0], case.kv_heads, case.page, case.dim, case.layout
+
+    def part(name, size, kind):
+        return case.packed[:, :, layout[name]:layout[name] + size].contiguous().view(kind).reshape(pages, heads, page, -1).numpy()
+
+    codes = part("off_kcodes", page * dim // 2, torch.uint8)
+    nibbles = np.stack([codes & 15, codes >> 4], -1).reshape(pages, heads, page, dim)
+    return nibbles & 7, nibbles >> 3, part("off_knorm", 4 * page, torch.float32)[..., 0], part("off_krnorm", 4 * page, torch.float32)[..., 0]
+
+
+def rounded(case):
+    """The outputs of 64-bit arithmetic in which what the kernel's header names is rounded: the rotated queries to fp16, relative to the
+    largest (of fp16 caches those of the residual part alone, the others being sums of two), centroids and residual norms to fp16 at the
+    scale where an fp16 cache's centroids lose least, the packed values to fp16, the probabilities of a bf16 cache's packed keys to fp16,
+    and the output to its type."""
+    half = lambda x: np.asarray(x, np.float16).astype(np.float64)  # noqa: E731
+    fp16 = case.dtype == torch.float16
+    tables = key_tables(head_dim=case.dim, bits=4, device="cpu")
+    centroids, s1, s2 = (x.numpy().astype(float) for x in (tables.centroids, tables.signs1, tables.signs2))
+    h, (index, sign, norm, rnorm) = hadamard(case.dim), packed_parts(case)
+    scales = 1 + np.arange(512 if fp16 else 1)[:, None] / 512
+    at = float(scales[np.argmin(((centroids * scales - half(centroids * scales)) ** 2 / scales ** 2).sum(1))][0])
+    out = torch.zeros(case.query.shape, dtype=torch.float64)
+    for b, (k, v) in enumerate(case.dense):
+        n, lq = case.lengths[b], case.quantized[b]
+        where = case.table[b].numpy()[np.arange(lq) // case.page], np.arange(lq) % case.page
+        for head, t in itertools.product(range(case.query.shape[1]), range(case.tokens)):
+            kvh = head // case.group
+            cells = where[0], kvh, where[1]
+            query = case.query[b, head, t].double().numpy()
+            q1 = h @ (s1 * query)
+            q2 = math.sqrt(math.pi / 2 / case.dim) * (h @ (s2 * q1))
+            top = max(np.abs(q1).max(), np.abs(q2).max())
+            score = (half(centroids * at) / at)[index[cells]] @ (q1 / top if fp16 else half(q1 / top))
+            score += half(rnorm[cells] * at) / at * ((2.0 * sign[cells] - 1) @ half(q2 / top))
+            score = np.concatenate([score * norm[cells] / case.dim * top, k[kvh][lq:] @ query]) * case.scaling
+            score = score[:n - case.tokens + t + 1]
+            w = np.exp(score - score.max())
+            w_v = w if fp16 else np.concatenate([half(w[:lq] * 128) / 128, w[lq:]])
+            out[b, head, t] = torch.from_numpy(w_v @ np.concatenate([half(v[kvh][:lq]), v[kvh][lq:]])[:len(w)] / w.sum())
+    return out.to(case.dtype).double()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,group,window,length", [
+    ("fp16", 128, 4, 128, 3000), ("fp16", 128, 16, 128, 2000), ("fp16", 256, 32, 64, 1500), ("fp16", 64, 8, 33, 1500), ("fp16", 128, 4, 256, 250),
+    ("fp16", 256, 8, 512, 480), ("bf16", 128, 4, 128, 3000), ("bf16", 256, 32, 64, 1500), ("bf16", 128, 4, 256, 250)])
+@pytest.mark.parametrize("exact_values", [False, True])
+def test_error_of_whole_outputs(cuda_device, dtype, dim, group, window, length, exact_values):
+    """Root mean square of the errors: that of 64-bit arithmetic with the roundings which the kernel says it makes, and 3 % for 32-bit
+    sums and for chance (thousands of outputs).  With residual norms of zero and values that fp16 holds, little is left but the output's own
+    rounding, so that queries or probabilities of a single fp16 would show in an fp16 cache."""
+    case = Case(lengths=[length], tokens=4, group=group, kv_heads=2, dim=dim, bits=4, page=16, window=window, dtype=dtype, device=cuda_device, seed=31)
+    if exact_values:
+        for t in range(case.quantized[0]):
+            pid, slot = int(case.table[0, t // 16]), t % 16
+            case.packed[pid, :, case.layout["off_krnorm"] + 4 * slot:case.layout["off_krnorm"] + 4 * slot + 4] = 0
+            for head, part in itertools.product(range(2), range(dim // 32)):
+                put_values(case, 0, t, head, part, scale=0.125, zero=(t * 7 + head + part) % 5 / 8 - 1)
+        case.dense[0][0][:, :case.quantized[0]] = keys_of(case)
+    want, _, _ = case.expected()
+    got = case.run().cpu().double()
+    rms = lambda x: float((x - want).square().mean().sqrt() / want.square().mean().sqrt())  # noqa: E731
+    print(f"{rms(got):.3e} and {rms(rounded(case)):.3e}")
+    assert rms(got) <= 1.03 * rms(rounded(case))
+
+
+def keys_of(case):
+    """De-quantized keys of sequence 0 of a 4-bit case, [KV heads, tokens, D]."""
+    tables, (index, sign, norm, rnorm) = key_tables(head_dim=case.dim, bits=4, device="cpu"), packed_parts(case)
+    t = np.arange(case.quantized[0])
+    index, sign, norm, rnorm = (x[case.table[0].numpy()[t // case.page], :, t % case.page].swapaxes(0, 1) for x in (index, sign, norm, rnorm))
+    h, s1, s2 = hadamard(case.dim), tables.signs1.numpy().astype(float), tables.signs2.numpy().astype(float)
+    rotated = tables.centroids.numpy().astype(float)[index] + math.sqrt(math.pi / 2 / case.dim) * rnorm[..., None] * (((2.0 * sign - 1.0) @ h) * s2)
+    return norm[..., None] / case.dim * (rotated @ h) * s1
