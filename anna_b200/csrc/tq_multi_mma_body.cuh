@@ -24,7 +24,8 @@
 // centroid and of the norm), value scales and zeros, probabilities and values to fp16 (2^-12 of themselves; for small ones see
 // kTopLog2).  Together they stay
 // below the rounding of a bf16 output (2^-9 of the value); for fp16 see kSplit.
-// Below 2^-14 fp16 has fewer bits, down to 2^-24.  Values beyond its range keep to it by powers of two: see `lift`.
+// Values beyond fp16's range keep to it by powers of two (see `lift`), so that beside this they are off by 2^-25 of the largest of a group's
+// dims in the keys of a tile of rows, at most.
 #pragma once
 
 #include "mbarrier_utils.cuh"
@@ -358,6 +359,22 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
   for (int i = 0; i < kRingStages - 1; ++i)
     if (i < my_steps) issue(i, (stage + i) % kRingStages);
 
+  // Scale and zero of this lane's column as B operand in one of the first tile's tokens 3, 7, 11 and 15, on their way behind the copies.
+  T first_scale = T(0.0f), first_zero = T(0.0f);
+  if constexpr (!std::is_same_v<T, __half>) {
+    if (my_steps > 0) {
+      const int in_tile = min(4 * tig + 3, q_end - 1 - t0 - warp * (kStepTiles * kTile)), ts = t0 + warp * (kStepTiles * kTile) + in_tile;
+      const int32_t pid = __shfl_sync(0xffffffffu, ids, in_tile / piece_tokens);
+      if (pid >= 0 && pid < p.num_pages) {
+        const int at = p.block_shift >= 0 ? ts & (p.block_size - 1) : ts % p.block_size;
+        const uint8_t* page = p.pages + ((int64_t)pid * p.kv_heads + kvh) * p.layout.chunk_bytes;
+        const int where = at * Cfg::kGroups + gid * (D / 8) / 32;
+        first_scale = reinterpret_cast<const T*>(page + p.layout.off_vscale)[where];
+        first_zero = reinterpret_cast<const T*>(page + p.layout.off_vzero)[where];
+      }
+    }
+  }
+
   // ---- rotated queries as A fragments ----------------------------------------------------------------------------------------
   float* factor = reinterpret_cast<float*>(smem + Cfg::kOffFactor);
   int* row_limit = reinterpret_cast<int*>(smem + Cfg::kOffLimit);
@@ -502,6 +519,19 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
   constexpr float kCodes = BITS == 2 ? 4.0f : 16.0f;  // above all codes
   float lift = 1.0f;
   bool exact = false, lifted = false;  // lifted: not every column at 1, or exact
+  auto lift_for = [&](float reach) {  // takes reach * kCodes to between 2^11 and 2^12
+    return __uint_as_float((uint32_t)(127 + 11 + 127 - (BITS == 2 ? 2 : 4)) * (1u << 23) - (__float_as_uint(fmaxf(reach, 0x1p-100f)) & 0x7f800000u));
+  };
+  // A bf16 cache may hold values far below fp16's range, too: a column whose first values stay below 2^-6 (or are zero, or in a hole) begins at
+  // a power above 1.  An fp16 cache's scales and zeros are multiples of 2^-24, and so are its values.
+  if constexpr (!std::is_same_v<T, __half>) {
+    const float a = fabsf(ElemTraits<T>::to_float(first_scale)), z = fabsf(ElemTraits<T>::to_float(first_zero));
+    float reach = a < INFINITY && z < INFINITY ? fmaf(z, 1.0f / kCodes, a) : 0.0f;
+    reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 1));
+    reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 2));
+    if (my_steps > 0 && reach < 0.015625f / kCodes) lift = lift_for(reach);
+    lifted = __any_sync(0xffffffffu, lift != 1.0f) != 0;
+  }
   // Steps whose scales and zeros stay below 2^14 (over the codes) look no further as long as no column is lifted: 2^14 in the type's bits,
   // each half with a bit on top that a larger magnitude, infinity and NaN take away.
   constexpr uint32_t kOne = std::is_same_v<T, __half> ? 15 << 10 : 127 << 7, kPower = std::is_same_v<T, __half> ? 1 << 10 : 1 << 7;
@@ -776,8 +806,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
             reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 1));
             reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 2));
             float next = lift;
-            if (reach * lift > 32768.0f / kCodes)  // to between 2^11 and 2^12
-              next = __uint_as_float((uint32_t)(127 + 11 + 127 - (BITS == 2 ? 2 : 4)) * (1u << 23) - (__float_as_uint(reach) & 0x7f800000u));
+            if (reach * lift > 32768.0f / kCodes) next = lift_for(reach);
             exact = __any_sync(0xffffffffu, cut && (!fine || (next != lift && next < 1.0f))) != 0;
             if (exact) next = 1.0f;
             lift_columns(next / lift);

@@ -211,3 +211,41 @@ def keys_of(case):
     h, s1, s2 = hadamard(case.dim), tables.signs1.numpy().astype(float), tables.signs2.numpy().astype(float)
     rotated = tables.centroids.numpy().astype(float)[index] + math.sqrt(math.pi / 2 / case.dim) * rnorm[..., None] * (((2.0 * sign - 1.0) @ h) * s2)
     return norm[..., None] / case.dim * (rotated @ h) * s1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,bits,page", [(128, 4, 16), (256, 3, 16), (64, 2, 16), (128, 2, 24), (64, 4, 8), (128, 4, 12)])
+@pytest.mark.parametrize("tokens,group", [(3, 2), (4, 4), (40, 3)])
+@pytest.mark.parametrize("power", [-6, -12, -17, -40, -90])
+def test_small_values(cuda_device, dim, bits, page, tokens, group, power):
+    """bf16 values down to 1e-27, as exact as others."""
+    case = Case(lengths=[700, 90, 33], tokens=tokens, group=group, kv_heads=2, dim=dim, bits=bits, page=page, window=9, dtype="bf16",
+                device=cuda_device, seed=17)
+    pages, groups = case.packed.shape[0], dim // 32
+    for name in ("off_vscale", "off_vzero"):
+        part = case.packed[:, :, case.layout[name]:case.layout[name] + page * groups * 2]
+        scaled = part.contiguous().view(torch.bfloat16).double().mul(2.0 ** power).to(torch.bfloat16)
+        part.copy_(scaled.view(torch.uint8).reshape(pages, 2, -1))
+    case.window_ring[:, 1] *= 2.0 ** power
+    for b in range(3):
+        case.dense[b][1][:] *= 2.0 ** power
+    check_each(case, case.run(), floor=0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,bits,page", [(128, 4, 16), (256, 3, 16), (64, 2, 16), (128, 2, 24)])
+@pytest.mark.parametrize("tokens,group", [(3, 2), (12, 6)])
+def test_small_and_ordinary_values_together(cuda_device, dim, bits, page, tokens, group):
+    """A group of dims with small values beside others, one that is zero at first, and one where an ordinary value comes late."""
+    case = Case(lengths=[700, 90], tokens=tokens, group=group, kv_heads=2, dim=dim, bits=bits, page=page, window=9, dtype="bf16",
+                device=cuda_device, seed=18)
+    for t in range(case.quantized[0]):
+        put_values(case, 0, t, 0, 1, scale=2e-7 * (1 + t % 7), zero=1e-6 * (t % 5 - 2))
+        late = t in (400, 689)
+        put_values(case, 0, t, 1, 0, scale=0.1 if late else 1e-6, zero=0.5 if late else 1e-5)
+        put_values(case, 0, t, 1, 1, scale=0.0 if t < 300 else 1e-6, zero=0.0 if t < 300 else 1e-5)
+    case.window_ring[case.slots[0], 1, 0, :, 32:64] *= 1e-6
+    case.window_ring[case.slots[0], 1, 1, :, :64] *= 1e-6
+    for t in range(case.quantized[0], 700):
+        case.dense[0][1][:, t] = case.window_ring[case.slots[0], 1, :, t % 9].double().numpy()
+    check_each(case, case.run(), floor=0.0)
