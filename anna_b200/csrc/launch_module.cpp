@@ -826,7 +826,8 @@ PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   // One token is the single-token decode (one row of 4000 tokens, 32/8 heads: 11.5 us there, 20.5 here), in scratch of its own; but pages
   // of an odd number of eights it reads on CUDA cores only (17 rows of 6-29 K tokens, 2/1 heads, pages of 24: 88 us there, 38 here).
   const bool eights = n[2] % 16 == 8 && code != ANNA_DTYPE_F32 && n[3] == 32;
-  if (tokens == 1 && !eights) {
+  const bool groups = n[3] % (code == ANNA_DTYPE_F32 ? 4 : 8) == 0;  // that it takes
+  if (tokens == 1 && !eights && groups) {
     int chunk = 0, chunks = 0;
     status = anna_tq_decode_plan((int)batch, kv_heads, max_blocks, (int)n[2], (int)n[1], &chunk, &chunks);
     if (status != 0) return failed("tq_paged_multi_decode", status);

@@ -249,3 +249,12 @@ def test_small_and_ordinary_values_together(cuda_device, dim, bits, page, tokens
     for t in range(case.quantized[0], 700):
         case.dense[0][1][:, t] = case.window_ring[case.slots[0], 1, :, t % 9].double().numpy()
     check_each(case, case.run(), floor=0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_small_value_groups(cuda_device, tokens):
+    for dtype, group in (("fp16", 4), ("bf16", 2), ("fp32", 2), ("fp32", 4), ("bf16", 8)):
+        case = Case(lengths=[90, 3], tokens=tokens, group=2, kv_heads=1, dim=128, bits=4, page=16, window=8, dtype=dtype, device=cuda_device,
+                    value_group=group)
+        case.check(case.run())
