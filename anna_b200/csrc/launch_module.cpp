@@ -823,11 +823,12 @@ PyObject* tq_multi_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const uint8_t* page_ptr = max_blocks > 0 ? static_cast<const uint8_t*>(pages->data_ptr()) : nullptr;
   const int32_t* table_ptr = max_blocks > 0 ? static_cast<const int32_t*>(table->data_ptr()) : nullptr;
   int status;
-  // One token is the single-token decode (one row of 4000 tokens, 32/8 heads: 11.5 us there, 20.5 here), in scratch of its own; but pages
-  // of an odd number of eights it reads on CUDA cores only (17 rows of 6-29 K tokens, 2/1 heads, pages of 24: 88 us there, 38 here).
-  const bool eights = n[2] % 16 == 8 && code != ANNA_DTYPE_F32 && n[3] == 32;
-  const bool groups = n[3] % (code == ANNA_DTYPE_F32 ? 4 : 8) == 0;  // that it takes
-  if (tokens == 1 && !eights && groups) {
+  // One token is the single-token decode, in scratch of its own, where that has 32 bits (CUDA cores: fp32 caches, pages or value groups that
+  // tensor cores do not read).  Elsewhere it scores with 8-bit queries, which one token of an answer must not have and the same token
+  // among several not: the caller chooses that with tq_paged_decode (one row of 4000 tokens, 32/8 heads: 13.4 us there, 18.5 here; 16 rows of
+  // 32768: 164 and 264).
+  const bool single = tokens == 1 && (code == ANNA_DTYPE_F32 || n[2] % 8 != 0 || n[3] != 32) && n[3] % (code == ANNA_DTYPE_F32 ? 4 : 8) == 0;
+  if (single) {
     int chunk = 0, chunks = 0;
     status = anna_tq_decode_plan((int)batch, kv_heads, max_blocks, (int)n[2], (int)n[1], &chunk, &chunks);
     if (status != 0) return failed("tq_paged_multi_decode", status);

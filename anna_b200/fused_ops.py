@@ -682,37 +682,17 @@ def _op_tq_paged_decode(query, packed_pages, page_table, window, window_slots, l
     return out
 
 
-def multi_scratch(device: torch.device, batch: int, heads: int, kv_heads: int, tokens: int, head_dim: int):
-    """(scratch, counters) of a multi-token decode.  The scratch is the call's own; the counters, zero between calls, are the
-    stream's, or under a graph capture the graph's (graphs may be replayed side by side)."""
-    floats, arrivals = _lib.tq_multi_decode_plan(batch, heads, kv_heads, tokens, head_dim)
-    scratch = torch.empty(floats, dtype=torch.float32, device=device)
-    with on_device(device):
-        if torch.cuda.is_current_stream_capturing():
-            return scratch, torch.zeros(arrivals, dtype=torch.int32, device=device)
-    return scratch, _SCRATCH.counters(device, arrivals)
-
-
-def multi_decode(name, query, packed_pages, page_table, window, window_slots, lengths, tables, scaling, gate, *, kv_heads, bits,
-                 residual_len, block_size, value_group):
-    """Launch of the multi-token decode on arguments that have been checked; pages and table may be None."""
-    device = query.device
-    batch, heads, tokens, dim = (int(v) for v in query.shape)
-    query = _last_dim_contiguous(query)
-    gate = None if gate is None else _last_dim_contiguous(gate)
-    out = torch.empty((batch, heads, tokens, dim), dtype=query.dtype, device=device)
-    if out.numel() == 0:
-        return out
-    max_blocks = 0 if page_table is None else int(page_table.shape[1])
-    scratch, counters = multi_scratch(device, batch, heads, kv_heads, tokens, dim)
-    with on_device(device):
-        _lib.check(_lib.lib().anna_tq_paged_multi_decode(
-            ptr(query), *query.stride()[:3], ptr(packed_pages) if max_blocks else None, ptr(page_table) if max_blocks else None,
-            page_table.stride(0) if max_blocks else 0, ptr(window), ptr(window_slots), ptr(lengths), ptr(tables.signs1),
-            ptr(tables.signs2), ptr(tables.centroids), ptr(gate), *((0, 0, 0) if gate is None else gate.stride()[:3]), ptr(out),
-            *out.stride()[:3], ptr(scratch), scratch.numel(), ptr(counters), batch, heads, kv_heads, tokens, dim, block_size,
-            residual_len, bits, value_group, int(packed_pages.shape[0]) if max_blocks else 0, max_blocks, float(scaling),
-            dtype_code(query.dtype), stream_ptr(device)), name)
+def multi_decode(name, query, packed_pages, page_table, window, window_slots, lengths, tables, scaling, gate, *, bits, residual_len,
+                 block_size, value_group):
+    """Launch of the multi-token decode on arguments that have been checked, query and gate in the layout that the kernels read; pages and
+    table may be None."""
+    if query.numel() == 0:
+        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    out = launch_module().tq_multi_decode(_last_dim_contiguous(query), None if gate is None else _last_dim_contiguous(gate), packed_pages,
+                                          page_table, window, window_slots, lengths, tables.signs1, tables.signs2, tables.centroids,
+                                          float(scaling), bits, residual_len, block_size, value_group)
+    if out is None:
+        raise RuntimeError(f"{name}: arguments that the kernels do not take")
     return out
 
 
@@ -748,8 +728,7 @@ def _op_tq_paged_multi_decode(query, packed_pages, page_table, window, window_sl
         page_table = page_table.contiguous()
     tables = key_tables(head_dim=dim, bits=bits, device=device)
     return multi_decode(name, query, packed_pages, page_table, window, window_slots.contiguous(), lengths.contiguous(), tables, scaling,
-                        gate, kv_heads=kv_heads, bits=bits, residual_len=residual_len, block_size=block_size,
-                        value_group=value_group_size)
+                        gate, bits=bits, residual_len=residual_len, block_size=block_size, value_group=value_group_size)
 
 
 _IMPLS = {
@@ -923,7 +902,8 @@ def run_tq_paged_multi_decode(*, query, packed_pages, page_table, window, window
     """Attention of the newest T tokens of every row over a packed TurboQuant cache: ``query`` ``[B, Hq, T, D]`` (any strides),
     ``lengths`` int64 ``[B]`` with the new tokens among them; query ``t`` sees the keys up to position ``lengths[b] - T + t``, one
     that sees none gives zeros.  ``gate`` (shape and dtype of the query): the output is multiplied by its sigmoid.  The cache is
-    given as for ``torch.ops.anna.tq_paged_decode``."""
+    given as for ``torch.ops.anna.tq_paged_decode``.  One token is as exact as one of several; ``tq_paged_decode`` scores 16-bit caches
+    with 8-bit queries (errors of 0.0013 in fp16 instead of 0.0003) in less time."""
     _resolve("tq_paged_multi_decode")
     op = _op_tq_paged_multi_decode  # same function the dispatcher would reach for CUDA tensors
     return op(query, packed_pages, page_table, window, window_slots, lengths, float(scaling), int(bits), int(residual_len),

@@ -11,6 +11,7 @@ import pytest
 import torch
 from test_gpu_tq_multi_decode import Case, hadamard
 
+import anna_b200
 from anna_b200.tq_tables import key_tables
 
 
@@ -211,6 +212,37 @@ def keys_of(case):
     h, s1, s2 = hadamard(case.dim), tables.signs1.numpy().astype(float), tables.signs2.numpy().astype(float)
     rotated = tables.centroids.numpy().astype(float)[index] + math.sqrt(math.pi / 2 / case.dim) * rnorm[..., None] * (((2.0 * sign - 1.0) @ h) * s2)
     return norm[..., None] / case.dim * (rotated @ h) * s1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,group,page,window,length", [
+    ("fp16", 128, 4, 16, 128, 3000), ("fp16", 128, 16, 32, 128, 2000), ("fp16", 256, 8, 16, 64, 1500), ("fp16", 64, 8, 16, 33, 1500),
+    ("fp16", 128, 4, 24, 64, 1500), ("fp16", 256, 8, 16, 512, 480), ("bf16", 128, 4, 16, 128, 3000), ("bf16", 256, 6, 32, 64, 1500)])
+def test_one_token_is_as_exact_as_one_of_several(cuda_device, dtype, dim, group, page, window, length):
+    """The error of a single new token has the bound of test_error_of_whole_outputs, and the same token among others the same answer but for
+    what the header's roundings may make of another running maximum: they are at the same places, so the two differ by less than twice that."""
+    rms = lambda x, want: float((x - want).square().mean().sqrt() / want.square().mean().sqrt())  # noqa: E731
+    case = Case(lengths=[length], tokens=4, group=group, kv_heads=2, dim=dim, bits=4, page=page, window=window, dtype=dtype, device=cuda_device, seed=32)
+    several = case.run()[:, :, 3:]
+    case.query, case.tokens = case.query[:, :, 3:], 1
+    want, _, _ = case.expected()
+    got, limit = case.run(), 1.03 * rms(rounded(case), want)
+    assert rms(got.cpu().double(), want) <= limit
+    assert rms(got.cpu().double(), several.cpu().double()) <= 2 * limit
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_layouts_that_change_nothing(cuda_device, tokens):
+    case = Case(lengths=[700, 90], tokens=tokens, group=4, kv_heads=2, dim=128, bits=4, page=16, window=16, dtype="fp16", device=cuda_device, seed=33)
+    want = case.run()
+    case.slots = torch.stack([case.slots, case.slots], 1)[:, 0]
+    case.table = torch.stack([case.table, case.table], 2)[..., 0]
+    put = lambda x: x.to(cuda_device) if x.is_contiguous() else torch.stack([x, x], -1).to(cuda_device)[..., 0]  # noqa: E731
+    got = anna_b200.run_tq_paged_multi_decode(
+        query=put(case.query), packed_pages=put(case.packed), page_table=put(case.table), window=put(case.window_ring), window_slots=put(case.slots),
+        lengths=put(torch.tensor([[700, 0], [90, 0]])[:, 0]), scaling=case.scaling, bits=4, residual_len=16, block_size=16, value_group_size=32)
+    assert torch.equal(got, want)
 
 
 @pytest.mark.gpu
