@@ -52,6 +52,7 @@ def rotary_tables(rotary_dim: int, *, theta: float = 10000.0, sections: Sequence
     if inverse_frequencies is not None:  # values, whatever holds them
         inverse_frequencies = tuple(float(f) for f in inverse_frequencies)
     sections = None if sections is None else tuple(int(s) for s in sections)
+    theta = float(theta)
     key = (rotary_dim, theta, sections, bool(interleaved), inverse_frequencies, device)
     found = _TABLES.get(key)
     if found is not None:
@@ -63,7 +64,7 @@ def rotary_tables(rotary_dim: int, *, theta: float = 10000.0, sections: Sequence
     if inverse_frequencies is None:
         if not theta > 0 or not math.isfinite(theta):
             raise ValueError(f"theta must be positive, got {theta}")
-        frequencies = [float(theta) ** (-i / pairs) for i in range(pairs)]
+        frequencies = [theta ** (-i / pairs) for i in range(pairs)]
     else:
         frequencies = list(inverse_frequencies)
         if len(frequencies) != pairs or not all(map(math.isfinite, frequencies)):
