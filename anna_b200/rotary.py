@@ -48,8 +48,15 @@ def pair_axes(rotary_dim: int, sections: Sequence[int] | None, interleaved: bool
 def rotary_tables(rotary_dim: int, *, theta: float = 10000.0, sections: Sequence[int] | None = None, interleaved: bool = False,
                   inverse_frequencies: Sequence[float] | None = None, device: torch.device) -> RotaryTables:
     """Rates and axes of the pairs on the device, made once for each set of parameters.  ``inverse_frequencies`` (radians per
-    position, one for each pair) stands in for the powers of ``theta``."""
+    position, one for each pair) stands in for the powers of ``theta``; a tensor in device memory is read back on every call."""
     if inverse_frequencies is not None:  # values, whatever holds them
+        if isinstance(inverse_frequencies, torch.Tensor):
+            if inverse_frequencies.is_cuda:
+                with on_device(inverse_frequencies.device):
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("inverse_frequencies in device memory cannot be read under graph capture: pass their values "
+                                           "(a list, or a tensor of the host)")
+            inverse_frequencies = inverse_frequencies.tolist()
         inverse_frequencies = tuple(float(f) for f in inverse_frequencies)
     sections = None if sections is None else tuple(int(s) for s in sections)
     theta = float(theta)

@@ -20,3 +20,36 @@ def test_theta_of_a_tensor_that_changes(cuda_device):
         want = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions, theta=float(theta))
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert rotary.rotary_tables(64, theta=theta, device=q.device) is rotary.rotary_tables(64, theta=5e5, device=q.device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+def test_frequencies_on_the_device(cuda_device, dtype):
+    q, k = states(2, 4, 2, 3, 64, torch.float32, cuda_device)
+    positions = torch.randint(0, 500, (2, 3), device=cuda_device)
+    frequencies = torch.logspace(0, -4, 32, device=cuda_device).to(dtype)
+    for _ in range(2):  # the second time with other values
+        got = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions, inverse_frequencies=frequencies)
+        want = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions, inverse_frequencies=[float(f) for f in frequencies])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        expected, bound = turned(q, positions, 64, frequencies=[float(f) for f in frequencies])
+        assert bool(((got[0].cpu().double() - expected.cpu()).abs() <= bound.cpu() + 2.0 ** -24 * expected.cpu().abs()).all())
+        frequencies.mul_(0.5)
+
+
+@pytest.mark.gpu
+def test_frequencies_on_the_device_are_refused_under_capture_which_goes_on(cuda_device):
+    q, k = states(2, 4, 2, 3, 64, torch.float32, cuda_device)
+    positions = torch.randint(0, 500, (2, 3), device=cuda_device)
+    frequencies = torch.logspace(0, -4, 32, device=cuda_device)
+    values = frequencies.tolist()
+    want = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions, inverse_frequencies=values)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="inverse_frequencies in device memory"):
+            anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions, inverse_frequencies=frequencies)
+        got = anna_b200.run_multi_axis_rotary(query=q, key=k, positions=positions, inverse_frequencies=torch.tensor(values))
+    got[0].zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
