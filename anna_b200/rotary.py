@@ -198,6 +198,8 @@ def check_rotary_arguments(name: str, query: torch.Tensor, key: torch.Tensor, po
     width = dim if rotary_dim is None else int(rotary_dim)
     if width > dim:
         raise RuntimeError(f"{name}: rotary_dim {width} is larger than head_dim {dim}")
+    if dim > 4096:
+        raise RuntimeError(f"{name}: head_dim {dim} is larger than 4096")
     float(attention_scaling)
     tables = rotary_tables(width, theta=theta, sections=sections, interleaved=interleaved, inverse_frequencies=inverse_frequencies,
                            device=device)

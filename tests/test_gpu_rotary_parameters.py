@@ -6,7 +6,7 @@ import torch
 from test_gpu_rotary import states, turned
 
 import anna_b200
-from anna_b200 import rotary
+from anna_b200 import KVCacheConfig, Qwen3DynamicCache, Qwen3PageAllocator, rotary
 
 
 @pytest.mark.gpu
@@ -53,3 +53,13 @@ def test_frequencies_on_the_device_are_refused_under_capture_which_goes_on(cuda_
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_an_append_of_heads_that_are_too_wide_counts_nothing(cuda_device):
+    config = KVCacheConfig(num_hidden_layers=1, cache_block_size=4)
+    cache = Qwen3DynamicCache(config, allocator=Qwen3PageAllocator(config), batch_size=1)
+    q, k = states(1, 2, 1, 3, 4098, torch.bfloat16, cuda_device)
+    with pytest.raises(RuntimeError, match="4096"):
+        cache.update_rotary(q, k, k, 0, rotary_dim=64)
+    assert cache.layer_lengths == [[0]] and cache.page_tables == [[[]]] and cache.allocator.layers[0].used_pages() == 0
