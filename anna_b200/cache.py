@@ -524,7 +524,10 @@ class Qwen3DynamicCache:
         ``positions`` (int64 ``[axes, B, T]`` or ``[B, T]``): None counts on from each row's length, plus the cache's
         ``rope_deltas`` where it has some (text behind images, ops.py:1900-1914).  ``rotary``: ``theta``, ``sections``,
         ``interleaved``, ``rotary_dim``, ``inverse_frequencies``, ``attention_scaling`` of ``run_multi_axis_rotary``.
-        Un-quantized layers turn and write in one launch."""
+        Un-quantized layers turn and write in one launch.
+
+        Blocks of a prompt that are found by its token ids (``set_prompt_token_ids``) are another sequence's keys as they were turned
+        there: call that for prompts alone whose positions follow from their ids, not where images of other sizes have the same ids."""
         if key_states.shape != value_states.shape or key_states.dim() != 4:
             raise ValueError("update_rotary expects matching [batch, kv_heads, tokens, head_dim] key and value tensors")
         if (query_states.dim() != 4 or query_states.shape[0] != key_states.shape[0] or query_states.shape[2:] != key_states.shape[2:]
@@ -983,7 +986,8 @@ class Qwen3DynamicCache:
         """Attention of the newest T tokens of every row, ``query_states`` ``[B, Hq, T, D]``, after ``update`` has appended them:
         drafted tokens, or a short chunk of a prompt, without the dense view of the cache.  Query ``t`` sees the keys up to its
         own position, keys of the same chunk among them (de-quantized where they have left the window); in a row of fewer than T
-        tokens the queries that see none give zeros.  One launch for the whole batch."""
+        tokens the queries that see none give zeros.  One launch for the whole batch; one token is as exact as one of several, which
+        ``turboquant_single_token_decode_attention`` with its 8-bit scores of 16-bit caches is not."""
         if not self.uses_turboquant_for_layer(layer_idx):
             raise ValueError(f"Layer {layer_idx} does not use TurboQuant-backed KV storage.")
         if query_states.ndim != 4:

@@ -15,17 +15,15 @@
 // the fewest instructions, and 2 * D/8 neighbouring dims of an output row.
 //
 // Bound: the packed bytes of a sequence from HBM, once for 16 or 32 of its queries; today the issue of instructions.  4 new tokens of 16 rows
-// of 32768, 32/8 heads of 128, 4 bits: 260 us, 2.5 TB/s, 542 instructions per tile and warp (56 % of the issue slots, logic pipe 50 %,
-// products 35 % of their pipe).  A CTA of eight warps splits a share's steps among them, so that a share of 32 tiles is two steps of each
+// of 32768, 32/8 heads of 128, 4 bits: 269 us, 2.4 TB/s, 556 instructions per tile and warp (55 % of the issue slots, logic pipe 53 %,
+// products 34 % of their pipe).  A CTA of eight warps splits a share's steps among them, so that a share of 32 tiles is two steps of each
 // warp and the merge of their rows is one per share; two CTAs per SM (16 rows, up to 128 dims) is what the 128 registers of a thread
-// leave.  32 rows a CTA (two row tiles) unpack a key once for both, with half the warps: 8 new tokens 395 us, twice 260 as two calls.
+// leave.  32 rows a CTA (two row tiles) unpack a key once for both, with half the warps: 8 new tokens 419 us, twice 269 as two calls.
 //
 // What is rounded below 32 bits: the rotated queries, centroids and residual norms to fp16 (2^-12 of the row's largest value, of the
-// centroid and of the norm), value scales and zeros, probabilities and values to fp16 (2^-12 of themselves; for small ones see
-// kTopLog2).  Together they stay
-// below the rounding of a bf16 output (2^-9 of the value); for fp16 see kSplit.
-// Values beyond fp16's range keep to it by powers of two (see `lift`), so that beside this they are off by 2^-25 of the largest of a group's
-// dims in the keys of a tile of rows, at most.
+// centroid and of the norm), probabilities and values to fp16 (2^-12 of themselves; small probabilities: see kTopLog2).  Together they
+// stay below the rounding of a bf16 output (2^-9 of the value); for fp16 see kSplit.  Values keep to fp16's range by powers of two (see
+// `lift`): those of a bf16 cache that are small beside others of their dims in a warp's keys are off by 2^-19 of the largest, at most.
 #pragma once
 
 #include "mbarrier_utils.cuh"
@@ -48,8 +46,8 @@ constexpr float kMoveLimit = 8.0f, kTopLog2 = 7.0f;
 template <typename T, int D, int BITS, int MT>
 struct MultiCfg {
   // An fp16 output shows what Q1 and P lose as one fp16 each, so that they are sums of two there, with a product for either part: 16 rows
-  // of 0.4-4 K tokens, 256 dims, 64 queries to a KV head, off by 2.9e-4 of the output instead of 3.9e-4 (2.1e-4 is its own rounding), 80 us
-  // instead of 70; 16 rows of 32768 tokens, 128 dims, 318 instead of 260.  A bf16 output hides it.
+  // of 0.4-4 K tokens, 256 dims, 64 queries to a KV head, off by 2.8e-4 of the output instead of 3.9e-4 (2.1e-4 is its own rounding), 84 us
+  // instead of 74; 16 rows of 32768 tokens, 128 dims, 328 instead of 269.  A bf16 output hides it.
   static constexpr bool kSplit = std::is_same_v<T, __half>;
   static constexpr int kPlanes = kSplit ? 3 : 2;
   static constexpr int kRows = 16 * MT;
@@ -614,7 +612,7 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[m][c][r] = 0.0f;
     {
-      // a lane's words of a token are loaded in two halves, which keeps the registers of four CTAs per SM (head_dim 128)
+      // a lane's words of a token are loaded in two halves: the others' registers are the products' (128 dims have 128 registers a thread)
       constexpr int kHalfWords = kKeyWords > 1 ? kKeyWords / 2 : 1, kPerLoad = BITS == 4 ? kHalfWords : 2 * kHalfWords;  // nibble words
       uint32_t words[kCols][kHalfWords], flips[kCols];  // flips: the residual norm at the centroids' scale, negative, twice in fp16
 #pragma unroll
@@ -1015,8 +1013,8 @@ __global__ void __launch_bounds__(kMultiMmaThreads, MultiCfg<T, D, BITS, MT>::kC
       if (tig == 0) stats[warp * Cfg::kRows + 16 * m + gid + 8 * k] = make_float2(m_run[m][k], l_run[m][k]);
     }
   __syncthreads();  // and nobody reads the ring or the queries any more
-  // a thread per row: what each warp's sums count, in place of its maximum; the row's maximum and denominator in place of its factor
-  // and its limit
+  // a thread per row: what each warp's sums count, in place of its maximum; the row's 1 / denominator, or 1 where the partials of
+  // several CTAs are merged, in place of its factor
   if (threadIdx.x < Cfg::kRows) {
     const int i = threadIdx.x;
     const float f = factor[i];

@@ -39,10 +39,14 @@ struct TqMultiParams {
   int block_size, block_shift, residual_len, value_group;
   int64_t num_pages, max_blocks, max_len;
   float scaling;
-  // What a stream costs a CTA beside its tiles (queries, first copies, merge), in tiles: 10 to 15 us.  By this number, 32 ragged rows of
-  // 0.5-16 K tokens, 20 queries to a KV head: 16 182 us, 32 141, 64 135, 96 139; 16 rows of 0.4-4 K of 256 dims 100, 84, 76, 82.
+  // What a stream costs a CTA beside its tiles (queries, first copies, merge), in tiles: 10 to 15 us.  By this number (16, 32, 64, 96),
+  // tensor cores: 32 ragged rows of 0.5-16 K tokens, 20 queries to a KV head 181, 137, 127, 132 us; 16 rows of 0.4-4 K of 256 dims 109, 88, 83,
+  // 90.  Of at most 16 queries and 128 dims, with shorter prologues, the same 32 rows 108, 88.4, 89.5, 92.4; 16 rows of 0.4-4 K 32.1, 28.4,
+  // 29.3, 31.5; 64 rows of 0.1-2 K 50.8, 49.1, 48.0, 45.9; one row of 4000 24.4, 19.7, 20.1, 19.9.  So 32 there, 64 otherwise.
   int stream_tiles;
-  int min_share;  // positions of the line that a CTA takes at least
+  // Positions of the line that a CTA takes at least, 32 with tensor cores: by this number (8, 16, 32, 64), one row of 16000 tokens, 4 new ones,
+  // 32/8 heads 27.7, 27.4, 26.8, 28.1 us; of 4000 20.9, 18.2, 19.7, 27.3; of 1000 18.3, 17.4, 20.4, 31.2; batches of 16 rows and more the same.
+  int min_share;
   int whole_tiles;  // streams of no more tiles, a CTA for each, are not cut: see multi_for_each_segment
   anna_tq_layout layout;
 };
