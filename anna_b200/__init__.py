@@ -22,6 +22,7 @@ from .fused_ops import (
 from .page_copy import run_page_copy, run_page_gather
 from .pools import Qwen3PagedLayerAllocator, TurboQuantLayerPool, resolve_value_group_size
 from .prefix_block_cache import PrefixBlockPool
+from .q8 import q8_page_bytes, run_q8_append, run_q8_gather, run_q8_paged_attention, run_q8_select_blocks
 from .rotary import run_multi_axis_rotary, run_rotary_paged_kv_write
 from .turboquant import VALID_KV_CACHE_QUANT_BITS, TurboQuantKVRow, TurboQuantTensorRow, turboquant_is_available
 
@@ -34,5 +35,5 @@ __all__ = [
     "run_gqa_decode_fused", "run_gqa_decode_splitkv_fused", "run_gqa_decode_splitkv_fused_out",
     "run_gqa_decode_splitkv_turboquant_fused_out", "run_paged_gqa_decode_fused", "grouped_query_attention",
     "run_multi_axis_rotary", "run_rotary_paged_kv_write", "run_page_copy", "run_page_gather",
-    "run_tq_paged_multi_decode",
+    "run_tq_paged_multi_decode", "q8_page_bytes", "run_q8_append", "run_q8_gather", "run_q8_paged_attention", "run_q8_select_blocks",
 ]

@@ -112,6 +112,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                           c_ptr, c_ptr, c_i32, c_ptr]),
     "anna_tq_materialize": (c_i32, [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64,
                                     c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_i64, c_i32, c_ptr]),
+    "anna_q8_page_bytes": (c_i32, [c_i32, c_i32, ctypes.POINTER(c_i64)]),
+    "anna_q8_append": (c_i32, [c_ptr, c_i64, c_i64, c_i64] * 2 + [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr] + [c_i32] * 5 +
+                       [c_i64, c_i64, c_i64, c_i32, c_ptr, c_ptr]),
+    "anna_q8_attention_plan": (c_i32, [c_i32] * 6 + [c_i64, c_i32, c_i32, ctypes.POINTER(c_i64), ctypes.POINTER(c_i32)]),
+    "anna_q8_attention": (c_i32, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i32] +
+                          [c_ptr, c_i64, c_i64, c_i64] * 2 + [c_ptr, c_i64, c_ptr] + [c_i32] * 6 +
+                          [c_i64, c_i64, c_i64, c_f32, c_i32, c_ptr]),
+    "anna_q8_select_blocks": (c_i32, [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_i32, c_i32, c_i32, c_ptr] +
+                              [c_i32] * 6 + [c_i64, c_i64, c_i32, c_ptr]),
+    "anna_q8_gather": (c_i32, [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32,
+                               c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, c_ptr]),
 }
 
 

@@ -1158,7 +1158,222 @@ PyObject* page_gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- 8-bit paged cache (q8.py) ---------------------------------------------------------------------------------------------------
+
+// What the calls on such a cache share; false where an argument is not the ordinary one.
+struct Q8Cache {
+  const at::Tensor *pages = nullptr, *table = nullptr, *window = nullptr, *slots = nullptr;
+  int64_t batch = 0, kv_heads = 0, dim = 0, block = 0;
+  int64_t num_pages() const { return pages->size(0); }
+  int64_t max_blocks() const { return table->size(1); }
+  int64_t num_slots() const { return window == nullptr ? 0 : window->size(0); }
+  uint8_t* page_ptr() const { return pages->numel() == 0 ? nullptr : static_cast<uint8_t*>(pages->data_ptr()); }
+  const int32_t* table_ptr() const { return table->numel() == 0 ? nullptr : static_cast<const int32_t*>(table->data_ptr()); }
+  int64_t table_stride() const { return table->stride(0); }
+  const int64_t* slot_ptr() const { return static_cast<const int64_t*>(slots->data_ptr()); }
+};
+bool q8_row_numbers(const at::Tensor* x, c10::Device device, int64_t batch) {
+  return x != nullptr && plain(*x, device, 1) && x->scalar_type() == at::kLong && x->size(0) == batch && x->is_contiguous();
+}
+bool q8_pages(Q8Cache* c, c10::Device device) {
+  int64_t bytes = 0;
+  if (c->pages == nullptr || c->table == nullptr || c->block <= 0 || c->block > INT32_MAX || c->dim > INT32_MAX || c->kv_heads <= 0 ||
+      c->kv_heads > INT32_MAX || c->batch > INT32_MAX || anna_q8_page_bytes((int)c->dim, (int)c->block, &bytes) != ANNA_OK)
+    return false;
+  if (!plain(*c->pages, device, 3) || c->pages->scalar_type() != at::kByte || !c->pages->is_contiguous() || c->pages->size(1) != c->kv_heads ||
+      c->pages->size(2) != bytes || !plain(*c->table, device, 2) || c->table->scalar_type() != at::kInt || c->table->size(0) != c->batch ||
+      (c->table->size(1) > 1 && c->table->stride(1) != 1))
+    return false;
+  return c->table->size(1) == 0 || c->pages->size(0) > 0;
+}
+bool q8_window(Q8Cache* c, c10::Device device, at::ScalarType type) {
+  if (c->window == nullptr || !plain(*c->window, device, 5) || c->window->scalar_type() != type || !c->window->is_contiguous() ||
+      c->window->numel() == 0 || c->window->size(1) != 2)
+    return false;
+  c->kv_heads = c->window->size(2);
+  c->block = c->window->size(3);
+  c->dim = c->window->size(4);
+  return q8_row_numbers(c->slots, device, c->batch);
+}
+// rows of 16-byte pieces, as the kernels load them
+bool q8_rows(const at::Tensor& x) {
+  const int64_t vec = 16 / x.element_size();
+  if (x.stride(3) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) return false;
+  for (int d = 0; d < 3; ++d)
+    if (x.size(d) > 1 && x.stride(d) % vec != 0) return false;
+  return true;
+}
+
+// q8_append(keys, values, pages, table, window, slots, past, new_lengths | None, status | None) -> True | None
+PyObject* q8_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) return PyErr_Format(PyExc_TypeError, "q8_append takes 9 arguments");
+  const at::Tensor *keys = tensor(args[0]), *values = tensor(args[1]), *past = tensor(args[6]);
+  bool ok = keys != nullptr && values != nullptr;
+  const at::Tensor *fresh = optional_tensor(args[7], &ok), *word = optional_tensor(args[8], &ok);
+  Q8Cache c{tensor(args[2]), tensor(args[3]), tensor(args[4]), tensor(args[5])};
+  int code = 0;
+  if (!ok || !keys->is_cuda() || !plain(*keys, keys->device(), 4) || !plain(*values, keys->device(), 4) || keys->sizes() != values->sizes() ||
+      keys->scalar_type() != values->scalar_type() || !dtype_code(keys->scalar_type(), &code) || keys->numel() == 0 || !q8_rows(*keys) ||
+      !q8_rows(*values) || keys->size(2) > INT32_MAX)
+    Py_RETURN_NONE;
+  const c10::Device device = keys->device();
+  c.batch = keys->size(0);
+  if (!q8_window(&c, device, keys->scalar_type()) || c.kv_heads != keys->size(1) || c.dim != keys->size(3) || !q8_pages(&c, device) ||
+      !q8_row_numbers(past, device, c.batch))
+    Py_RETURN_NONE;
+  if (fresh != nullptr && (!q8_row_numbers(fresh, device, c.batch) || fresh->data_ptr() == past->data_ptr())) Py_RETURN_NONE;
+  if (word != nullptr && (word->device() != device || word->scalar_type() != at::kInt || word->numel() < 1)) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(device);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  int status;
+  {
+    pybind11::gil_scoped_release unlocked;
+    status = anna_q8_append(keys->data_ptr(), keys->stride(0), keys->stride(1), keys->stride(2), values->data_ptr(), values->stride(0),
+                            values->stride(1), values->stride(2), c.page_ptr(), c.table_ptr(), c.table_stride(), c.window->data_ptr(),
+                            c.slot_ptr(), static_cast<const int64_t*>(past->data_ptr()), static_cast<int64_t*>(address(fresh)),
+                            (int)c.batch, (int)c.kv_heads, (int)keys->size(2), (int)c.dim, (int)c.block, c.num_pages(), c.max_blocks(),
+                            c.num_slots(), code, static_cast<int32_t*>(address(word)), stream);
+  }
+  if (status != 0) return failed("q8_append", status);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// a query of attention or of a selection
+bool q8_query(const at::Tensor* query, int* code) {
+  return query != nullptr && query->is_cuda() && plain(*query, query->device(), 4) && query->stride(3) == 1 && query->numel() != 0 &&
+         query->size(0) <= INT32_MAX && query->size(1) <= INT32_MAX && query->size(2) <= INT32_MAX && query->size(3) <= INT32_MAX &&
+         dtype_code(query->scalar_type(), code);
+}
+
+// q8_attention(query, gate | None, pages, table, window, slots, lengths, blocks | None, scaling) -> output | None
+PyObject* q8_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) return PyErr_Format(PyExc_TypeError, "q8_attention takes 9 arguments");
+  bool ok = true;
+  const at::Tensor *query = tensor(args[0]), *gate = optional_tensor(args[1], &ok), *lengths = tensor(args[6]),
+                   *blocks = optional_tensor(args[7], &ok);
+  Q8Cache c{tensor(args[2]), tensor(args[3]), tensor(args[4]), tensor(args[5])};
+  const double scaling = PyFloat_AsDouble(args[8]);
+  if (scaling == -1.0 && PyErr_Occurred()) return nullptr;
+  int code = 0;
+  if (!ok || !q8_query(query, &code)) Py_RETURN_NONE;
+  const c10::Device device = query->device();
+  const int64_t heads = query->size(1), tokens = query->size(2);
+  c.batch = query->size(0);
+  if (!q8_window(&c, device, query->scalar_type()) || c.dim != query->size(3) || heads % c.kv_heads != 0 || !q8_pages(&c, device) ||
+      !q8_row_numbers(lengths, device, c.batch))
+    Py_RETURN_NONE;
+  if (gate != nullptr && (!plain(*gate, device, 4) || gate->stride(3) != 1 || gate->scalar_type() != query->scalar_type() ||
+                          gate->sizes() != query->sizes()))
+    Py_RETURN_NONE;
+  if (blocks != nullptr && (!plain(*blocks, device, 4) || blocks->scalar_type() != at::kInt || !blocks->is_contiguous() ||
+                            blocks->size(0) != c.batch || blocks->size(1) != c.kv_heads || blocks->size(2) != tokens || blocks->size(3) == 0 ||
+                            blocks->size(3) > INT32_MAX))
+    Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(device);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  const int width = blocks == nullptr ? 0 : (int)blocks->size(3);
+  int64_t floats_needed = 0;
+  int arrivals = 0;
+  int status = anna_q8_attention_plan((int)c.batch, (int)heads, (int)c.kv_heads, (int)tokens, (int)c.dim, (int)c.block, c.max_blocks(), width,
+                                      code, &floats_needed, &arrivals);
+  if (status != 0) return failed("q8_paged_attention", status);
+  at::Tensor out = at::empty(query->sizes(), query->options());
+  at::Tensor scratch = at::empty({floats_needed}, query->options().dtype(at::kFloat)), counters = arrival_counters(device, stream, arrivals);
+  {
+    pybind11::gil_scoped_release unlocked;
+    status = anna_q8_attention(
+        query->data_ptr(), query->stride(0), query->stride(1), query->stride(2), c.page_ptr(), c.table_ptr(), c.table_stride(),
+        c.window->data_ptr(), c.slot_ptr(), static_cast<const int64_t*>(lengths->data_ptr()), static_cast<const int32_t*>(address(blocks)),
+        width, address(gate), gate == nullptr ? 0 : gate->stride(0), gate == nullptr ? 0 : gate->stride(1),
+        gate == nullptr ? 0 : gate->stride(2), out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), scratch.data_ptr<float>(),
+        floats_needed, static_cast<int32_t*>(counters.data_ptr()), (int)c.batch, (int)heads, (int)c.kv_heads, (int)tokens, (int)c.dim,
+        (int)c.block, c.num_pages(), c.max_blocks(), c.num_slots(), (float)scaling, code, stream);
+  }
+  if (status != 0) return failed("q8_paged_attention", status);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// q8_select(query, pages, table, lengths, block_size, count, first, recent) -> blocks | None
+PyObject* q8_select(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) return PyErr_Format(PyExc_TypeError, "q8_select takes 8 arguments");
+  const at::Tensor *query = tensor(args[0]), *lengths = tensor(args[3]);
+  Q8Cache c{tensor(args[1]), tensor(args[2])};
+  int64_t n[4];  // block_size, count, first, recent
+  if (!int_args(args + 4, 4, n)) return nullptr;
+  int code = 0;
+  if (!q8_query(query, &code) || c.pages == nullptr || c.pages->dim() != 3) Py_RETURN_NONE;
+  const c10::Device device = query->device();
+  const int64_t heads = query->size(1), tokens = query->size(2);
+  c.batch = query->size(0);
+  c.kv_heads = c.pages->size(1);
+  c.dim = query->size(3);
+  c.block = n[0];
+  if (!q8_pages(&c, device) || heads % c.kv_heads != 0 || !q8_row_numbers(lengths, device, c.batch)) Py_RETURN_NONE;
+  for (int i = 1; i < 4; ++i)
+    if (n[i] < 0 || n[i] > INT32_MAX) Py_RETURN_NONE;
+  if (n[1] == 0 || n[2] + n[3] > n[1]) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(device);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  at::Tensor blocks = at::empty({c.batch, c.kv_heads, tokens, n[1]}, query->options().dtype(at::kInt));
+  at::Tensor scores = at::empty({c.batch * c.kv_heads * tokens * c.max_blocks()}, query->options().dtype(at::kInt));
+  int status;
+  {
+    pybind11::gil_scoped_release unlocked;
+    status = anna_q8_select_blocks(query->data_ptr(), query->stride(0), query->stride(1), query->stride(2), c.page_ptr(), c.table_ptr(),
+                                   c.table_stride(), static_cast<const int64_t*>(lengths->data_ptr()), blocks.data_ptr<int32_t>(), (int)n[1],
+                                   (int)n[2], (int)n[3], reinterpret_cast<uint32_t*>(scores.data_ptr()), (int)c.batch, (int)heads,
+                                   (int)c.kv_heads, (int)tokens, (int)c.dim, (int)c.block, c.num_pages(), c.max_blocks(), code, stream);
+  }
+  if (status != 0) return failed("q8_select_blocks", status);
+  return THPVariable_Wrap(std::move(blocks));
+  END_HANDLE_TH_ERRORS
+}
+
+// q8_gather(pages, table, window, slots, lengths, max_len) -> (keys, values) | None
+PyObject* q8_gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 6) return PyErr_Format(PyExc_TypeError, "q8_gather takes 6 arguments");
+  Q8Cache c{tensor(args[0]), tensor(args[1]), tensor(args[2]), tensor(args[3])};
+  const at::Tensor* lengths = tensor(args[4]);
+  int64_t max_len;
+  if (!int_args(args + 5, 1, &max_len)) return nullptr;
+  int code = 0;
+  if (c.window == nullptr || !c.window->is_cuda() || !dtype_code(c.window->scalar_type(), &code) || c.table == nullptr || c.table->dim() != 2 ||
+      max_len < 0)
+    Py_RETURN_NONE;
+  const c10::Device device = c.window->device();
+  c.batch = c.table->size(0);
+  if (!q8_window(&c, device, c.window->scalar_type()) || !q8_pages(&c, device) || !q8_row_numbers(lengths, device, c.batch)) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(device);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  at::Tensor keys = at::empty({c.batch, c.kv_heads, max_len, c.dim}, c.window->options()), values = at::empty_like(keys);
+  int status = 0;
+  if (keys.numel() > 0) {
+    pybind11::gil_scoped_release unlocked;
+    status = anna_q8_gather(c.page_ptr(), c.table_ptr(), c.table_stride(), c.window->data_ptr(), c.slot_ptr(),
+                            static_cast<const int64_t*>(lengths->data_ptr()), keys.data_ptr(), values.data_ptr(), keys.stride(0),
+                            keys.stride(1), keys.stride(2), (int)c.batch, (int)c.kv_heads, (int)c.dim, (int)c.block, c.num_pages(),
+                            c.max_blocks(), c.num_slots(), max_len, code, stream);
+  }
+  if (status != 0) return failed("q8_gather", status);
+  PyObject *k = THPVariable_Wrap(std::move(keys)), *v = THPVariable_Wrap(std::move(values));
+  PyObject* pair = k == nullptr || v == nullptr ? nullptr : PyTuple_Pack(2, k, v);
+  Py_XDECREF(k);
+  Py_XDECREF(v);
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"q8_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(q8_append)), METH_FASTCALL, nullptr},
+    {"q8_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(q8_attention)), METH_FASTCALL, nullptr},
+    {"q8_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(q8_select)), METH_FASTCALL, nullptr},
+    {"q8_gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(q8_gather)), METH_FASTCALL, nullptr},
     {"tq_multi_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tq_multi_decode)), METH_FASTCALL, nullptr},
     {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
     {"rotary_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary_write)), METH_FASTCALL, nullptr},

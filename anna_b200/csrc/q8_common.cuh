@@ -1,0 +1,102 @@
+// The 8-bit paged cache: layout of a page and what its kernels share (q8_append.cu, q8_attention.cu, q8_attention_mma.cu, q8_select.cu).
+//
+// A page holds S tokens of one KV head: key codes int8 [S, D], value codes int8 [S, D], their two scales, and the bounds of the key
+// codes, int8 [2, D].  Codes of keys and values lie next to one another and the scales behind them, so that a kernel that reads all of
+// a page reads one run; the bounds, which the selection alone reads, are next to the scale that it needs, too.
+#pragma once
+
+#include "tq_multi_params.cuh"
+
+namespace anna {
+
+constexpr int kQ8MaxBlockSize = 1024;
+
+__host__ __device__ __forceinline__ int q8_scale_offset(int head_dim, int block_size) { return 2 * block_size * head_dim; }
+__host__ __device__ __forceinline__ int q8_bounds_offset(int head_dim, int block_size) { return 2 * block_size * head_dim + 16; }
+__host__ __device__ __forceinline__ int q8_page_bytes(int head_dim, int block_size) {
+  return (2 * block_size * head_dim + 16 + 2 * head_dim + 127) / 128 * 128;
+}
+inline bool q8_head_dim(int head_dim) { return head_dim == 64 || head_dim == 128 || head_dim == 256; }
+
+// Attention (q8_attention.cu): the multi-token decode's parameters, of which packed codes, signs and centroids are not used.  The keys of
+// a stream lie on an axis: its full pages, or with `blocks` the pages that its list names, `width` of them; behind those the tokens of
+// the ring.  Row tiles: of all rows, or with `blocks` of the rows of one query token, since each has a list of its own.
+struct Q8Params : TqMultiParams {
+  int page_bytes;
+  const int32_t* blocks;  // [B, Hkv, T, width]
+  int width;
+  int tiles_per_token;    // row tiles of one query token (blocks only)
+  int splits;             // CTAs of a stream (blocks only)
+  int64_t num_slots;
+};
+
+// What a stream reads: rows row0 .. row0 + count - 1 (row = token * groups + head of the group).
+struct Q8Stream {
+  int64_t len, full;    // tokens of the sequence, of those in full pages
+  int64_t packed;       // tokens of the axis that lie in pages
+  int row0, count;
+  const int32_t* list;  // the blocks on the axis, or null: all in order
+};
+
+template <int ROWS>
+__device__ __forceinline__ Q8Stream q8_stream(const Q8Params& p, int64_t b, int kvh, int tile) {
+  Q8Stream s;
+  s.len = max((int64_t)0, min(p.lengths[b], p.max_len));
+  const int blocks = p.block_shift >= 0 ? (int)(s.len >> p.block_shift) : (int)s.len / p.block_size;
+  s.full = (int64_t)blocks * p.block_size;
+  s.list = nullptr;
+  if (p.blocks == nullptr) {
+    s.packed = s.full;
+    s.row0 = tile * ROWS;
+    s.count = min(ROWS, p.rows - s.row0);
+  } else {
+    const int token = tile / p.tiles_per_token, part = tile - token * p.tiles_per_token;
+    s.packed = (int64_t)p.width * p.block_size;
+    s.row0 = token * p.groups + part * ROWS;
+    s.count = min(ROWS, p.groups - part * ROWS);
+    s.list = p.blocks + ((b * p.kv_heads + kvh) * p.tokens + token) * p.width;
+  }
+  return s;
+}
+
+// Page of entry `entry` of the axis, in bytes from the pool's start, -1: none; *block is its place in the sequence.
+__device__ __forceinline__ int64_t q8_page_at(const Q8Params& p, const Q8Stream& s, int64_t b, int kvh, int entry, int* block) {
+  const int j = s.list != nullptr ? s.list[entry] : entry;
+  *block = j;
+  if (j < 0 || (int64_t)j * p.block_size >= s.full || j >= p.max_blocks) return -1;
+  const int32_t pid = p.block_table[b * p.table_stride + j];
+  return pid >= 0 && pid < p.num_pages ? ((int64_t)pid * p.kv_heads + kvh) * p.page_bytes : -1;
+}
+
+// Calls segment(b, kvh, tile, t0, t1, partial) for this CTA's part of the axes; see multi_for_each_segment.  With blocks all axes are as
+// long, and the host has cut them: `splits` CTAs to a stream, 16-token tiles dealt evenly.
+template <typename T, int D, int THREADS, bool kBlocks, typename Fn>
+__device__ __forceinline__ void q8_for_each_segment(const Q8Params& p, int row_tiles, Fn&& segment) {
+  if constexpr (kBlocks) {
+    const int stream = blockIdx.x / p.splits, split = blockIdx.x - stream * p.splits;
+    const int tile = stream % row_tiles, head = stream / row_tiles % p.kv_heads;
+    const int64_t b = stream / row_tiles / p.kv_heads;
+    const int64_t len = max((int64_t)0, min(p.lengths[b], p.max_len));
+    const int64_t end = (int64_t)p.width * p.block_size + len % p.block_size;
+    const int64_t tiles = (end + kBalancedTileTokens - 1) / kBalancedTileTokens;
+    const int64_t t0 = tiles * split / p.splits * kBalancedTileTokens, t1 = min(end, tiles * (split + 1) / p.splits * kBalancedTileTokens);
+    segment(b, head, tile, t0, t1, MultiPartial{stream * p.splits, p.splits, split});
+  } else {
+    multi_for_each_segment<T, D, THREADS>(p, row_tiles, segment);
+  }
+}
+
+// Rows of a tile, CTAs and the scratch of a call; q8_attention.cu plans, both kernels go by it.
+struct Q8Plan {
+  bool tensor_cores;
+  int rows;       // of a row tile
+  int row_tiles;  // of a (sequence, KV head)
+  int tiles_per_token, splits;
+  int64_t ctas;   // at most
+  int64_t floats;
+  int counters;
+};
+
+int launch_q8_mma(const Q8Params& p, const Q8Plan& plan, int head_dim, int dtype, int ctas, cudaStream_t stream);
+
+}  // namespace anna

@@ -135,10 +135,10 @@ __device__ __forceinline__ void multi_for_each_segment(const TqMultiParams& p, i
 // has the same four dims of several rows and several partials on their way at a time (33 partials of 16 rows, a thread's rows one
 // after the other: one row of 4000 tokens 46 us, 31 so).
 template <typename T, int D, int WARPS, int ROWS>
-__device__ __forceinline__ void multi_merge(const TqMultiParams& p, int64_t b, int kvh, int tile, int tiles, int count,
-                                            const MultiPartial& part, float* weights) {
+__device__ __forceinline__ void multi_merge_rows(const TqMultiParams& p, int64_t b, int kvh, int tile, int tiles, int row0, int count,
+                                                 const MultiPartial& part, float* weights) {
   if (!merge_arrive(FusedCombine{p.counters}, (b * p.kv_heads + kvh) * tiles + tile, part.count)) return;
-  const int chunks = part.count, row0 = tile * ROWS;
+  const int chunks = part.count;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float2* all_stats = reinterpret_cast<const float2*>(p.stats);
   for (int i = warp; i < count; i += WARPS) {
@@ -198,6 +198,13 @@ __device__ __forceinline__ void multi_merge(const TqMultiParams& p, int64_t b, i
     const float out[4] = {acc[r].x, acc[r].y, acc[r].z, acc[r].w};
     if (i < count) multi_store<T, 4>(p, b, kvh, row0 + i, 4 * col, out);
   }
+}
+
+// The same, the tiles of a (sequence, KV head) all of ROWS rows but the last.
+template <typename T, int D, int WARPS, int ROWS>
+__device__ __forceinline__ void multi_merge(const TqMultiParams& p, int64_t b, int kvh, int tile, int tiles, int count,
+                                            const MultiPartial& part, float* weights) {
+  multi_merge_rows<T, D, WARPS, ROWS>(p, b, kvh, tile, tiles, tile * ROWS, count, part, weights);
 }
 
 // Tensor-core form (tq_multi_mma.cu): 16-bit caches, head_dim 64, 128 and 256, value groups of 32, pages of a multiple of 8 tokens.

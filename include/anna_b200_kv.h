@@ -495,6 +495,78 @@ int anna_tq_tensor_dequantize(const uint8_t* idx, const float* norms, int64_t ca
                               int64_t stride_h, int64_t stride_t, int heads, int tokens, int head_dim, int bits,
                               const float* signs1, const float* centroids, int dtype, anna_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Paged cache in 8 bits.  No counterpart in the reference.
+ *
+ * Pool: uint8 [P, Hkv, page_bytes]; what a page of S = block_size tokens holds of one KV head:
+ *   key codes int8 [S, D] | value codes int8 [S, D] | float32 scale of the keys, of the values, 8 bytes that nothing reads |
+ *   bounds int8 [2, D]: the largest key code and the largest negated key code of every dim | up to a multiple of 128 bytes.
+ * A code is the whole number next to 127 x / m (of two the even one), m the page's and head's largest magnitude among its keys
+ * (values), and stands for scale * code, scale = m / 127 in float32.  Keys (values) with an infinity or a NaN among them get the scale
+ * NaN and codes of 0: what looks at them gets NaN.  Full pages alone are in the pool: of a sequence of n tokens, token t < n / S * S in
+ * block t / S of its table row, slot t % S.  The tokens of the last, unfinished page are in window [slots, 2, Hkv, S, D] (index 0 =
+ * keys, 1 = values) of the element type, token t in slot t % S of the sequence's ring.  head_dim 64, 128 and 256, S up to 1024.
+ * Entries of window_slots outside [0, num_slots) and page ids outside the pool are no memory: what would be read there is left out,
+ * what would be written is not.
+ */
+int anna_q8_page_bytes(int head_dim, int block_size, int64_t* bytes);
+
+/*
+ * Appends T tokens to every row: pages that they fill are quantized, from the ring and the new tokens, the tokens of the unfinished page
+ * go to the ring.  What is stored does not depend on how tokens are cut into calls.
+ *   k_new, v_new   [B, Hkv, T, D], element strides of their own, multiples of 16 bytes on 16-byte aligned rows; last dim contiguous
+ *   page_table     int32 [B, table_stride >= max_blocks];  window_slots, past_lengths int64 [B], no slot twice
+ *   new_lengths    NULL or int64 [B] apart from past_lengths: receives past_lengths[b] + T
+ *   status         optional device int32: ANNA_DEV_BAD_PAGE is OR-ed in when a page or slot that is needed is none
+ */
+int anna_q8_append(const void* k_new, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t, const void* v_new, int64_t v_stride_b,
+                   int64_t v_stride_h, int64_t v_stride_t, uint8_t* pages, const int32_t* page_table, int64_t table_stride, void* window,
+                   const int64_t* window_slots, const int64_t* past_lengths, int64_t* new_lengths, int batch, int kv_heads, int new_tokens,
+                   int head_dim, int block_size, int64_t num_pages, int64_t max_blocks, int64_t num_slots, int dtype, int32_t* status,
+                   anna_stream_t stream);
+
+/*
+ * Attention of the newest T tokens of every row: q [B, Hq, T, D], query t of row b sees the keys at positions up to
+ * lengths[b] - T + t; one that sees none gives zeros.  softmax in fp32, optional sigmoid(gate) epilogue.
+ *   blocks         NULL: all pages.  int32 [B, Hkv, T, width] contiguous: query t of KV head h sees, of the full pages, those that its
+ *                  list names (in any order; one that is named twice counts twice, what is no full page of the row is left out), and the
+ *                  unfinished one
+ *   scratch        float32, 16-byte aligned, as many as the plan says; counters int32, zero on entry and on return
+ * anna_q8_attention_plan: sizes for these arguments (width 0: no blocks).
+ */
+int anna_q8_attention_plan(int batch, int q_heads, int kv_heads, int tokens, int head_dim, int block_size, int64_t max_blocks, int width,
+                           int dtype, int64_t* scratch_size, int* counters);
+int anna_q8_attention(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, const uint8_t* pages,
+                      const int32_t* page_table, int64_t table_stride, const void* window, const int64_t* window_slots,
+                      const int64_t* lengths, const int32_t* blocks, int width, const void* gate, int64_t gate_stride_b,
+                      int64_t gate_stride_h, int64_t gate_stride_t, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                      int64_t out_stride_t, float* scratch, int64_t scratch_size, int32_t* counters, int batch, int q_heads, int kv_heads,
+                      int tokens, int head_dim, int block_size, int64_t num_pages, int64_t max_blocks, int64_t num_slots, float scaling,
+                      int dtype, anna_stream_t stream);
+
+/*
+ * Which full pages a query should look at: blocks int32 [B, Hkv, T, count] receives for query t of row b and KV head h the indices, in
+ * ascending order and followed by -1, of the `count` pages of the best score among those with a token that the query sees, the `first`
+ * first and the `recent` last of them in any case.  The score bounds the head's products with the page's keys from above:
+ *   max over the query heads g of the KV head of  m_g * scale * sum_d max(r_gd * high_d, -r_gd * negated_d)
+ * r_gd the whole number next to 32767 q_gd / m_g, m_g the largest magnitude in q_g; the sums are exact, the products are rounded to
+ * float32 from the left.  Of equal scores the lower index counts as the better one; NaN is the best.  Pages that are no memory are left out.
+ *   scores         uint32 scratch [B, Hkv, T, max_blocks]
+ */
+int anna_q8_select_blocks(const void* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, const uint8_t* pages,
+                          const int32_t* page_table, int64_t table_stride, const int64_t* lengths, int32_t* blocks, int count, int first,
+                          int recent, uint32_t* scores, int batch, int q_heads, int kv_heads, int tokens, int head_dim, int block_size,
+                          int64_t num_pages, int64_t max_blocks, int dtype, anna_stream_t stream);
+
+/*
+ * Dense view of the cache: key_out, value_out [B, Hkv, max_len, D] (element strides, the same for both, multiples of 16 bytes on 16-byte
+ * aligned rows; last dim contiguous); zeros at and past a row's length and where a page is none.
+ */
+int anna_q8_gather(const uint8_t* pages, const int32_t* page_table, int64_t table_stride, const void* window, const int64_t* window_slots,
+                   const int64_t* lengths, void* key_out, void* value_out, int64_t out_stride_b, int64_t out_stride_h,
+                   int64_t out_stride_t, int batch, int kv_heads, int head_dim, int block_size, int64_t num_pages, int64_t max_blocks,
+                   int64_t num_slots, int64_t max_len, int dtype, anna_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
