@@ -124,16 +124,21 @@ __device__ __forceinline__ void q8_store_codes(uint8_t* to, const int (&code)[N]
   else *reinterpret_cast<uint32_t*>(to) = w[0];
 }
 
-template <typename T, int D>
+// PER warps, one or all of the CTA, to an item.
+template <typename T, int D, int PER>
 __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8AppendParams p) {
+  static_assert(PER == 1 || PER == kQ8AppendWarps, "a warp or a CTA");
   constexpr int kN = ElemTraits<T>::kVec;
   constexpr int kVecs = D / kN;                               // of a token
   constexpr int kLanes = kVecs < 32 ? kVecs : 32;              // that share a token
   constexpr int kCols = kVecs / kLanes;                        // vectors of a lane and token
-  constexpr int kAtOnce = 32 / kLanes;                         // tokens of a warp
+  constexpr int kAtOnce = PER * (32 / kLanes);                 // tokens of the item's warps
   constexpr int kHeld = 16 / kCols;                            // rounds whose values stay in registers
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * kQ8AppendWarps + (threadIdx.x >> 5);
+  __shared__ __align__(16) float s_extremes[PER == 1 ? 1 : 2 * PER * D];
+  q8_let_next_start();
+  q8_wait_for_previous();
+  const int lane = threadIdx.x & 31, part = PER == 1 ? 0 : threadIdx.x >> 5;
+  const int64_t item = PER == 1 ? (int64_t)blockIdx.x * kQ8AppendWarps + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
   const int which = (int)(item & 1);  // keys, values
   int64_t rest = item >> 1;
   const int unit = (int)(rest % p.units);
@@ -143,7 +148,7 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
   if (b >= p.batch) return;
   const int S = p.block_size;
   const int64_t past = p.past_lengths[b], total = past + p.tokens;
-  if (p.new_lengths != nullptr && unit == 0 && h == 0 && which == 0 && lane == 0) p.new_lengths[b] = total;
+  if (p.new_lengths != nullptr && unit == 0 && h == 0 && which == 0 && lane == 0 && part == 0) p.new_lengths[b] = total;
   if (past < 0) return;
   const int64_t block = past / S + unit;
   const T* fresh = reinterpret_cast<const T*>(p.in[which]) + b * p.stride_b[which] + h * p.stride_h[which];
@@ -151,14 +156,14 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
   const int64_t slot = unit == 0 ? p.window_slots[b] : -1;
   T* ring = slot >= 0 && slot < p.num_slots ? reinterpret_cast<T*>(p.window) + ((slot * 2 + which) * p.kv_heads + h) * S * D : nullptr;
   const int64_t begin = block * S;  // position of the page's first token
-  const int col = lane % kLanes * kN, row = lane / kLanes;
+  const int col = lane % kLanes * kN, row = part * (32 / kLanes) + lane / kLanes;
 
   const bool closes = begin + S <= total;
   int32_t pid = -1;
   if (closes && block < p.max_blocks) pid = p.page_table[b * p.table_stride + block];
   const bool there = pid >= 0 && pid < p.num_pages;
   const bool needs_ring = unit == 0 && (past % S != 0 || total % S != 0);
-  if (p.status != nullptr && lane == 0 && ((closes && !there) || (needs_ring && ring == nullptr)))
+  if (p.status != nullptr && lane == 0 && part == 0 && ((closes && !there) || (needs_ring && ring == nullptr)))
     atomicOr(p.status, (int)ANNA_DEV_BAD_PAGE);
   if (closes && there && (begin >= past || ring != nullptr)) {
     uint8_t* page = p.pages + ((int64_t)pid * p.kv_heads + h) * p.page_bytes;
@@ -177,6 +182,28 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
       for (int mask = kLanes; mask < 32; mask *= 2)
 #pragma unroll
         for (int c = 0; c < kCols; ++c) seen[c].exchange(mask);
+      if constexpr (PER > 1) {
+        float* mine = s_extremes + part * 2 * D + col;
+        if (lane < kLanes) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+              mine[c * 32 * kN + i] = seen[c].high[i];
+              mine[D + c * 32 * kN + i] = seen[c].low[i];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < PER; ++w)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+              seen[c].high[i] = Q8Extremes<T>::larger(seen[c].high[i], s_extremes[w * 2 * D + col + c * 32 * kN + i]);
+              seen[c].low[i] = Q8Extremes<T>::smaller(seen[c].low[i], s_extremes[w * 2 * D + D + col + c * 32 * kN + i]);
+            }
+      }
       float top = seen[0].magnitude();
 #pragma unroll
       for (int c = 1; c < kCols; ++c) top = Q8Extremes<T>::larger(top, seen[c].magnitude());
@@ -184,7 +211,7 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
       for (int mask = 1; mask < kLanes; mask *= 2) top = Q8Extremes<T>::larger(top, __shfl_xor_sync(0xffffffffu, top, mask));
       const bool fine = top < INFINITY;  // neither an infinity nor a NaN
       const bool some = fine && top > 0.0f;
-      if (lane == 0)
+      if (lane == 0 && part == 0)
         reinterpret_cast<float*>(page + q8_scale_offset(D, S))[which] = fine ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fc00000);
       const Q8Coder<T> coder(some ? top : 1.0f);
       auto put = [&](const float (&x)[kN], float sign, uint8_t* to) {
@@ -249,7 +276,8 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
     }
   }
   if (unit != 0 || ring == nullptr) return;
-  __syncwarp();  // the ring has been read
+  if constexpr (PER == 1) __syncwarp();  // the ring has been read
+  else __syncthreads();
   const int64_t open = total / S * S;  // first position of the unfinished page
   const int64_t from = max(past, open);
   for (int64_t at = from + row; at < total; at += kAtOnce)
@@ -269,19 +297,25 @@ struct Q8GatherParams {
   void* out[2];
   int64_t stride_b, stride_h, stride_t;
   int batch, kv_heads, block_size, page_bytes;
+  int shares;  // of a block
   int64_t num_pages, max_blocks, num_slots, max_len, spans;
 };
+constexpr int kQ8GatherPieces = 128;  // of 16 codes, of a warp
 
-// Dense view: a warp writes the keys or the values of one block of one KV head; a lane de-quantizes 16 codes, which is 32 bytes of a
+// Dense view: a warp writes 2048 keys' or values' dims of one block of one KV head; a lane de-quantizes 16 codes, which is 32 bytes of a
 // 16-bit cache, at a time.  Bound: HBM, of which the output is two thirds.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) q8_gather_kernel(const Q8GatherParams p) {
   constexpr int kN = ElemTraits<T>::kVec;
   constexpr int kPieces = D / 16;  // of a token
+  q8_let_next_start();
+  q8_wait_for_previous();
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int which = (int)(item & 1);
   int64_t rest = item >> 1;
+  const int share = (int)(rest % p.shares);
+  rest /= p.shares;
   const int64_t block = rest % p.spans;
   rest /= p.spans;
   const int h = (int)(rest % p.kv_heads);
@@ -306,8 +340,11 @@ __global__ void __launch_bounds__(128) q8_gather_kernel(const Q8GatherParams p) 
   }
   T* out = reinterpret_cast<T*>(p.out[which]) + b * p.stride_b + h * p.stride_h;
   const int pieces = (int)min((int64_t)S, p.max_len - begin) * kPieces;
-#pragma unroll 4
-  for (int i = lane; i < pieces; i += 32) {
+  const int end = min(pieces, (share + 1) * kQ8GatherPieces);
+#pragma unroll
+  for (int round = 0; round < kQ8GatherPieces / 32; ++round) {
+    const int i = share * kQ8GatherPieces + round * 32 + lane;
+    if (i >= end) break;
     const int token = i / kPieces, d = i % kPieces * 16;
     uint4 x[16 / kN];
     if (codes != nullptr) {
@@ -372,12 +409,16 @@ extern "C" int anna_q8_append(const void* k_new, int64_t k_stride_b, int64_t k_s
   p.batch = batch; p.kv_heads = kv_heads; p.tokens = new_tokens; p.block_size = block_size;
   p.units = (int)(((int64_t)new_tokens + block_size - 2) / block_size) + 1;
   p.page_bytes = (int)bytes; p.num_pages = num_pages; p.max_blocks = max_blocks; p.num_slots = num_slots; p.status = status;
-  const int64_t ctas = ((int64_t)batch * kv_heads * p.units * 2 + kQ8AppendWarps - 1) / kQ8AppendWarps;
+  // A CTA to an item where a warp would have more than 8 vectors a lane, or where the GPU has room for that: 64 rows of one token
+  // PLACEHOLDER
+  const int64_t items = (int64_t)batch * kv_heads * p.units * 2;
+  const bool whole = block_size * head_dim / vec > 256 || items <= 148 * 8;
+  const int64_t ctas = whole ? items : (items + kQ8AppendWarps - 1) / kQ8AppendWarps;
   ANNA_REQUIRE(ctas < (1ll << 31), "%s: too many tokens", what);
   return ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
-      q8_append_kernel<T, D><<<(unsigned)ctas, kQ8AppendWarps * 32, 0, (cudaStream_t)stream>>>(p);
-      return check_launch("q8_append_kernel");
+      return q8_launch("q8_append_kernel", whole ? q8_append_kernel<T, D, kQ8AppendWarps> : q8_append_kernel<T, D, 1>, dim3((unsigned)ctas),
+                       kQ8AppendWarps * 32, 0, (cudaStream_t)stream, p);
     });
   });
 }
@@ -406,12 +447,12 @@ extern "C" int anna_q8_gather(const uint8_t* pages, const int32_t* page_table, i
   p.batch = batch; p.kv_heads = kv_heads; p.block_size = block_size; p.page_bytes = (int)bytes;
   p.num_pages = num_pages; p.max_blocks = max_blocks; p.num_slots = num_slots; p.max_len = max_len;
   p.spans = (max_len + block_size - 1) / block_size;
-  const int64_t warps = (int64_t)batch * kv_heads * p.spans * 2;
+  p.shares = (block_size * head_dim / 16 + kQ8GatherPieces - 1) / kQ8GatherPieces;
+  const int64_t warps = (int64_t)batch * kv_heads * p.spans * p.shares * 2;
   ANNA_REQUIRE(p.spans < (1ll << 31) && warps / 4 < (1ll << 31) - 1, "%s: too many tokens", what);
   return ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
-      q8_gather_kernel<T, D><<<(unsigned)((warps + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p);
-      return check_launch("q8_gather_kernel");
+      return q8_launch("q8_gather_kernel", q8_gather_kernel<T, D>, dim3((unsigned)((warps + 3) / 4)), 128, 0, (cudaStream_t)stream, p);
     });
   });
 }

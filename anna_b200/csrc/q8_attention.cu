@@ -27,6 +27,8 @@ __global__ void __launch_bounds__(kQ8Threads<D>) q8_attention_kernel(const Q8Par
   __shared__ int64_t sm_position[kQ8Tokens];     // in the sequence; past its end for what is not there
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  q8_let_next_start();
+  q8_wait_for_previous();
   q8_for_each_segment<T, D, kThreads, kBlocks>(p, row_tiles, [&](int64_t b, int kvh, int tile, int64_t t0, int64_t t1, const MultiPartial& part) {
   const Q8Stream st = q8_stream<kQ8Rows>(p, b, kvh, tile);
   const int row0 = st.row0, count = st.count;
@@ -318,8 +320,7 @@ extern "C" int anna_q8_attention(const void* q, int64_t q_stride_b, int64_t q_st
         constexpr int smem = kQ8SmemFloats<D> * 4;
         auto kernel = width > 0 ? q8_attention_kernel<T, D, true> : q8_attention_kernel<T, D, false>;
         ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        kernel<<<ctas, kQ8Threads<D>, smem, (cudaStream_t)stream>>>(p, plan.row_tiles);
-        return check_launch("q8_attention_kernel");
+        return q8_launch("q8_attention_kernel", kernel, dim3((unsigned)ctas), kQ8Threads<D>, smem, (cudaStream_t)stream, p, plan.row_tiles);
       });
     });
     if (rc != ANNA_OK) return rc;

@@ -81,6 +81,8 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
   float* rate = reinterpret_cast<float*>(smem + Cfg::kOffRate);
   float2* stats = reinterpret_cast<float2*>(smem + Cfg::kOffStats);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  q8_let_next_start();
+  q8_wait_for_previous();
 
   q8_for_each_segment<T, D, Cfg::kThreads, kBlocks>(p, row_tiles, [&](int64_t b, int kvh, int tile, int64_t t0, int64_t t1, const MultiPartial& part) {
   const Q8Stream st = q8_stream<Cfg::kRows>(p, b, kvh, tile);
@@ -485,8 +487,7 @@ static int launch(const Q8Params& p, int row_tiles, int ctas, cudaStream_t strea
   using Cfg = Q8Cfg<D, NT>;
   auto kernel = p.blocks != nullptr ? q8_mma_kernel<T, D, NT, true> : q8_mma_kernel<T, D, NT, false>;
   ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
-  kernel<<<ctas, Cfg::kThreads, Cfg::kSmem, stream>>>(p, row_tiles);
-  return check_launch("q8_mma_kernel");
+  return q8_launch("q8_mma_kernel", kernel, dim3((unsigned)ctas), Cfg::kThreads, Cfg::kSmem, stream, p, row_tiles);
 }
 
 int launch_q8_mma(const Q8Params& p, const Q8Plan& plan, int head_dim, int dtype, int ctas, cudaStream_t stream) {

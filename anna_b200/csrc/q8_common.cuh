@@ -86,6 +86,28 @@ __device__ __forceinline__ void q8_for_each_segment(const Q8Params& p, int row_t
   }
 }
 
+// Launches of this cache follow one another (append, selection, choice, attention), each of a few microseconds.  They go out with leave to
+// start while the kernel in front of them ends, and touch no memory before that has ended and its writes are there.
+__device__ __forceinline__ void q8_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void q8_let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+template <typename... Params, typename... Args>
+int q8_launch(const char* what, void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, Args&&... args) {
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = (size_t)smem;
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+  if (err != cudaSuccess) return set_error(ANNA_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(err));
+  return ANNA_OK;
+}
+
 // Rows of a tile, CTAs and the scratch of a call; q8_attention.cu plans, both kernels go by it.
 struct Q8Plan {
   bool tensor_cores;

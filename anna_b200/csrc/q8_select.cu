@@ -7,8 +7,8 @@
 // u < 256, v < 128), with signed bytes: integer mma, 16 pages to a tile, 8 query heads.
 //
 // Scores: a warp takes 16 pages at a time, for all heads and several tokens.  Bound: HBM (2 D + 4 bytes a page and head), or the launch.
-// Choice: a CTA per query token and KV head finds the score of the last page that is taken, 8 bits at a time, counting how many scores
-// share the bits so far; then the pages above it, and of those equal to it the first, are written in order.
+// Choice: a CTA per query token and KV head finds the score of the last page that is taken, 8 bits at a time from the first bit in which
+// scores differ, counting how many share the bits so far; then the pages above it, and of those equal to it the first, are written in order.
 #include "q8_common.cuh"
 
 namespace anna {
@@ -25,11 +25,13 @@ struct Q8SelectParams {
   int kv_heads, groups, tokens, block_size, page_bytes;
   int count, first, recent;
   int head_tiles, tokens_at_once;  // tiles of 8 query heads of a token; tokens of a CTA
+  int rounds;                      // tiles of a warp
   int64_t num_pages, max_blocks;
 };
 
 constexpr int kQ8SelectWarps = 8;
 constexpr int kQ8SelectTile = 16;  // pages of a warp at a time
+constexpr int kQ8SelectRounds = 8;   // tiles of a warp at most
 constexpr uint32_t kQ8Forced = 0xffffffffu;
 
 // Full pages of which query t sees a token.
@@ -53,9 +55,11 @@ __device__ __forceinline__ uint32_t q8_ordered(float x) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kQ8SelectWarps * 32) q8_score_kernel(const Q8SelectParams p) {
+__global__ void __launch_bounds__(kQ8SelectWarps * 32, D == 256 ? 1 : 2) q8_score_kernel(const Q8SelectParams p) {
   constexpr int kChunks = 2 * D / 64;  // of 64 bounds, 16 of them a lane's
   extern __shared__ __align__(16) uint8_t smem[];
+  q8_let_next_start();
+  q8_wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int64_t b = blockIdx.y / p.kv_heads;
   const int kvh = blockIdx.y % p.kv_heads;
@@ -63,6 +67,39 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32) q8_score_kernel(const Q8S
   const int head_tiles = p.head_tiles, tiles = here * head_tiles;
   uint4* parts = reinterpret_cast<uint4*>(smem);                                              // [2][tiles][kChunks][32 lanes]
   float* tops = reinterpret_cast<float*>(smem + p.tokens_at_once * head_tiles * 2 * kChunks * 512);  // [tiles][8]
+
+  // ---- this CTA's pages: `rounds` tiles of every warp -----------------------------------------------------------------------------------
+  const int most = q8_candidates(p, b, token0 + here - 1);
+  const int first_tile = blockIdx.x * p.rounds * kQ8SelectWarps + warp;
+  if ((int)blockIdx.x * p.rounds * kQ8SelectWarps * kQ8SelectTile >= most) return;
+  struct Tile {
+    uint4 w[2][kChunks];
+    float scale[2];
+    bool there[2];
+  };
+  int32_t ids[2];  // pages of the tile after next
+  auto find = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = tile * kQ8SelectTile + gid + 8 * i;
+      ids[i] = j < most ? p.block_table[b * p.table_stride + j] : -1;
+    }
+  };
+  auto load = [&](Tile& x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x.there[i] = ids[i] >= 0 && ids[i] < p.num_pages;
+      const uint8_t* page = p.pages + (x.there[i] ? ((int64_t)ids[i] * p.kv_heads + kvh) * p.page_bytes : 0);
+      x.scale[i] = __ldg(reinterpret_cast<const float*>(page + q8_scale_offset(D, p.block_size)));
+      const uint4* bounds = reinterpret_cast<const uint4*>(page + q8_bounds_offset(D, p.block_size));
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) x.w[i][c] = ldg_stream16(bounds + 4 * c + tig);
+    }
+  };
+  Tile now, next;
+  find(first_tile);
+  load(now);
+  find(first_tile + kQ8SelectWarps);
 
   // ---- queries in whole numbers --------------------------------------------------------------------------------------------------
   for (int row = warp; row < tiles * 8; row += kQ8SelectWarps) {
@@ -102,22 +139,12 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32) q8_score_kernel(const Q8S
   __syncthreads();
 
   // ---- 16 pages at a time -----------------------------------------------------------------------------------------------------------
-  const int most = q8_candidates(p, b, token0 + here - 1);
-  for (int tile = blockIdx.x * kQ8SelectWarps + warp; tile * kQ8SelectTile < most; tile += gridDim.x * kQ8SelectWarps) {
-    uint4 w[2][kChunks];
-    float scale[2];
-    bool there[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int j = tile * kQ8SelectTile + gid + 8 * i;
-      int32_t pid = -1;
-      if (j < most) pid = p.block_table[b * p.table_stride + j];
-      there[i] = pid >= 0 && pid < p.num_pages;
-      const uint8_t* page = p.pages + (there[i] ? ((int64_t)pid * p.kv_heads + kvh) * p.page_bytes : 0);
-      scale[i] = *reinterpret_cast<const float*>(page + q8_scale_offset(D, p.block_size));
-      const uint4* bounds = reinterpret_cast<const uint4*>(page + q8_bounds_offset(D, p.block_size));
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) w[i][c] = ldg_stream16(bounds + 4 * c + tig);
+  for (int round = 0; round < p.rounds; ++round) {
+    const int tile = first_tile + round * kQ8SelectWarps;
+    if (tile * kQ8SelectTile >= most) break;
+    if (round + 1 < p.rounds) {
+      load(next);
+      find(tile + 2 * kQ8SelectWarps);
     }
     for (int t = 0; t < here; ++t) {
       float best[2] = {-INFINITY, -INFINITY};
@@ -127,17 +154,17 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32) q8_score_kernel(const Q8S
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           const uint4 u = at[c * 32], v = at[(tiles * kChunks + c) * 32];
-          mma_s8u8(hi, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, u.x, u.y);
-          mma_s8u8(lo, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, v.x, v.y);
-          mma_s8u8(hi, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, u.z, u.w);
-          mma_s8u8(lo, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, v.z, v.w);
+          mma_s8u8(hi, now.w[0][c].x, now.w[1][c].x, now.w[0][c].y, now.w[1][c].y, u.x, u.y);
+          mma_s8u8(lo, now.w[0][c].x, now.w[1][c].x, now.w[0][c].y, now.w[1][c].y, v.x, v.y);
+          mma_s8u8(hi, now.w[0][c].z, now.w[1][c].z, now.w[0][c].w, now.w[1][c].w, u.z, u.w);
+          mma_s8u8(lo, now.w[0][c].z, now.w[1][c].z, now.w[0][c].w, now.w[1][c].w, v.z, v.w);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int g = h * 8 + 2 * tig + (r & 1);
           if (g >= p.groups) continue;
           const float top = tops[(t * head_tiles + h) * 8 + 2 * tig + (r & 1)];
-          const float x = __fmul_rn(__fmul_rn(top, scale[r / 2]), __int2float_rn(128 * hi[r] + lo[r]));
+          const float x = __fmul_rn(__fmul_rn(top, now.scale[r / 2]), __int2float_rn(128 * hi[r] + lo[r]));
           best[r / 2] = isnan(x) ? INFINITY : fmaxf(best[r / 2], x);
         }
       }
@@ -149,123 +176,199 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32) q8_score_kernel(const Q8S
         const int j = tile * kQ8SelectTile + gid + 8 * i;
         if (tig == 0 && j < candidates) {
           const bool forced = j < p.first || j >= candidates - p.recent;
-          p.scores[((int64_t)blockIdx.y * p.tokens + token0 + t) * p.max_blocks + j] = !there[i] ? 0u : forced ? kQ8Forced : q8_ordered(best[i]);
+          p.scores[((int64_t)blockIdx.y * p.tokens + token0 + t) * p.max_blocks + j] = !now.there[i] ? 0u : forced ? kQ8Forced : q8_ordered(best[i]);
         }
       }
     }
+    now = next;
   }
 }
 
-constexpr int kQ8PickThreads = 256;
-constexpr int kQ8PickHeld = 12288;  // scores that are kept in shared memory
-
-// Exclusive sums of x and y over the CTA's threads.
-__device__ __forceinline__ void q8_scan2(int& x, int& y, int* smem) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int a = x, b = y;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, a, d), v = __shfl_up_sync(0xffffffffu, b, d);
-    if (lane >= d) {
-      a += u;
-      b += v;
-    }
-  }
-  if (lane == 31) {
-    smem[2 * warp] = a;
-    smem[2 * warp + 1] = b;
-  }
-  __syncthreads();
-  int before_a = 0, before_b = 0;
-  for (int w = 0; w < warp; ++w) {
-    before_a += smem[2 * w];
-    before_b += smem[2 * w + 1];
-  }
-  x = before_a + a - x;
-  y = before_b + b - y;
-}
-
-template <bool kHeld>
-__global__ void __launch_bounds__(kQ8PickThreads) q8_pick_kernel(const Q8SelectParams p) {
-  constexpr int kWarps = kQ8PickThreads / 32;
-  extern __shared__ __align__(16) uint32_t held[];
-  __shared__ int histogram[256], s_sums[2 * kWarps], s_digit, s_left;
+// A CTA's choice of a query token and KV head.  kHeld scores a thread are kept in registers, thread i has the scores i, i + THREADS, ...; with
+// kHeld = 0 they are read again wherever they are looked at.
+template <int THREADS, int kHeld>
+__global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p) {
+  constexpr int kWarps = THREADS / 32, kRounds = kHeld == 0 ? 1 : kHeld;
+  __shared__ int histogram[256], s_before[kRounds * kWarps], s_digit, s_left, s_same, s_taken;
+  __shared__ uint32_t s_high[kWarps], s_low[kWarps];
+  __shared__ int s_some[kWarps];
+  q8_let_next_start();
+  q8_wait_for_previous();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t stream = blockIdx.x;
   const int64_t b = stream / p.tokens / p.kv_heads;
-  const int t = (int)(stream % p.tokens);
-  const int n = q8_candidates(p, b, t);
+  const int n = q8_candidates(p, b, (int)(stream % p.tokens));
   const uint32_t* scores = p.scores + stream * p.max_blocks;
   int32_t* out = p.blocks + stream * p.count;
-  // place of score i in shared memory: a thread's run of scores and the next one's begin in different banks
-  const int run = (n + kQ8PickThreads - 1) / kQ8PickThreads;
-  auto score = [&](int i) { return kHeld ? held[i + i / 32] : __ldcg(scores + i); };
-  if (kHeld)
-    for (int i = threadIdx.x; i < n; i += kQ8PickThreads) held[i + i / 32] = __ldcg(scores + i);
-  // ---- the score of the last page that is taken, and how many of that score --------------------------------------------------------
-  uint32_t least = 1, known = 0;  // `known`: the bits of `least` that have been found
-  int left = p.count;
+  const int rounds = (n + THREADS - 1) / THREADS;
+  uint32_t held[kRounds] = {};
+  auto score = [&](int k) {
+    const int i = k * THREADS + (int)threadIdx.x;
+    return i < n ? __ldcg(scores + i) : 0u;
+  };
+  auto each = [&](auto&& fn) {
+    if constexpr (kHeld > 0) {
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k) fn(k, held[k]);
+    } else {
+      for (int k = 0; k < rounds; ++k) fn(k, score(k));
+    }
+  };
+  if constexpr (kHeld > 0) {
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) held[k] = score(k);
+  }
+  // ---- pages with a score above `least` are taken, and of those with that score the first `left` ----------------------------------------
+  uint32_t least = 0;
+  int left = 0;
   if (n > p.count) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      histogram[threadIdx.x] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += kQ8PickThreads) {
-        const uint32_t x = score(i);
-        if (x != 0 && (x & known) == (least & known)) atomicAdd(&histogram[(x >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (threadIdx.x < 32) {  // a lane has eight digits, the largest first
-        const int lane = threadIdx.x;
-        int mine[8], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += mine[i] = histogram[255 - 8 * lane - i];
-        int up_to = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, up_to, d);
-          if (lane >= d) up_to += v;
-        }
-        const bool crosses = up_to >= left && up_to - sum < left;
-        if (lane == 0) s_digit = -1;
-        __syncwarp();
-        if (crosses) {
-          int before = up_to - sum, i = 0;
-          while (before + mine[i] < left) before += mine[i++];
-          s_digit = 255 - 8 * lane - i;
-          s_left = left - before;
-        }
-      }
-      __syncthreads();
-      if (s_digit < 0) break;  // fewer candidates than are asked for: only in the first round, as all are then taken
-      least = (known == 0 ? 0u : least & known) | (uint32_t)s_digit << shift;
-      known |= 255u << shift;
-      left = s_left;
+    uint32_t high = 0, low = 0xffffffffu;
+    int some = 0;
+    each([&](int, uint32_t x) {
+      high = max(high, x);
+      low = min(low, x - 1u);  // 0 is no candidate
+      some += x != 0;
+    });
+    high = __reduce_max_sync(0xffffffffu, high);
+    low = __reduce_min_sync(0xffffffffu, low);
+    some = __reduce_add_sync(0xffffffffu, some);
+    if (lane == 0) {
+      s_high[warp] = high;
+      s_low[warp] = low;
+      s_some[warp] = some;
     }
-    if (known == 0) left = p.count;
-  }
-  const bool all = known == 0;  // every candidate is taken
-  __syncthreads();
-  // ---- in order ------------------------------------------------------------------------------------------------------------------
-  const int begin = min((int)threadIdx.x * run, n), end = min(begin + run, n);
-  int above = 0, equal = 0;
-  for (int i = begin; i < end; ++i) {
-    const uint32_t x = score(i);
-    above += all ? x != 0 : x > least;
-    equal += !all && x == least;
-  }
-  const int mine_above = above, mine_equal = equal;
-  q8_scan2(above, equal, s_sums);
-  int at = above + min(equal, left), ties = equal;
-  for (int i = begin; i < end; ++i) {
-    const uint32_t x = score(i);
-    if (all ? x != 0 : x > least) {
-      out[at++] = i;
-    } else if (!all && x == least) {
-      if (ties++ < left) out[at++] = i;
+    __syncthreads();
+    some = 0;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+      high = max(high, s_high[v]);
+      low = min(low, s_low[v]);
+      some += s_some[v];
+    }
+    low += 1u;
+    if (some > p.count) {
+      // `known`: the bits that all scores share, and further down those of the score that is looked for
+      int bits = high == low ? 0 : 32 - __clz(high ^ low);  // still unknown
+      uint32_t known = bits == 32 ? 0u : 0xffffffffu << bits;
+      least = high & known;
+      left = p.count;
+      while (bits > 0) {
+        const int width = min(bits, 8), shift = bits - width;
+        for (int i = threadIdx.x; i < 256; i += THREADS) histogram[i] = 0;
+        __syncthreads();
+        each([&](int, uint32_t x) {
+          if (x != 0 && (x & known) == least) atomicAdd(&histogram[(x >> shift) & ((1u << width) - 1u)], 1);
+        });
+        __syncthreads();
+        if (threadIdx.x < 32) {  // a lane has eight digits, the largest first
+          int mine[8], sum = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum += mine[i] = histogram[255 - 8 * lane - i];
+          int up_to = sum;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, up_to, d);
+            if (lane >= d) up_to += v;
+          }
+          if (up_to >= left && up_to - sum < left) {
+            int before = up_to - sum;
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (!found && before + mine[i] >= left) {
+                found = true;
+                s_digit = 255 - 8 * lane - i;
+                s_left = left - before;
+                s_same = mine[i];
+              }
+              before += mine[i];
+            }
+          }
+        }
+        __syncthreads();
+        least |= (uint32_t)s_digit << shift;
+        known |= ((1u << width) - 1u) << shift;
+        left = s_left;
+        bits = shift;
+        if (s_same == left && least != 0) {  // all that share these bits are taken
+          least -= 1u;
+          left = 0;
+          break;
+        }
+      }
     }
   }
-  if (threadIdx.x == kQ8PickThreads - 1) s_digit = above + mine_above + min(equal + mine_equal, all ? 0 : left);
+  // ---- in order: scores of a round of a warp, 32 neighbours, are counted by votes --------------------------------------------------------
+  if constexpr (kHeld > 0) {
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const unsigned above = __ballot_sync(0xffffffffu, held[k] > least), same = __ballot_sync(0xffffffffu, held[k] == least && held[k] != 0);
+      if (lane == 0) s_before[k * kWarps + warp] = __popc(above) | __popc(same) << 16;
+    }
+    __syncthreads();
+    if (warp == 0) {  // no more than 2^14 scores are held, so both counts fit into 16 bits
+      constexpr int kEach = (kRounds * kWarps + 31) / 32;
+      int mine[kEach], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int at = lane * kEach + i;
+        mine[i] = at < kRounds * kWarps ? s_before[at] : 0;
+        sum += mine[i];
+      }
+      int up_to = sum;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, up_to, d);
+        if (lane >= d) up_to += v;
+      }
+      int before = up_to - sum;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int at = lane * kEach + i;
+        if (at < kRounds * kWarps) s_before[at] = before;
+        before += mine[i];
+      }
+      if (lane == 31) s_taken = (up_to & 0xffff) + min(up_to >> 16, left);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const bool is_above = held[k] > least, is_same = held[k] == least && held[k] != 0;
+      const unsigned above = __ballot_sync(0xffffffffu, is_above), same = __ballot_sync(0xffffffffu, is_same);
+      const unsigned before = (1u << lane) - 1u;
+      const int base = s_before[k * kWarps + warp];
+      const int rank = (base & 0xffff) + __popc(above & before), ties = (base >> 16) + __popc(same & before);
+      if (is_above || (is_same && ties < left)) out[rank + min(ties, left)] = k * THREADS + (int)threadIdx.x;
+    }
+  } else {
+    int taken = 0, ties = 0;  // in front of the round
+    for (int k = 0; k < rounds; ++k) {
+      const uint32_t x = score(k);
+      const bool is_above = x > least, is_same = x == least && x != 0;
+      const unsigned above = __ballot_sync(0xffffffffu, is_above), same = __ballot_sync(0xffffffffu, is_same);
+      if (lane == 0) s_before[warp] = __popc(above) | __popc(same) << 16;
+      __syncthreads();
+      int rank = taken, tie = ties;
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        const int c = s_before[v];
+        if (v < warp) {
+          rank += c & 0xffff;
+          tie += c >> 16;
+        }
+        taken += c & 0xffff;
+        ties += c >> 16;
+      }
+      const unsigned before = (1u << lane) - 1u;
+      rank += __popc(above & before);
+      tie += __popc(same & before);
+      if (is_above || (is_same && tie < left)) out[rank + min(tie, left)] = k * THREADS + (int)threadIdx.x;
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) s_taken = taken + min(ties, left);
+  }
   __syncthreads();
-  for (int i = s_digit + threadIdx.x; i < p.count; i += kQ8PickThreads) out[i] = -1;
+  for (int i = s_taken + threadIdx.x; i < p.count; i += THREADS) out[i] = -1;
 }
 
 }  // namespace anna
@@ -303,25 +406,28 @@ extern "C" int anna_q8_select_blocks(const void* q, int64_t q_stride_b, int64_t 
   const int chunks = (tokens + p.tokens_at_once - 1) / p.tokens_at_once;
   ANNA_REQUIRE(chunks < 65536, "%s: too many tokens", what);
   if (max_blocks > 0) {
-    const int64_t tiles = (max_blocks + kQ8SelectTile - 1) / kQ8SelectTile, most = (tiles + kQ8SelectWarps - 1) / kQ8SelectWarps;
-    int64_t splits = 148 * 2 / ((int64_t)batch * kv_heads * chunks);
-    splits = splits < 1 ? 1 : splits > most ? most : splits;
+    // one wave where the pages are that few; a CTA whose pages lie behind its row's end leaves at once
+    const int64_t tiles = (max_blocks + kQ8SelectTile - 1) / kQ8SelectTile, wave = 148 * (head_dim == 256 ? 1 : 2) * kQ8SelectWarps;
+    const int64_t rounds = ((int64_t)batch * kv_heads * chunks * tiles + wave - 1) / wave;
+    p.rounds = (int)(rounds > kQ8SelectRounds ? kQ8SelectRounds : rounds);
+    const int64_t splits = (tiles + p.rounds * kQ8SelectWarps - 1) / (p.rounds * kQ8SelectWarps);
     const int rc = ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
       return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
         auto kernel = q8_score_kernel<T, D>;
         ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        kernel<<<dim3((unsigned)splits, (unsigned)(batch * kv_heads), (unsigned)chunks), kQ8SelectWarps * 32, smem, (cudaStream_t)stream>>>(p);
-        return check_launch("q8_score_kernel");
+        return q8_launch("q8_score_kernel", kernel, dim3((unsigned)splits, (unsigned)(batch * kv_heads), (unsigned)chunks), kQ8SelectWarps * 32,
+                         smem, (cudaStream_t)stream, p);
       });
     });
     if (rc != ANNA_OK) return rc;
   }
-  if (max_blocks <= kQ8PickHeld) {
-    const int held = (int)(max_blocks + max_blocks / 32 + 1) * 4;
-    ANNA_CUDA_CHECK(cudaFuncSetAttribute(q8_pick_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kQ8PickHeld + kQ8PickHeld / 32 + 1) * 4));
-    q8_pick_kernel<true><<<(unsigned)streams, kQ8PickThreads, held, (cudaStream_t)stream>>>(p);
-  } else {
-    q8_pick_kernel<false><<<(unsigned)streams, kQ8PickThreads, 0, (cudaStream_t)stream>>>(p);
-  }
-  return check_launch("q8_pick_kernel");
+  auto pick = [&](auto kernel, int threads) {
+    return q8_launch("q8_pick_kernel", kernel, dim3((unsigned)streams), threads, 0, (cudaStream_t)stream, p);
+  };
+  if (max_blocks <= 1024) return pick(q8_pick_kernel<256, 4>, 256);
+  if (max_blocks <= 2048) return pick(q8_pick_kernel<256, 8>, 256);
+  if (max_blocks <= 4096) return pick(q8_pick_kernel<512, 8>, 512);
+  if (max_blocks <= 8192) return pick(q8_pick_kernel<1024, 8>, 1024);
+  if (max_blocks <= 16384) return pick(q8_pick_kernel<1024, 16>, 1024);
+  return pick(q8_pick_kernel<1024, 0>, 1024);
 }
