@@ -1,18 +1,20 @@
 // Attention over the 8-bit paged cache on tensor cores: 16-bit caches, pages of a multiple of 16 tokens.
 //
-// Keys and values are the first operand of mma.sync m16n8k16 (S^T = K Q^T with tokens as rows, O^T = V^T P^T with dims as rows), the
-// queries that share a KV head its eight columns (NT times eight of a CTA).  Codes are whole numbers up to 127, which fp16 holds exactly:
-// a byte with its top bit flipped under the exponent of 1024 reads as 1152 + code, and taking 1152 off is exact, too; a permute and half a
-// subtraction per code.  The order of dims and tokens inside a product is free, so a lane's share of a tile is whole 16-byte pieces of
-// rows, and tiles go from global memory to registers without a stop in shared memory.
+// Keys and values are the first operand of mma.sync (S^T = K Q^T with 16 tokens as rows, O^T = V^T P^T with 16 dims as rows), the queries that
+// share a KV head its eight columns (NT times eight of a CTA).
 //
-// Queries are scaled by a power of two that brings their largest magnitude under 2^15, so bf16 ones fit into fp16 and lose no bit that is
-// worth 2^-29 of the largest.  Scores take the keys' scale of the page in 32 bits.  Weights are 2^14 times exp2 of the score below the
-// running maximum, rounded to fp16: all down to 2^-28 of the largest have 11 bits.  A tile's products are added to the sums in 32 bits, times
-// the values' scale of its page, so pages of any scales may meet.
+// Scores: codes go into the integer product as they are.  A query is a whole number of 24 bits, 2^22 to 2^23 for its head's largest
+// magnitude: three bytes, three products, whose sums are exact; what is not is the last bit of a query, 2^-24 of its largest magnitude.
+// Sums: a code with its top bit flipped is code + 128, which as the low byte of an fp16 is 2^-24 times that, a subnormal; so values take a mask
+// each and nothing more.  128 times the sum of the weights comes off in 32 bits, as what the product is added to (one product with -2^-17
+// everywhere gives it).  Weights are 2^14 times exp2 of the score below the running maximum, rounded to fp16: all down to 2^-28 of the
+// largest have 11 bits.  A tile's products are added to the sums in 32 bits, times the values' scale of its page, so pages of any scales may meet.
+//
+// The order of dims and tokens inside a product is free, so a lane's share of a tile is 16-byte pieces of rows.  A warp copies its own tiles,
+// 16 bytes a lane and instruction, into a ring of its own; pieces are swizzled so that the reads of a tile are free of bank conflicts.
 //
 // Tokens of the unfinished page take the same way as 16-token tiles of the ring: keys times queries in the cache's type, scaled by a power
-// of two as well, and weights as a sum of two numbers of it.
+// of two, and weights as a sum of two numbers of it.
 #include "mma_utils.cuh"
 #include "q8_common.cuh"
 
@@ -20,43 +22,83 @@ namespace anna {
 
 template <int D, int NT>
 struct Q8Cfg {
-  static constexpr int kWarps = NT == 1 && D <= 128 ? 8 : 4;
+  static constexpr int kWarps = 4;
   static constexpr int kThreads = kWarps * 32;
-  // per SM, by registers: 128, 168 or 255 a thread
-  static constexpr int kCtas = NT == 1 ? (D <= 128 ? 2 : 3) : NT == 2 && D <= 128 ? 3 : 2;
+  static constexpr int kCtas = D == 256 ? 2 : NT <= 2 ? 3 : 2;  // per SM
+  static constexpr int kStages = D == 64 ? 4 : D == 256 && NT == 2 ? 2 : 3;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kSteps = D / 16;          // products over the dims of a key
   static constexpr int kChunks = D / 64;         // 16-byte pieces of a lane's key
   static constexpr int kVWords = D / 32;         // 4-byte words of a lane's value
+  static constexpr int kTileBytes = 32 * D;      // keys and values of 16 tokens
   static constexpr int kMergeStride = D + 4;     // floats
-  static constexpr int kOffFrags = 0;                                   // [NT][steps][32 lanes] uint2: queries as second operands
-  static constexpr int kOffRing = kOffFrags + NT * kSteps * 256;        // [rows][D] queries in the cache's type
-  static constexpr int kOffStats = kOffRing + kRows * D * 2;             // [warps][rows] float2
+  static constexpr int kOffParts = 0;                                   // [NT][chunks][3][32 lanes] uint4: bytes of queries as second operands
+  static constexpr int kOffRing = kOffParts + NT * kChunks * 3 * 512;   // [rows][D] queries in the cache's type
+  static constexpr int kOffStats = kOffRing + kRows * D * 2;            // [warps][rows] float2
   static constexpr int kOffRate = kOffStats + kWarps * kRows * 8;       // [rows] to units of log2 of a weight; in the end 1 / denominator
-  static constexpr int kOffMerge = kOffRate + kRows * 4;                // [warps][8][stride] floats, or the weights of a merge
+  static constexpr int kOffRingRate = kOffRate + kRows * 4;             // [rows] the same for keys of the ring
+  static constexpr int kOffTiles = (kOffRingRate + kRows * 4 + 127) / 128 * 128;  // [warps][stages] tiles; in the end sums of the warps, weights of a merge
   static constexpr int kMergeBytes = kWarps * 8 * kMergeStride * 4;
   static constexpr int kWeightBytes = kRows * kMultiMaxPartials * 4;
-  static constexpr int kSmem = kOffMerge + (kMergeBytes > kWeightBytes ? kMergeBytes : kWeightBytes);
+  static constexpr int kRingBytes = kWarps * kStages * kTileBytes;
+  static constexpr int kSmem = kOffTiles + (kRingBytes > kWeightBytes ? kRingBytes : kWeightBytes);
+  static_assert(kMergeBytes <= kRingBytes && kCtas * (kSmem + 1024 + 5120) <= 228 * 1024, "shared memory");
 };
 
-__device__ __forceinline__ uint32_t q8_sub_half2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+// Place of the 16-byte piece `piece` of token `token` in a tile.  Reads of keys take pieces D / 64 t .. of tokens g and g + 8 (t = lane % 4, g = lane / 4),
+// reads of values those of dims D / 8 g .. of tokens 2 t + const: eight lanes of either always in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t q8_place(int token, int piece) {
+  if constexpr (D == 64) {  // two tokens to a line of 128 bytes
+    return token / 2 * 128 + ((((token & 1) << 2 | piece) ^ (token & 6)) << 4);
+  } else if constexpr (D == 128) {
+    return token * 128 + ((piece ^ (token & 7)) << 4);
+  } else {  // a token has two lines
+    const int turn = (token & 4) | (token & 1) << 1 | ((token >> 1 & 1) ^ piece >> 3);
+    return token * 256 + (piece & 8) * 16 + (((piece & 7) ^ turn) << 4);
+  }
 }
-// Bytes (flipped codes) 0 and 1, or 2 and 3, of x as two fp16.
-template <int PAIR>
-__device__ __forceinline__ uint32_t q8_halves(uint32_t x) {
-  return q8_sub_half2(__byte_perm(x, 0x64646464u, PAIR == 0 ? 0x4140 : 0x4342), 0x64806480u);
+// What one lane's places differ by, so that few of them have to be worked out: the copy of pieces 32 i + lane, value tokens 2 t and 2 t + 1.
+// (All of them from q8_place in the loop took two thirds of its instructions: 16 rows of 32768 tokens 199 us.)
+template <int D>
+__host__ __device__ constexpr uint32_t kQ8CopyTurn(int i) {
+  return D == 64 ? 0u : D == 128 ? (uint32_t)(i & 1) << 6 : (uint32_t)((i >> 1 & 1) << 2 | (i & 1)) << 4;
 }
-template <typename T>
-__device__ __forceinline__ void q8_mma_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void q8_mma_zero<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+template <int D>
+constexpr uint32_t kQ8OddTurn = D == 64 ? 64u : D == 128 ? 16u : 32u;
+template <int D>
+constexpr uint32_t kQ8OddStep = D == 64 ? 0u : D;  // bytes from a token's line to the next one's
+
+__device__ __forceinline__ uint4 q8_shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 q8_shared8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+
+// d += a . b of signed bytes with signed or unsigned ones.
+template <bool kSigned>
+__device__ __forceinline__ void q8_mma_bytes(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (kSigned)
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a . b + c
+__device__ __forceinline__ void q8_mma_onto(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[2]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]));
 }
 __device__ __forceinline__ float q8_exp2(float x) {
   float r;
@@ -75,12 +117,21 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
   using Cfg = Q8Cfg<D, NT>;
   constexpr int kTile = kBalancedTileTokens;
   constexpr int kFar = 0x7fff0000;  // position of a token that nobody sees
-  constexpr float kRingFactor = std::is_same_v<T, __half> ? 1.0f : 1.0f / 16384.0f;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const uint2* frags = reinterpret_cast<const uint2*>(smem + Cfg::kOffFrags) + (threadIdx.x & 31);
+  // Queries of the ring are under 2^15 in fp16 and under 2 in bf16, whose keys may be as large as a product; for the same reason sums are 2^14
+  // times what they stand for in fp16 alone.
+  constexpr bool kHalf = std::is_same_v<T, __half>;
+  constexpr float kWeight = 16384.0f;                        // of the largest
+  constexpr float kRingWeight = kHalf ? kWeight : 1.0f;
+  extern __shared__ __align__(128) uint8_t smem[];
   float* rate = reinterpret_cast<float*>(smem + Cfg::kOffRate);
+  float* ring_rate = reinterpret_cast<float*>(smem + Cfg::kOffRingRate);
   float2* stats = reinterpret_cast<float2*>(smem + Cfg::kOffStats);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  const uint32_t tiles = smem_u32(smem + Cfg::kOffTiles) + warp * Cfg::kStages * Cfg::kTileBytes, tiles_end = tiles + Cfg::kStages * Cfg::kTileBytes;
+  // this lane's places in a tile: what it copies, keys, values of tokens 2 t; see kQ8CopyTurn
+  const uint32_t copy_place = q8_place<D>(lane / (D / 16), lane % (D / 16)), key_place = q8_place<D>(gid, Cfg::kChunks * tig);
+  const uint32_t value_place = 16 * D + (D == 64 ? q8_place<D>(2 * tig, gid / 2) + gid % 2 * 8 : q8_place<D>(2 * tig, D / 128 * gid));
+  const uint32_t parts = smem_u32(smem + Cfg::kOffParts) + lane * 16;
   q8_let_next_start();
   q8_wait_for_previous();
 
@@ -111,71 +162,70 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
     }
     return x;
   };
-  auto scales = [&](Pages& x) {
-    // a tile's keys begin `slot` rows behind its page
-    if (x.position != kFar)
-      x.scale = __ldg(reinterpret_cast<const float2*>(x.keys + (int64_t)(2 * p.block_size - x.position % p.block_size) * D));
-  };
-  uint4 key[2][Cfg::kChunks];
-  uint32_t val[4][Cfg::kVWords];
-  auto load_keys = [&](const uint8_t* keys) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int c = 0; c < Cfg::kChunks; ++c) key[i][c] = ldg_stream16(keys + (gid + 8 * i) * D + 64 * c + 16 * tig);
-  };
-  const int values_at = p.block_size * D;
-  auto load_values = [&](const uint8_t* keys) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t* from = keys + values_at + (2 * tig + (i & 1) + 8 * (i / 2)) * D + gid * (D / 8);
-      if constexpr (D == 64) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(from));
-        val[i][0] = v.x; val[i][1] = v.y;
-      } else {
-#pragma unroll
-        for (int c = 0; c < D / 128; ++c) {
-          const uint4 v = ldg_stream16(from + 16 * c);
-          val[i][4 * c] = v.x; val[i][4 * c + 1] = v.y; val[i][4 * c + 2] = v.z; val[i][4 * c + 3] = v.w;
-        }
-      }
+  auto scales = [&](Pages& x) {  // a tile's keys begin `slot` rows behind its page
+    if (x.position != kFar) {
+      const int slot = p.block_shift >= 0 ? x.position & (p.block_size - 1) : x.position % p.block_size;
+      x.scale = __ldg(reinterpret_cast<const float2*>(x.keys + (int64_t)(2 * p.block_size - slot) * D));
     }
   };
-  auto broadcast = [&](const uint8_t* x, int from) {
-    return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)x, from));
+  const int values_at = p.block_size * D;
+  auto copy_tile = [&](const uint8_t* keys, uint32_t to) {
+    const uint8_t* from = keys + lane * 16;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) cp_async16(to + (copy_place ^ kQ8CopyTurn<D>(i)) + i * 512, from + i * 512, 16);
+    from += values_at;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) cp_async16(to + (copy_place ^ kQ8CopyTurn<D>(i)) + 16 * D + i * 512, from + i * 512, 16);
   };
   Pages now = find(0), next = now;
-  const uint8_t* at = broadcast(now.keys, 0);
-  if (mine > 0) {
-    load_keys(at);
-    load_values(at);
-    scales(now);
-    if (mine > 32) next = find(32);
-  }
+  uint32_t to = tiles;  // where the next copy goes
+  auto start = [&](int i, int done) {  // copies of tile i, while `now` is of the 32 tiles that `done` is of
+    if (i < mine) {
+      const unsigned long long keys = (i >> 5) == (done >> 5) ? (unsigned long long)now.keys : (unsigned long long)next.keys;
+      copy_tile(reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, keys, i & 31)), to);
+    }
+    to = to + Cfg::kTileBytes == tiles_end ? tiles : to + Cfg::kTileBytes;
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < Cfg::kStages - 1; ++i) start(i, 0);
+  scales(now);
+  if (mine > 32) next = find(32);
 
   // ---- queries -----------------------------------------------------------------------------------------------------------------------
   for (int i = warp; i < Cfg::kRows; i += Cfg::kWarps) {
     constexpr int E = D / 32;
     float x[E], top = 0.0f;
+    bool fine = true;
     const int row = st.row0 + min(i, st.count - 1), t = multi_token_of(p, row), h = kvh * p.groups + row - t * p.groups;
     const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_stride_b + h * p.q_stride_h + t * p.q_stride_t + lane * E;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       x[j] = ElemTraits<T>::to_float(q[j]);
+      fine = fine && fabsf(x[j]) < INFINITY;
       top = fmaxf(top, fabsf(x[j]));
     }
+    fine = __all_sync(0xffffffffu, fine);
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    int up = top > 0.0f && top < INFINITY ? 14 + 127 - (int)(__float_as_uint(top) >> 23) : 0;  // top * 2^up is in [2^14, 2^15)
-    up = min(up, 126);
-    const float factor = __uint_as_float((uint32_t)(up + 127) << 23);
-    if (lane == 0) rate[i] = p.scaling * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - up) << 23);
+    // top * 2^up is in [1, 2)
+    const int up = fine && top > 0.0f ? min(127 - (int)(__float_as_uint(top) >> 23), 126) : 0;
+    const float factor = __uint_as_float((uint32_t)(max(up, -126) + 127) << 23) * (up < -126 ? 0.5f : 1.0f);
+    const float back = p.scaling * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - up) << 23);
+    constexpr float kRingFactor = kHalf ? 16384.0f : 1.0f;
+    if (lane == 0) {
+      rate[i] = fine ? back / 4194304.0f : __int_as_float(0x7fc00000);
+      ring_rate[i] = back / kRingFactor;
+    }
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const int d = lane * E + j;
-      const int place = ((i / 8 * Cfg::kSteps + d / 64 * 4 + d % 16 / 4) * 32 + i % 8 * 4 + d % 64 / 16) * 4 + d % 4;
-      reinterpret_cast<__half*>(smem + Cfg::kOffFrags)[place] = __float2half_rn(x[j] * factor);
-      // under 2^15 in fp16, under 2 in bf16, whose keys may be as large as a product
+      const int whole = fine ? __float2int_rn(x[j] * factor * 4194304.0f) : 0;
+      // dims D / 4 t + 16 c .. are lane t's piece c
+      const int place = (((i / 8 * Cfg::kChunks + d % (D / 4) / 16) * 3) * 32 + i % 8 * 4 + d / (D / 4)) * 16 + d % 16;
+      smem[Cfg::kOffParts + place] = (uint8_t)(whole >> 16);
+      smem[Cfg::kOffParts + place + 512] = (uint8_t)(whole >> 8);
+      smem[Cfg::kOffParts + place + 1024] = (uint8_t)whole;
       reinterpret_cast<T*>(smem + Cfg::kOffRing)[i * D + d] = ElemTraits<T>::from_float(x[j] * factor * kRingFactor);
     }
   }
@@ -227,7 +277,7 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float base = m_run[j][k] == -INFINITY ? 0.0f : m_run[j][k] - 14.0f;
+        const float base = m_run[j][k] == -INFINITY ? 0.0f : m_run[j][k] - 14.0f;  // log2 of kWeight
         s[j][k] = q8_exp2(s[j][k] - base);
         s[j][k + 2] = q8_exp2(s[j][k + 2] - base);
         l_run[j][k] += s[j][k] + s[j][k + 2];
@@ -235,44 +285,44 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
   };
 
   // ---- packed tiles -------------------------------------------------------------------------------------------------------------------
+  uint32_t at = tiles;  // of the tile that is read
   for (int i = 0; i < mine; ++i) {
     const int position = __shfl_sync(0xffffffffu, now.position, i & 31);
     const float2 scale = make_float2(__shfl_sync(0xffffffffu, now.scale.x, i & 31), __shfl_sync(0xffffffffu, now.scale.y, i & 31));
-    if ((i & 31) == 31 && i + 1 < mine) {
-      now = next;
-      scales(now);
-      if (i + 33 < mine) next = find(i + 33);
-    }
-    at = broadcast(now.keys, (i + 1) & 31);
-    float s[NT][4];
+    cp_async_wait<Cfg::kStages - 2>();
+    __syncwarp();  // the tile is there, and the one in front of it has been read
+    start(i + Cfg::kStages - 1, i);
+    int whole[NT][3][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[j][r] = 0.0f;
+      for (int x = 0; x < 3; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) whole[j][x][r] = 0;
 #pragma unroll
     for (int c = 0; c < Cfg::kChunks; ++c) {
-      const uint32_t wa[4] = {key[0][c].x, key[0][c].y, key[0][c].z, key[0][c].w};
-      const uint32_t wb[4] = {key[1][c].x, key[1][c].y, key[1][c].z, key[1][c].w};
+      const uint4 u = q8_shared16(at + (key_place ^ c << 4)), v = q8_shared16(at + (key_place ^ c << 4) + 8 * D);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint32_t ua = wa[x] ^ 0x80808080u, ub = wb[x] ^ 0x80808080u;
-        const uint32_t a[4] = {q8_halves<0>(ua), q8_halves<0>(ub), q8_halves<1>(ua), q8_halves<1>(ub)};
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const uint2 q = frags[(j * Cfg::kSteps + 4 * c + x) * 32];
-          mma_m16n8k16<__half>(s[j], a, q.x, q.y);
-        }
+      for (int j = 0; j < NT; ++j) {
+        const uint32_t q = parts + (j * Cfg::kChunks + c) * 1536;
+        const uint4 q0 = q8_shared16(q), q1 = q8_shared16(q + 512), q2 = q8_shared16(q + 1024);
+        q8_mma_bytes<true>(whole[j][0], u.x, v.x, u.y, v.y, q0.x, q0.y);
+        q8_mma_bytes<false>(whole[j][1], u.x, v.x, u.y, v.y, q1.x, q1.y);
+        q8_mma_bytes<false>(whole[j][2], u.x, v.x, u.y, v.y, q2.x, q2.y);
+        q8_mma_bytes<true>(whole[j][0], u.z, v.z, u.w, v.w, q0.z, q0.w);
+        q8_mma_bytes<false>(whole[j][1], u.z, v.z, u.w, v.w, q1.z, q1.w);
+        q8_mma_bytes<false>(whole[j][2], u.z, v.z, u.w, v.w, q2.z, q2.w);
       }
     }
-    if (i + 1 < mine) load_keys(at);
-    float by[NT][2];
+    float s[NT][4], by[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const float x = scale.x * to_log2[j][k];
-        s[j][k] *= x;
-        s[j][k + 2] *= x;
+#pragma unroll
+        for (int r = k; r < 4; r += 2)  // the lower two bytes' sums are below 2^23 each: together below 2^31
+          s[j][r] = fmaf(__int2float_rn(whole[j][0][r]), 65536.0f, __int2float_rn(whole[j][1][r] * 256 + whole[j][2][r])) * x;
         by[j][k] = scale.y;
       }
     if (position + kTile - 1 > first_seen) {  // tokens that some rows do not see, or a page that is none
@@ -288,30 +338,63 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
     }
     softmax(s);
     uint32_t w[NT][2];
+    float off[NT][2];  // what the flipped bits are too much
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) w[j][k] = movmatrix_trans(pack2<__half>(s[j][2 * k], s[j][2 * k + 1]));
+      const uint32_t flipped[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+      const float zero[2] = {0.0f, 0.0f};
+      float sum[4];
+      q8_mma_onto(sum, flipped, w[j][0], w[j][1], zero);
+      off[j][0] = sum[0];
+      off[j][1] = sum[1];
+    }
+    uint32_t val[4][Cfg::kVWords];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t from = (value_place ^ ((k & 1) ? kQ8OddTurn<D> : 0u)) + (k & 1) * kQ8OddStep<D> + k / 2 * 8 * D;
+      if constexpr (D == 64) {
+        const uint2 v = q8_shared8(at + from);
+        val[k][0] = v.x; val[k][1] = v.y;
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 128; ++c) {
+          const uint4 v = q8_shared16(at + (from ^ c << 4));
+          val[k][4 * c] = v.x; val[k][4 * c + 1] = v.y; val[k][4 * c + 2] = v.z; val[k][4 * c + 3] = v.w;
+        }
+      }
+    }
 #pragma unroll
     for (int v = 0; v < Cfg::kVWords; ++v) {
-      uint32_t u[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = val[k][v] ^ 0x80808080u;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint32_t x = __byte_perm(u[0], u[1], half == 0 ? 0x5140 : 0x7362), z = __byte_perm(u[2], u[3], half == 0 ? 0x5140 : 0x7362);
-        const uint32_t a[4] = {q8_halves<0>(x), q8_halves<1>(x), q8_halves<0>(z), q8_halves<1>(z)};
+        const uint32_t x = __byte_perm(val[0][v], val[1][v], half == 0 ? 0x5410 : 0x7632), z = __byte_perm(val[2][v], val[3][v], half == 0 ? 0x5410 : 0x7632);
+        const uint32_t a[4] = {(x & 0x00ff00ffu) ^ 0x00800080u, (x >> 8 & 0x00ff00ffu) ^ 0x00800080u, (z & 0x00ff00ffu) ^ 0x00800080u,
+                               (z >> 8 & 0x00ff00ffu) ^ 0x00800080u};
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           float sum[4];
-          q8_mma_zero<__half>(sum, a, w[j][0], w[j][1]);
+          q8_mma_onto(sum, a, w[j][0], w[j][1], off[j]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[j][2 * v + half][r] = fmaf(sum[r], by[j][r & 1], o[j][2 * v + half][r]);
         }
       }
     }
-    if (i + 1 < mine) load_values(at);
+    if ((i & 31) == 16 && i + 16 < mine) scales(next);
+    at = at + Cfg::kTileBytes == tiles_end ? tiles : at + Cfg::kTileBytes;
+    if ((i & 31) == 31 && i + 1 < mine) {
+      now = next;
+      if (i + 33 < mine) next = find(i + 33);
+    }
   }
+  // from 2^-24 of the codes' units to those of the ring
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[j][d][r] *= 16777216.0f / kWeight * kRingWeight;
 
   // ---- tiles of the ring ----------------------------------------------------------------------------------------------------------------
   const int64_t ring_from = max(t0, st.packed);
@@ -347,7 +430,7 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int token = gid + 8 * (r / 2);
-          s[j][r] = token >= valid || position + token > limit(j, r & 1) ? -INFINITY : s[j][r] * (to_log2[j][r & 1] / kRingFactor);
+          s[j][r] = token >= valid || position + token > limit(j, r & 1) ? -INFINITY : s[j][r] * ring_rate[8 * j + 2 * tig + (r & 1)];
         }
       softmax(s);
       // weights as a sum of two of the type, so that they keep 16 bits and more
@@ -356,7 +439,7 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float x = s[j][2 * k], y = s[j][2 * k + 1];
+          const float x = s[j][2 * k] * (kRingWeight / kWeight), y = s[j][2 * k + 1] * (kRingWeight / kWeight);
           const uint32_t most = pack2<T>(x, y);
           const T* parts = reinterpret_cast<const T*>(&most);
           w[j][k] = movmatrix_trans(most);
@@ -408,6 +491,7 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
   }
 
   // ---- the warps' rows together ----------------------------------------------------------------------------------------------------------
+  cp_async_wait<0>();
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -431,13 +515,14 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
       stats[v * Cfg::kRows + i].x = by;
       den = fmaf(x.y, by, den);
     }
+    den *= kRingWeight / kWeight;  // in the sums' units
     // a NaN among the scores has to stay one, so only a row without a key is zero
     rate[i] = part.count > 1 ? 1.0f : den == 0.0f ? 0.0f : 1.0f / den;
     if (part.count > 1 && i < st.count)
       reinterpret_cast<float2*>(p.stats)[multi_partial_row(part, part.mine, Cfg::kRows) + i] = make_float2(top * 0.6931471805599453f, den);
   }
   __syncthreads();
-  float* merged = reinterpret_cast<float*>(smem + Cfg::kOffMerge);
+  float* merged = reinterpret_cast<float*>(smem + Cfg::kOffTiles);
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
 #pragma unroll
