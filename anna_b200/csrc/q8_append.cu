@@ -32,6 +32,7 @@ struct Q8AppendParams {
 };
 
 constexpr int kQ8AppendWarps = 4;
+constexpr int64_t kQ8MaxLength = 1ll << 30;  // of a table, and of a call's tokens
 
 // The lanes' 16 bytes as values, and what follows of their extremes.
 template <typename T>
@@ -138,24 +139,28 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
   q8_let_next_start();
   q8_wait_for_previous();
   const int lane = threadIdx.x & 31, part = PER == 1 ? 0 : threadIdx.x >> 5;
-  const int64_t item = PER == 1 ? (int64_t)blockIdx.x * kQ8AppendWarps + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-  const int which = (int)(item & 1);  // keys, values
-  int64_t rest = item >> 1;
-  const int unit = (int)(rest % p.units);
-  rest /= p.units;
-  const int h = (int)(rest % p.kv_heads);
-  const int64_t b = rest / p.kv_heads;
+  const uint32_t item = PER == 1 ? blockIdx.x * kQ8AppendWarps + (threadIdx.x >> 5) : blockIdx.x;
+  const int which = (int)(item & 1u);  // keys, values
+  uint32_t rest = item >> 1;
+  const int unit = (int)(rest % (uint32_t)p.units);
+  rest /= (uint32_t)p.units;
+  const int h = (int)(rest % (uint32_t)p.kv_heads);
+  const int64_t b = rest / (uint32_t)p.kv_heads;
   if (b >= p.batch) return;
   const int S = p.block_size;
-  const int64_t past = p.past_lengths[b], total = past + p.tokens;
-  if (p.new_lengths != nullptr && unit == 0 && h == 0 && which == 0 && lane == 0 && part == 0) p.new_lengths[b] = total;
-  if (past < 0) return;
-  const int64_t block = past / S + unit;
+  const int64_t past_length = p.past_lengths[b];
+  if (p.new_lengths != nullptr && unit == 0 && h == 0 && which == 0 && lane == 0 && part == 0) p.new_lengths[b] = past_length + p.tokens;
+  if (past_length < 0) return;
+  if (past_length >= kQ8MaxLength) {  // behind any table
+    if (p.status != nullptr && unit == 0 && lane == 0) atomicOr(p.status, (int)ANNA_DEV_BAD_PAGE);
+    return;
+  }
+  const int past = (int)past_length, total = past + p.tokens, block = past / S + unit;
   const T* fresh = reinterpret_cast<const T*>(p.in[which]) + b * p.stride_b[which] + h * p.stride_h[which];
   const int64_t step = p.stride_t[which];
   const int64_t slot = unit == 0 ? p.window_slots[b] : -1;
   T* ring = slot >= 0 && slot < p.num_slots ? reinterpret_cast<T*>(p.window) + ((slot * 2 + which) * p.kv_heads + h) * S * D : nullptr;
-  const int64_t begin = block * S;  // position of the page's first token
+  const int begin = block * S;  // position of the page's first token
   const int col = lane % kLanes * kN, row = part * (32 / kLanes) + lane / kLanes;
 
   const bool closes = begin + S <= total;
@@ -169,8 +174,8 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
     uint8_t* page = p.pages + ((int64_t)pid * p.kv_heads + h) * p.page_bytes;
     uint8_t* codes = page + which * S * D;
     auto source = [&](int token) {
-      const int64_t at = begin + token;
-      return at < past ? ring + (int64_t)token * D : fresh + (at - past) * step;
+      const int at = begin + token;
+      return at < past ? ring + token * D : fresh + (at - past) * step;
     };
     const int rounds = (S + kAtOnce - 1) / kAtOnce;
     Q8Extremes<T> seen[kCols];
@@ -278,9 +283,8 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
   if (unit != 0 || ring == nullptr) return;
   if constexpr (PER == 1) __syncwarp();  // the ring has been read
   else __syncthreads();
-  const int64_t open = total / S * S;  // first position of the unfinished page
-  const int64_t from = max(past, open);
-  for (int64_t at = from + row; at < total; at += kAtOnce)
+  const int open = total / S * S;  // first position of the unfinished page
+  for (int at = max(past, open) + row; at < total; at += kAtOnce)
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
       *reinterpret_cast<uint4*>(ring + (at - open) * D + c * 32 * kN + col) =
@@ -298,7 +302,8 @@ struct Q8GatherParams {
   int64_t stride_b, stride_h, stride_t;
   int batch, kv_heads, block_size, page_bytes;
   int shares;  // of a block
-  int64_t num_pages, max_blocks, num_slots, max_len, spans;
+  int spans;   // blocks
+  int64_t num_pages, max_blocks, num_slots, max_len;
 };
 constexpr int kQ8GatherPieces = 128;  // of 16 codes, of a warp
 
@@ -311,19 +316,20 @@ __global__ void __launch_bounds__(128) q8_gather_kernel(const Q8GatherParams p) 
   q8_let_next_start();
   q8_wait_for_previous();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int which = (int)(item & 1);
-  int64_t rest = item >> 1;
-  const int share = (int)(rest % p.shares);
-  rest /= p.shares;
-  const int64_t block = rest % p.spans;
-  rest /= p.spans;
-  const int h = (int)(rest % p.kv_heads);
-  const int64_t b = rest / p.kv_heads;
+  const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int which = (int)(item & 1u);
+  uint32_t rest = item >> 1;
+  const int share = (int)(rest % (uint32_t)p.shares);
+  rest /= (uint32_t)p.shares;
+  const int block = (int)(rest % (uint32_t)p.spans);
+  rest /= (uint32_t)p.spans;
+  const int h = (int)(rest % (uint32_t)p.kv_heads);
+  const int64_t b = rest / (uint32_t)p.kv_heads;
   if (b >= p.batch) return;
   const int S = p.block_size;
-  const int64_t len = max((int64_t)0, min(p.lengths[b], p.max_len)), begin = block * S;
-  const bool full = begin + S <= p.lengths[b];
+  const int64_t length = p.lengths[b];
+  const int len = (int)max((int64_t)0, min(length, p.max_len)), begin = block * S;
+  const bool full = begin + S <= length;
   const uint8_t* codes = nullptr;
   const T* ring = nullptr;
   float scale = 0.0f;
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(128) q8_gather_kernel(const Q8GatherParams p) 
     if (slot >= 0 && slot < p.num_slots) ring = reinterpret_cast<const T*>(p.window) + ((slot * 2 + which) * p.kv_heads + h) * S * D;
   }
   T* out = reinterpret_cast<T*>(p.out[which]) + b * p.stride_b + h * p.stride_h;
-  const int pieces = (int)min((int64_t)S, p.max_len - begin) * kPieces;
+  const int pieces = min(S, (int)p.max_len - begin) * kPieces;
   const int end = min(pieces, (share + 1) * kQ8GatherPieces);
 #pragma unroll
   for (int round = 0; round < kQ8GatherPieces / 32; ++round) {
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(128) q8_gather_kernel(const Q8GatherParams p) 
       for (int j = 0; j < 16 / kN; ++j)
         x[j] = ring != nullptr && begin + token < len ? *reinterpret_cast<const uint4*>(ring + token * D + d + j * kN) : make_uint4(0u, 0u, 0u, 0u);
     }
-    T* to = out + (begin + token) * p.stride_t + d;
+    T* to = out + (int64_t)(begin + token) * p.stride_t + d;
 #pragma unroll
     for (int j = 0; j < 16 / kN; ++j) *reinterpret_cast<uint4*>(to + j * kN) = x[j];
   }
@@ -412,9 +418,9 @@ extern "C" int anna_q8_append(const void* k_new, int64_t k_stride_b, int64_t k_s
   // A CTA to an item where a warp would have more than 8 vectors a lane, or where the GPU has room for that: 64 rows of one token
   // PLACEHOLDER
   const int64_t items = (int64_t)batch * kv_heads * p.units * 2;
+  ANNA_REQUIRE(new_tokens < kQ8MaxLength && max_blocks < kQ8MaxLength / block_size && items < (1ll << 31), "%s: too many tokens", what);
   const bool whole = block_size * head_dim / vec > 256 || items <= 148 * 8;
   const int64_t ctas = whole ? items : (items + kQ8AppendWarps - 1) / kQ8AppendWarps;
-  ANNA_REQUIRE(ctas < (1ll << 31), "%s: too many tokens", what);
   return ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
       return q8_launch("q8_append_kernel", whole ? q8_append_kernel<T, D, kQ8AppendWarps> : q8_append_kernel<T, D, 1>, dim3((unsigned)ctas),
@@ -446,10 +452,11 @@ extern "C" int anna_q8_gather(const uint8_t* pages, const int32_t* page_table, i
   p.stride_b = out_stride_b; p.stride_h = out_stride_h; p.stride_t = out_stride_t;
   p.batch = batch; p.kv_heads = kv_heads; p.block_size = block_size; p.page_bytes = (int)bytes;
   p.num_pages = num_pages; p.max_blocks = max_blocks; p.num_slots = num_slots; p.max_len = max_len;
-  p.spans = (max_len + block_size - 1) / block_size;
+  ANNA_REQUIRE(max_len < kQ8MaxLength, "%s: too many tokens", what);
+  p.spans = (int)((max_len + block_size - 1) / block_size);
   p.shares = (block_size * head_dim / 16 + kQ8GatherPieces - 1) / kQ8GatherPieces;
   const int64_t warps = (int64_t)batch * kv_heads * p.spans * p.shares * 2;
-  ANNA_REQUIRE(p.spans < (1ll << 31) && warps / 4 < (1ll << 31) - 1, "%s: too many tokens", what);
+  ANNA_REQUIRE(warps < (1ll << 31), "%s: too many tokens", what);
   return ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
       return q8_launch("q8_gather_kernel", q8_gather_kernel<T, D>, dim3((unsigned)((warps + 3) / 4)), 128, 0, (cudaStream_t)stream, p);

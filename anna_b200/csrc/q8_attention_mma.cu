@@ -5,10 +5,11 @@
 //
 // Scores: codes go into the integer product as they are.  A query is a whole number of 24 bits, 2^22 to 2^23 for its head's largest
 // magnitude: three bytes, three products, whose sums are exact; what is not is the last bit of a query, 2^-24 of its largest magnitude.
-// Sums: a code with its top bit flipped is code + 128, which as the low byte of an fp16 is 2^-24 times that, a subnormal; so values take a mask
-// each and nothing more.  128 times the sum of the weights comes off in 32 bits, as what the product is added to (one product with -2^-17
-// everywhere gives it).  Weights are 2^14 times exp2 of the score below the running maximum, rounded to fp16: all down to 2^-28 of the
-// largest have 11 bits.  A tile's products are added to the sums in 32 bits, times the values' scale of its page, so pages of any scales may meet.
+// Sums: a code with its top bit flipped, as the low byte of an fp16 of exponent 1024, reads as 1152 + code, and taking 1152 off is exact.  Weights
+// are 2^14 times exp2 of the score below the running maximum, rounded to fp16: all down to 2^-28 of the largest have 11 bits.  The scale of a
+// page's values goes into its weights where it is within 2^6 of the largest so far; where it is smaller, the tile's product is added to the sums
+// in 32 bits, times the scale, so pages of any scales may meet.  (The product of each tile added in 32 bits, with codes as fp16 subnormals, which
+// are one operation a pair instead of two: 16 rows of 32768 tokens, 4 queries a KV head PLACEHOLDER.)
 //
 // The order of dims and tokens inside a product is free, so a lane's share of a tile is 16-byte pieces of rows.  A warp copies its own tiles,
 // 16 bytes a lane and instruction, into a ring of its own; pieces are swizzled so that the reads of a tile are free of bank conflicts.
@@ -79,26 +80,31 @@ __device__ __forceinline__ uint2 q8_shared8(uint32_t at) {
   return v;
 }
 
-// d += a . b of signed bytes with signed or unsigned ones.
-template <bool kSigned>
+// d += a . b of signed bytes with signed or unsigned ones; kFirst: d = a . b.
+template <bool kSigned, bool kFirst>
 __device__ __forceinline__ void q8_mma_bytes(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (kSigned)
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+#define ANNA_Q8_MMA(TYPE, C0, C1, C2, C3)                                                                                              \
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8." TYPE ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"      \
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                                        \
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(C0), "r"(C1), "r"(C2), "r"(C3))
+  if constexpr (kSigned && kFirst) ANNA_Q8_MMA("s8", 0, 0, 0, 0);
+  else if constexpr (kSigned) ANNA_Q8_MMA("s8", d[0], d[1], d[2], d[3]);
+  else if constexpr (kFirst) ANNA_Q8_MMA("u8", 0, 0, 0, 0);
+  else ANNA_Q8_MMA("u8", d[0], d[1], d[2], d[3]);
+#undef ANNA_Q8_MMA
 }
-// d = a . b + c
-__device__ __forceinline__ void q8_mma_onto(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[2]) {
+// d = a . b
+__device__ __forceinline__ void q8_mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// The codes in bytes 0 and 2 of x as two fp16.
+__device__ __forceinline__ uint32_t q8_halves(uint32_t x) {
+  uint32_t r;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"((x & 0x00ff00ffu) ^ 0x64806480u), "r"(0x64806480u));
+  return r;
 }
 __device__ __forceinline__ float q8_exp2(float x) {
   float r;
@@ -247,13 +253,14 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
       for (int r = 0; r < 4; ++r) o[j][d][r] = 0.0f;
   auto limit = [&](int j, int k) { return first_seen + multi_token_of(p, st.row0 + 8 * j + 2 * tig + k); };  // newest key that a row sees
 
-  // Scores of 16 tokens (rows gid and gid + 8 of every column pair) become weights, at 2^14 times their size.
+  // Scores of 16 tokens (rows gid and gid + 8 of every column pair) become weights, at 2^14 times their size.  A score may be up to 1 above the
+  // running maximum (a weight of 2^15) before that is raised: the sums are scaled anew less often.
   auto softmax = [&](float (&s)[NT][4]) {
     bool more = false;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) more = more || fmaxf(s[j][k], s[j][k + 2]) > m_run[j][k];
+      for (int k = 0; k < 2; ++k) more = more || fmaxf(s[j][k], s[j][k + 2]) > m_run[j][k] + 1.0f;
     if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
@@ -286,6 +293,7 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
 
   // ---- packed tiles -------------------------------------------------------------------------------------------------------------------
   uint32_t at = tiles;  // of the tile that is read
+  int unit = -120;         // of the sums, as a power of two
   for (int i = 0; i < mine; ++i) {
     const int position = __shfl_sync(0xffffffffu, now.position, i & 31);
     const float2 scale = make_float2(__shfl_sync(0xffffffffu, now.scale.x, i & 31), __shfl_sync(0xffffffffu, now.scale.y, i & 31));
@@ -294,27 +302,26 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
     start(i + Cfg::kStages - 1, i);
     int whole[NT][3][4];
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int x = 0; x < 3; ++x)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) whole[j][x][r] = 0;
-#pragma unroll
     for (int c = 0; c < Cfg::kChunks; ++c) {
       const uint4 u = q8_shared16(at + (key_place ^ c << 4)), v = q8_shared16(at + (key_place ^ c << 4) + 8 * D);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const uint32_t q = parts + (j * Cfg::kChunks + c) * 1536;
         const uint4 q0 = q8_shared16(q), q1 = q8_shared16(q + 512), q2 = q8_shared16(q + 1024);
-        q8_mma_bytes<true>(whole[j][0], u.x, v.x, u.y, v.y, q0.x, q0.y);
-        q8_mma_bytes<false>(whole[j][1], u.x, v.x, u.y, v.y, q1.x, q1.y);
-        q8_mma_bytes<false>(whole[j][2], u.x, v.x, u.y, v.y, q2.x, q2.y);
-        q8_mma_bytes<true>(whole[j][0], u.z, v.z, u.w, v.w, q0.z, q0.w);
-        q8_mma_bytes<false>(whole[j][1], u.z, v.z, u.w, v.w, q1.z, q1.w);
-        q8_mma_bytes<false>(whole[j][2], u.z, v.z, u.w, v.w, q2.z, q2.w);
+        auto both = [&](auto first) {
+          constexpr bool kFirst = decltype(first)::value;
+          q8_mma_bytes<true, kFirst>(whole[j][0], u.x, v.x, u.y, v.y, q0.x, q0.y);
+          q8_mma_bytes<false, kFirst>(whole[j][1], u.x, v.x, u.y, v.y, q1.x, q1.y);
+          q8_mma_bytes<false, kFirst>(whole[j][2], u.x, v.x, u.y, v.y, q2.x, q2.y);
+        };
+        if (c == 0) both(std::true_type{});
+        else both(std::false_type{});
+        q8_mma_bytes<true, false>(whole[j][0], u.z, v.z, u.w, v.w, q0.z, q0.w);
+        q8_mma_bytes<false, false>(whole[j][1], u.z, v.z, u.w, v.w, q1.z, q1.w);
+        q8_mma_bytes<false, false>(whole[j][2], u.z, v.z, u.w, v.w, q2.z, q2.w);
       }
     }
-    float s[NT][4], by[NT][2];
+    float s[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -323,9 +330,9 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
 #pragma unroll
         for (int r = k; r < 4; r += 2)  // the lower two bytes' sums are below 2^23 each: together below 2^31
           s[j][r] = fmaf(__int2float_rn(whole[j][0][r]), 65536.0f, __int2float_rn(whole[j][1][r] * 256 + whole[j][2][r])) * x;
-        by[j][k] = scale.y;
       }
-    if (position + kTile - 1 > first_seen) {  // tokens that some rows do not see, or a page that is none
+    const bool cut = position + kTile - 1 > first_seen;  // tokens that some rows do not see, or a page that is none
+    if (cut) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -333,23 +340,31 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
           const int last = limit(j, k);
           if (position + gid > last) s[j][k] = -INFINITY;
           if (position + gid + 8 > last) s[j][k + 2] = -INFINITY;
-          if (position > last) by[j][k] = 0.0f;  // the scale may be NaN
         }
     }
     softmax(s);
-    uint32_t w[NT][2];
-    float off[NT][2];  // what the flipped bits are too much
+    // The sums count in units of a power of two above the largest scale so far.
+    const int exponent = (int)(__float_as_uint(scale.y) >> 23) - 126;
+    if (exponent > unit && exponent < 129) {
+      const float by = unit + 126 < exponent ? 0.0f : __uint_as_float((uint32_t)(127 + unit - exponent) << 23);
+      unit = exponent;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) w[j][k] = movmatrix_trans(pack2<__half>(s[j][2 * k], s[j][2 * k + 1]));
-      const uint32_t flipped[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
-      const float zero[2] = {0.0f, 0.0f};
-      float sum[4];
-      q8_mma_onto(sum, flipped, w[j][0], w[j][1], zero);
-      off[j][0] = sum[0];
-      off[j][1] = sum[1];
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[j][d][r] *= by;
     }
+    const float share = scale.y * __uint_as_float((uint32_t)(127 - unit) << 23);
+    const bool near = share <= 1.0f && (share >= 1.0f / 64.0f || share == 0.0f);  // the weights may take the scale
+    uint32_t w[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float f = near ? share : 1.0f;
+        w[j][k] = movmatrix_trans(pack2<__half>(s[j][2 * k] * f, s[j][2 * k + 1] * f));
+      }
     uint32_t val[4][Cfg::kVWords];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -365,21 +380,32 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
         }
       }
     }
+    auto sums = [&](auto&& add) {
 #pragma unroll
-    for (int v = 0; v < Cfg::kVWords; ++v) {
+      for (int v = 0; v < Cfg::kVWords; ++v) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t x = __byte_perm(val[0][v], val[1][v], half == 0 ? 0x5410 : 0x7632), z = __byte_perm(val[2][v], val[3][v], half == 0 ? 0x5410 : 0x7632);
-        const uint32_t a[4] = {(x & 0x00ff00ffu) ^ 0x00800080u, (x >> 8 & 0x00ff00ffu) ^ 0x00800080u, (z & 0x00ff00ffu) ^ 0x00800080u,
-                               (z >> 8 & 0x00ff00ffu) ^ 0x00800080u};
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t x = __byte_perm(val[0][v], val[1][v], half == 0 ? 0x5410 : 0x7632), z = __byte_perm(val[2][v], val[3][v], half == 0 ? 0x5410 : 0x7632);
+          const uint32_t a[4] = {q8_halves(x), q8_halves(x >> 8), q8_halves(z), q8_halves(z >> 8)};
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          float sum[4];
-          q8_mma_onto(sum, a, w[j][0], w[j][1], off[j]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[j][2 * v + half][r] = fmaf(sum[r], by[j][r & 1], o[j][2 * v + half][r]);
+          for (int j = 0; j < NT; ++j) add(j, o[j][2 * v + half], a);
         }
       }
+    };
+    if (near) {
+      sums([&](int j, float (&sum)[4], const uint32_t (&a)[4]) { mma_m16n8k16<__half>(sum, a, w[j][0], w[j][1]); });
+    } else {  // a scale far below the largest, or NaN
+      float by[NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) by[j][k] = cut && position > limit(j, k) ? 0.0f : share;  // rows that see nothing of the tile
+      sums([&](int j, float (&sum)[4], const uint32_t (&a)[4]) {
+        float part[4];
+        q8_mma_first(part, a, w[j][0], w[j][1]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] = fmaf(part[r], by[j][r & 1], sum[r]);
+      });
     }
     if ((i & 31) == 16 && i + 16 < mine) scales(next);
     at = at + Cfg::kTileBytes == tiles_end ? tiles : at + Cfg::kTileBytes;
@@ -388,13 +414,14 @@ __global__ void __launch_bounds__(Q8Cfg<D, NT>::kThreads, Q8Cfg<D, NT>::kCtas) q
       if (i + 33 < mine) next = find(i + 33);
     }
   }
-  // from 2^-24 of the codes' units to those of the ring
+  // to the units of the ring
+  const float units = __uint_as_float((uint32_t)(127 + unit) << 23);
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[j][d][r] *= 16777216.0f / kWeight * kRingWeight;
+      for (int r = 0; r < 4; ++r) o[j][d][r] = o[j][d][r] * (kRingWeight / kWeight) * units;
 
   // ---- tiles of the ring ----------------------------------------------------------------------------------------------------------------
   const int64_t ring_from = max(t0, st.packed);

@@ -36,9 +36,9 @@ constexpr uint32_t kQ8Forced = 0xffffffffu;
 
 // Full pages of which query t sees a token.
 __device__ __forceinline__ int q8_candidates(const Q8SelectParams& p, int64_t b, int t) {
-  const int64_t len = max((int64_t)0, min(p.lengths[b], p.max_blocks * p.block_size + p.block_size - 1));
-  const int64_t seen = len - p.tokens + t + 1;
-  return seen <= 0 ? 0 : (int)min(len / p.block_size, (seen + p.block_size - 1) / p.block_size);
+  const int len = (int)max((int64_t)0, min(p.lengths[b], p.max_blocks * p.block_size + p.block_size - 1));  // below 2^30
+  const int seen = len - p.tokens + t + 1;
+  return seen <= 0 ? 0 : min(len / p.block_size, (seen + p.block_size - 1) / p.block_size);
 }
 
 __device__ __forceinline__ void mma_s8u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -61,14 +61,15 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, D == 256 ? 1 : 2) q8_scor
   q8_let_next_start();
   q8_wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-  const int64_t b = blockIdx.y / p.kv_heads;
-  const int kvh = blockIdx.y % p.kv_heads;
+  const int b = blockIdx.y / p.kv_heads, kvh = blockIdx.y - b * p.kv_heads;
   const int token0 = blockIdx.z * p.tokens_at_once, here = min(p.tokens_at_once, p.tokens - token0);
   const int head_tiles = p.head_tiles, tiles = here * head_tiles;
   uint4* parts = reinterpret_cast<uint4*>(smem);                                              // [2][tiles][kChunks][32 lanes]
   float* tops = reinterpret_cast<float*>(smem + p.tokens_at_once * head_tiles * 2 * kChunks * 512);  // [tiles][8]
 
   // ---- this CTA's pages: `rounds` tiles of every warp -----------------------------------------------------------------------------------
+  __shared__ int candidates_of[8];
+  if (threadIdx.x < here) candidates_of[threadIdx.x] = q8_candidates(p, b, token0 + threadIdx.x);
   const int most = q8_candidates(p, b, token0 + here - 1);
   const int first_tile = blockIdx.x * p.rounds * kQ8SelectWarps + warp;
   if ((int)blockIdx.x * p.rounds * kQ8SelectWarps * kQ8SelectTile >= most) return;
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, D == 256 ? 1 : 2) q8_scor
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int j = tile * kQ8SelectTile + gid + 8 * i;
-      ids[i] = j < most ? p.block_table[b * p.table_stride + j] : -1;
+      ids[i] = j < most ? p.block_table[(int64_t)b * p.table_stride + j] : -1;
     }
   };
   auto load = [&](Tile& x) {
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, D == 256 ? 1 : 2) q8_scor
     for (int j = 0; j < D / 32; ++j) {
       x[j] = 0.0f;
       if (g < p.groups)
-        x[j] = ElemTraits<T>::to_float(reinterpret_cast<const T*>(p.q)[b * p.q_stride_b + (int64_t)(kvh * p.groups + g) * p.q_stride_h +
+        x[j] = ElemTraits<T>::to_float(reinterpret_cast<const T*>(p.q)[(int64_t)b * p.q_stride_b + (int64_t)(kvh * p.groups + g) * p.q_stride_h +
                                                                       (int64_t)(token0 + t) * p.q_stride_t + lane + 32 * j]);
       top = fmaxf(top, fabsf(x[j]));
       fine = fine && fabsf(x[j]) < INFINITY;
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, D == 256 ? 1 : 2) q8_scor
           best[r / 2] = isnan(x) ? INFINITY : fmaxf(best[r / 2], x);
         }
       }
-      const int candidates = q8_candidates(p, b, token0 + t);
+      const int candidates = candidates_of[t];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 1));
@@ -196,8 +197,8 @@ __global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p
   q8_wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t stream = blockIdx.x;
-  const int64_t b = stream / p.tokens / p.kv_heads;
-  const int n = q8_candidates(p, b, (int)(stream % p.tokens));
+  const int head = blockIdx.x / p.tokens, b = head / p.kv_heads;
+  const int n = q8_candidates(p, b, blockIdx.x - head * p.tokens);
   const uint32_t* scores = p.scores + stream * p.max_blocks;
   int32_t* out = p.blocks + stream * p.count;
   const int rounds = (n + THREADS - 1) / THREADS;
