@@ -24,14 +24,20 @@ struct Q8SelectParams {
   uint32_t* scores;  // [B, Hkv, T, max_blocks], larger is better, 0: no candidate
   int kv_heads, groups, tokens, block_size, page_bytes;
   int count, first, recent;
-  int head_tiles, tokens_at_once;  // tiles of 8 query heads of a token; tokens of a CTA
-  int rounds;                      // tiles of a warp
+  int row_group;       // rows of a token: its query heads, padded to 8 where they do not divide 8; see q8_score_kernel
+  int group_shift, head_tiles;  // log2 of rows of a token in one tile; tiles of a token that has more
+  int tokens_at_once;  // of a CTA
+  int batch, chunks;   // chunks of tokens_at_once
+  int rounds;          // tiles of a warp, where CTAs take parts
   int64_t num_pages, max_blocks;
 };
 
 constexpr int kQ8SelectWarps = 8;
 constexpr int kQ8SelectTile = 16;  // pages of a warp at a time
-constexpr int kQ8SelectRounds = 8;   // tiles of a warp at most
+constexpr int kQ8SelectCost = 16;    // tiles
+constexpr int kQ8SelectRows = 64;    // rows of a CTA, where a token has no more
+template <int D>
+constexpr int kQ8SelectCtas = D == 256 ? 1 : 3;
 constexpr uint32_t kQ8Forced = 0xffffffffu;
 
 // Full pages of which query t sees a token.
@@ -54,31 +60,33 @@ __device__ __forceinline__ uint32_t q8_ordered(float x) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kQ8SelectWarps * 32, D == 256 ? 1 : 2) q8_score_kernel(const Q8SelectParams p) {
+// Rows are the query heads of several tokens, one behind the other: the heads of a token are in one tile of 8 rows where their number divides 8, else
+// a token has tiles of its own.
+//
+// CTAs: a part of a stream (sequence, KV head and tokens) each where the GPU holds them all at once; else one resident wave that takes even shares of
+// the line of all streams' tiles, kQ8SelectCost tiles in front of each for its queries (32 rows of 20000 to 32768 tokens, 8 KV heads: 42 us in
+// parts, PLACEHOLDER so).
+template <typename T, int D, bool kShares>
+__global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_score_kernel(const Q8SelectParams p) {
   constexpr int kChunks = 2 * D / 64;  // of 64 bounds, 16 of them a lane's
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int candidates_of[kQ8SelectRows];
+  __shared__ int s_prefix[kShares ? kBalancedMaxRows + 1 : 1];
   q8_let_next_start();
   q8_wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-  const int b = blockIdx.y / p.kv_heads, kvh = blockIdx.y - b * p.kv_heads;
-  const int token0 = blockIdx.z * p.tokens_at_once, here = min(p.tokens_at_once, p.tokens - token0);
-  const int head_tiles = p.head_tiles, tiles = here * head_tiles;
-  uint4* parts = reinterpret_cast<uint4*>(smem);                                              // [2][tiles][kChunks][32 lanes]
-  float* tops = reinterpret_cast<float*>(smem + p.tokens_at_once * head_tiles * 2 * kChunks * 512);  // [tiles][8]
 
-  // ---- this CTA's pages: `rounds` tiles of every warp -----------------------------------------------------------------------------------
-  __shared__ int candidates_of[8];
-  if (threadIdx.x < here) candidates_of[threadIdx.x] = q8_candidates(p, b, token0 + threadIdx.x);
+  // The pages of tiles [begin, end) of 16, for tokens token0 .. of row b and KV head kvh.
+  auto segment = [&](int b, int kvh, int chunk, int begin, int end) {
+  const int token0 = chunk * p.tokens_at_once, here = min(p.tokens_at_once, p.tokens - token0);
+  const int tiles = (here * p.row_group + 7) / 8;
+  uint4* parts = reinterpret_cast<uint4*>(smem);                                           // [2][tiles][kChunks][32 lanes]
+  float* tops = reinterpret_cast<float*>(smem + tiles * 2 * kChunks * 512);                // [tiles][8]
   const int most = q8_candidates(p, b, token0 + here - 1);
-  const int first_tile = blockIdx.x * p.rounds * kQ8SelectWarps + warp;
-  if ((int)blockIdx.x * p.rounds * kQ8SelectWarps * kQ8SelectTile >= most) return;
-  struct Tile {
-    uint4 w[2][kChunks];
-    float scale[2];
-    bool there[2];
-  };
-  int32_t ids[2];  // pages of the tile after next
+  if ((int)threadIdx.x < here) candidates_of[threadIdx.x] = q8_candidates(p, b, token0 + threadIdx.x);
+  const int first_tile = begin + warp;
+  uint32_t* scores = p.scores + (((int64_t)b * p.kv_heads + kvh) * p.tokens + token0) * p.max_blocks;
+  int32_t ids[2];  // pages of the next tile
   auto find = [&](int tile) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -86,31 +94,33 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, D == 256 ? 1 : 2) q8_scor
       ids[i] = j < most ? p.block_table[(int64_t)b * p.table_stride + j] : -1;
     }
   };
-  auto load = [&](Tile& x) {
+  uint4 w[2][kChunks];
+  float scale[2];
+  bool there[2];
+  auto load = [&] {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      x.there[i] = ids[i] >= 0 && ids[i] < p.num_pages;
-      const uint8_t* page = p.pages + (x.there[i] ? ((int64_t)ids[i] * p.kv_heads + kvh) * p.page_bytes : 0);
-      x.scale[i] = __ldg(reinterpret_cast<const float*>(page + q8_scale_offset(D, p.block_size)));
+      there[i] = ids[i] >= 0 && ids[i] < p.num_pages;
+      const uint8_t* page = p.pages + (there[i] ? ((int64_t)ids[i] * p.kv_heads + kvh) * p.page_bytes : 0);
+      scale[i] = __ldg(reinterpret_cast<const float*>(page + q8_scale_offset(D, p.block_size)));
       const uint4* bounds = reinterpret_cast<const uint4*>(page + q8_bounds_offset(D, p.block_size));
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) x.w[i][c] = ldg_stream16(bounds + 4 * c + tig);
+      for (int c = 0; c < kChunks; ++c) w[i][c] = ldg_stream16(bounds + 4 * c + tig);
     }
   };
-  Tile now, next;
   find(first_tile);
-  load(now);
+  load();
   find(first_tile + kQ8SelectWarps);
 
   // ---- queries in whole numbers --------------------------------------------------------------------------------------------------
   for (int row = warp; row < tiles * 8; row += kQ8SelectWarps) {
-    const int t = row / (8 * head_tiles), g = row % (8 * head_tiles);
+    const int t = row / p.row_group, g = row - t * p.row_group;
     float x[D / 32], top = 0.0f;
     bool fine = true;
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       x[j] = 0.0f;
-      if (g < p.groups)
+      if (t < here && g < p.groups)
         x[j] = ElemTraits<T>::to_float(reinterpret_cast<const T*>(p.q)[(int64_t)b * p.q_stride_b + (int64_t)(kvh * p.groups + g) * p.q_stride_h +
                                                                       (int64_t)(token0 + t) * p.q_stride_t + lane + 32 * j]);
       top = fmaxf(top, fabsf(x[j]));
@@ -140,48 +150,103 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, D == 256 ? 1 : 2) q8_scor
   __syncthreads();
 
   // ---- 16 pages at a time -----------------------------------------------------------------------------------------------------------
-  for (int round = 0; round < p.rounds; ++round) {
-    const int tile = first_tile + round * kQ8SelectWarps;
-    if (tile * kQ8SelectTile >= most) break;
-    if (round + 1 < p.rounds) {
-      load(next);
-      find(tile + 2 * kQ8SelectWarps);
+  for (int tile = first_tile; tile < end && tile * kQ8SelectTile < most; tile += kQ8SelectWarps) {
+    if (tile > first_tile) {
+      load();
+      find(tile + kQ8SelectWarps);
     }
-    for (int t = 0; t < here; ++t) {
-      float best[2] = {-INFINITY, -INFINITY};
-      for (int h = 0; h < head_tiles; ++h) {
-        int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-        const uint4* at = parts + (t * head_tiles + h) * kChunks * 32 + lane;
+    float best[2] = {-INFINITY, -INFINITY};  // of one token
+    for (int n = 0, t0 = 0, h = 0; n < tiles; ++n) {
+      int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+      const uint4* at = parts + n * kChunks * 32 + lane;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const uint4 u = at[c * 32], v = at[(tiles * kChunks + c) * 32];
-          mma_s8u8(hi, now.w[0][c].x, now.w[1][c].x, now.w[0][c].y, now.w[1][c].y, u.x, u.y);
-          mma_s8u8(lo, now.w[0][c].x, now.w[1][c].x, now.w[0][c].y, now.w[1][c].y, v.x, v.y);
-          mma_s8u8(hi, now.w[0][c].z, now.w[1][c].z, now.w[0][c].w, now.w[1][c].w, u.z, u.w);
-          mma_s8u8(lo, now.w[0][c].z, now.w[1][c].z, now.w[0][c].w, now.w[1][c].w, v.z, v.w);
-        }
+      for (int c = 0; c < kChunks; ++c) {
+        const uint4 u = at[c * 32], v = at[(tiles * kChunks + c) * 32];
+        mma_s8u8(hi, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, u.x, u.y);
+        mma_s8u8(lo, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, v.x, v.y);
+        mma_s8u8(hi, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, u.z, u.w);
+        mma_s8u8(lo, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, v.z, v.w);
+      }
+      const float2 top = *reinterpret_cast<const float2*>(tops + 8 * n + 2 * tig);
+      float x[4];  // rows 2 tig and 2 tig + 1 of pages gid and gid + 8
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int g = h * 8 + 2 * tig + (r & 1);
-          if (g >= p.groups) continue;
-          const float top = tops[(t * head_tiles + h) * 8 + 2 * tig + (r & 1)];
-          const float x = __fmul_rn(__fmul_rn(top, now.scale[r / 2]), __int2float_rn(128 * hi[r] + lo[r]));
-          best[r / 2] = isnan(x) ? INFINITY : fmaxf(best[r / 2], x);
+      for (int r = 0; r < 4; ++r) {
+        x[r] = __fmul_rn(__fmul_rn(r & 1 ? top.y : top.x, scale[r / 2]), __int2float_rn(128 * hi[r] + lo[r]));
+        if (isnan(x[r])) x[r] = INFINITY;
+      }
+      auto put = [&](int t, int i, float score) {  // of token t and page gid + 8 i
+        const int j = tile * kQ8SelectTile + gid + 8 * i, candidates = candidates_of[t];
+        if (j >= candidates) return;
+        const bool forced = j < p.first || j >= candidates - p.recent;
+        scores[(int64_t)t * p.max_blocks + j] = !there[i] ? 0u : forced ? kQ8Forced : q8_ordered(score);
+      };
+      if (p.group_shift == 0) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (8 * n + 2 * tig + (r & 1) < here) put(8 * n + 2 * tig + (r & 1), r / 2, x[r]);
+        continue;
+      }
+      if (p.group_shift == 3) {  // rows past a token's heads
+        const int g = 8 * h + 2 * tig;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (g >= p.groups) x[2 * i] = -INFINITY;
+          if (g + 1 >= p.groups) x[2 * i + 1] = -INFINITY;
         }
       }
-      const int candidates = candidates_of[t];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 1));
-        best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 2));
-        const int j = tile * kQ8SelectTile + gid + 8 * i;
-        if (tig == 0 && j < candidates) {
-          const bool forced = j < p.first || j >= candidates - p.recent;
-          p.scores[((int64_t)blockIdx.y * p.tokens + token0 + t) * p.max_blocks + j] = !now.there[i] ? 0u : forced ? kQ8Forced : q8_ordered(best[i]);
-        }
+        float score = fmaxf(x[2 * i], x[2 * i + 1]);
+        if (p.group_shift >= 2) score = fmaxf(score, __shfl_xor_sync(0xffffffffu, score, 1));
+        if (p.group_shift == 3) score = fmaxf(score, __shfl_xor_sync(0xffffffffu, score, 2));
+        best[i] = fmaxf(best[i], score);
       }
+      if (++h < p.head_tiles) continue;  // more tiles of this token follow
+      const int t = t0 + (2 * tig >> p.group_shift);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (t < here && (2 * tig & ((1 << p.group_shift) - 1)) == 0) put(t, i, best[i]);
+        best[i] = -INFINITY;
+      }
+      t0 += 8 >> p.group_shift;
+      h = 0;
     }
-    now = next;
+  }
+  };
+
+  if constexpr (!kShares) {
+    const int b = blockIdx.y / p.kv_heads, begin = blockIdx.x * p.rounds * kQ8SelectWarps;
+    if (begin * kQ8SelectTile < q8_candidates(p, b, p.tokens - 1))
+      segment(b, blockIdx.y - b * p.kv_heads, blockIdx.z, begin, begin + p.rounds * kQ8SelectWarps);
+  } else {
+    constexpr int kThreads = kQ8SelectWarps * 32;
+    const int per_row = p.kv_heads * p.chunks, each = (p.batch + kThreads - 1) / kThreads;
+    int tiles_of_rows[kBalancedRowsPerThread<kThreads>], streams;
+#pragma unroll
+    for (int i = 0; i < kBalancedRowsPerThread<kThreads>; ++i) {
+      const int b = threadIdx.x * each + i;
+      tiles_of_rows[i] = i < each && b < p.batch ? (q8_candidates(p, b, p.tokens - 1) + kQ8SelectTile - 1) / kQ8SelectTile : 0;
+    }
+    balanced_scan<kThreads>(tiles_of_rows, p.batch, per_row, s_prefix, kQ8SelectCost, 0, &streams);
+    const int total = s_prefix[p.batch], share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 2 * kQ8SelectWarps);
+    int pos = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
+    const int stop = min(pos + share, total);
+    int b = 0, above = p.batch;  // s_prefix[b] <= pos < s_prefix[above]
+    while (above - b > 1) {
+      const int mid = (b + above) >> 1;
+      if (s_prefix[mid] <= pos) b = mid;
+      else above = mid;
+    }
+    while (pos < stop) {
+      while (s_prefix[b + 1] <= pos) ++b;
+      const int n = (s_prefix[b + 1] - s_prefix[b]) / per_row;  // of a stream, its cost among them
+      const int stream = (pos - s_prefix[b]) / n, at = pos - s_prefix[b] - stream * n, to = min(n, at + stop - pos);
+      if (to > kQ8SelectCost) {
+        segment(b, stream / p.chunks, stream % p.chunks, max(0, at - kQ8SelectCost), to - kQ8SelectCost);
+        __syncthreads();  // queries and candidates have been read
+      }
+      pos += to - at;
+    }
   }
 }
 
@@ -398,26 +463,35 @@ extern "C" int anna_q8_select_blocks(const void* q, int64_t q_stride_b, int64_t 
   p.pages = pages; p.block_table = page_table; p.table_stride = table_stride; p.lengths = lengths; p.blocks = blocks; p.scores = scores;
   p.kv_heads = kv_heads; p.groups = q_heads / kv_heads; p.tokens = tokens; p.block_size = block_size; p.page_bytes = (int)bytes;
   p.count = count; p.first = first; p.recent = recent; p.num_pages = num_pages; p.max_blocks = max_blocks;
-  p.head_tiles = (p.groups + 7) / 8;
-  p.tokens_at_once = p.head_tiles >= 8 ? 1 : 8 / p.head_tiles;
+  p.row_group = p.groups <= 8 && 8 % p.groups == 0 ? p.groups : (p.groups + 7) / 8 * 8;
+  p.group_shift = p.row_group == 1 ? 0 : p.row_group == 2 ? 1 : p.row_group == 4 ? 2 : 3;
+  p.head_tiles = (p.row_group + 7) / 8;
+  p.tokens_at_once = p.row_group >= kQ8SelectRows ? 1 : kQ8SelectRows / p.row_group;
   if (p.tokens_at_once > tokens) p.tokens_at_once = tokens;
-  const int row_tiles = p.tokens_at_once * p.head_tiles;
+  const int row_tiles = (p.tokens_at_once * p.row_group + 7) / 8;
   const int smem = row_tiles * (2 * (2 * head_dim / 64) * 512 + 32);
   if (smem > 200 * 1024) return set_error(ANNA_ERR_UNSUPPORTED, "%s: too many query heads (%d) to a KV head", what, p.groups);
   const int chunks = (tokens + p.tokens_at_once - 1) / p.tokens_at_once;
   ANNA_REQUIRE(chunks < 65536, "%s: too many tokens", what);
   if (max_blocks > 0) {
-    // one wave where the pages are that few; a CTA whose pages lie behind its row's end leaves at once
-    const int64_t tiles = (max_blocks + kQ8SelectTile - 1) / kQ8SelectTile, wave = 148 * (head_dim == 256 ? 1 : 2) * kQ8SelectWarps;
-    const int64_t rounds = ((int64_t)batch * kv_heads * chunks * tiles + wave - 1) / wave;
-    p.rounds = (int)(rounds > kQ8SelectRounds ? kQ8SelectRounds : rounds);
-    const int64_t splits = (tiles + p.rounds * kQ8SelectWarps - 1) / (p.rounds * kQ8SelectWarps);
+    const int64_t tiles = (max_blocks + kQ8SelectTile - 1) / kQ8SelectTile, ctas = 148 * (head_dim == 256 ? kQ8SelectCtas<256> : kQ8SelectCtas<128>);
+    const int64_t parts = (int64_t)batch * kv_heads * chunks, line = parts * (tiles + kQ8SelectCost);
+    const int64_t wave = ctas * kQ8SelectWarps;
+    p.batch = batch;
+    p.chunks = chunks;
+    p.rounds = (int)((parts * tiles + wave - 1) / wave);
+    int64_t splits = (tiles + p.rounds * kQ8SelectWarps - 1) / (p.rounds * kQ8SelectWarps);
+    const bool shares = parts * splits > ctas && batch <= kBalancedMaxRows && line < (1ll << 30);
+    if (!shares && p.rounds > 8) {
+      p.rounds = 8;
+      splits = (tiles + 8 * kQ8SelectWarps - 1) / (8 * kQ8SelectWarps);
+    }
+    const dim3 grid = shares ? dim3((unsigned)ctas) : dim3((unsigned)splits, (unsigned)(batch * kv_heads), (unsigned)chunks);
     const int rc = ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
       return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
-        auto kernel = q8_score_kernel<T, D>;
+        auto kernel = shares ? q8_score_kernel<T, D, true> : q8_score_kernel<T, D, false>;
         ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        return q8_launch("q8_score_kernel", kernel, dim3((unsigned)splits, (unsigned)(batch * kv_heads), (unsigned)chunks), kQ8SelectWarps * 32,
-                         smem, (cudaStream_t)stream, p);
+        return q8_launch("q8_score_kernel", kernel, grid, kQ8SelectWarps * 32, smem, (cudaStream_t)stream, p);
       });
     });
     if (rc != ANNA_OK) return rc;
