@@ -1,6 +1,6 @@
 // Attention of the newest T tokens of every sequence over the 8-bit paged cache: the CUDA-core form and the entry points.
 //
-// This form serves fp32 caches and pages that are no multiple of 16 tokens; everything in it is 32 bits.  A CTA brings 32 tokens at a
+// This form serves pages that are no multiple of 8 tokens; everything in it is 32 bits.  A CTA brings 32 tokens at a
 // time into shared memory, as floats without their scale, for its 8 rows; a warp scores two rows (256 dims: one) with a token a lane.
 // Bound: issue, of which the reads of shared memory are as many as the FMAs.
 #include "q8_common.cuh"
@@ -213,11 +213,11 @@ constexpr int kQ8MinTiles = 4;   // of a CTA with blocks, CUDA cores
 Q8Plan q8_plan(int batch, int q_heads, int kv_heads, int tokens, int head_dim, int block_size, int64_t max_blocks, int width, int dtype) {
   Q8Plan plan{};
   const int groups = q_heads / kv_heads, rows = width > 0 ? groups : tokens * groups;
-  plan.tensor_cores = dtype != ANNA_DTYPE_F32 && block_size % kBalancedTileTokens == 0;
+  plan.tensor_cores = block_size % 8 == 0;
   const Q8Shape shape = plan.tensor_cores ? q8_mma_shape(head_dim, rows)
                                           : Q8Shape{kQ8Rows, head_dim == 64 ? kQ8Ctas<64> : head_dim == 128 ? kQ8Ctas<128> : kQ8Ctas<256>, 4};
   plan.rows = shape.rows;
-  const int per_sm = shape.ctas, min_tiles = plan.tensor_cores ? shape.warps : kQ8MinTiles;
+  const int per_sm = shape.ctas, min_tiles = plan.tensor_cores ? 4 * shape.warps : kQ8MinTiles;
   const int tiles = (rows + plan.rows - 1) / plan.rows;
   plan.tiles_per_token = tiles;
   plan.row_tiles = width > 0 ? tokens * tiles : tiles;
@@ -300,7 +300,7 @@ extern "C" int anna_q8_attention(const void* q, int64_t q_stride_b, int64_t q_st
     if ((1 << s) == block_size) p.block_shift = s;
   p.num_pages = num_pages; p.max_blocks = max_blocks; p.max_len = max_blocks * block_size + block_size - 1;
   p.scaling = scaling;
-  p.stream_tiles = plan.tensor_cores ? 16 : 4;
+  p.stream_tiles = plan.tensor_cores ? 32 : 4;
   p.min_share = plan.tensor_cores ? 16 : 4;
   p.whole_tiles = 0;
   // The line of a launch without blocks has room for so many rows and positions: larger batches go in several, one behind the other.
@@ -314,8 +314,8 @@ extern "C" int anna_q8_attention(const void* q, int64_t q_stride_b, int64_t q_st
   for (int at = 0; at < batch; at += most) {
     p.batch = batch - at < most ? batch - at : most;
     const int ctas = width > 0 ? (int)plan.ctas : multi_ctas(p, plan.row_tiles, (int)(plan.ctas / 148));
-    const int rc = plan.tensor_cores ? launch_q8_mma(p, plan, head_dim, dtype, ctas, (cudaStream_t)stream)
-                                     : ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+    const int rc = ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+      if (plan.tensor_cores) return launch_q8_mma_of<T>(p, plan, head_dim, ctas, (cudaStream_t)stream);
       return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
         constexpr int smem = kQ8SmemFloats<D> * 4;
         auto kernel = width > 0 ? q8_attention_kernel<T, D, true> : q8_attention_kernel<T, D, false>;

@@ -119,11 +119,12 @@ struct Q8Plan {
   int counters;
 };
 
-// Tensor-core form (q8_attention_mma.cu): 16-bit caches, pages of a multiple of 16 tokens.
+// Tensor-core form (q8_attention_mma_body.cuh): pages of a multiple of 8 tokens.
 struct Q8Shape {
   int rows, ctas, warps;  // of a row tile; of an SM; of a CTA
 };
 Q8Shape q8_mma_shape(int head_dim, int rows);
-int launch_q8_mma(const Q8Params& p, const Q8Plan& plan, int head_dim, int dtype, int ctas, cudaStream_t stream);
+template <typename T>
+int launch_q8_mma_of(const Q8Params& p, const Q8Plan& plan, int head_dim, int ctas, cudaStream_t stream);
 
 }  // namespace anna
