@@ -156,6 +156,17 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kC
   const int packed_tiles = max(0, (int)(min(t1, st.packed) - t0 + kTile - 1)) / kTile;
   const int mine = packed_tiles > warp ? (packed_tiles - warp + Cfg::kWarps - 1) / Cfg::kWarps : 0;  // tiles of this warp: every kWarps-th
 
+  // queries, on their way while the pages are found
+  constexpr int E = D / 32, kMyRows = Cfg::kRows / Cfg::kWarps;
+  T query[kMyRows][E];
+#pragma unroll
+  for (int k = 0; k < kMyRows; ++k) {
+    const int row = st.row0 + min(warp + k * Cfg::kWarps, st.count - 1), t = multi_token_of(p, row), h = kvh * p.groups + row - t * p.groups;
+    const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_stride_b + h * p.q_stride_h + t * p.q_stride_t + lane * E;
+#pragma unroll
+    for (int j = 0; j < E; ++j) query[k][j] = q[j];
+  }
+
   // ---- pages of 32 of the warp's tiles, one tile a lane -------------------------------------------------------------------------------
   struct Pages {
     const uint8_t* keys[kPages];
@@ -225,21 +236,19 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kC
   if (mine > 32) next = find(32);
 
   // ---- queries -----------------------------------------------------------------------------------------------------------------------
-  for (int i = warp; i < Cfg::kRows; i += Cfg::kWarps) {
-    constexpr int E = D / 32;
+#pragma unroll
+  for (int k = 0; k < kMyRows; ++k) {
+    const int i = warp + k * Cfg::kWarps;
     float x[E], top = 0.0f;
     bool fine = true;
-    const int row = st.row0 + min(i, st.count - 1), t = multi_token_of(p, row), h = kvh * p.groups + row - t * p.groups;
-    const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_stride_b + h * p.q_stride_h + t * p.q_stride_t + lane * E;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      x[j] = ElemTraits<T>::to_float(q[j]);
+      x[j] = ElemTraits<T>::to_float(query[k][j]);
       fine = fine && fabsf(x[j]) < INFINITY;
       top = fmaxf(top, fabsf(x[j]));
     }
     fine = __all_sync(0xffffffffu, fine);
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
     // top * 2^up is in [1, 2)
     const int up = fine && top > 0.0f ? min(127 - (int)(__float_as_uint(top) >> 23), 126) : 0;
     const float factor = __uint_as_float((uint32_t)(max(up, -126) + 127) << 23) * (up < -126 ? 0.5f : 1.0f);
@@ -249,17 +258,26 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kC
       rate[i] = fine ? back / 4194304.0f : __int_as_float(0x7fc00000);
       ring_rate[i] = back / kRingFactor;
     }
+    // dims D / 4 t + 16 c .. are lane t's piece c; this lane's E dims lie in one piece, next to one another
+    const int d0 = lane * E, place = (((i / 8 * Cfg::kChunks + d0 % (D / 4) / 16) * 3) * 32 + i % 8 * 4 + d0 / (D / 4)) * 16 + d0 % 16;
+    uint32_t bytes[3][E >= 4 ? E / 4 : 1] = {};
+    T scaled[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const int d = lane * E + j;
       const int whole = fine ? __float2int_rn(x[j] * factor * 4194304.0f) : 0;
-      // dims D / 4 t + 16 c .. are lane t's piece c
-      const int place = (((i / 8 * Cfg::kChunks + d % (D / 4) / 16) * 3) * 32 + i % 8 * 4 + d / (D / 4)) * 16 + d % 16;
-      smem[Cfg::kOffParts + place] = (uint8_t)(whole >> 16);
-      smem[Cfg::kOffParts + place + 512] = (uint8_t)(whole >> 8);
-      smem[Cfg::kOffParts + place + 1024] = (uint8_t)whole;
-      reinterpret_cast<T*>(smem + Cfg::kOffRing)[i * D + d] = ElemTraits<T>::from_float(x[j] * factor * kRingFactor);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) bytes[n][j / 4] |= ((uint32_t)whole >> (16 - 8 * n) & 255u) << (8 * (j % 4));
+      scaled[j] = ElemTraits<T>::from_float(x[j] * factor * kRingFactor);
     }
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      uint8_t* to = smem + Cfg::kOffParts + place + 512 * n;
+      if constexpr (E == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)bytes[n][0];
+      else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(to) = bytes[n][0];
+      else *reinterpret_cast<uint2*>(to) = make_uint2(bytes[n][0], bytes[n][E / 4 - 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) reinterpret_cast<T*>(smem + Cfg::kOffRing)[i * D + d0 + j] = scaled[j];
   }
   __syncthreads();
   float to_log2[NT][2], m_run[NT][2], l_run[NT][2], o[NT][D / 16][4];

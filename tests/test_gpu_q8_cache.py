@@ -214,6 +214,17 @@ def test_dense_view_of_missing_pages_is_zero(cuda_device):
     (128, 16, 2, 4, 1), (128, 16, 1, 8, 4), (64, 16, 2, 3, 1), (64, 32, 2, 1, 7), (256, 32, 1, 8, 1), (256, 16, 2, 5, 6),
     (128, 64, 1, 12, 3), (128, 24, 2, 4, 2), (64, 8, 1, 6, 5), (256, 1, 1, 2, 1), (128, 16, 1, 16, 9), (128, 112, 2, 2, 2)])
 def test_attention(cuda_device, dtype, dim, page, heads, group, tokens):
+    run_attention(cuda_device, dtype, dim, page, heads, group, tokens)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim,page,heads,group,tokens", [(256, 32, 2, 8, 8), (128, 16, 1, 4, 17), (64, 24, 1, 8, 9), (256, 8, 1, 3, 23), (128, 64, 1, 16, 5),
+                                                         (128, 1024, 1, 8, 12), (64, 48, 2, 40, 1)])
+def test_attention_of_many_queries(cuda_device, dtype, dim, page, heads, group, tokens):
+    run_attention(cuda_device, dtype, dim, page, heads, group, tokens)
+
+
+def run_attention(cuda_device, dtype, dim, page, heads, group, tokens):
     lengths = [0, 1, page - 1, page, page + 1, 5 * page + page // 2, 333, 16, 15, 17]
     cache, gpu = filled(cuda_device, lengths, heads, dim, page, dtype, seed=dim + page)
     query = torch.randn((len(lengths), heads * group, tokens, dim), generator=cache.gen).to(dtype)
@@ -257,9 +268,10 @@ def test_many_rows(cuda_device):
     check_attention(cache, gpu, query, cuda_device, blocks=torch.randint(0, 3, (rows, 1, 1, 2), generator=gen).int())
 
 
-@pytest.mark.parametrize("dtype,page", [(BF16, 16), (FP16, 16), (FP32, 16), (BF16, 24)])
-def test_keys_that_a_query_does_not_see_do_not_matter(cuda_device, dtype, page):
-    """Infinities and NaN in newer tokens, in rings behind the last token, in pages that are not there or not named."""
+@pytest.mark.parametrize("dtype,page,copies", [(BF16, 16, 1), (FP16, 16, 1), (FP32, 16, 1), (BF16, 24, 1), (FP16, 5, 1), (BF16, 16, 5), (FP16, 24, 5)])
+def test_keys_that_a_query_does_not_see_do_not_matter(cuda_device, dtype, page, copies):
+    """Infinities and NaN in newer tokens, in rings behind the last token, in pages that are not there or not named.  `copies`: of every head,
+    for kernels of many rows."""
     tokens = 3
     lengths = [page * 3 + 1, page * 2, page + 2]
     cache, _ = filled(cuda_device, lengths, 2, 128, page, dtype)
@@ -273,7 +285,11 @@ def test_keys_that_a_query_does_not_see_do_not_matter(cuda_device, dtype, page):
     gpu = cache.on(cuda_device)
     query = torch.randn((3, 8, tokens, 128), generator=cache.gen).to(dtype)
     scaling = 128 ** -0.5
-    out = anna_b200.run_q8_paged_attention(query=query.to(cuda_device), lengths=cache.lengths.to(cuda_device), scaling=scaling, **gpu).cpu()
+    wide = query.repeat_interleave(copies, dim=1)
+    out = anna_b200.run_q8_paged_attention(query=wide.to(cuda_device), lengths=cache.lengths.to(cuda_device), scaling=scaling, **gpu).cpu()
+    for i in range(1, copies):
+        assert torch.equal(out[:, i::copies].isfinite(), out[:, ::copies].isfinite())
+    out = out[:, ::copies]
     rows = [cache.dense(b) for b in range(3)]
     checked = []
     for b, n in enumerate(lengths):
@@ -309,8 +325,8 @@ def test_missing_pages_and_rings_are_left_out(cuda_device, dtype, page):
             assert bool(((out[b, :, t] - want[0, :, 0]).abs() <= attention_bound(want, dtype, 64, reach, most)[0, :, 0]).all())
 
 
-@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
-def test_small_weights_and_pages_of_very_different_scales_count(cuda_device, dtype):
+@pytest.mark.parametrize("dtype,copies", [(BF16, 1), (FP16, 1), (FP32, 1), (BF16, 10), (FP16, 10)])
+def test_small_weights_and_pages_of_very_different_scales_count(cuda_device, dtype, copies):
     """One key that takes nearly all weight has no value; what the others add is still exact.  Pages whose scales differ by 2^12."""
     cache = Cache(2, 1, 128, 16, dtype, 40)
     key, value = cache.new_tokens(600)
@@ -322,7 +338,9 @@ def test_small_weights_and_pages_of_very_different_scales_count(cuda_device, dty
     cache.append(key, value)
     gpu = cache.on(cuda_device)
     rows = [cache.dense(b) for b in range(2)]
-    out = anna_b200.run_q8_paged_attention(query=query.to(cuda_device), lengths=cache.lengths.to(cuda_device), scaling=0.09, **gpu).cpu().double()
+    wide = query.repeat_interleave(copies, dim=1)  # many rows
+    out = anna_b200.run_q8_paged_attention(query=wide.to(cuda_device), lengths=cache.lengths.to(cuda_device), scaling=0.09, **gpu).cpu().double()
+    out = out[:, ::copies]
     for b in range(2):
         score = torch.einsum("hd,nd->hn", query[b, :, 0].double(), rows[b][0, 0]) * 0.09
         weight = torch.softmax(score, dim=-1)
