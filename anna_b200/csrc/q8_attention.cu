@@ -24,15 +24,15 @@ __global__ void __launch_bounds__(kQ8Threads<D>) q8_attention_kernel(const Q8Par
   float* vals = keys + kQ8Tokens * (D + 1);      // [tokens][D]
   float* weight = vals + kQ8Tokens * D;          // [rows][tokens]
   __shared__ float sm_scale[kQ8Tokens], sm_rescale[kQ8Rows];
-  __shared__ int64_t sm_position[kQ8Tokens];     // in the sequence; past its end for what is not there
+  __shared__ int sm_position[kQ8Tokens];         // in the sequence; past its end for what is not there
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   q8_let_next_start();
   q8_wait_for_previous();
-  q8_for_each_segment<T, D, kThreads, kBlocks>(p, row_tiles, [&](int64_t b, int kvh, int tile, int64_t t0, int64_t t1, const MultiPartial& part) {
-  const Q8Stream st = q8_stream<kQ8Rows>(p, b, kvh, tile);
+  q8_for_each_segment<T, D, kThreads, kBlocks>(p, row_tiles, [&](int64_t b, int kvh, int tile, int t0, int t1, int len, const MultiPartial& part) {
+  const Q8Stream st = q8_stream<kQ8Rows>(p, b, kvh, tile, len);
   const int row0 = st.row0, count = st.count;
-  const int64_t first_seen = st.len - p.tokens;  // newest key that query 0 sees
+  const int first_seen = st.len - p.tokens;  // newest key that query 0 sees
 
   for (int i = warp; i < count; i += kWarps) {
     const int t = multi_token_of(p, row0 + i), h = kvh * p.groups + row0 + i - t * p.groups;
@@ -56,29 +56,29 @@ __global__ void __launch_bounds__(kQ8Threads<D>) q8_attention_kernel(const Q8Par
   const int64_t slot = st.len > st.full ? p.window_slots[b] : -1;
   const T* ring = slot >= 0 && slot < p.num_slots ? reinterpret_cast<const T*>(p.window) + (slot * 2 * p.kv_heads + kvh) * p.block_size * D : nullptr;
   const int64_t ring_values = (int64_t)p.kv_heads * p.block_size * D;
-  for (int64_t base = t0; base < t1;) {
+  for (int base = t0; base < t1;) {
     const bool packed = base < st.packed;
-    const int64_t stop = min(packed ? min(st.packed, t1) : t1, base + kQ8Tokens);
-    const int n = (int)(stop - base);
+    const int stop = min(packed ? min(st.packed, t1) : t1, base + kQ8Tokens), n = stop - base;
     __syncthreads();
     // ---- 32 tokens into shared memory: a lane finds its token, then a warp takes a token at a time --------------------------------
-    int64_t page = -1, position = INT64_MAX;
+    int64_t page = -1;
+    int position = INT32_MAX;
     int in_page = 0;
     float value_scale = 0.0f;
     if (lane < n) {
       if (packed) {
-        const int entry = (int)((base + lane) / p.block_size);
-        in_page = (int)(base + lane - (int64_t)entry * p.block_size);
+        const int entry = (base + lane) / p.block_size;
+        in_page = base + lane - entry * p.block_size;
         int block;
         page = q8_page_at(p, st, b, kvh, entry, &block);
         if (page >= 0) {
-          position = (int64_t)block * p.block_size + in_page;
+          position = block * p.block_size + in_page;
           const float2 scale = *reinterpret_cast<const float2*>(p.pages + page + q8_scale_offset(D, p.block_size));
           value_scale = scale.y;
           if (warp == 0) sm_scale[lane] = scale.x;
         }
       } else {
-        in_page = (int)(base + lane - st.packed);
+        in_page = base + lane - st.packed;
         page = ring != nullptr ? 0 : -1;
         if (page >= 0) position = st.full + in_page;
         value_scale = 1.0f;

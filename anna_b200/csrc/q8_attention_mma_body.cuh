@@ -150,10 +150,10 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kC
   q8_let_next_start();
   q8_wait_for_previous();
 
-  q8_for_each_segment<T, D, Cfg::kThreads, kBlocks>(p, row_tiles, [&](int64_t b, int kvh, int tile, int64_t t0, int64_t t1, const MultiPartial& part) {
-  const Q8Stream st = q8_stream<Cfg::kRows>(p, b, kvh, tile);
-  const int first_seen = (int)(st.len - p.tokens);  // newest key that query 0 sees
-  const int packed_tiles = max(0, (int)(min(t1, st.packed) - t0 + kTile - 1)) / kTile;
+  q8_for_each_segment<T, D, Cfg::kThreads, kBlocks>(p, row_tiles, [&](int64_t b, int kvh, int tile, int t0, int t1, int len, const MultiPartial& part) {
+  const Q8Stream st = q8_stream<Cfg::kRows>(p, b, kvh, tile, len);
+  const int first_seen = st.len - p.tokens;  // newest key that query 0 sees
+  const int packed_tiles = max(0, min(t1, st.packed) - t0 + kTile - 1) / kTile;
   const int mine = packed_tiles > warp ? (packed_tiles - warp + Cfg::kWarps - 1) / Cfg::kWarps : 0;  // tiles of this warp: every kWarps-th
 
   // queries, on their way while the pages are found
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kC
       x.keys[h] = p.pages;
       x.position[h] = kFar;
       x.scale[h] = make_float2(0.0f, 0.0f);
-      const int at = (int)t0 + (warp + i * Cfg::kWarps) * kTile + kPageTokens * h;
+      const int at = t0 + (warp + i * Cfg::kWarps) * kTile + kPageTokens * h;
       if (i < mine && (!kHalves || at < st.packed)) {
         const int entry = p.block_shift >= 0 ? at >> p.block_shift : at / p.block_size, slot = at - entry * p.block_size;
         int block;
@@ -239,6 +239,10 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kC
 #pragma unroll
   for (int k = 0; k < kMyRows; ++k) {
     const int i = warp + k * Cfg::kWarps;
+    if (i >= st.count) {  // a row that is not there: whatever its columns hold is not looked at
+      if (lane == 0) rate[i] = ring_rate[i] = 0.0f;
+      continue;
+    }
     float x[E], top = 0.0f;
     bool fine = true;
 #pragma unroll
@@ -497,12 +501,12 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kC
       for (int r = 0; r < 4; ++r) o[j][d][r] = o[j][d][r] * (kRingWeight / kWeight) * units;
 
   // ---- tiles of the ring ----------------------------------------------------------------------------------------------------------------
-  const int64_t ring_from = max(t0, st.packed);
+  const int ring_from = max(t0, st.packed);
   const int64_t slot = ring_from < t1 ? p.window_slots[b] : -1;
   if (slot >= 0 && slot < p.num_slots) {
     const T* keys = reinterpret_cast<const T*>(p.window) + (slot * 2 * p.kv_heads + kvh) * p.block_size * D;
     const T* values = keys + (int64_t)p.kv_heads * p.block_size * D;
-    const int begin = (int)(ring_from - st.packed), end = (int)(t1 - st.packed), full = (int)st.full;  // ring slots; position of slot 0
+    const int begin = ring_from - st.packed, end = t1 - st.packed, full = st.full;  // ring slots; position of slot 0
     for (int from = begin + (warp + Cfg::kWarps - packed_tiles % Cfg::kWarps) % Cfg::kWarps * kTile; from < end; from += Cfg::kWarps * kTile) {
       const int valid = min(kTile, end - from), position = full + from;
       auto row_of = [&](int token) { return (int64_t)(from + min(token, valid - 1)) * D; };

@@ -32,18 +32,18 @@ struct Q8Params : TqMultiParams {
 
 // What a stream reads: rows row0 .. row0 + count - 1 (row = token * groups + head of the group).
 struct Q8Stream {
-  int64_t len, full;    // tokens of the sequence, of those in full pages
-  int64_t packed;       // tokens of the axis that lie in pages
+  int len, full;        // tokens of the sequence, of those in full pages
+  int packed;           // tokens of the axis that lie in pages
   int row0, count;
   const int32_t* list;  // the blocks on the axis, or null: all in order
 };
 
 template <int ROWS>
-__device__ __forceinline__ Q8Stream q8_stream(const Q8Params& p, int64_t b, int kvh, int tile) {
+__device__ __forceinline__ Q8Stream q8_stream(const Q8Params& p, int64_t b, int kvh, int tile, int len) {
   Q8Stream s;
-  s.len = max((int64_t)0, min(p.lengths[b], p.max_len));
-  const int blocks = p.block_shift >= 0 ? (int)(s.len >> p.block_shift) : (int)s.len / p.block_size;
-  s.full = (int64_t)blocks * p.block_size;
+  s.len = len;
+  const int blocks = p.block_shift >= 0 ? len >> p.block_shift : len / p.block_size;
+  s.full = blocks * p.block_size;
   s.list = nullptr;
   if (p.blocks == nullptr) {
     s.packed = s.full;
@@ -51,7 +51,7 @@ __device__ __forceinline__ Q8Stream q8_stream(const Q8Params& p, int64_t b, int 
     s.count = min(ROWS, p.rows - s.row0);
   } else {
     const int token = tile / p.tiles_per_token, part = tile - token * p.tiles_per_token;
-    s.packed = (int64_t)p.width * p.block_size;
+    s.packed = p.width * p.block_size;
     s.row0 = token * p.groups + part * ROWS;
     s.count = min(ROWS, p.groups - part * ROWS);
     s.list = p.blocks + ((b * p.kv_heads + kvh) * p.tokens + token) * p.width;
@@ -63,26 +63,83 @@ __device__ __forceinline__ Q8Stream q8_stream(const Q8Params& p, int64_t b, int 
 __device__ __forceinline__ int64_t q8_page_at(const Q8Params& p, const Q8Stream& s, int64_t b, int kvh, int entry, int* block) {
   const int j = s.list != nullptr ? s.list[entry] : entry;
   *block = j;
-  if (j < 0 || (int64_t)j * p.block_size >= s.full || j >= p.max_blocks) return -1;
+  if (j < 0 || (int64_t)j * p.block_size >= s.full) return -1;  // a sequence has no more full pages than the table has columns
   const int32_t pid = p.block_table[b * p.table_stride + j];
   return pid >= 0 && pid < p.num_pages ? ((int64_t)pid * p.kv_heads + kvh) * p.page_bytes : -1;
 }
 
-// Calls segment(b, kvh, tile, t0, t1, partial) for this CTA's part of the axes; see multi_for_each_segment.  With blocks all axes are as
-// long, and the host has cut them: `splits` CTAs to a stream, 16-token tiles dealt evenly.
+// Calls segment(b, kvh, tile, t0, t1, length, partial) for this CTA's part of the axes.
+//
+// With blocks all axes are as long, and the host has cut them: `splits` CTAs to a stream, 16-token tiles dealt evenly.  Else CTAs take even shares of a
+// line of all streams, as multi_for_each_segment cuts it; at most 32 rows are lined up by every warp by itself, without barriers and with one read of
+// the lengths (one row of 4000 tokens: 12.3 us, 11.7 so).
 template <typename T, int D, int THREADS, bool kBlocks, typename Fn>
 __device__ __forceinline__ void q8_for_each_segment(const Q8Params& p, int row_tiles, Fn&& segment) {
   if constexpr (kBlocks) {
     const int stream = blockIdx.x / p.splits, split = blockIdx.x - stream * p.splits;
-    const int tile = stream % row_tiles, head = stream / row_tiles % p.kv_heads;
-    const int64_t b = stream / row_tiles / p.kv_heads;
-    const int64_t len = max((int64_t)0, min(p.lengths[b], p.max_len));
-    const int64_t end = (int64_t)p.width * p.block_size + len % p.block_size;
-    const int64_t tiles = (end + kBalancedTileTokens - 1) / kBalancedTileTokens;
-    const int64_t t0 = tiles * split / p.splits * kBalancedTileTokens, t1 = min(end, tiles * (split + 1) / p.splits * kBalancedTileTokens);
-    segment(b, head, tile, t0, t1, MultiPartial{stream * p.splits, p.splits, split});
+    const int rest = stream / row_tiles, tile = stream - rest * row_tiles, b = rest / p.kv_heads, head = rest - b * p.kv_heads;
+    const int len = (int)max((int64_t)0, min(p.lengths[b], p.max_len));
+    const int ring = p.block_shift >= 0 ? len & (p.block_size - 1) : len % p.block_size, end = p.width * p.block_size + ring;
+    const int tiles = (end + kBalancedTileTokens - 1) / kBalancedTileTokens, each = tiles / p.splits, more = tiles - each * p.splits;
+    const int t0 = (each * split + min(split, more)) * kBalancedTileTokens, t1 = min(end, t0 + (each + (split < more ? 1 : 0)) * kBalancedTileTokens);
+    segment(b, head, tile, t0, t1, len, MultiPartial{stream * p.splits, p.splits, split});
   } else {
-    multi_for_each_segment<T, D, THREADS>(p, row_tiles, segment);
+    __shared__ int s_prefix[kBalancedMaxRows + 1];
+    const bool few = p.batch <= 32;
+    const int per_row = p.kv_heads * row_tiles;
+    WarpLine line{};
+    int total, most;
+    if (few) {
+      line.load(p.lengths, p.max_len, p.batch, 0);
+      total = line.scan(per_row, p.stream_tiles, 0);
+      most = __reduce_max_sync(0xffffffffu, line.tiles);
+    } else {
+      int tiles[kBalancedRowsPerThread<THREADS>], streams;
+      balanced_load_tiles<THREADS>(p.lengths, p.max_len, p.batch, 0, tiles);
+      most = balanced_scan<THREADS>(tiles, p.batch, per_row, s_prefix, p.stream_tiles, 0, &streams);
+      total = s_prefix[p.batch];
+    }
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {  // rows without a key
+      if (few ? __shfl_sync(0xffffffffu, line.tiles, b & 31) != 0 : s_prefix[b + 1] != s_prefix[b]) continue;
+      for (int item = threadIdx.x; item < p.kv_heads * p.rows * (D / 4); item += THREADS) {
+        const float zeros[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int row = item / (D / 4);
+        multi_store<T, 4>(p, b, row / p.rows, row % p.rows, item % (D / 4) * 4, zeros);
+      }
+    }
+    const int share = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_share), (most + kMultiMaxPartials - 3) / (kMultiMaxPartials - 2));
+    int pos = (int)min((int64_t)blockIdx.x * share, (int64_t)total), b = 0;
+    const int end = min(pos + share, total);
+    if (!few && pos < end) {
+      int above = p.batch;  // s_prefix[b] <= pos < s_prefix[above]
+      while (above - b > 1) {
+        const int mid = (b + above) >> 1;
+        if (s_prefix[mid] <= pos) b = mid;
+        else above = mid;
+      }
+    }
+    while (pos < end) {
+      int len, first_of_row;
+      if (few) {
+        b = __popc(__ballot_sync(0xffffffffu, line.next <= pos));  // rows that end at or before it (never all: pos < total)
+        len = __shfl_sync(0xffffffffu, line.len, b);
+        first_of_row = __shfl_sync(0xffffffffu, line.first, b);
+      } else {
+        while (s_prefix[b + 1] <= pos) ++b;
+        len = (int)max((int64_t)0, min(p.lengths[b], p.max_len));
+        first_of_row = s_prefix[b];
+      }
+      const int n = (len + kBalancedTileTokens - 1) / kBalancedTileTokens + p.stream_tiles;
+      const int stream = (pos - first_of_row) / n, at = pos - first_of_row - stream * n, stop = min(n, at + end - pos);
+      if (stop > p.stream_tiles) {
+        const int begin = first_of_row + stream * n, first = (begin + p.stream_tiles) / share;
+        const int head = stream / row_tiles;
+        segment(b, head, stream - head * row_tiles, max(0, at - p.stream_tiles) * kBalancedTileTokens,
+                min(len, (stop - p.stream_tiles) * kBalancedTileTokens), len,
+                MultiPartial{first, (begin + n - 1) / share - first + 1, (int)blockIdx.x - first});
+      }
+      pos += stop - at;
+    }
   }
 }
 
