@@ -27,14 +27,15 @@ struct Q8SelectParams {
   int row_group;       // rows of a token: its query heads, padded to 8 where they do not divide 8; see q8_score_kernel
   int group_shift, head_tiles;  // log2 of rows of a token in one tile; tiles of a token that has more
   int tokens_at_once;  // of a CTA
-  int batch, chunks;   // chunks of tokens_at_once
-  int rounds;          // tiles of a warp, where CTAs take parts
+  int heads_at_once;   // KV heads of a CTA
+  int batch, chunks, head_groups;  // chunks of tokens_at_once, groups of heads_at_once
+  int part_tiles;      // of a CTA, where CTAs take parts
   int64_t num_pages, max_blocks;
 };
 
 constexpr int kQ8SelectWarps = 8;
 constexpr int kQ8SelectTile = 16;  // pages of a warp at a time
-constexpr int kQ8SelectCost = 16;    // tiles
+constexpr int kQ8SelectCost = 4;     // tiles, of all KV heads of a CTA
 constexpr int kQ8SelectRows = 64;    // rows of a CTA, where a token has no more
 template <int D>
 constexpr int kQ8SelectCtas = D == 256 ? 1 : 3;
@@ -61,11 +62,11 @@ __device__ __forceinline__ uint32_t q8_ordered(float x) {
 }
 
 // Rows are the query heads of several tokens, one behind the other: the heads of a token are in one tile of 8 rows where their number divides 8, else
-// a token has tiles of its own.
+// a token has tiles of its own.  The KV heads of a page lie next to one another, and a CTA's warps take them together: a page costs one translation of its
+// address and one stretch of memory (32 rows of 20000 to 32768 tokens in scattered pages, 8 KV heads: PLACEHOLDER us with CTAs of one KV head).
 //
-// CTAs: a part of a stream (sequence, KV head and tokens) each where the GPU holds them all at once; else one resident wave that takes even shares of
-// the line of all streams' tiles, kQ8SelectCost tiles in front of each for its queries (32 rows of 20000 to 32768 tokens, 8 KV heads: 42 us in
-// parts, PLACEHOLDER so).
+// CTAs: a part of a stream (sequence, tokens, KV heads) each where the GPU holds them all at once; else one resident wave that takes even shares of the
+// line of all streams' tiles, kQ8SelectCost tiles in front of each for its queries.
 template <typename T, int D, bool kShares>
 __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_score_kernel(const Q8SelectParams p) {
   constexpr int kChunks = 2 * D / 64;  // of 64 bounds, 16 of them a lane's
@@ -76,98 +77,115 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
   q8_wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
 
-  // The pages of tiles [begin, end) of 16, for tokens token0 .. of row b and KV head kvh.
-  auto segment = [&](int b, int kvh, int chunk, int begin, int end) {
-  const int token0 = chunk * p.tokens_at_once, here = min(p.tokens_at_once, p.tokens - token0);
-  const int tiles = (here * p.row_group + 7) / 8;
-  uint4* parts = reinterpret_cast<uint4*>(smem);                                           // [2][tiles][kChunks][32 lanes]
-  float* tops = reinterpret_cast<float*>(smem + tiles * 2 * kChunks * 512);                // [tiles][8]
+  // The pages of tiles [begin, end) of 16, for a chunk of tokens and a group of KV heads of row b.
+  auto segment = [&](int b, int stream, int begin, int end) {
+  const int heads0 = stream / p.chunks * p.heads_at_once, heads = min(p.heads_at_once, p.kv_heads - heads0);
+  const int token0 = stream % p.chunks * p.tokens_at_once, here = min(p.tokens_at_once, p.tokens - token0);
+  const int tiles = (here * p.row_group + 7) / 8;                                           // of a KV head
+  uint4* parts = reinterpret_cast<uint4*>(smem);                                            // [2][heads][tiles][kChunks][32 lanes]
+  float* tops = reinterpret_cast<float*>(smem + heads * tiles * 2 * kChunks * 512);         // [heads][tiles][8]
+  const int plane = heads * tiles * kChunks * 32;
   const int most = q8_candidates(p, b, token0 + here - 1);
   if ((int)threadIdx.x < here) candidates_of[threadIdx.x] = q8_candidates(p, b, token0 + threadIdx.x);
-  const int first_tile = begin + warp;
-  uint32_t* scores = p.scores + (((int64_t)b * p.kv_heads + kvh) * p.tokens + token0) * p.max_blocks;
-  int32_t ids[2];  // pages of the next tile
-  auto find = [&](int tile) {
+  // this warp's items: tiles with their KV heads, these first
+  int tile = begin + warp / heads, head = warp % heads;
+  const int tile_step = kQ8SelectWarps / heads, head_step = kQ8SelectWarps - tile_step * heads;
+  int32_t ids[2];  // pages of the next item
+  auto find = [&](int of) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int j = tile * kQ8SelectTile + gid + 8 * i;
-      ids[i] = j < most ? p.block_table[(int64_t)b * p.table_stride + j] : -1;
+      const int j = of * kQ8SelectTile + gid + 8 * i;
+      ids[i] = of < end && j < most ? p.block_table[(int64_t)b * p.table_stride + j] : -1;
     }
   };
   uint4 w[2][kChunks];
   float scale[2];
   bool there[2];
-  auto load = [&] {
+  auto load = [&](int h) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       there[i] = ids[i] >= 0 && ids[i] < p.num_pages;
-      const uint8_t* page = p.pages + (there[i] ? ((int64_t)ids[i] * p.kv_heads + kvh) * p.page_bytes : 0);
+      const uint8_t* page = p.pages + (there[i] ? ((int64_t)ids[i] * p.kv_heads + heads0 + h) * p.page_bytes : 0);
       scale[i] = __ldg(reinterpret_cast<const float*>(page + q8_scale_offset(D, p.block_size)));
       const uint4* bounds = reinterpret_cast<const uint4*>(page + q8_bounds_offset(D, p.block_size));
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) w[i][c] = ldg_stream16(bounds + 4 * c + tig);
     }
   };
-  find(first_tile);
-  load();
-  find(first_tile + kQ8SelectWarps);
+  auto next_tile = [&] { return tile + tile_step + (head + head_step >= heads ? 1 : 0); };
+  find(tile);
+  load(head);
+  find(next_tile());
 
-  // ---- queries in whole numbers --------------------------------------------------------------------------------------------------
-  for (int row = warp; row < tiles * 8; row += kQ8SelectWarps) {
-    const int t = row / p.row_group, g = row - t * p.row_group;
-    float x[D / 32], top = 0.0f;
-    bool fine = true;
+  // ---- queries in whole numbers; rows that are not there stay as they are --------------------------------------------------------------
+  const int of_head = here * p.groups, rows = heads * of_head;
+  constexpr int kAhead = 4;  // rows on their way
+  for (int from = warp * kAhead; from < rows; from += kQ8SelectWarps * kAhead) {
+    T raw[kAhead][D / 32];
+    int place_of[kAhead];
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      x[j] = 0.0f;
-      if (t < here && g < p.groups)
-        x[j] = ElemTraits<T>::to_float(reinterpret_cast<const T*>(p.q)[(int64_t)b * p.q_stride_b + (int64_t)(kvh * p.groups + g) * p.q_stride_h +
-                                                                      (int64_t)(token0 + t) * p.q_stride_t + lane + 32 * j]);
-      top = fmaxf(top, fabsf(x[j]));
-      fine = fine && fabsf(x[j]) < INFINITY;
+    for (int k = 0; k < kAhead; ++k) {
+      const int row = min(from + k, rows - 1), h = row / of_head, t = (row - h * of_head) / p.groups, g = row - h * of_head - t * p.groups;
+      place_of[k] = 8 * h * tiles + t * p.row_group + g;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+        raw[k][j] = reinterpret_cast<const T*>(p.q)[(int64_t)b * p.q_stride_b + (int64_t)((heads0 + h) * p.groups + g) * p.q_stride_h +
+                                                  (int64_t)(token0 + t) * p.q_stride_t + lane + 32 * j];
     }
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    fine = __all_sync(0xffffffffu, fine);
-    if (lane == 0) tops[row] = fine ? top : __int_as_float(0x7fc00000);
-    // the whole number next to 32767 x / top, as q8_append.cu finds codes: a quotient that is no tie is at least 2^-40 of its power of
-    // two away from one, the product is off by 2^-51 of it at most
-    const double rate = fine && top > 0.0f ? 32767.0 / (double)top : 0.0;
+    for (int k = 0; k < kAhead; ++k) {
+      if (from + k >= rows) break;
+      float x[D / 32], top = 0.0f;
+      bool fine = true;
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      const double r = fine ? __dmul_rn((double)x[j], rate) : 0.0, c = __dmul_rn(r, 257.0);
-      const int whole = __double2int_rn(__dsub_rn(c, __dsub_rn(c, r)));
-      const int d = lane + 32 * j;
+      for (int j = 0; j < D / 32; ++j) {
+        x[j] = ElemTraits<T>::to_float(raw[k][j]);
+        top = fmaxf(top, fabsf(x[j]));
+        fine = fine && fabsf(x[j]) < INFINITY;
+      }
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+      fine = __all_sync(0xffffffffu, fine);
+      if (lane == 0) tops[place_of[k]] = fine ? top : __int_as_float(0x7fc00000);
+      // the whole number next to 32767 x / top, as q8_append.cu finds codes: a quotient that is no tie is at least 2^-40 of its power of
+      // two away from one, the product is off by 2^-51 of it at most
+      const double rate = fine && top > 0.0f ? 32767.0 / (double)top : 0.0;
 #pragma unroll
-      for (int negated = 0; negated < 2; ++negated) {
-        const int n = max(negated ? -whole : whole, 0), at = d + negated * D;
-        const int place = ((row / 8 * kChunks + at / 64) * 32 + row % 8 * 4 + at % 64 / 16) * 16 + at % 16;
-        smem[place] = (uint8_t)(n >> 7);
-        smem[tiles * kChunks * 512 + place] = (uint8_t)(n & 127);
+      for (int j = 0; j < D / 32; ++j) {
+        const double r = fine ? __dmul_rn((double)x[j], rate) : 0.0, c = __dmul_rn(r, 257.0);
+        const int whole = __double2int_rn(__dsub_rn(c, __dsub_rn(c, r)));
+        const int d = lane + 32 * j;
+#pragma unroll
+        for (int negated = 0; negated < 2; ++negated) {
+          const int n = max(negated ? -whole : whole, 0), at = d + negated * D;
+          const int place = ((place_of[k] / 8 * kChunks + at / 64) * 32 + place_of[k] % 8 * 4 + at % 64 / 16) * 16 + at % 16;
+          smem[place] = (uint8_t)(n >> 7);
+          smem[plane * 16 + place] = (uint8_t)(n & 127);
+        }
       }
     }
   }
   __syncthreads();
 
-  // ---- 16 pages at a time -----------------------------------------------------------------------------------------------------------
-  for (int tile = first_tile; tile < end && tile * kQ8SelectTile < most; tile += kQ8SelectWarps) {
-    if (tile > first_tile) {
-      load();
-      find(tile + kQ8SelectWarps);
+  // ---- 16 pages of a KV head at a time ---------------------------------------------------------------------------------------------------
+  for (bool first = true; tile < end && tile * kQ8SelectTile < most; first = false) {
+    if (!first) {
+      load(head);
+      find(next_tile());
     }
+    uint32_t* scores = p.scores + (((int64_t)b * p.kv_heads + heads0 + head) * p.tokens + token0) * p.max_blocks;
     float best[2] = {-INFINITY, -INFINITY};  // of one token
     for (int n = 0, t0 = 0, h = 0; n < tiles; ++n) {
       int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-      const uint4* at = parts + n * kChunks * 32 + lane;
+      const uint4* at = parts + (head * tiles + n) * kChunks * 32 + lane;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        const uint4 u = at[c * 32], v = at[(tiles * kChunks + c) * 32];
+        const uint4 u = at[c * 32], v = at[plane + c * 32];
         mma_s8u8(hi, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, u.x, u.y);
         mma_s8u8(lo, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, v.x, v.y);
         mma_s8u8(hi, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, u.z, u.w);
         mma_s8u8(lo, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, v.z, v.w);
       }
-      const float2 top = *reinterpret_cast<const float2*>(tops + 8 * n + 2 * tig);
+      const float2 top = *reinterpret_cast<const float2*>(tops + 8 * (head * tiles + n) + 2 * tig);
       float x[4];  // rows 2 tig and 2 tig + 1 of pages gid and gid + 8
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -211,16 +229,17 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
       t0 += 8 >> p.group_shift;
       h = 0;
     }
+    tile = next_tile();
+    head += head_step - (head + head_step >= heads ? heads : 0);
   }
   };
 
   if constexpr (!kShares) {
-    const int b = blockIdx.y / p.kv_heads, begin = blockIdx.x * p.rounds * kQ8SelectWarps;
-    if (begin * kQ8SelectTile < q8_candidates(p, b, p.tokens - 1))
-      segment(b, blockIdx.y - b * p.kv_heads, blockIdx.z, begin, begin + p.rounds * kQ8SelectWarps);
+    const int begin = blockIdx.x * p.part_tiles;
+    if (begin * kQ8SelectTile < q8_candidates(p, blockIdx.y, p.tokens - 1)) segment(blockIdx.y, blockIdx.z, begin, begin + p.part_tiles);
   } else {
     constexpr int kThreads = kQ8SelectWarps * 32;
-    const int per_row = p.kv_heads * p.chunks, each = (p.batch + kThreads - 1) / kThreads;
+    const int per_row = p.chunks * p.head_groups, each = (p.batch + kThreads - 1) / kThreads;
     int tiles_of_rows[kBalancedRowsPerThread<kThreads>], streams;
 #pragma unroll
     for (int i = 0; i < kBalancedRowsPerThread<kThreads>; ++i) {
@@ -228,7 +247,7 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
       tiles_of_rows[i] = i < each && b < p.batch ? (q8_candidates(p, b, p.tokens - 1) + kQ8SelectTile - 1) / kQ8SelectTile : 0;
     }
     balanced_scan<kThreads>(tiles_of_rows, p.batch, per_row, s_prefix, kQ8SelectCost, 0, &streams);
-    const int total = s_prefix[p.batch], share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 2 * kQ8SelectWarps);
+    const int total = s_prefix[p.batch], share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
     int pos = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
     const int stop = min(pos + share, total);
     int b = 0, above = p.batch;  // s_prefix[b] <= pos < s_prefix[above]
@@ -242,7 +261,7 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
       const int n = (s_prefix[b + 1] - s_prefix[b]) / per_row;  // of a stream, its cost among them
       const int stream = (pos - s_prefix[b]) / n, at = pos - s_prefix[b] - stream * n, to = min(n, at + stop - pos);
       if (to > kQ8SelectCost) {
-        segment(b, stream / p.chunks, stream % p.chunks, max(0, at - kQ8SelectCost), to - kQ8SelectCost);
+        segment(b, stream, max(0, at - kQ8SelectCost), to - kQ8SelectCost);
         __syncthreads();  // queries and candidates have been read
       }
       pos += to - at;
@@ -457,7 +476,7 @@ extern "C" int anna_q8_select_blocks(const void* q, int64_t q_stride_b, int64_t 
   ANNA_REQUIRE(aligned_to(pages, 16), "%s: pages must be 16-byte aligned", what);
   ANNA_REQUIRE(max_blocks < (1ll << 30) / block_size - 1, "%s: too many pages", what);
   const int64_t streams = (int64_t)batch * kv_heads * tokens;
-  ANNA_REQUIRE(streams < (1ll << 31) && (int64_t)batch * kv_heads < 65536, "%s: too many queries", what);
+  ANNA_REQUIRE(streams < (1ll << 31), "%s: too many queries", what);
   Q8SelectParams p{};
   p.q = q; p.q_stride_b = batch > 1 ? q_stride_b : 0; p.q_stride_h = q_heads > 1 ? q_stride_h : 0; p.q_stride_t = tokens > 1 ? q_stride_t : 0;
   p.pages = pages; p.block_table = page_table; p.table_stride = table_stride; p.lengths = lengths; p.blocks = blocks; p.scores = scores;
@@ -466,27 +485,32 @@ extern "C" int anna_q8_select_blocks(const void* q, int64_t q_stride_b, int64_t 
   p.row_group = p.groups <= 8 && 8 % p.groups == 0 ? p.groups : (p.groups + 7) / 8 * 8;
   p.group_shift = p.row_group == 1 ? 0 : p.row_group == 2 ? 1 : p.row_group == 4 ? 2 : 3;
   p.head_tiles = (p.row_group + 7) / 8;
-  p.tokens_at_once = p.row_group >= kQ8SelectRows ? 1 : kQ8SelectRows / p.row_group;
+  // As many KV heads as shared memory has room for with one token, then as many tokens.
+  const int tile_bytes = 2 * (2 * head_dim / 64) * 512 + 32, room = 64 * 1024 / tile_bytes;
+  // Where warps have few tiles each, one KV head: what counts is how soon a CTA's queries are ready (one row of 8191 pages, 8 KV heads: all at once 20.0 us,
+  // one 17.4).
+  const int64_t page_tiles = (max_blocks + kQ8SelectTile - 1) / kQ8SelectTile, ctas = 148 * (head_dim == 256 ? kQ8SelectCtas<256> : kQ8SelectCtas<128>);
+  const bool few = (int64_t)batch * kv_heads * page_tiles <= 2 * ctas * kQ8SelectWarps;
+  p.heads_at_once = few || room / p.head_tiles < 1 ? 1 : room / p.head_tiles > kv_heads ? kv_heads : room / p.head_tiles;
+  p.tokens_at_once = room / p.heads_at_once * 8 / p.row_group;
+  if (p.tokens_at_once > kQ8SelectRows / p.row_group) p.tokens_at_once = kQ8SelectRows / p.row_group;
   if (p.tokens_at_once > tokens) p.tokens_at_once = tokens;
-  const int row_tiles = (p.tokens_at_once * p.row_group + 7) / 8;
-  const int smem = row_tiles * (2 * (2 * head_dim / 64) * 512 + 32);
+  if (p.tokens_at_once < 1) p.tokens_at_once = 1;
+  const int smem = p.heads_at_once * ((p.tokens_at_once * p.row_group + 7) / 8) * tile_bytes;
   if (smem > 200 * 1024) return set_error(ANNA_ERR_UNSUPPORTED, "%s: too many query heads (%d) to a KV head", what, p.groups);
-  const int chunks = (tokens + p.tokens_at_once - 1) / p.tokens_at_once;
-  ANNA_REQUIRE(chunks < 65536, "%s: too many tokens", what);
+  p.chunks = (tokens + p.tokens_at_once - 1) / p.tokens_at_once;
+  p.head_groups = (kv_heads + p.heads_at_once - 1) / p.heads_at_once;
+  p.batch = batch;
   if (max_blocks > 0) {
-    const int64_t tiles = (max_blocks + kQ8SelectTile - 1) / kQ8SelectTile, ctas = 148 * (head_dim == 256 ? kQ8SelectCtas<256> : kQ8SelectCtas<128>);
-    const int64_t parts = (int64_t)batch * kv_heads * chunks, line = parts * (tiles + kQ8SelectCost);
-    const int64_t wave = ctas * kQ8SelectWarps;
-    p.batch = batch;
-    p.chunks = chunks;
-    p.rounds = (int)((parts * tiles + wave - 1) / wave);
-    int64_t splits = (tiles + p.rounds * kQ8SelectWarps - 1) / (p.rounds * kQ8SelectWarps);
-    const bool shares = parts * splits > ctas && batch <= kBalancedMaxRows && line < (1ll << 30);
-    if (!shares && p.rounds > 8) {
-      p.rounds = 8;
-      splits = (tiles + 8 * kQ8SelectWarps - 1) / (8 * kQ8SelectWarps);
-    }
-    const dim3 grid = shares ? dim3((unsigned)ctas) : dim3((unsigned)splits, (unsigned)(batch * kv_heads), (unsigned)chunks);
+    const int64_t tiles = page_tiles;
+    const int64_t streams_of_all = (int64_t)batch * p.chunks * p.head_groups, line = streams_of_all * (tiles + kQ8SelectCost);
+    // tiles of a CTA: at least one for every warp
+    const int64_t least = (kQ8SelectWarps + p.heads_at_once - 1) / p.heads_at_once, even = (streams_of_all * tiles + ctas - 1) / ctas;
+    p.part_tiles = (int)(even < least ? least : even > 64 ? 64 : even);
+    const int64_t splits = (tiles + p.part_tiles - 1) / p.part_tiles;
+    const bool shares = ((!few && batch > 1) || streams_of_all * splits > ctas) && batch <= kBalancedMaxRows && line < (1ll << 30);
+    ANNA_REQUIRE(shares || (batch < 65536 && p.chunks * p.head_groups < 65536), "%s: too many queries", what);
+    const dim3 grid = shares ? dim3((unsigned)ctas) : dim3((unsigned)splits, (unsigned)batch, (unsigned)(p.chunks * p.head_groups));
     const int rc = ANNA_DISPATCH_DTYPE(dtype, T, [&]() -> int {
       return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
         auto kernel = shares ? q8_score_kernel<T, D, true> : q8_score_kernel<T, D, false>;
