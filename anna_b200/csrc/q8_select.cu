@@ -61,6 +61,39 @@ __device__ __forceinline__ uint32_t q8_ordered(float x) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+// The whole number next to 32767 x / top, of two the even one; 0 where top is.  Of 16-bit values (11 bits) in 32 bits: the quotient is off by less than
+// 0.01, and what 32767 x exceeds n top by is exact, a product in two parts less another (the first difference has no more than 24 bits, as n top and
+// 32767 x lie that close).  (64-bit arithmetic, as fp32 values take it: 4 to 6 us until a CTA's queries were ready, PLACEHOLDER so.)
+template <typename T>
+struct Q8Whole {
+  float factor, top, rate;
+  __device__ __forceinline__ explicit Q8Whole(float most) {
+    const int up = most > 0.0f ? min(max(127 - (int)(__float_as_uint(most) >> 23), -126), 126) : 0;  // top is in [1, 4), or all is as good as 0
+    factor = __uint_as_float((uint32_t)(up + 127) << 23);
+    top = most * factor;
+    rate = most > 0.0f ? __fdiv_rn(32767.0f, top) : 0.0f;
+  }
+  __device__ __forceinline__ int whole(float value) const {
+    const float x = value * factor, n = rintf(x * rate);
+    const float product = __fmul_rn(32767.0f, x), rest = __fmaf_rn(32767.0f, x, -product);
+    const float over = __fadd_rn(__fmaf_rn(-n, top, product), rest), half = 0.5f * top;
+    const int i = __float2int_rn(n);
+    const bool odd = i & 1;
+    return i + (over > half || (over == half && odd) ? 1 : 0) - (over < -half || (over == -half && odd) ? 1 : 0);
+  }
+};
+// fp32 values: a quotient that is no tie is at least 2^-40 of its power of two away from one, the product is off by 2^-51 of it at most; rounded to 45 bits
+// (as q8_append.cu does it) ties are ties again.
+template <>
+struct Q8Whole<float> {
+  double rate;
+  __device__ __forceinline__ explicit Q8Whole(float top) { rate = top > 0.0f ? 32767.0 / (double)top : 0.0; }
+  __device__ __forceinline__ int whole(float value) const {
+    const double r = __dmul_rn((double)value, rate), c = __dmul_rn(r, 257.0);
+    return __double2int_rn(__dsub_rn(c, __dsub_rn(c, r)));
+  }
+};
+
 // Rows are the query heads of several tokens, one behind the other: the heads of a token are in one tile of 8 rows where their number divides 8, else
 // a token has tiles of its own.  The KV heads of a page lie next to one another, and a CTA's warps take them together: a page costs one translation of its
 // address and one stretch of memory (32 rows of 20000 to 32768 tokens in scattered pages, 8 KV heads: PLACEHOLDER us with CTAs of one KV head).
@@ -121,24 +154,25 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
   const int of_head = here * p.groups, rows = heads * of_head;
   constexpr int kAhead = 4;  // rows on their way
   for (int from = warp * kAhead; from < rows; from += kQ8SelectWarps * kAhead) {
-    T raw[kAhead][D / 32];
+    constexpr int E = D / 32;  // neighbouring dims of a lane
+    T raw[kAhead][E];
     int place_of[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int row = min(from + k, rows - 1), h = row / of_head, t = (row - h * of_head) / p.groups, g = row - h * of_head - t * p.groups;
       place_of[k] = 8 * h * tiles + t * p.row_group + g;
+      const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_stride_b + (int64_t)((heads0 + h) * p.groups + g) * p.q_stride_h +
+                   (int64_t)(token0 + t) * p.q_stride_t + lane * E;
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j)
-        raw[k][j] = reinterpret_cast<const T*>(p.q)[(int64_t)b * p.q_stride_b + (int64_t)((heads0 + h) * p.groups + g) * p.q_stride_h +
-                                                  (int64_t)(token0 + t) * p.q_stride_t + lane + 32 * j];
+      for (int j = 0; j < E; ++j) raw[k][j] = q[j];
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (from + k >= rows) break;
-      float x[D / 32], top = 0.0f;
+      float x[E], top = 0.0f;
       bool fine = true;
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
+      for (int j = 0; j < E; ++j) {
         x[j] = ElemTraits<T>::to_float(raw[k][j]);
         top = fmaxf(top, fabsf(x[j]));
         fine = fine && fabsf(x[j]) < INFINITY;
@@ -146,20 +180,31 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
       top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
       fine = __all_sync(0xffffffffu, fine);
       if (lane == 0) tops[place_of[k]] = fine ? top : __int_as_float(0x7fc00000);
-      // the whole number next to 32767 x / top, as q8_append.cu finds codes: a quotient that is no tie is at least 2^-40 of its power of
-      // two away from one, the product is off by 2^-51 of it at most
-      const double rate = fine && top > 0.0f ? 32767.0 / (double)top : 0.0;
+      const Q8Whole<T> rounder(fine ? top : 0.0f);
+      uint32_t upper[2][(E + 3) / 4] = {}, lower[2][(E + 3) / 4] = {};  // bytes of positive and of negative numbers
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const double r = fine ? __dmul_rn((double)x[j], rate) : 0.0, c = __dmul_rn(r, 257.0);
-        const int whole = __double2int_rn(__dsub_rn(c, __dsub_rn(c, r)));
-        const int d = lane + 32 * j;
+      for (int j = 0; j < E; ++j) {
+        const int whole = fine ? rounder.whole(x[j]) : 0;
 #pragma unroll
         for (int negated = 0; negated < 2; ++negated) {
-          const int n = max(negated ? -whole : whole, 0), at = d + negated * D;
-          const int place = ((place_of[k] / 8 * kChunks + at / 64) * 32 + place_of[k] % 8 * 4 + at % 64 / 16) * 16 + at % 16;
-          smem[place] = (uint8_t)(n >> 7);
-          smem[plane * 16 + place] = (uint8_t)(n & 127);
+          const uint32_t n = (uint32_t)max(negated ? -whole : whole, 0);
+          upper[negated][j / 4] |= (n >> 7) << (8 * (j % 4));
+          lower[negated][j / 4] |= (n & 127u) << (8 * (j % 4));
+        }
+      }
+      const int d = lane * E;
+#pragma unroll
+      for (int negated = 0; negated < 2; ++negated) {
+        uint8_t* to = smem + ((place_of[k] / 8 * kChunks + d / 64 + negated * (D / 64)) * 32 + place_of[k] % 8 * 4 + d % 64 / 16) * 16 + d % 16;
+        if constexpr (E == 2) {
+          *reinterpret_cast<uint16_t*>(to) = (uint16_t)upper[negated][0];
+          *reinterpret_cast<uint16_t*>(to + plane * 16) = (uint16_t)lower[negated][0];
+        } else if constexpr (E == 4) {
+          *reinterpret_cast<uint32_t*>(to) = upper[negated][0];
+          *reinterpret_cast<uint32_t*>(to + plane * 16) = lower[negated][0];
+        } else {
+          *reinterpret_cast<uint2*>(to) = make_uint2(upper[negated][0], upper[negated][E / 4 - 1]);
+          *reinterpret_cast<uint2*>(to + plane * 16) = make_uint2(lower[negated][0], lower[negated][E / 4 - 1]);
         }
       }
     }
@@ -238,28 +283,47 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
     const int begin = blockIdx.x * p.part_tiles;
     if (begin * kQ8SelectTile < q8_candidates(p, blockIdx.y, p.tokens - 1)) segment(blockIdx.y, blockIdx.z, begin, begin + p.part_tiles);
   } else {
+    // at most 32 rows are lined up by every warp by itself
     constexpr int kThreads = kQ8SelectWarps * 32;
-    const int per_row = p.chunks * p.head_groups, each = (p.batch + kThreads - 1) / kThreads;
-    int tiles_of_rows[kBalancedRowsPerThread<kThreads>], streams;
+    const bool few = p.batch <= 32;
+    const int per_row = p.chunks * p.head_groups;
+    auto tiles_of = [&](int b) { return b < p.batch ? (q8_candidates(p, b, p.tokens - 1) + kQ8SelectTile - 1) / kQ8SelectTile : 0; };
+    WarpLine line{};
+    int total;
+    if (few) {
+      line.tiles = tiles_of(lane);
+      total = line.scan(per_row, kQ8SelectCost, 0);
+    } else {
+      const int each = (p.batch + kThreads - 1) / kThreads;
+      int tiles_of_rows[kBalancedRowsPerThread<kThreads>], streams;
 #pragma unroll
-    for (int i = 0; i < kBalancedRowsPerThread<kThreads>; ++i) {
-      const int b = threadIdx.x * each + i;
-      tiles_of_rows[i] = i < each && b < p.batch ? (q8_candidates(p, b, p.tokens - 1) + kQ8SelectTile - 1) / kQ8SelectTile : 0;
+      for (int i = 0; i < kBalancedRowsPerThread<kThreads>; ++i) tiles_of_rows[i] = i < each ? tiles_of(threadIdx.x * each + i) : 0;
+      balanced_scan<kThreads>(tiles_of_rows, p.batch, per_row, s_prefix, kQ8SelectCost, 0, &streams);
+      total = s_prefix[p.batch];
     }
-    balanced_scan<kThreads>(tiles_of_rows, p.batch, per_row, s_prefix, kQ8SelectCost, 0, &streams);
-    const int total = s_prefix[p.batch], share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
-    int pos = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
+    const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+    int pos = (int)min((int64_t)blockIdx.x * share, (int64_t)total), b = 0;
     const int stop = min(pos + share, total);
-    int b = 0, above = p.batch;  // s_prefix[b] <= pos < s_prefix[above]
-    while (above - b > 1) {
-      const int mid = (b + above) >> 1;
-      if (s_prefix[mid] <= pos) b = mid;
-      else above = mid;
+    if (!few && pos < stop) {
+      int above = p.batch;  // s_prefix[b] <= pos < s_prefix[above]
+      while (above - b > 1) {
+        const int mid = (b + above) >> 1;
+        if (s_prefix[mid] <= pos) b = mid;
+        else above = mid;
+      }
     }
     while (pos < stop) {
-      while (s_prefix[b + 1] <= pos) ++b;
-      const int n = (s_prefix[b + 1] - s_prefix[b]) / per_row;  // of a stream, its cost among them
-      const int stream = (pos - s_prefix[b]) / n, at = pos - s_prefix[b] - stream * n, to = min(n, at + stop - pos);
+      int first, n;  // positions in front of the row; of a stream, its cost among them
+      if (few) {
+        b = __popc(__ballot_sync(0xffffffffu, line.next <= pos));
+        first = __shfl_sync(0xffffffffu, line.first, b);
+        n = __shfl_sync(0xffffffffu, line.tiles, b) + kQ8SelectCost;
+      } else {
+        while (s_prefix[b + 1] <= pos) ++b;
+        first = s_prefix[b];
+        n = (s_prefix[b + 1] - first) / per_row;
+      }
+      const int stream = (pos - first) / n, at = pos - first - stream * n, to = min(n, at + stop - pos);
       if (to > kQ8SelectCost) {
         segment(b, stream, max(0, at - kQ8SelectCost), to - kQ8SelectCost);
         __syncthreads();  // queries and candidates have been read
