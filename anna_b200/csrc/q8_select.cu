@@ -55,6 +55,12 @@ __device__ __forceinline__ void mma_s8u8(int (&d)[4], uint32_t a0, uint32_t a1, 
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 16 bytes that are read once; half lines are fetched from memory, as bounds end a little way into a line (320 bytes a page of 128 dims instead of 384).
+__device__ __forceinline__ uint4 q8_ldg64(const uint4* ptr) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::64B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
+  return v;
+}
 // Order of floats as order of whole numbers, none of them 0.
 __device__ __forceinline__ uint32_t q8_ordered(float x) {
   const uint32_t bits = __float_as_uint(x + 0.0f);  // -0 counts as 0
@@ -142,21 +148,17 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
       scale[i] = __ldg(reinterpret_cast<const float*>(page + q8_scale_offset(D, p.block_size)));
       const uint4* bounds = reinterpret_cast<const uint4*>(page + q8_bounds_offset(D, p.block_size));
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) w[i][c] = ldg_stream16(bounds + 4 * c + tig);
+      for (int c = 0; c < kChunks; ++c) w[i][c] = q8_ldg64(bounds + 4 * c + tig);
     }
   };
   auto next_tile = [&] { return tile + tile_step + (head + head_step >= heads ? 1 : 0); };
-  find(tile);
-  load(head);
-  find(next_tile());
-
-  // ---- queries in whole numbers; rows that are not there stay as they are --------------------------------------------------------------
+  // queries: the first of them are asked for ahead of the bounds, behind which they would wait
   const int of_head = here * p.groups, rows = heads * of_head;
   constexpr int kAhead = 4;  // rows on their way
-  for (int from = warp * kAhead; from < rows; from += kQ8SelectWarps * kAhead) {
-    constexpr int E = D / 32;  // neighbouring dims of a lane
-    T raw[kAhead][E];
-    int place_of[kAhead];
+  constexpr int E = D / 32;  // neighbouring dims of a lane
+  T raw[kAhead][E];
+  int place_of[kAhead];
+  auto fetch = [&](int from) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int row = min(from + k, rows - 1), h = row / of_head, t = (row - h * of_head) / p.groups, g = row - h * of_head - t * p.groups;
@@ -166,6 +168,15 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
 #pragma unroll
       for (int j = 0; j < E; ++j) raw[k][j] = q[j];
     }
+  };
+  find(tile);
+  fetch(warp * kAhead);
+  load(head);
+  find(next_tile());
+
+  // ---- queries in whole numbers; rows that are not there stay as they are --------------------------------------------------------------
+  for (int from = warp * kAhead; from < rows; from += kQ8SelectWarps * kAhead) {
+    if (from > warp * kAhead) fetch(from);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (from + k >= rows) break;
