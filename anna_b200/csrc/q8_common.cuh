@@ -144,9 +144,13 @@ __device__ __forceinline__ void q8_for_each_segment(const Q8Params& p, int row_t
 }
 
 // Launches of this cache follow one another (append, selection, choice, attention), each of a few microseconds.  They go out with leave to
-// start while the kernel in front of them ends, and touch no memory before that has ended and its writes are there.
+// start while the kernel in front of them ends, and touch no memory before that has ended and its writes are there.  A kernel of more than two CTAs per
+// SM lets the next one start at its end alone: CTAs that wait beside it cost more than that saves (a prompt of 3001 tokens appended and viewed 16.4 us,
+// 11.7 so; a selection of one row 18.5 us without an early start, 17.6 with it).
 __device__ __forceinline__ void q8_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void q8_let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void q8_let_next_start() {
+  if (gridDim.x * gridDim.y * gridDim.z <= 2 * 148) asm volatile("griddepcontrol.launch_dependents;");
+}
 
 template <typename... Params, typename... Args>
 int q8_launch(const char* what, void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, Args&&... args) {
