@@ -208,16 +208,25 @@ using namespace anna;
 namespace {
 
 constexpr int kQ8MinTiles = 4;   // of a CTA with blocks, CUDA cores
+// Tensor cores.  What a stream costs a CTA beside its tiles, in tiles; by this number (8, 16, 32, 64) 64 ragged rows of 0.5-16 K tokens 106, 105, 102,
+// 103 us, 16 rows of 0.4-4 K tokens of 256 dims 72, 67, 61, 67.  Positions of the line that a CTA takes at least; by this number (8, 16, 32, 64) one row of
+// 4000 tokens 13.4, 12.3, 14.1, 18.4; tiles of a list alike (one row's 256 pages: 4 to 12 tiles 15.2-13.3, 16 12.4, 24 and 32 13.3-13.7).
+constexpr int kQ8StreamTiles = 32, kQ8MinShare = 16;
 
 // What a call takes; the sizes have been checked.
 Q8Plan q8_plan(int batch, int q_heads, int kv_heads, int tokens, int head_dim, int block_size, int64_t max_blocks, int width, int dtype) {
   Q8Plan plan{};
   const int groups = q_heads / kv_heads, rows = width > 0 ? groups : tokens * groups;
   plan.tensor_cores = block_size % 8 == 0;
-  const Q8Shape shape = plan.tensor_cores ? q8_mma_shape(head_dim, rows)
+  // key tiles of all streams, with what a stream costs beside its own; a stream has one row tile where `few` counts
+  const int64_t axis = width > 0 ? (int64_t)(width + 1) * block_size : max_blocks * block_size + block_size - 1;
+  const int64_t key_tiles = (axis + kBalancedTileTokens - 1) / kBalancedTileTokens;
+  const bool few = (int64_t)batch * kv_heads * (width > 0 ? tokens * key_tiles : key_tiles + kQ8StreamTiles) <= 148 * kQ8MinShare;
+  const Q8Shape shape = plan.tensor_cores ? q8_mma_shape(head_dim, rows, few)
                                           : Q8Shape{kQ8Rows, head_dim == 64 ? kQ8Ctas<64> : head_dim == 128 ? kQ8Ctas<128> : kQ8Ctas<256>, 4};
   plan.rows = shape.rows;
-  const int per_sm = shape.ctas, min_tiles = plan.tensor_cores ? 4 * shape.warps : kQ8MinTiles;
+  plan.warps = shape.warps;
+  const int per_sm = shape.ctas, min_tiles = plan.tensor_cores ? 16 : kQ8MinTiles;
   const int tiles = (rows + plan.rows - 1) / plan.rows;
   plan.tiles_per_token = tiles;
   plan.row_tiles = width > 0 ? tokens * tiles : tiles;
@@ -225,7 +234,6 @@ Q8Plan q8_plan(int batch, int q_heads, int kv_heads, int tokens, int head_dim, i
   plan.splits = 1;
   plan.ctas = wave;
   if (width > 0) {
-    const int64_t key_tiles = ((int64_t)(width + 1) * block_size + kBalancedTileTokens - 1) / kBalancedTileTokens;
     int64_t splits = wave / (streams < 1 ? 1 : streams);
     if (splits > key_tiles / min_tiles) splits = key_tiles / min_tiles;
     if (splits > kMultiMaxPartials) splits = kMultiMaxPartials;
@@ -300,8 +308,8 @@ extern "C" int anna_q8_attention(const void* q, int64_t q_stride_b, int64_t q_st
     if ((1 << s) == block_size) p.block_shift = s;
   p.num_pages = num_pages; p.max_blocks = max_blocks; p.max_len = max_blocks * block_size + block_size - 1;
   p.scaling = scaling;
-  p.stream_tiles = plan.tensor_cores ? 32 : 4;
-  p.min_share = plan.tensor_cores ? 16 : 4;
+  p.stream_tiles = plan.tensor_cores ? kQ8StreamTiles : 4;
+  p.min_share = plan.tensor_cores ? kQ8MinShare : 4;
   p.whole_tiles = 0;
   // The line of a launch without blocks has room for so many rows and positions: larger batches go in several, one behind the other.
   int most = batch;

@@ -28,11 +28,12 @@
 
 namespace anna {
 
-template <typename T, int D, int NT>
+// W warps: four, with several CTAs to an SM; eight, with one, where the tiles of a call are few (one row of 4000 tokens: 11.5 us, PLACEHOLDER with eight).
+template <typename T, int D, int NT, int W>
 struct Q8Cfg {
-  static constexpr int kWarps = 4;
+  static constexpr int kWarps = W;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kCtas = D == 256 ? 2 : NT <= 2 ? 3 : 2;  // per SM
+  static constexpr int kCtas = W == 8 ? 1 : D == 256 ? 2 : NT <= 2 ? 3 : 2;  // per SM
   static constexpr int kStages = D == 64 ? 4 : D == 256 && (NT == 2 || sizeof(T) == 4) ? 2 : 3;
   static constexpr int kRows = 8 * NT;
   static constexpr int kChunks = D / 64;         // 16-byte pieces of a lane's key
@@ -125,9 +126,9 @@ __device__ __forceinline__ uint32_t q8_finite_halves(uint32_t x) {
   return ((x & kExp) != kExp ? 0x0000ffffu : 0u) | ((x >> 16 & kExp) != kExp ? 0xffff0000u : 0u);
 }
 
-template <typename T, int D, int NT, bool kBlocks, bool kHalves>
-__global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kCtas) q8_mma_kernel(const Q8Params p, int row_tiles) {
-  using Cfg = Q8Cfg<T, D, NT>;
+template <typename T, int D, int NT, int W, bool kBlocks, bool kHalves>
+__global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, W>::kCtas) q8_mma_kernel(const Q8Params p, int row_tiles) {
+  using Cfg = Q8Cfg<T, D, NT, W>;
   constexpr bool kFloat = std::is_same_v<T, float>;
   constexpr int kPages = kHalves ? 2 : 1, kPageTokens = 16 / kPages;  // of a tile
   constexpr int kTile = kBalancedTileTokens;
@@ -705,25 +706,24 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT>::kThreads, Q8Cfg<T, D, NT>::kC
   });
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int W = 4>
 static int launch(const Q8Params& p, int row_tiles, int ctas, cudaStream_t stream) {
-  using Cfg = Q8Cfg<T, D, NT>;
+  using Cfg = Q8Cfg<T, D, NT, W>;
   const bool halves = p.block_size % kBalancedTileTokens != 0;
-  auto kernel = p.blocks != nullptr ? (halves ? q8_mma_kernel<T, D, NT, true, true> : q8_mma_kernel<T, D, NT, true, false>)
-                                    : (halves ? q8_mma_kernel<T, D, NT, false, true> : q8_mma_kernel<T, D, NT, false, false>);
+  auto kernel = p.blocks != nullptr ? (halves ? q8_mma_kernel<T, D, NT, W, true, true> : q8_mma_kernel<T, D, NT, W, true, false>)
+                                    : (halves ? q8_mma_kernel<T, D, NT, W, false, true> : q8_mma_kernel<T, D, NT, W, false, false>);
   ANNA_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
   return q8_launch("q8_mma_kernel", kernel, dim3((unsigned)ctas), Cfg::kThreads, Cfg::kSmem, stream, p, row_tiles);
 }
 
 template <typename T>
 int launch_q8_mma_of(const Q8Params& p, const Q8Plan& plan, int head_dim, int ctas, cudaStream_t stream) {
-  if (head_dim == 64)
-    return plan.rows == 8 ? launch<T, 64, 1>(p, plan.row_tiles, ctas, stream) : plan.rows == 16 ? launch<T, 64, 2>(p, plan.row_tiles, ctas, stream)
-                                                                                              : launch<T, 64, 4>(p, plan.row_tiles, ctas, stream);
-  if (head_dim == 128)
-    return plan.rows == 8 ? launch<T, 128, 1>(p, plan.row_tiles, ctas, stream) : plan.rows == 16 ? launch<T, 128, 2>(p, plan.row_tiles, ctas, stream)
-                                                                                               : launch<T, 128, 4>(p, plan.row_tiles, ctas, stream);
-  return plan.rows == 8 ? launch<T, 256, 1>(p, plan.row_tiles, ctas, stream) : launch<T, 256, 2>(p, plan.row_tiles, ctas, stream);
+  return ANNA_DISPATCH_TQ_DIM(head_dim, D, [&]() -> int {
+    if (plan.rows == 8) return plan.warps == 8 ? launch<T, D, 1, 8>(p, plan.row_tiles, ctas, stream) : launch<T, D, 1>(p, plan.row_tiles, ctas, stream);
+    if (D == 256 || plan.rows == 16) return launch<T, D, 2>(p, plan.row_tiles, ctas, stream);
+    if constexpr (D != 256) return launch<T, D, 4>(p, plan.row_tiles, ctas, stream);
+    return ANNA_OK;
+  });
 }
 
 }  // namespace anna

@@ -173,6 +173,7 @@ int q8_launch(const char* what, void (*kernel)(Params...), dim3 grid, int thread
 struct Q8Plan {
   bool tensor_cores;
   int rows;       // of a row tile
+  int warps;      // of a CTA (tensor cores)
   int row_tiles;  // of a (sequence, KV head)
   int tiles_per_token, splits;
   int64_t ctas;   // at most
@@ -184,7 +185,7 @@ struct Q8Plan {
 struct Q8Shape {
   int rows, ctas, warps;  // of a row tile; of an SM; of a CTA
 };
-Q8Shape q8_mma_shape(int head_dim, int rows);
+Q8Shape q8_mma_shape(int head_dim, int rows, bool few);  // few: one row tile, and no more key tiles than a CTA to an SM has quick work of
 template <typename T>
 int launch_q8_mma_of(const Q8Params& p, const Q8Plan& plan, int head_dim, int ctas, cudaStream_t stream);
 
