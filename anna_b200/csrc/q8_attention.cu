@@ -216,6 +216,7 @@ constexpr int kQ8StreamTiles = 32, kQ8MinShare = 16;
 // What a call takes; the sizes have been checked.
 Q8Plan q8_plan(int batch, int q_heads, int kv_heads, int tokens, int head_dim, int block_size, int64_t max_blocks, int width, int dtype) {
   Q8Plan plan{};
+  if (max_blocks == 0) width = 0;  // a table without columns has no page to choose: the kernels go by the ring alone
   const int groups = q_heads / kv_heads, rows = width > 0 ? groups : tokens * groups;
   plan.tensor_cores = block_size % 8 == 0;
   // key tiles of all streams, with what a stream costs beside its own; a stream has one row tile where `few` counts
@@ -285,6 +286,10 @@ extern "C" int anna_q8_attention(const void* q, int64_t q_stride_b, int64_t q_st
   ANNA_REQUIRE(max_blocks == 0 || (pages && page_table && num_pages > 0), "%s: a block table needs pages", what);
   ANNA_REQUIRE(aligned_to(pages, 16) && aligned_to(window, 16), "%s: pages and window must be 16-byte aligned", what);
   ANNA_REQUIRE(aligned_to(scratch, 16), "%s: scratch must be 16-byte aligned", what);
+  if (max_blocks == 0) {  // as q8_plan has it; there may be no pool either
+    blocks = nullptr;
+    width = 0;
+  }
   const Q8Plan plan = q8_plan(batch, q_heads, kv_heads, tokens, head_dim, block_size, max_blocks, width, dtype);
   if (scratch_size < plan.floats)
     return set_error(ANNA_ERR_WORKSPACE, "%s: scratch holds %lld floats, %lld are needed", what, (long long)scratch_size, (long long)plan.floats);
