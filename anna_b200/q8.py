@@ -81,7 +81,7 @@ def run_q8_append(*, key: torch.Tensor, value: torch.Tensor, packed_pages: torch
     """Appends ``key`` and ``value`` ``[B, Hkv, T, D]`` (any strides) to rows of ``past_lengths`` tokens, int64 ``[B]``.  Pages that are
     filled are quantized into the page that ``page_table`` has for their block; what is stored does not depend on how tokens are cut into
     calls.  ``new_lengths`` (int64 ``[B]``, other memory than ``past_lengths``) receives ``past_lengths + T``.  ``status``: int32, bit 0
-    is set when a page or ring that is needed is none (its tokens are not written)."""
+    is set when a page or ring that is needed is none (its tokens are not written), or a row would be 2^30 tokens or longer."""
     name = "q8_append"
     if launch_module().q8_append(key, value, packed_pages, page_table, window, window_slots, past_lengths, new_lengths, status):
         return

@@ -517,7 +517,8 @@ int anna_q8_page_bytes(int head_dim, int block_size, int64_t* bytes);
  *   k_new, v_new   [B, Hkv, T, D], element strides of their own, multiples of 16 bytes on 16-byte aligned rows; last dim contiguous
  *   page_table     int32 [B, table_stride >= max_blocks];  window_slots, past_lengths int64 [B], no slot twice
  *   new_lengths    NULL or int64 [B] apart from past_lengths: receives past_lengths[b] + T
- *   status         optional device int32: ANNA_DEV_BAD_PAGE is OR-ed in when a page or slot that is needed is none
+ *   new_tokens     at least one; rows of a negative length, and those that would be 2^30 tokens or more, are left out
+ *   status         optional device int32: ANNA_DEV_BAD_PAGE is OR-ed in when a page or slot that is needed is none, or a row too long
  */
 int anna_q8_append(const void* k_new, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t, const void* v_new, int64_t v_stride_b,
                    int64_t v_stride_h, int64_t v_stride_t, uint8_t* pages, const int32_t* page_table, int64_t table_stride, void* window,
@@ -532,6 +533,7 @@ int anna_q8_append(const void* k_new, int64_t k_stride_b, int64_t k_stride_h, in
  *                  list names (in any order; one that is named twice counts twice, what is no full page of the row is left out), and the
  *                  unfinished one
  *   scratch        float32, 16-byte aligned, as many as the plan says; counters int32, zero on entry and on return
+ *                  (lengths are cut at what the table and the ring hold, max_blocks * S + S - 1)
  * anna_q8_attention_plan: sizes for these arguments (width 0: no blocks).
  */
 int anna_q8_attention_plan(int batch, int q_heads, int kv_heads, int tokens, int head_dim, int block_size, int64_t max_blocks, int width,
