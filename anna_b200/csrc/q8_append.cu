@@ -12,6 +12,9 @@
 // 2^-22.4 of it at most.  Rounded to 21 bits (Veltkamp's splitting: c = 9 q, c - (c - q)) a tie is one again, and all else stays on its
 // side.  fp32 values take the same steps in 64 bits (24 significant bits, rounded to 41).
 #include "q8_common.cuh"
+#include "tq_bulk.cuh"
+
+#include <type_traits>
 
 namespace anna {
 
@@ -34,62 +37,54 @@ struct Q8AppendParams {
 constexpr int kQ8AppendWarps = 4;
 constexpr int64_t kQ8MaxLength = 1ll << 30;  // of a row, a table, and a call's tokens
 
-// The lanes' 16 bytes as values, and what follows of their extremes.
+// The larger and the smaller of the values in a word, one or two; a NaN stays one.
 template <typename T>
-struct Q8Vec {
-  static constexpr int kN = ElemTraits<T>::kVec;
-  uint4 raw;
-  __device__ __forceinline__ void load(const T* from) { raw = *reinterpret_cast<const uint4*>(from); }
-  __device__ __forceinline__ void values(float (&x)[kN]) const { widen16<T>(raw, x); }
-};
+__device__ __forceinline__ uint32_t q8_larger(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, float>) asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else if constexpr (std::is_same_v<T, __half>) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t q8_smaller(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, float>) asm("min.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else if constexpr (std::is_same_v<T, __half>) asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
-// Running extremes of a lane's dims; a NaN stays one.
+// Running extremes of a lane's dims, 16 bytes each, in the cache's type.
 template <typename T>
 struct Q8Extremes {
-  static constexpr int kN = ElemTraits<T>::kVec;
-  float high[kN], low[kN];
+  uint4 high, low;
   __device__ __forceinline__ void start() {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      high[i] = -INFINITY;
-      low[i] = INFINITY;
-    }
+    constexpr uint32_t kInf = std::is_same_v<T, float> ? 0x7f800000u : std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t kSigns = std::is_same_v<T, float> ? 0x80000000u : 0x80008000u;
+    low = make_uint4(kInf, kInf, kInf, kInf);
+    high = make_uint4(kInf | kSigns, kInf | kSigns, kInf | kSigns, kInf | kSigns);
   }
-  static __device__ __forceinline__ float larger(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-  }
-  static __device__ __forceinline__ float smaller(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-  }
-  __device__ __forceinline__ void take(const Q8Vec<T>& v) {
-    float x[kN];
-    v.values(x);
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      high[i] = larger(high[i], x[i]);
-      low[i] = smaller(low[i], x[i]);
-    }
+  __device__ __forceinline__ void take(const uint4& h, const uint4& l) {
+    high = make_uint4(q8_larger<T>(high.x, h.x), q8_larger<T>(high.y, h.y), q8_larger<T>(high.z, h.z), q8_larger<T>(high.w, h.w));
+    low = make_uint4(q8_smaller<T>(low.x, l.x), q8_smaller<T>(low.y, l.y), q8_smaller<T>(low.z, l.z), q8_smaller<T>(low.w, l.w));
   }
   __device__ __forceinline__ void exchange(int mask) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      high[i] = larger(high[i], __shfl_xor_sync(0xffffffffu, high[i], mask));
-      low[i] = smaller(low[i], __shfl_xor_sync(0xffffffffu, low[i], mask));
-    }
+    auto other = [&](uint32_t x) { return __shfl_xor_sync(0xffffffffu, x, mask); };
+    const uint4 h = make_uint4(other(high.x), other(high.y), other(high.z), other(high.w));
+    take(h, make_uint4(other(low.x), other(low.y), other(low.z), other(low.w)));
   }
-  __device__ __forceinline__ float magnitude() const {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) m = larger(m, larger(fabsf(high[i]), fabsf(low[i])));
-    return m;
+  // the largest magnitude, of one dim or of two
+  __device__ __forceinline__ uint32_t magnitude() const {
+    constexpr uint32_t kValue = std::is_same_v<T, float> ? 0x7fffffffu : 0x7fff7fffu;
+    auto larger = [](uint32_t a, uint32_t b) { return q8_larger<T>(a & kValue, b & kValue); };
+    return larger(larger(larger(high.x, low.x), larger(high.y, low.y)), larger(larger(high.z, low.z), larger(high.w, low.w)));
   }
 };
 
-// Turns values into codes (see above).  Tiny pages are lifted, so that 127 / m is finite.
+// Turns 16 bytes of values into codes (see above), of which the lowest byte is looked at.  Two at a time, as the GPU has packed products; 9 q is
+// 8 q + q, and a packed product with a sum behind it, which may be contracted, is one of the first step alone, where that rounds once less.  Tiny pages are
+// lifted, so that 127 / m is finite.
 template <typename T>
 struct Q8Coder {
   float lift, rate;
@@ -97,19 +92,38 @@ struct Q8Coder {
     lift = top < 8.6736174e-19f ? 1.2676506e30f : 1.0f;  // 2^-60, 2^100
     rate = __fdiv_rn(127.0f, top * lift);
   }
-  __device__ __forceinline__ int code(float x) const {
-    const float q = __fmul_rn(x * lift, rate), c = __fmul_rn(q, 9.0f);
-    const float tie = __fsub_rn(c, __fsub_rn(c, q));
-    return __float_as_int(__fadd_rn(tie, 12582912.0f));  // 1.5 * 2^23: the lowest byte is the code
+  __device__ __forceinline__ void codes(const uint4& raw, float sign, int (&code)[8]) const {
+    float x[8];
+    widen16<T>(raw, x);
+    if (lift != 1.0f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= lift;
+    }
+    const uint64_t rates = pair_of(sign * rate, sign * rate), eight = pair_of(8.0f, 8.0f), minus = pair_of(-1.0f, -1.0f);
+    const uint64_t to_whole = pair_of(12582912.0f, 12582912.0f);  // 1.5 * 2^23
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const uint64_t q = mul_pair(pair_of(x[i], x[i + 1]), rates), c = fma_pair(q, eight, q);
+      const uint64_t tie = add_pair(c, fma_pair(c, minus, q));
+      float a, b;
+      halves_of(add_pair(tie, to_whole), a, b);
+      code[i] = __float_as_int(a);
+      code[i + 1] = __float_as_int(b);
+    }
   }
 };
 template <>
 struct Q8Coder<float> {
   double rate;
   __device__ __forceinline__ explicit Q8Coder(float top) { rate = 127.0 / (double)top; }
-  __device__ __forceinline__ int code(float x) const {
-    const double q = __dmul_rn((double)x, rate), c = __dmul_rn(q, 4097.0);
-    return (int)rint(__dsub_rn(c, __dsub_rn(c, q)));
+  __device__ __forceinline__ void codes(const uint4& raw, float sign, int (&code)[4]) const {
+    float x[4];
+    widen16<float>(raw, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double q = __dmul_rn((double)(sign * x[i]), rate), c = __dmul_rn(q, 4097.0);
+      code[i] = (int)rint(__dsub_rn(c, __dsub_rn(c, q)));
+    }
   }
 };
 
@@ -134,8 +148,8 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
   constexpr int kLanes = kVecs < 32 ? kVecs : 32;              // that share a token
   constexpr int kCols = kVecs / kLanes;                        // vectors of a lane and token
   constexpr int kAtOnce = PER * (32 / kLanes);                 // tokens of the item's warps
-  constexpr int kHeld = 16 / kCols;                            // rounds whose values stay in registers
-  __shared__ __align__(16) float s_extremes[PER == 1 ? 1 : 2 * PER * D];
+  constexpr int kHeld = (PER == 1 ? 8 : 16) / kCols;           // rounds whose values stay in registers
+  __shared__ uint4 s_extremes[PER == 1 ? 1 : 2 * PER * kVecs];
   q8_let_next_start();
   q8_wait_for_previous();
   const int lane = threadIdx.x & 31, part = PER == 1 ? 0 : threadIdx.x >> 5;
@@ -188,71 +202,67 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
 #pragma unroll
         for (int c = 0; c < kCols; ++c) seen[c].exchange(mask);
       if constexpr (PER > 1) {
-        float* mine = s_extremes + part * 2 * D + col;
+        uint4* mine = s_extremes + part * 2 * kVecs + lane;
         if (lane < kLanes) {
 #pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-              mine[c * 32 * kN + i] = seen[c].high[i];
-              mine[D + c * 32 * kN + i] = seen[c].low[i];
-            }
+          for (int c = 0; c < kCols; ++c) {
+            mine[c * 32] = seen[c].high;
+            mine[kVecs + c * 32] = seen[c].low;
+          }
         }
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < PER; ++w)
 #pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-              seen[c].high[i] = Q8Extremes<T>::larger(seen[c].high[i], s_extremes[w * 2 * D + col + c * 32 * kN + i]);
-              seen[c].low[i] = Q8Extremes<T>::smaller(seen[c].low[i], s_extremes[w * 2 * D + D + col + c * 32 * kN + i]);
-            }
+          for (int c = 0; c < kCols; ++c) {
+            const uint4* theirs = s_extremes + w * 2 * kVecs + lane % kLanes + c * 32;
+            seen[c].take(theirs[0], theirs[kVecs]);
+          }
       }
-      float top = seen[0].magnitude();
+      uint32_t word = seen[0].magnitude();
 #pragma unroll
-      for (int c = 1; c < kCols; ++c) top = Q8Extremes<T>::larger(top, seen[c].magnitude());
+      for (int c = 1; c < kCols; ++c) word = q8_larger<T>(word, seen[c].magnitude());
 #pragma unroll
-      for (int mask = 1; mask < kLanes; mask *= 2) top = Q8Extremes<T>::larger(top, __shfl_xor_sync(0xffffffffu, top, mask));
+      for (int mask = 1; mask < kLanes; mask *= 2) word = q8_larger<T>(word, __shfl_xor_sync(0xffffffffu, word, mask));
+      float pair[kN];
+      widen16<T>(make_uint4(word, word, word, word), pair);
+      const float top = __uint_as_float(q8_larger<float>(__float_as_uint(pair[0]), __float_as_uint(pair[1])));
       const bool fine = top < INFINITY;  // neither an infinity nor a NaN
       const bool some = fine && top > 0.0f;
       if (lane == 0 && part == 0)
         reinterpret_cast<float*>(page + q8_scale_offset(D, S))[which] = fine ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fc00000);
       const Q8Coder<T> coder(some ? top : 1.0f);
-      auto put = [&](const float (&x)[kN], float sign, uint8_t* to) {
-        int code[kN];
-#pragma unroll
-        for (int i = 0; i < kN; ++i) code[i] = some ? coder.code(sign * x[i]) : 0;
+      auto put = [&](const uint4& raw, float sign, uint8_t* to) {
+        int code[kN] = {};
+        if (some) coder.codes(raw, sign, code);
         q8_store_codes<kN>(to, code);
       };
-      each([&](const Q8Vec<T>& v, int token, int c) {
-        float x[kN];
-        v.values(x);
-        if (token < S) put(x, 1.0f, codes + token * D + c * 32 * kN + col);
+      each([&](const uint4& v, int token, int c) {
+        if (token < S) put(v, 1.0f, codes + token * D + c * 32 * kN + col);
       });
       if (which == 0 && row == 0) {
-        int8_t* bounds = reinterpret_cast<int8_t*>(page + q8_bounds_offset(D, S));
+        uint8_t* bounds = page + q8_bounds_offset(D, S);
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
-          put(seen[c].high, 1.0f, reinterpret_cast<uint8_t*>(bounds) + c * 32 * kN + col);
-          put(seen[c].low, -1.0f, reinterpret_cast<uint8_t*>(bounds) + D + c * 32 * kN + col);
+          put(seen[c].high, 1.0f, bounds + c * 32 * kN + col);
+          put(seen[c].low, -1.0f, bounds + D + c * 32 * kN + col);
         }
       }
     };
     if (rounds <= kHeld) {
-      Q8Vec<T> held[kHeld][kCols];
+      uint4 held[kHeld][kCols];
 #pragma unroll
       for (int r = 0; r < kHeld; ++r)
         if (r < rounds) {
           const T* from = source(min(r * kAtOnce + row, S - 1));
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) held[r][c].load(from + c * 32 * kN + col);
+          for (int c = 0; c < kCols; ++c) held[r][c] = *reinterpret_cast<const uint4*>(from + c * 32 * kN + col);
         }
 #pragma unroll
       for (int r = 0; r < kHeld; ++r)
         if (r < rounds) {
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) seen[c].take(held[r][c]);
+          for (int c = 0; c < kCols; ++c) seen[c].take(held[r][c], held[r][c]);
         }
       finish([&](auto&& one) {
 #pragma unroll
@@ -269,14 +279,10 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
           const int token = r * kAtOnce + row;
           const T* from = source(min(token, S - 1));
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            Q8Vec<T> v;
-            v.load(from + c * 32 * kN + col);
-            one(v, token, c);
-          }
+          for (int c = 0; c < kCols; ++c) one(*reinterpret_cast<const uint4*>(from + c * 32 * kN + col), token, c);
         }
       };
-      walk([&](const Q8Vec<T>& v, int, int c) { seen[c].take(v); });
+      walk([&](const uint4& v, int, int c) { seen[c].take(v, v); });
       finish(walk);
     }
   }
