@@ -351,9 +351,9 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
 template <int THREADS, int kHeld>
 __global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p) {
   constexpr int kWarps = THREADS / 32, kRounds = kHeld == 0 ? 1 : kHeld;
-  __shared__ int histogram[256], s_before[kRounds * kWarps], s_digit, s_left, s_same, s_taken;
-  __shared__ uint32_t s_high[kWarps], s_low[kWarps];
-  __shared__ int s_some[kWarps];
+  __shared__ int histogram[256], s_before[kRounds * kWarps], s_digit, s_left, s_same, s_taken, s_few;
+  __shared__ uint32_t s_high[kWarps], s_low[kWarps], few[32];
+  __shared__ int s_some[kWarps], s_forced[kWarps];
   q8_let_next_start();
   q8_wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -384,42 +384,52 @@ __global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p
   uint32_t least = 0;
   int left = 0;
   if (n > p.count) {
+    // of those that are not taken in any case
     uint32_t high = 0, low = 0xffffffffu;
-    int some = 0;
+    int some = 0, forced = 0;
     each([&](int, uint32_t x) {
-      high = max(high, x);
+      high = max(high, x == kQ8Forced ? 0u : x);
       low = min(low, x - 1u);  // 0 is no candidate
       some += x != 0;
+      forced += x == kQ8Forced;
     });
     high = __reduce_max_sync(0xffffffffu, high);
     low = __reduce_min_sync(0xffffffffu, low);
     some = __reduce_add_sync(0xffffffffu, some);
+    forced = __reduce_add_sync(0xffffffffu, forced);
     if (lane == 0) {
       s_high[warp] = high;
       s_low[warp] = low;
       s_some[warp] = some;
+      s_forced[warp] = forced;
     }
+    if (threadIdx.x == 0) s_few = 0;
     __syncthreads();
-    some = 0;
+    some = forced = 0;
 #pragma unroll
     for (int v = 0; v < kWarps; ++v) {
       high = max(high, s_high[v]);
       low = min(low, s_low[v]);
       some += s_some[v];
+      forced += s_forced[v];
     }
     low += 1u;
-    if (some > p.count) {
+    left = p.count - forced;  // no more than the first and the recent ones: not negative
+    if (some <= p.count) {
+      left = 0;
+    } else if (left == 0) {
+      least = kQ8Forced - 1u;
+    } else {
       // `known`: the bits that all scores share, and further down those of the score that is looked for
       int bits = high == low ? 0 : 32 - __clz(high ^ low);  // still unknown
       uint32_t known = bits == 32 ? 0u : 0xffffffffu << bits;
       least = high & known;
-      left = p.count;
       while (bits > 0) {
         const int width = min(bits, 8), shift = bits - width;
         for (int i = threadIdx.x; i < 256; i += THREADS) histogram[i] = 0;
         __syncthreads();
         each([&](int, uint32_t x) {
-          if (x != 0 && (x & known) == least) atomicAdd(&histogram[(x >> shift) & ((1u << width) - 1u)], 1);
+          if (x != 0 && x != kQ8Forced && (x & known) == least) atomicAdd(&histogram[(x >> shift) & ((1u << width) - 1u)], 1);
         });
         __syncthreads();
         if (threadIdx.x < 32) {  // a lane has eight digits, the largest first
@@ -455,6 +465,24 @@ __global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p
         if (s_same == left && least != 0) {  // all that share these bits are taken
           least -= 1u;
           left = 0;
+          break;
+        }
+        if (bits > 0 && s_same <= 32) {  // the left-th largest of a warp's scores, without more counting
+          each([&](int, uint32_t x) {
+            if (x != 0 && x != kQ8Forced && (x & known) == least) few[atomicAdd(&s_few, 1)] = x;
+          });
+          __syncthreads();
+          const uint32_t mine = lane < s_few ? few[lane] : 0u;
+          int larger = 0, same = 0;
+#pragma unroll
+          for (int v = 0; v < 32; ++v) {
+            const uint32_t other = __shfl_sync(0xffffffffu, mine, v);
+            larger += other > mine;
+            same += other == mine;
+          }
+          const unsigned here = __ballot_sync(0xffffffffu, mine != 0 && larger < left && larger + same >= left);
+          least = __shfl_sync(0xffffffffu, mine, __ffs(here) - 1);
+          left -= __shfl_sync(0xffffffffu, larger, __ffs(here) - 1);
           break;
         }
       }
