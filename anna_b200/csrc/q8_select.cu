@@ -7,8 +7,8 @@
 // u < 256, v < 128), with signed bytes: integer mma, 16 pages to a tile, 8 query heads.
 //
 // Scores: a warp takes 16 pages at a time, for all heads and several tokens.  Bound: HBM (2 D + 4 bytes a page and head), or the launch.
-// Choice: a CTA per query token and KV head finds the score of the last page that is taken, 8 bits at a time from the first bit in which
-// scores differ, counting how many share the bits so far; then the pages above it, and of those equal to it the first, are written in order.
+// Choice: a CTA per query token and KV head finds the score of the last page that is taken, in a 256th of the scores' range at a time, counting how many
+// lie in each, until a warp holds all that are left; then the pages above it, and of those equal to it the first, are written in order.
 #include "q8_common.cuh"
 
 namespace anna {
@@ -405,31 +405,24 @@ __global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p
     }
     if (threadIdx.x == 0) s_few = 0;
     __syncthreads();
-    some = forced = 0;
-#pragma unroll
-    for (int v = 0; v < kWarps; ++v) {
-      high = max(high, s_high[v]);
-      low = min(low, s_low[v]);
-      some += s_some[v];
-      forced += s_forced[v];
-    }
-    low += 1u;
+    high = __reduce_max_sync(0xffffffffu, s_high[lane % kWarps]);
+    low = __reduce_min_sync(0xffffffffu, s_low[lane % kWarps]) + 1u;
+    some = __reduce_add_sync(0xffffffffu, lane < kWarps ? s_some[lane % kWarps] : 0);
+    forced = __reduce_add_sync(0xffffffffu, lane < kWarps ? s_forced[lane % kWarps] : 0);
     left = p.count - forced;  // no more than the first and the recent ones: not negative
     if (some <= p.count) {
       left = 0;
     } else if (left == 0) {
       least = kQ8Forced - 1u;
     } else {
-      // `known`: the bits that all scores share, and further down those of the score that is looked for
-      int bits = high == low ? 0 : 32 - __clz(high ^ low);  // still unknown
-      uint32_t known = bits == 32 ? 0u : 0xffffffffu << bits;
-      least = high & known;
-      while (bits > 0) {
-        const int width = min(bits, 8), shift = bits - width;
+      // the score that is looked for is in low .. low + span, of those there the left-th largest; neither 0 nor kQ8Forced is
+      uint32_t span = high - low;
+      while (span > 0) {
+        const int shift = max(24 - __clz(span), 0);
         for (int i = threadIdx.x; i < 256; i += THREADS) histogram[i] = 0;
         __syncthreads();
         each([&](int, uint32_t x) {
-          if (x != 0 && x != kQ8Forced && (x & known) == least) atomicAdd(&histogram[(x >> shift) & ((1u << width) - 1u)], 1);
+          if (x - low <= span) atomicAdd(&histogram[(x - low) >> shift], 1);
         });
         __syncthreads();
         if (threadIdx.x < 32) {  // a lane has eight digits, the largest first
@@ -458,18 +451,17 @@ __global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p
           }
         }
         __syncthreads();
-        least |= (uint32_t)s_digit << shift;
-        known |= ((1u << width) - 1u) << shift;
+        low += (uint32_t)s_digit << shift;
+        span = min(span - ((uint32_t)s_digit << shift), (1u << shift) - 1u);
         left = s_left;
-        bits = shift;
-        if (s_same == left && least != 0) {  // all that share these bits are taken
-          least -= 1u;
+        if (s_same == left) {  // all of them are taken
+          low -= 1u;
           left = 0;
           break;
         }
-        if (bits > 0 && s_same <= 32) {  // the left-th largest of a warp's scores, without more counting
+        if (span > 0 && s_same <= 32) {  // the left-th largest of a warp's scores, without more counting
           each([&](int, uint32_t x) {
-            if (x != 0 && x != kQ8Forced && (x & known) == least) few[atomicAdd(&s_few, 1)] = x;
+            if (x - low <= span) few[atomicAdd(&s_few, 1)] = x;
           });
           __syncthreads();
           const uint32_t mine = lane < s_few ? few[lane] : 0u;
@@ -481,11 +473,12 @@ __global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p
             same += other == mine;
           }
           const unsigned here = __ballot_sync(0xffffffffu, mine != 0 && larger < left && larger + same >= left);
-          least = __shfl_sync(0xffffffffu, mine, __ffs(here) - 1);
+          low = __shfl_sync(0xffffffffu, mine, __ffs(here) - 1);
           left -= __shfl_sync(0xffffffffu, larger, __ffs(here) - 1);
           break;
         }
       }
+      least = low;
     }
   }
   // ---- in order: scores of a round of a warp, 32 neighbours, are counted by votes --------------------------------------------------------
