@@ -20,8 +20,8 @@
 // Tokens of the unfinished page take the same way as 16-token tiles of the ring: keys times queries in the cache's type, scaled by a power
 // of two, and weights as a sum of two numbers of it.
 //
-// fp32 caches: weights are a sum of two fp16, the second 2^12 times what the first leaves, and all products are added in 32 bits; tokens of the ring
-// are scored and summed on CUDA cores.
+// fp16 and fp32 caches: weights are a sum of two fp16.  fp32 caches: all products are added in 32 bits, and tokens of the ring are scored and summed on
+// CUDA cores.
 #pragma once
 #include "mma_utils.cuh"
 #include "q8_common.cuh"
@@ -138,6 +138,11 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr float kWeight = 16384.0f;                        // of the largest
   constexpr float kRingWeight = kHalf ? kWeight : 1.0f;
+  // Weights of 11 bits are an eighth as coarse as a bf16 output.  Beside an fp16 output they would show (an error of 0.00029 of the whole instead of 0.00021),
+  // so those of fp16 and fp32 caches are sums of two fp16, the second kRest times what the first leaves (16 rows of 0.4-4 K tokens, 64 queries of 256 dims
+  // to a KV head: 58.2 us, 57.3 with one).
+  constexpr bool kTwo = kFloat || kHalf;
+  constexpr float kRest = kFloat ? 4096.0f : 1.0f;
   extern __shared__ __align__(128) uint8_t smem[];
   float* rate = reinterpret_cast<float*>(smem + Cfg::kOffRate);
   float* ring_rate = reinterpret_cast<float*>(smem + Cfg::kOffRingRate);
@@ -333,9 +338,10 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float base = m_run[j][k] == -INFINITY ? 0.0f : m_run[j][k] - 14.0f;  // log2 of kWeight
-        s[j][k] = q8_exp2(s[j][k] - base);
-        s[j][k + 2] = q8_exp2(s[j][k + 2] - base);
+        // log2 of kWeight; a difference near 14 is off by 2^-21, so fp32 caches multiply
+        const float base = m_run[j][k] == -INFINITY ? 0.0f : m_run[j][k] - (kFloat ? 0.0f : 14.0f);
+        s[j][k] = q8_exp2(s[j][k] - base) * (kFloat ? kWeight : 1.0f);
+        s[j][k + 2] = q8_exp2(s[j][k + 2] - base) * (kFloat ? kWeight : 1.0f);
         l_run[j][k] += s[j][k] + s[j][k + 2];
       }
   };
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
       share[h] = scale[h].y * __uint_as_float((uint32_t)(127 - unit) << 23);
       near = near && share[h] <= 1.0f && (share[h] >= 1.0f / 64.0f || share[h] == 0.0f);
     }
-    uint32_t w[NT][2], rest[kFloat ? NT : 1][2];
+    uint32_t w[NT][2], rest[kTwo ? NT : 1][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -428,9 +434,9 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
         const float f = near ? share[k * (kPages - 1)] : 1.0f;
         const uint32_t most = pack2<__half>(s[j][2 * k] * f, s[j][2 * k + 1] * f);
         w[j][k] = movmatrix_trans(most);
-        if constexpr (kFloat) {
+        if constexpr (kTwo) {
           const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&most));
-          rest[j][k] = movmatrix_trans(pack2<__half>((s[j][2 * k] - x.x) * 4096.0f, (s[j][2 * k + 1] - x.y) * 4096.0f));
+          rest[j][k] = movmatrix_trans(pack2<__half>(fmaf(s[j][2 * k], f, -x.x) * kRest, fmaf(s[j][2 * k + 1], f, -x.y) * kRest));
         }
       }
     uint32_t val[4][Cfg::kVWords];
@@ -461,7 +467,10 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
       }
     };
     if (near) {
-      sums([&](int j, float (&sum)[4], const uint32_t (&a)[4]) { mma_m16n8k16<__half>(sum, a, w[j][0], w[j][1]); });
+      sums([&](int j, float (&sum)[4], const uint32_t (&a)[4]) {
+        mma_m16n8k16<__half>(sum, a, w[j][0], w[j][1]);
+        if constexpr (kTwo) mma_m16n8k16<__half>(sum, a, rest[j][0], rest[j][1]);
+      });
     } else {  // a scale far below the largest, or NaN, or an fp32 cache
       float by[kPages][NT][2];
 #pragma unroll
@@ -477,10 +486,10 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
           q8_mma_first(part, a, kHalves && h == 1 ? 0u : w[j][0], kHalves && h == 0 ? 0u : w[j][1]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) sum[r] = fmaf(part[r], by[h][j][r & 1], sum[r]);
-          if constexpr (kFloat) {
+          if constexpr (kTwo) {
             q8_mma_first(part, a, kHalves && h == 1 ? 0u : rest[j][0], kHalves && h == 0 ? 0u : rest[j][1]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum[r] = fmaf(part[r], by[h][j][r & 1] * (1.0f / 4096.0f), sum[r]);
+            for (int r = 0; r < 4; ++r) sum[r] = fmaf(part[r], by[h][j][r & 1] * (1.0f / kRest), sum[r]);
           }
         }
       });
@@ -528,7 +537,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float4 q = raw[(8 * j + (r & 1)) * (D / 4) + d];
-              s[j][r] = fmaf(k[r / 2].w, q.w, fmaf(k[r / 2].z, q.z, fmaf(k[r / 2].y, q.y, fmaf(k[r / 2].x, q.x, s[j][r]))));
+              s[j][r] += fmaf(k[r / 2].w, q.w, fmaf(k[r / 2].z, q.z, fmaf(k[r / 2].y, q.y, k[r / 2].x * q.x)));  // a quarter of the roundings of one chain
             }
         }
       } else {

@@ -129,10 +129,10 @@ def attention_bound(out: torch.Tensor, dtype: torch.dtype, dim: int, reach: floa
 
     A score is a sum of `dim` products in 32 bits (queries of 16-bit caches are exact, or off by 2^-25 of the largest): off by
     (dim + 3) 2^-24 of the sum of magnitudes, and what a softmax makes of scores that are off by s is off by 2 s of the largest value.  exp2 and
-    the sums behind it: 2^-20.  16-bit caches weigh values with weights in fp16, each off by half a step, 2^-11.  The output is rounded to its
-    type, half a step again."""
+    the sums behind it: 2^-20.  bf16 caches weigh values with weights in fp16, each off by half a step, 2^-11; others with sums of two.  The
+    output is rounded to its type, half a step again."""
     weights = 2.0 * (dim + 3) * 2.0 ** -24 * reach + 2.0 ** -20
-    if dtype != torch.float32:
+    if dtype == torch.bfloat16:
         weights += 2.0 ** -11
     return most * weights + torch.finfo(dtype).eps / 2 * out.abs() + torch.finfo(dtype).smallest_normal
 
