@@ -4,8 +4,9 @@
 // Keys and values are the first operand of mma.sync (S^T = K Q^T with 16 tokens as rows, O^T = V^T P^T with 16 dims as rows), the queries that
 // share a KV head its eight columns (NT times eight of a CTA).
 //
-// Scores: codes go into the integer product as they are.  A query is a whole number of 24 bits, 2^22 to 2^23 for its head's largest
-// magnitude: three bytes, three products, whose sums are exact; what is not is the last bit of a query, 2^-24 of its largest magnitude.
+// Scores: codes go into the integer product as they are.  A query is a whole number of 24 bits, -2^23 to 2^23 - 1, with 2^22 and more for its head's
+// largest magnitude: three bytes, the first signed, three products, whose sums are exact.  What is not is a query: its entries are off by half a unit,
+// 2^-23 of the head's largest magnitude at most.
 // Sums: a code with its top bit flipped, as the low byte of an fp16 of exponent 1024, reads as 1152 + code, and taking 1152 off is exact.  Weights
 // are 2^14 times exp2 of the score below the running maximum, rounded to fp16: all down to 2^-28 of the largest have 11 bits.  The scale of a
 // page's values goes into its weights where it is within 2^6 of the largest so far; where it is smaller, the tile's product is added to the sums
@@ -274,7 +275,8 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
     T scaled[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const int whole = fine ? __float2int_rn(x[j] * factor * 4194304.0f) : 0;
+      // the top byte is signed, so what rounds up to 2^23 (fp32: 2^k less its last bit) stays half a unit below, as far off as any tie
+      const int whole = fine ? min(__float2int_rn(x[j] * factor * 4194304.0f), 8388607) : 0;
 #pragma unroll
       for (int n = 0; n < 3; ++n) bytes[n][j / 4] |= ((uint32_t)whole >> (16 - 8 * n) & 255u) << (8 * (j % 4));
       scaled[j] = ElemTraits<T>::from_float(x[j] * factor * kRingFactor);
