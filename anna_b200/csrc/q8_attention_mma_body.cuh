@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
     for (int h = 0; h < kPages; ++h)
       if (x.position[h] != kFar) {
         const int slot = p.block_shift >= 0 ? x.position[h] & (p.block_size - 1) : x.position[h] % p.block_size;
-        x.scale[h] = __ldg(reinterpret_cast<const float2*>(x.keys[h] + (int64_t)(2 * p.block_size - slot) * D));
+        x.scale[h] = *reinterpret_cast<const float2*>(x.keys[h] + (int64_t)(2 * p.block_size - slot) * D);
       }
   };
   const int values_at = p.block_size * D;

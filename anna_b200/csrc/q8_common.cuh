@@ -147,6 +147,9 @@ __device__ __forceinline__ void q8_for_each_segment(const Q8Params& p, int row_t
 // start while the kernel in front of them ends, and touch no memory before that has ended and its writes are there.  A kernel of more than two CTAs per
 // SM lets the next one start at its end alone: CTAs that wait beside it cost more than that saves (a prompt of 3001 tokens appended and viewed 16.4 us,
 // 11.7 so; a selection of one row 18.5 us without an early start, 17.6 with it).
+//
+// So a kernel is on the GPU while the one in front of it still writes pages, and pages change their contents between two kernels on one SM: what is read of the
+// pool goes by coherent loads alone (__ldg and ld.global.nc are for memory that stays as it is while the kernel lives).
 __device__ __forceinline__ void q8_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void q8_let_next_start() {
   if (gridDim.x * gridDim.y * gridDim.z <= 2 * 148) asm volatile("griddepcontrol.launch_dependents;");

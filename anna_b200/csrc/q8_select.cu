@@ -55,10 +55,11 @@ __device__ __forceinline__ void mma_s8u8(int (&d)[4], uint32_t a0, uint32_t a1, 
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes that are read once; half lines are fetched from memory, as bounds end a little way into a line (320 bytes a page of 128 dims instead of 384).
-__device__ __forceinline__ uint4 q8_ldg64(const uint4* ptr) {
+// 16 bytes that are read once, coherently (see q8_wait_for_previous); half lines are fetched from memory, as bounds end a little way into a line (320 bytes a
+// page of 128 dims instead of 384).  (Past L1, as ld.global.cg: 32 rows of 20000 to 32768 tokens and the attention behind it 85.7 us, 80.2 so.)
+__device__ __forceinline__ uint4 q8_load64(const uint4* ptr) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::64B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
+  asm volatile("ld.global.L1::no_allocate.L2::64B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
   return v;
 }
 // Order of floats as order of whole numbers, none of them 0.
@@ -147,10 +148,10 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
     for (int i = 0; i < 2; ++i) {
       there[i] = ids[i] >= 0 && ids[i] < p.num_pages;
       const uint8_t* page = p.pages + (there[i] ? ((int64_t)ids[i] * p.kv_heads + heads0 + h) * p.page_bytes : 0);
-      scale[i] = __ldg(reinterpret_cast<const float*>(page + q8_scale_offset(D, p.block_size)));
+      scale[i] = *reinterpret_cast<const float*>(page + q8_scale_offset(D, p.block_size));
       const uint4* bounds = reinterpret_cast<const uint4*>(page + q8_bounds_offset(D, p.block_size));
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) w[i][c] = q8_ldg64(bounds + 4 * c + tig);
+      for (int c = 0; c < kChunks; ++c) w[i][c] = q8_load64(bounds + 4 * c + tig);
     }
   };
   auto next_tile = [&] { return tile + tile_step + (head + head_step >= heads ? 1 : 0); };
