@@ -8,7 +8,7 @@
 // largest magnitude: three bytes, the first signed, three products, whose sums are exact.  What is not is a query: its entries are off by half a unit,
 // 2^-23 of the head's largest magnitude at most.
 // Sums: a code with its top bit flipped, as the low byte of an fp16 of exponent 1024, reads as 1152 + code, and taking 1152 off is exact.  Weights
-// are 2^14 times exp2 of the score below the running maximum, rounded to fp16: all down to 2^-28 of the largest have 11 bits.  The scale of a
+// are 2^14 times exp2 of the score below the running maximum, as sums of two fp16: all down to 2^-28 of the largest have 11 bits and more.  The scale of a
 // page's values goes into its weights where it is within 2^6 of the largest so far; where it is smaller, the tile's product is added to the sums
 // in 32 bits, times the scale, so pages of any scales may meet.  (The product of each tile added in 32 bits, with codes as fp16 subnormals, which
 // are one operation a pair instead of two: 16 rows of 32768 tokens, 4 queries a KV head, take 204 us both ways; four tokens each 293 us, 280 so.)
@@ -21,7 +21,7 @@
 // Tokens of the unfinished page take the same way as 16-token tiles of the ring: keys times queries in the cache's type, scaled by a power
 // of two, and weights as a sum of two numbers of it.
 //
-// fp16 and fp32 caches: weights are a sum of two fp16.  fp32 caches: all products are added in 32 bits, and tokens of the ring are scored and summed on
+// fp32 caches: all products are added in 32 bits, and tokens of the ring are scored and summed on
 // CUDA cores.
 #pragma once
 #include "mma_utils.cuh"
@@ -139,10 +139,9 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr float kWeight = 16384.0f;                        // of the largest
   constexpr float kRingWeight = kHalf ? kWeight : 1.0f;
-  // Weights of 11 bits are an eighth as coarse as a bf16 output.  Beside an fp16 output they would show (an error of 0.00029 of the whole instead of 0.00021),
-  // so those of fp16 and fp32 caches are sums of two fp16, the second kRest times what the first leaves (16 rows of 0.4-4 K tokens, 64 queries of 256 dims
-  // to a KV head: 58.2 us, 57.3 with one).
-  constexpr bool kTwo = kFloat || kHalf;
+  // One fp16 of 11 bits would show in an output, of fp16 (an error of 0.00029 of the whole instead of 0.00021) and of bf16 (0.00168 instead of 0.00166), so
+  // weights are sums of two, the second kRest times what the first leaves (16 rows of 32768 tokens, 4 queries a KV head: 174 us with one, 186 so; of four tokens
+  // 260 and 292).
   constexpr float kRest = kFloat ? 4096.0f : 1.0f;
   extern __shared__ __align__(128) uint8_t smem[];
   float* rate = reinterpret_cast<float*>(smem + Cfg::kOffRate);
@@ -428,7 +427,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
       share[h] = scale[h].y * __uint_as_float((uint32_t)(127 - unit) << 23);
       near = near && share[h] <= 1.0f && (share[h] >= 1.0f / 64.0f || share[h] == 0.0f);
     }
-    uint32_t w[NT][2], rest[kTwo ? NT : 1][2];
+    uint32_t w[NT][2], rest[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -436,10 +435,8 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
         const float f = near ? share[k * (kPages - 1)] : 1.0f;
         const uint32_t most = pack2<__half>(s[j][2 * k] * f, s[j][2 * k + 1] * f);
         w[j][k] = movmatrix_trans(most);
-        if constexpr (kTwo) {
-          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&most));
-          rest[j][k] = movmatrix_trans(pack2<__half>(fmaf(s[j][2 * k], f, -x.x) * kRest, fmaf(s[j][2 * k + 1], f, -x.y) * kRest));
-        }
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&most));
+        rest[j][k] = movmatrix_trans(pack2<__half>(fmaf(s[j][2 * k], f, -x.x) * kRest, fmaf(s[j][2 * k + 1], f, -x.y) * kRest));
       }
     uint32_t val[4][Cfg::kVWords];
 #pragma unroll
@@ -471,7 +468,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
     if (near) {
       sums([&](int j, float (&sum)[4], const uint32_t (&a)[4]) {
         mma_m16n8k16<__half>(sum, a, w[j][0], w[j][1]);
-        if constexpr (kTwo) mma_m16n8k16<__half>(sum, a, rest[j][0], rest[j][1]);
+        mma_m16n8k16<__half>(sum, a, rest[j][0], rest[j][1]);
       });
     } else {  // a scale far below the largest, or NaN, or an fp32 cache
       float by[kPages][NT][2];
@@ -488,11 +485,9 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
           q8_mma_first(part, a, kHalves && h == 1 ? 0u : w[j][0], kHalves && h == 0 ? 0u : w[j][1]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) sum[r] = fmaf(part[r], by[h][j][r & 1], sum[r]);
-          if constexpr (kTwo) {
-            q8_mma_first(part, a, kHalves && h == 1 ? 0u : rest[j][0], kHalves && h == 0 ? 0u : rest[j][1]);
+          q8_mma_first(part, a, kHalves && h == 1 ? 0u : rest[j][0], kHalves && h == 0 ? 0u : rest[j][1]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum[r] = fmaf(part[r], by[h][j][r & 1] * (1.0f / kRest), sum[r]);
-          }
+          for (int r = 0; r < 4; ++r) sum[r] = fmaf(part[r], by[h][j][r & 1] * (1.0f / kRest), sum[r]);
         }
       });
     }

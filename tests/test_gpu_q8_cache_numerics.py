@@ -4,7 +4,9 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_q8_cache import FP32, check_attention, filled
+import anna_b200
+from q8_reference import Cache, attention
+from test_gpu_q8_cache import BF16, FP16, FP32, check_attention, filled
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +27,26 @@ def test_fp32_queries_just_below_a_power_of_two(cuda_device, dim, page, group, t
         check_attention(cache, gpu, query, cuda_device, scaling=0.3 / power)
         blocks = torch.randint(0, 7, (3, 2, tokens, 3), generator=cache.gen).int()
         check_attention(cache, gpu, query, cuda_device, blocks=blocks, scaling=0.3 / power)
+
+
+@pytest.mark.parametrize("dim,page,group,tokens", [(64, 16, 1, 1), (128, 16, 4, 1), (128, 24, 2, 2), (256, 32, 8, 2), (128, 16, 8, 4), (128, 5, 2, 1)])
+@pytest.mark.parametrize("ring", [0, 3])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_weights_of_16_bit_caches_leave_the_rounding_to_the_output(cuda_device, dtype, dim, page, group, tokens, ring):
+    """Values that nearly cancel, so that an output shows what its weights are off by."""
+    lengths = [4 * page + ring, page + ring]
+    cache = Cache(2, 2, dim, page, dtype, 5, seed=dim + ring)
+    key, value = cache.new_tokens(max(lengths), spread=0.05)
+    value = torch.where(torch.arange(max(lengths))[:, None] % 2 == 0, 1.0, -1.0) * (1.0 + value.float().abs())
+    for b, n in enumerate(lengths):
+        cache.append(key[:, :, :n], value[:, :, :n].to(dtype), rows=[b])
+    gpu = cache.on(cuda_device)
+    query = torch.randn((2, 2 * group, tokens, dim), generator=cache.gen).to(dtype)
+    scaling = dim ** -0.5
+    out = anna_b200.run_q8_paged_attention(query=query.to(cuda_device), lengths=cache.lengths.to(cuda_device), scaling=scaling, **gpu).cpu().double()
+    want, reach, most = attention(query, [cache.dense(b) for b in range(2)], scaling)
+    # as for fp32 caches (scores and sums in 32 bits), but a weight is a sum of two fp16, for tokens of the ring of two numbers of the type: off by
+    # half a step of the second, 2^-11 of at most 2^-11 of it (bf16: 2^-8 of 2^-8)
+    share = 2.0 ** -22 if dtype == FP16 or ring == 0 else 2.0 ** -16
+    bound = most * (2.0 * (dim + 3) * 2.0 ** -24 * reach + 2.0 ** -20 + share) + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal
+    assert bool(((out - want).abs() <= bound).all()), float(((out - want).abs() / bound).max())
