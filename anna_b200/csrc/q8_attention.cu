@@ -150,10 +150,13 @@ __global__ void __launch_bounds__(kQ8Threads<D>) q8_attention_kernel(const Q8Par
     for (int r = 0; r < kOutRows; ++r) acc[r] *= sm_rescale[out_row0 + r];
     for (int i = 0; i < n; ++i) {
       const float v = vals[i * D + place];
+      if (fabsf(v) < INFINITY) {
 #pragma unroll
-      for (int r = 0; r < kOutRows; ++r) {
-        const float w = weight[(out_row0 + r) * kQ8Tokens + i];
-        if (w != 0.0f) acc[r] = fmaf(w, v, acc[r]);  // a value that the row does not see may be infinite or NaN
+        for (int r = 0; r < kOutRows; ++r) acc[r] = fmaf(weight[(out_row0 + r) * kQ8Tokens + i], v, acc[r]);
+      } else {  // infinite or NaN: for the rows that see it, however small its weight
+#pragma unroll
+        for (int r = 0; r < kOutRows; ++r)
+          if (sm_position[i] <= first_seen + multi_token_of(p, row0 + out_row0 + r)) acc[r] += v;
       }
     }
     base = stop;

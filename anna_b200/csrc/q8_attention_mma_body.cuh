@@ -561,6 +561,8 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
           s[j][r] = token >= valid || position + token > limit(j, r & 1) ? -INFINITY : s[j][r] * ring_rate[8 * j + 2 * tig + (r & 1)];
         }
       softmax(s);
+      // Infinite and NaN values are left out of the sums, as they must not meet a weight of 0: of a row that does not see them, of a rest.
+      bool strange = false;
       if constexpr (kFloat) {
         for (int token = 0; token < valid; ++token) {
           float weight[NT][2];
@@ -573,14 +575,17 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
 #pragma unroll
           for (int d = 0; d < D / 32; ++d) {
             const float4 got = value[d];
-            const float v[4] = {got.x, got.y, got.z, got.w};
+            float v[4] = {got.x, got.y, got.z, got.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+              const bool fine = fabsf(v[i]) < INFINITY;
+              strange = strange || !fine;
+              v[i] = fine ? v[i] : 0.0f;
 #pragma unroll
               for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int k = 0; k < 2; ++k)  // a value that the row does not see may be infinite or NaN
-                  if (weight[j][k] != 0.0f) o[j][2 * d + i / 2][2 * (i & 1) + k] = fmaf(weight[j][k], v[i], o[j][2 * d + i / 2][2 * (i & 1) + k]);
+                for (int k = 0; k < 2; ++k) o[j][2 * d + i / 2][2 * (i & 1) + k] = fmaf(weight[j][k], v[i], o[j][2 * d + i / 2][2 * (i & 1) + k]);
+            }
           }
         }
       } else {
@@ -596,7 +601,6 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
           w[j][k] = movmatrix_trans(most);
           rest[j][k] = movmatrix_trans(pack2<T>(x - ElemTraits<T>::to_float(parts[0]), y - ElemTraits<T>::to_float(parts[1])));
         }
-      bool strange = false;
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {  // 8 of a lane's dims
         uint32_t x[4][4];
@@ -606,7 +610,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
           const uint4 got = token < valid ? *reinterpret_cast<const uint4*>(values + row_of(token) + gid * (D / 8) + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
           x[k][0] = got.x; x[k][1] = got.y; x[k][2] = got.z; x[k][3] = got.w;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {  // an infinite or NaN value must not meet a weight of 0: of a row that does not see it, of a rest
+          for (int v = 0; v < 4; ++v) {
             const uint32_t fine = q8_finite_halves<T>(x[k][v]);
             strange = strange || fine != 0xffffffffu;
             x[k][v] &= fine;
@@ -623,7 +627,8 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
           }
         }
       }
-      if (__any_sync(0xffffffffu, strange)) {  // what was left out, for the rows that see it
+      }
+      if (__any_sync(0xffffffffu, strange)) {  // what was left out, for the rows that see it, however small its weight
         for (int token = 0; token < valid; ++token) {
           const T* value = values + row_of(token) + gid * (D / 8);
 #pragma unroll
@@ -637,7 +642,6 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
                 if (position + token <= limit(j, k)) o[j][d / 2][2 * (d & 1) + k] += x;
           }
         }
-      }
       }
     }
   }

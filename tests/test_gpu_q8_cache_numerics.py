@@ -1,6 +1,8 @@
 """Attention over the 8-bit paged cache where its numbers come close to the ends of their formats, against a restatement in 64 bits."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -50,3 +52,31 @@ def test_weights_of_16_bit_caches_leave_the_rounding_to_the_output(cuda_device, 
     share = 2.0 ** -22 if dtype == FP16 or ring == 0 else 2.0 ** -16
     bound = most * (2.0 * (dim + 3) * 2.0 ** -24 * reach + 2.0 ** -20 + share) + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal
     assert bool(((out - want).abs() <= bound).all()), float(((out - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("page,pages,copies", [(16, 4, 1), (24, 4, 1), (5, 4, 1), (16, 4, 9), (16, 130, 1), (5, 300, 1)])
+def test_what_a_query_sees_shows_however_small_its_weight(cuda_device, dtype, page, pages, copies):
+    """A NaN among the values of a page or of the ring, and an infinity there, under a key that takes all weight."""
+    dim, extra = 64, 3
+    n = page * pages + extra
+    cache = Cache(4, 1, dim, page, dtype, pages)
+    key, value = cache.new_tokens(n, spread=0.1)
+    key[:, 0, :, 0] = 0.0
+    key[:, 0, n - 1, 0] = 100.0  # a score of 1000
+    value[0, 0, 2, 7] = math.nan       # in the first page: all of its values are NaN
+    value[1, 0, n - 2, 7] = math.nan   # in the ring
+    value[2, 0, n - 2, 9] = -math.inf
+    cache.append(key, value)
+    gpu = cache.on(cuda_device)
+    query = torch.zeros((4, 2 * copies, 1, dim), dtype=dtype)
+    query[..., 0] = 10.0
+    out = anna_b200.run_q8_paged_attention(query=query.to(cuda_device), lengths=cache.lengths.to(cuda_device), scaling=1.0, **gpu).cpu()
+    assert bool(torch.isnan(out[0]).all())
+    assert bool(torch.isnan(out[1, ..., 7]).all()) and bool(torch.isfinite(out[1, ..., torch.arange(dim) != 7]).all())
+    assert not bool(torch.isfinite(out[2, ..., 9]).any()) and bool(torch.isfinite(out[2, ..., torch.arange(dim) != 9]).all())
+    assert torch.equal(out[3], value[3, :, n - 1:].expand(2 * copies, 1, dim))
+    # the same tokens behind the queries' own are not seen
+    query = torch.cat((query, query), dim=2)
+    out = anna_b200.run_q8_paged_attention(query=query.to(cuda_device), lengths=(cache.lengths - 1).to(cuda_device), scaling=1.0, **gpu).cpu()
+    assert bool(torch.isfinite(out[1:3, :, 0]).all()) and not bool(torch.isfinite(out[1, :, 1, 7]).any()) and not bool(torch.isfinite(out[2, :, 1, 9]).any())
