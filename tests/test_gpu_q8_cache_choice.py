@@ -7,7 +7,7 @@ import torch
 
 import anna_b200
 from q8_reference import Cache
-from test_gpu_q8_cache import BF16
+from test_gpu_q8_cache import BF16, FP16, FP32
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,59 @@ def test_choice_at_every_width(cuda_device, columns, spread):
             for h in range(heads):
                 score = scores[b][h][table[b, :lengths[b] // page].numpy()]
                 assert got[b, h, 0].tolist() == best(score, count, first, recent), (count, b, h)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 4), (256, 2)])
+def test_the_page_of_the_largest_product_is_chosen(cuda_device, dtype, dim, group):
+    """Pages as the append writes them: their bounds hold for all of their keys, and a page with a key whose product no other page's bound reaches is the
+    first that is chosen."""
+    page, blocks = 16, 40
+    cache = Cache(1, 1, dim, page, dtype, blocks, seed=dim)
+    gpu = cache.on(cuda_device)
+    key, value = cache.new_tokens(page * blocks)
+    query = torch.randn((1, group, blocks, dim), generator=cache.gen).to(dtype)
+    targets = torch.randperm(blocks, generator=cache.gen)[:8].tolist()
+    for i, j in enumerate(targets):  # the key that query i looks for
+        key[0, 0, j * page + i] = 6.0 * query[0, i % group, i]
+    anna_b200.run_q8_append(key=key.to(cuda_device), value=value.to(cuda_device), past_lengths=torch.zeros(1, dtype=torch.long, device=cuda_device), **gpu)
+    size = 2 * page * dim
+    rows = gpu["packed_pages"].cpu()[cache.table[0].long(), 0]
+    codes = rows[:, :page * dim].contiguous().view(torch.int8).view(blocks, page, dim).double()
+    scale = rows[:, size:size + 4].contiguous().view(torch.float32).double()  # [blocks, 1]
+    bounds = rows[:, size + 16:size + 16 + 2 * dim].contiguous().view(torch.int8).view(blocks, 2, dim).double()
+    assert torch.equal(bounds[:, 0], codes.amax(1)) and torch.equal(bounds[:, 1], (-codes).amax(1))
+    for i, j in enumerate(targets):
+        q = query[0, :, i].double()
+        product = torch.einsum("gd,bsd->gbs", q, codes).amax(2) * scale.T
+        reach = (q.clamp_min(0) @ bounds[:, 0].T + (-q).clamp_min(0) @ bounds[:, 1].T) * scale.T  # [group, blocks]
+        assert bool((product <= reach).all())
+        others = reach.amax(0)
+        others[j] = -1.0
+        # queries in whole numbers are off by half of 1 / 32767 of the largest entry
+        assert float(product[:, j].max()) > 1.01 * float(others.max())
+        got = anna_b200.run_q8_select_blocks(query=query[:, :, i:i + 1].to(cuda_device), packed_pages=gpu["packed_pages"], page_table=gpu["page_table"],
+                                             lengths=torch.tensor([page * blocks], device=cuda_device), block_size=page, count=1, first=0, recent=0)
+        assert got.flatten().tolist() == [j]
+
+
+def test_an_append_writes_the_pages_that_are_there_and_no_others(cuda_device):
+    """Rows whose block has no column in the table, that have a negative length, and one that fills its second page."""
+    cache = Cache(3, 1, 64, 16, FP16, 2)
+    key, value = cache.new_tokens(31)
+    cache.append(key, value, rows=[2])
+    gpu = cache.on(cuda_device)
+    before = {k: v.clone() for k, v in gpu.items()}
+    key, value = cache.new_tokens(1)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    anna_b200.run_q8_append(key=key.to(cuda_device), value=value.to(cuda_device), past_lengths=torch.tensor([47, -5, 31], device=cuda_device), status=status,
+                            **gpu)
+    assert status.item() == 1  # of row 0
+    cache.append(key, value, rows=[2])
+    page = int(cache.table[2, 1])
+    changed = (gpu["packed_pages"] != before["packed_pages"]).flatten(1).any(1).cpu()
+    assert changed.nonzero().flatten().tolist() == [page]
+    known = cache.known_bytes()
+    assert torch.equal(gpu["packed_pages"].cpu()[page][:, known], cache.pages[page][:, known])
+    # row 0 closes a page that is none and row 2 one that is: neither leaves a token in its ring; row 1 is left out
+    assert torch.equal(gpu["window"].cpu().view(torch.uint8), before["window"].cpu().view(torch.uint8))
