@@ -8,10 +8,11 @@
 // largest magnitude: three bytes, the first signed, three products, whose sums are exact.  What is not is a query: its entries are off by half a unit,
 // 2^-23 of the head's largest magnitude at most.
 // Sums: a code with its top bit flipped, as the low byte of an fp16 of exponent 1024, reads as 1152 + code, and taking 1152 off is exact.  Weights
-// are 2^14 times exp2 of the score below the running maximum, as sums of two fp16: all down to 2^-28 of the largest have 11 bits and more.  The scale of a
-// page's values goes into its weights where it is within 2^6 of the largest so far; where it is smaller, the tile's product is added to the sums
-// in 32 bits, times the scale, so pages of any scales may meet.  (The product of each tile added in 32 bits, with codes as fp16 subnormals, which
-// are one operation a pair instead of two: 16 rows of 32768 tokens, 4 queries a KV head, take 204 us both ways; four tokens each 293 us, 280 so.)
+// are 2^14 times exp2 of the score below the running maximum, as sums of two fp16.  The scale of a page's values goes into its weights where it is within
+// 2^6 of the power of two above the largest so far, as a share of that power; where it is smaller, the tile's product is added to the sums in 32 bits,
+// times the scale, so pages of any scales may meet.  A weight, times its share where it has one, is off by 2^-23 of itself (half a step of the second fp16),
+// but where the largest weight is 2^14 by no less than half a step of subnormals, 2^-25: a weight whose share is 1 keeps 2^-23 down to 2^-16 of the
+// largest and 2^-11 down to 2^-28, one whose share is 1/64 down to 2^-10 and 2^-22.
 //
 // The order of dims and tokens inside a product is free, so a lane's share of a tile is 16-byte pieces of rows.  A warp copies its own tiles,
 // 16 bytes a lane and instruction, into a ring of its own; pieces are swizzled so that the reads of a tile are free of bank conflicts.
@@ -21,8 +22,7 @@
 // Tokens of the unfinished page take the same way as 16-token tiles of the ring: keys times queries in the cache's type, scaled by a power
 // of two, and weights as a sum of two numbers of it.
 //
-// fp32 caches: all products are added in 32 bits, and tokens of the ring are scored and summed on
-// CUDA cores.
+// fp32 caches: all products are added in 32 bits, and tokens of the ring are scored and summed on CUDA cores.
 #pragma once
 #include "mma_utils.cuh"
 #include "q8_common.cuh"

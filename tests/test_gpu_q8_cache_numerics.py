@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import anna_b200
-from q8_reference import Cache, attention
+from q8_reference import Cache, attention, quantized
 from test_gpu_q8_cache import BF16, FP16, FP32, check_attention, filled
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +80,43 @@ def test_what_a_query_sees_shows_however_small_its_weight(cuda_device, dtype, pa
     query = torch.cat((query, query), dim=2)
     out = anna_b200.run_q8_paged_attention(query=query.to(cuda_device), lengths=(cache.lengths - 1).to(cuda_device), scaling=1.0, **gpu).cpu()
     assert bool(torch.isfinite(out[1:3, :, 0]).all()) and not bool(torch.isfinite(out[1, :, 1, 7]).any()) and not bool(torch.isfinite(out[2, :, 1, 9]).any())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("ratio", [63.0, 65.0])
+@pytest.mark.parametrize("copies", [1, 10])
+def test_small_weights_of_pages_with_small_scales(cuda_device, dtype, ratio, copies):
+    """A page with much larger values, of which a query sees a key that takes nearly all weight and has no value; what pages with scales just within and just
+    past 2^6 of it add, at weights of 2^-20 to 2^-30."""
+    page, dim, blocks = 16, 128, 40
+    cache = Cache(2, 1, dim, page, dtype, blocks)
+    key, value = cache.new_tokens(page * blocks)
+    query = torch.zeros((2, 4, 1, dim), dtype=dtype)
+    query[..., 0] = 1.0
+    scaling = math.log(2.0)
+    key *= 0.25
+    key[..., 0] = torch.randint(-30, -19, key.shape[:3], generator=cache.gen).to(dtype)  # log2 of a weight
+    value[:, :, page:] = 512.0 * value[:, :, page:].clamp(-1.0, 1.0)
+    value[:, :, page::page, 0] = 512.0       # the scale is 512 / 127
+    value[:, :, :page] *= 0.0
+    value[:, :, 1, 0] = 512.0 * ratio        # a large value at a small weight
+    key[:, :, :page, 0] = -30.0
+    key[:, :, 5, 0] = 0.0
+    cache.append(key, value)
+    gpu = cache.on(cuda_device)
+    rows = [cache.dense(b) for b in range(2)]
+    wide = query.repeat_interleave(copies, dim=1)
+    out = anna_b200.run_q8_paged_attention(query=wide.to(cuda_device), lengths=cache.lengths.to(cuda_device), scaling=scaling, **gpu).cpu().double()
+    for b in range(2):
+        score = torch.einsum("hd,nd->hn", query[b, :, 0].double(), rows[b][0, 0]) * scaling
+        weight = torch.softmax(score, dim=-1)
+        want = (weight @ rows[b][1, 0]).repeat_interleave(copies, dim=0)
+        reach = float(score.abs().max())
+        share = (2.0 * (dim + 3) * 2.0 ** -24 * reach + 2.0 ** -20 + 2.0 ** -22) * (weight @ rows[b][1, 0].abs())
+        # A weight, times the scale of its page in units of at most twice the largest scale, is rounded to a multiple of 2^-24, of which the largest weight has
+        # 2^14 or more: it loses 2^-39 of that at most, and is there for a code.
+        codes = torch.cat([quantized(cache.tokens[b][1, :, j * page:(j + 1) * page])[0][0] for j in range(blocks)]).double()
+        scale = torch.cat([quantized(cache.tokens[b][1, :, j * page:(j + 1) * page])[1] for j in range(blocks)]).double()
+        lost = 2.0 ** -39 * weight.amax() * 2.0 * scale.max() * codes.abs().sum(0)
+        bound = (share + lost).repeat_interleave(copies, dim=0) + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert bool(((out[b, :, 0] - want).abs() <= bound).all()), (b, float(((out[b, :, 0] - want).abs() / bound).max()))
