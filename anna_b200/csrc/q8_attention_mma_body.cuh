@@ -245,8 +245,12 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
 #pragma unroll
   for (int k = 0; k < kMyRows; ++k) {
     const int i = warp + k * Cfg::kWarps;
-    if (i >= st.count) {  // a row that is not there: whatever its columns hold is not looked at
+    // A row that is not there: its columns are not stored, but its scores count where the softmax asks whether any is above its maximum, so they must not
+    // follow from what lies in shared memory.  Those of packed tiles are whole numbers times 0.
+    if (i >= st.count) {
       if (lane == 0) rate[i] = ring_rate[i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) reinterpret_cast<T*>(smem + Cfg::kOffRing)[i * D + lane * E + j] = ElemTraits<T>::from_float(0.0f);
       continue;
     }
     float x[E], top = 0.0f;

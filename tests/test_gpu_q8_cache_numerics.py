@@ -120,3 +120,36 @@ def test_small_weights_of_pages_with_small_scales(cuda_device, dtype, ratio, cop
         lost = 2.0 ** -39 * weight.amax() * 2.0 * scale.max() * codes.abs().sum(0)
         bound = (share + lost).repeat_interleave(copies, dim=0) + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
         assert bool(((out[b, :, 0] - want).abs() <= bound).all()), (b, float(((out[b, :, 0] - want).abs() / bound).max()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim,group", [(128, 4), (256, 20), (128, 20), (64, 9), (128, 33), (256, 3)])
+def test_outputs_do_not_depend_on_what_calls_before_left_behind(cuda_device, dtype, dim, group):
+    """The same call again after others have left pages where its tiles have no rows: as numbers of the type some 2^127, whose products with keys are infinite
+    or, with keys of zero, are not.  Scores of a warp's second tile are above those of its first by less than 1 (in powers of two), where the running maximum may
+    stay or be raised."""
+    page, heads = 128, 40
+    lengths = [79, 127, 80]
+    cache = Cache(3, heads, dim, page, dtype, 2)
+    key, value = cache.new_tokens(127)
+    key = torch.where(torch.arange(127)[:, None] < 16, -4.0 - key.float() / 2, 0.0).to(dtype)
+    for b, n in enumerate(lengths):
+        cache.append(key[:, :, :n], value[:, :, :n], rows=[b])
+    gpu = cache.on(cuda_device)
+    past = cache.lengths.to(cuda_device)
+    query = (1.0 + torch.randn((3, heads * group, 1, dim), generator=cache.gen) / 16).to(dtype).to(cuda_device)
+    other = Cache(4, heads, 64, 16, dtype, 40)
+    size = 2 * 16 * 64
+    pages = torch.tensor([0, 0x7f], dtype=torch.uint8).repeat(other.pages.shape[2] // 2).expand(other.pages.shape).contiguous()
+    pages[:, :, size:size + 8] = torch.ones((pages.shape[0], heads, 2)).view(torch.uint8)
+    left = dict(other.on(cuda_device), packed_pages=pages.to(cuda_device))
+    plain = dict(left, packed_pages=torch.zeros_like(left["packed_pages"]))
+    n = torch.full((4,), 640, dtype=torch.long, device=cuda_device)
+    results = []
+    for tensors in (plain, left, plain, left):
+        for other_group in (1, 8):
+            noise = torch.randn((4, heads * other_group, 1, 64), generator=cache.gen).to(dtype).to(cuda_device)
+            anna_b200.run_q8_paged_attention(query=noise, lengths=n, scaling=0.01, **tensors)
+        results.append(anna_b200.run_q8_paged_attention(query=query, lengths=past, scaling=0.5 * math.log(2.0) / (4 * dim), **gpu))
+    for got in results[1:]:
+        assert int((got != results[0]).sum()) == 0
