@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
   // weights are sums of two, the second kRest times what the first leaves (16 rows of 32768 tokens, 4 queries a KV head: 174 us with one, 186 so; of four tokens
   // 260 and 292).
   constexpr float kRest = kFloat ? 4096.0f : 1.0f;
+  constexpr float kUnit = 1.0f / 4194304.0f;                 // of a query entry, its head's largest magnitude in [1, 2)
   extern __shared__ __align__(128) uint8_t smem[];
   float* rate = reinterpret_cast<float*>(smem + Cfg::kOffRate);
   float* ring_rate = reinterpret_cast<float*>(smem + Cfg::kOffRingRate);
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
     const float back = p.scaling * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - up) << 23);
     constexpr float kRingFactor = kHalf ? 16384.0f : 1.0f;
     if (lane == 0) {
-      rate[i] = fine ? back / 4194304.0f : __int_as_float(0x7fc00000);
+      rate[i] = fine ? back : __int_as_float(0x7fc00000);
       ring_rate[i] = back / kRingFactor;
     }
     // dims D / 4 t + 16 c .. are lane t's piece c; this lane's E dims lie in one piece, next to one another
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       // the top byte is signed, so what rounds up to 2^23 (fp32: 2^k less its last bit) stays half a unit below, as far off as any tie
-      const int whole = fine ? min(__float2int_rn(x[j] * factor * 4194304.0f), 8388607) : 0;
+      const int whole = fine ? min(__float2int_rn(x[j] * factor / kUnit), 8388607) : 0;
 #pragma unroll
       for (int n = 0; n < 3; ++n) bytes[n][j / 4] |= ((uint32_t)whole >> (16 - 8 * n) & 255u) << (8 * (j % 4));
       scaled[j] = ElemTraits<T>::from_float(x[j] * factor * kRingFactor);
@@ -390,8 +391,10 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)  // the lower two bytes' sums are below 2^23 each: together below 2^31
-        s[j][r] = fmaf(__int2float_rn(whole[j][0][r]), 65536.0f, __int2float_rn(whole[j][1][r] * 256 + whole[j][2][r])) *
+      // The lower two bytes' sums are below 2^23 each: together below 2^31.  The unit goes into the numbers and not into the rates, which for tiny queries
+      // (of huge keys) are small as it is.
+      for (int r = 0; r < 4; ++r)
+        s[j][r] = fmaf(__int2float_rn(whole[j][0][r]), 65536.0f * kUnit, __int2float_rn(whole[j][1][r] * 256 + whole[j][2][r]) * kUnit) *
                   (scale[r / 2 * (kPages - 1)].x * to_log2[j][r & 1]);
     bool cut = false;  // tokens that some rows do not see, or a page that is none
 #pragma unroll

@@ -153,3 +153,18 @@ def test_outputs_do_not_depend_on_what_calls_before_left_behind(cuda_device, dty
         results.append(anna_b200.run_q8_paged_attention(query=query, lengths=past, scaling=0.5 * math.log(2.0) / (4 * dim), **gpu))
     for got in results[1:]:
         assert int((got != results[0]).sum()) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("dim,page,group", [(64, 16, 1), (128, 24, 4), (256, 32, 10), (128, 5, 2)])
+@pytest.mark.parametrize("power", [-120, -108, 100, 116])
+def test_tiny_queries_of_huge_keys_and_huge_ones_of_tiny(cuda_device, dtype, dim, page, group, power):
+    """Scores of ordinary size from factors near the ends of the type."""
+    lengths = [3 * page + 3, 2 * page]
+    cache = Cache(2, 2, dim, page, dtype, 4, seed=dim)
+    key, value = cache.new_tokens(max(lengths))
+    key = (key.double() * 2.0 ** (-4 - power)).to(dtype)
+    for b, n in enumerate(lengths):
+        cache.append(key[:, :, :n], value[:, :, :n], rows=[b])
+    query = (torch.randn((2, 2 * group, 1, dim), generator=cache.gen).double() * 2.0 ** (power + 4)).to(dtype)
+    check_attention(cache, cache.on(cuda_device), query, cuda_device)
