@@ -150,7 +150,6 @@ __global__ void __launch_bounds__(kQ8AppendWarps * 32) q8_append_kernel(const Q8
   constexpr int kAtOnce = PER * (32 / kLanes);                 // tokens of the item's warps
   constexpr int kHeld = (PER == 1 ? 8 : 16) / kCols;           // rounds whose values stay in registers
   __shared__ uint4 s_extremes[PER == 1 ? 1 : 2 * PER * kVecs];
-  q8_let_next_start();
   q8_wait_for_previous();
   const int lane = threadIdx.x & 31, part = PER == 1 ? 0 : threadIdx.x >> 5;
   const uint32_t item = PER == 1 ? blockIdx.x * kQ8AppendWarps + (threadIdx.x >> 5) : blockIdx.x;
@@ -319,7 +318,6 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) q8_gather_kernel(const Q8GatherParams p) {
   constexpr int kN = ElemTraits<T>::kVec;
   constexpr int kPieces = D / 16;  // of a token
-  q8_let_next_start();
   q8_wait_for_previous();
   const int lane = threadIdx.x & 31;
   const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 5);

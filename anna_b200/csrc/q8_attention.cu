@@ -27,7 +27,6 @@ __global__ void __launch_bounds__(kQ8Threads<D>) q8_attention_kernel(const Q8Par
   __shared__ int sm_position[kQ8Tokens];         // in the sequence; past its end for what is not there
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  q8_let_next_start();
   q8_wait_for_previous();
   q8_for_each_segment<T, D, kThreads, kBlocks>(p, row_tiles, [&](int64_t b, int kvh, int tile, int t0, int t1, int len, const MultiPartial& part) {
   const Q8Stream st = q8_stream<kQ8Rows>(p, b, kvh, tile, len);

@@ -154,7 +154,6 @@ __global__ void __launch_bounds__(Q8Cfg<T, D, NT, W>::kThreads, Q8Cfg<T, D, NT, 
   const uint32_t copy_place = q8_place<D>(lane / (D / 16), lane % (D / 16)), key_place = q8_place<D>(gid, Cfg::kChunks * tig);
   const uint32_t value_place = 16 * D + (D == 64 ? q8_place<D>(2 * tig, gid / 2) + gid % 2 * 8 : q8_place<D>(2 * tig, D / 128 * gid));
   const uint32_t parts = smem_u32(smem + Cfg::kOffParts) + lane * 16;
-  q8_let_next_start();
   q8_wait_for_previous();
 
   q8_for_each_segment<T, D, Cfg::kThreads, kBlocks>(p, row_tiles, [&](int64_t b, int kvh, int tile, int t0, int t1, int len, const MultiPartial& part) {

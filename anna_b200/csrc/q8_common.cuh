@@ -143,17 +143,14 @@ __device__ __forceinline__ void q8_for_each_segment(const Q8Params& p, int row_t
   }
 }
 
-// Launches of this cache follow one another (append, selection, choice, attention), each of a few microseconds.  They go out with leave to
-// start while the kernel in front of them ends, and touch no memory before that has ended and its writes are there.  A kernel of more than two CTAs per
-// SM lets the next one start at its end alone: CTAs that wait beside it cost more than that saves (a prompt of 3001 tokens appended and viewed 16.4 us,
-// 11.7 so; a selection of one row 18.5 us without an early start, 17.6 with it).
+// Launches of this cache follow one another (append, selection, choice, attention), each of a few microseconds.  They go out with leave to be set up
+// while the kernel in front of them ends, and touch no memory before that has ended and its writes are there.  No kernel lets the next one start ahead of
+// its own end, as CTAs that wait beside it cost more than that saves: an append and attention of one row of 4000 tokens 11.9 us, 12.5 with early starts, 16.4
+// without leave; choice of 128 pages of 32 rows and attention 71.6, 81.7, 79.3; dense view of a prompt behind its append 10.8, 10.8, 14.4.
 //
-// So a kernel is on the GPU while the one in front of it still writes pages, and pages change their contents between two kernels on one SM: what is read of the
-// pool goes by coherent loads alone (__ldg and ld.global.nc are for memory that stays as it is while the kernel lives).
+// A kernel may be on the GPU all the same while the one in front of it still writes pages, and pages change their contents between two kernels on one SM: what is read
+// of the pool goes by coherent loads alone (__ldg and ld.global.nc are for memory that stays as it is while the kernel lives).
 __device__ __forceinline__ void q8_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void q8_let_next_start() {
-  if (gridDim.x * gridDim.y * gridDim.z <= 2 * 148) asm volatile("griddepcontrol.launch_dependents;");
-}
 
 template <typename... Params, typename... Args>
 int q8_launch(const char* what, void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, Args&&... args) {

@@ -115,7 +115,6 @@ __global__ void __launch_bounds__(kQ8SelectWarps * 32, kQ8SelectCtas<D>) q8_scor
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int candidates_of[kQ8SelectRows];
   __shared__ int s_prefix[kShares ? kBalancedMaxRows + 1 : 1];
-  q8_let_next_start();
   q8_wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
 
@@ -355,7 +354,6 @@ __global__ void __launch_bounds__(THREADS) q8_pick_kernel(const Q8SelectParams p
   __shared__ int histogram[256], s_before[kRounds * kWarps], s_digit, s_left, s_same, s_taken, s_few;
   __shared__ uint32_t s_high[kWarps], s_low[kWarps], few[32];
   __shared__ int s_some[kWarps], s_forced[kWarps];
-  q8_let_next_start();
   q8_wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t stream = blockIdx.x;
