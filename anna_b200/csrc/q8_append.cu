@@ -419,8 +419,9 @@ extern "C" int anna_q8_append(const void* k_new, int64_t k_stride_b, int64_t k_s
   p.batch = batch; p.kv_heads = kv_heads; p.tokens = new_tokens; p.block_size = block_size;
   p.units = (int)(((int64_t)new_tokens + block_size - 2) / block_size) + 1;
   p.page_bytes = (int)bytes; p.num_pages = num_pages; p.max_blocks = max_blocks; p.num_slots = num_slots; p.status = status;
-  // A CTA to an item where a warp would have more than 8 vectors a lane, or where the GPU has room for that: one row of one
-  // token and 8 KV heads takes 5.2 us so, 6.0 with a warp to an item; 512 tokens of 256 dims in pages of 32 14.5 and 24.6.
+  // A CTA to an item where a warp would have more than 8 vectors a lane, or where the GPU has room for that: 512 tokens of 256 dims in pages of 32
+  // take 4.5 us so, 7.8 with a warp to an item, 3001 such tokens 6.6 and 12.6, one token of 8 KV heads that fills its page 3.5 and 3.7.  A warp otherwise: 8 rows
+  // of 2048 tokens of 128 dims in pages of 16 take 16.4 us so, 45.7 with CTAs.
   const int64_t items = (int64_t)batch * kv_heads * p.units * 2;
   ANNA_REQUIRE(new_tokens < kQ8MaxLength && max_blocks < kQ8MaxLength / block_size && items < (1ll << 31), "%s: too many tokens", what);
   const bool whole = block_size * head_dim / vec > 256 || items <= 148 * 8;

@@ -2,7 +2,9 @@
 //
 // This form serves pages that are no multiple of 8 tokens; everything in it is 32 bits.  A CTA brings 32 tokens at a
 // time into shared memory, as floats without their scale, for its 8 rows; a warp scores two rows (256 dims: one) with a token a lane.
-// Bound: issue, of which the reads of shared memory are as many as the FMAs.
+// Bound: issue, of which the reads of shared memory are as many as the FMAs (16 rows of 32768 tokens in pages of 20, 4 queries a KV head, 3.2 ms; in pages of
+// 24, which tensor cores read, 0.21).  A tile of 16 tokens of those lies in one page or half and half in two; pages of other sizes would take a page lookup, scales and
+// a copy of their own for every token.
 #include "q8_common.cuh"
 
 namespace anna {
@@ -210,9 +212,9 @@ using namespace anna;
 namespace {
 
 constexpr int kQ8MinTiles = 4;   // of a CTA with blocks, CUDA cores
-// Tensor cores.  What a stream costs a CTA beside its tiles, in tiles; by this number (8, 16, 32, 64) 64 ragged rows of 0.5-16 K tokens 106, 105, 102,
-// 103 us, 16 rows of 0.4-4 K tokens of 256 dims 72, 67, 61, 67.  Positions of the line that a CTA takes at least; by this number (8, 16, 32, 64) one row of
-// 4000 tokens 13.4, 12.3, 14.1, 18.4; tiles of a list alike (one row's 256 pages: 4 to 12 tiles 15.2-13.3, 16 12.4, 24 and 32 13.3-13.7).
+// Tensor cores.  What a stream costs a CTA beside its tiles, in tiles; by this number (8, 16, 32, 64) 64 ragged rows of 0.5-16 K tokens 113, 107, 107,
+// 112 us, 16 rows of 0.4-4 K tokens of 256 dims 70, 68, 63, 70.  Positions of the line that a CTA takes at least; by this number (8, 16, 32, 64) one row of
+// 4000 tokens 11.5, 9.9, 11.2, 14.8; tiles of a list alike (one row's 256 pages: 4 to 12 tiles 9.8, 16 9.3, 24 10.9, 32 11.2).
 constexpr int kQ8StreamTiles = 32, kQ8MinShare = 16;
 
 // What a call takes; the sizes have been checked.

@@ -29,7 +29,7 @@
 
 namespace anna {
 
-// W warps: four, with several CTAs to an SM; eight, with one, where the tiles of a call are few (one row of 4000 tokens: 11.5 us with four, 10.7 with eight).
+// W warps: four, with several CTAs to an SM; eight, with one, where the tiles of a call are few (one row of 4000 tokens: 11.0 us with four, 9.9 with eight).
 template <typename T, int D, int NT, int W>
 struct Q8Cfg {
   static constexpr int kWarps = W;
@@ -68,7 +68,7 @@ __device__ __forceinline__ uint32_t q8_place(int token, int piece) {
   }
 }
 // What one lane's places differ by, so that few of them have to be worked out: the copy of pieces 32 i + lane, value tokens 2 t and 2 t + 1.
-// (All of them from q8_place in the loop: 469 instead of 430 instructions a tile, 16 rows of 32768 tokens 219 us, 213 so.)
+// (All of them from q8_place in the loop: 39 instructions a tile more, 3 % of the time of 16 rows of 32768 tokens.)
 template <int D>
 __host__ __device__ constexpr uint32_t kQ8CopyTurn(int i) {
   return D == 64 ? 0u : D == 128 ? (uint32_t)(i & 1) << 6 : (uint32_t)((i >> 1 & 1) << 2 | (i & 1)) << 4;

@@ -72,7 +72,7 @@ __device__ __forceinline__ int64_t q8_page_at(const Q8Params& p, const Q8Stream&
 //
 // With blocks all axes are as long, and the host has cut them: `splits` CTAs to a stream, 16-token tiles dealt evenly.  Else CTAs take even shares of a
 // line of all streams, as multi_for_each_segment cuts it; at most 32 rows are lined up by every warp by itself, without barriers and with one read of
-// the lengths (one row of 4000 tokens: 12.3 us, 11.7 so).
+// the lengths (one row of 4000 tokens 9.9 us either way; 12.3 and 11.7 when its tiles were scored with four warps).
 template <typename T, int D, int THREADS, bool kBlocks, typename Fn>
 __device__ __forceinline__ void q8_for_each_segment(const Q8Params& p, int row_tiles, Fn&& segment) {
   if constexpr (kBlocks) {

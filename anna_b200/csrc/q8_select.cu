@@ -56,7 +56,7 @@ __device__ __forceinline__ void mma_s8u8(int (&d)[4], uint32_t a0, uint32_t a1, 
 }
 
 // 16 bytes that are read once, coherently (see q8_wait_for_previous); half lines are fetched from memory, as bounds end a little way into a line (320 bytes a
-// page of 128 dims instead of 384).  (Past L1, as ld.global.cg: 32 rows of 20000 to 32768 tokens and the attention behind it 85.7 us, 80.2 so.)
+// page of 128 dims instead of 384).  (Past L1, as ld.global.cg: 32 rows of 20000 to 32768 tokens and the attention behind it take 5.5 us more.)
 __device__ __forceinline__ uint4 q8_load64(const uint4* ptr) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.L2::64B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
@@ -104,7 +104,7 @@ struct Q8Whole<float> {
 
 // Rows are the query heads of several tokens, one behind the other: the heads of a token are in one tile of 8 rows where their number divides 8, else
 // a token has tiles of its own.  The KV heads of a page lie next to one another, and a CTA's warps take them together: a page costs one translation of its
-// address and one stretch of memory (32 rows of 20000 to 32768 tokens in scattered pages, 8 KV heads: 39.6 us, 47.5 with CTAs of one
+// address and one stretch of memory (32 rows of 20000 to 32768 tokens in scattered pages, 8 KV heads: 34.5 us, 45.6 with CTAs of one
 // KV head).
 //
 // CTAs: a part of a stream (sequence, tokens, KV heads) each where the GPU holds them all at once; else one resident wave that takes even shares of the
@@ -584,8 +584,8 @@ extern "C" int anna_q8_select_blocks(const void* q, int64_t q_stride_b, int64_t 
   p.head_tiles = (p.row_group + 7) / 8;
   // As many KV heads as shared memory has room for with one token, then as many tokens.
   const int tile_bytes = 2 * (2 * head_dim / 64) * 512 + 32, room = 64 * 1024 / tile_bytes;
-  // Where warps have few tiles each, one KV head: what counts is how soon a CTA's queries are ready (one row of 8191 pages, 8 KV heads: all at once 20.0 us,
-  // one 17.4).
+  // Where warps have few tiles each, one KV head: what counts is how soon a CTA's queries are ready (8 KV heads, one row of 8191 pages: all at once 17.4 us,
+  // one 17.0; a row of 49160 tokens in pages of 16 12.7, 11.7).
   const int64_t page_tiles = (max_blocks + kQ8SelectTile - 1) / kQ8SelectTile, ctas = 148 * (head_dim == 256 ? kQ8SelectCtas<256> : kQ8SelectCtas<128>);
   const bool few = (int64_t)batch * kv_heads * page_tiles <= 2 * ctas * kQ8SelectWarps;
   p.heads_at_once = few || room / p.head_tiles < 1 ? 1 : room / p.head_tiles > kv_heads ? kv_heads : room / p.head_tiles;

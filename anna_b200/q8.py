@@ -12,6 +12,10 @@ unfinished page are as they came, in a ring (``include/anna_b200_kv.h`` has the 
 Pages are plain memory: ``run_page_copy`` copies them (and rings) for forks, a full page may be in the tables of several rows.  head_dim is
 64, 128 or 256, ``block_size`` at most 1024, types float32, float16 and bfloat16.  Calls work on the current stream, can be captured into a
 CUDA graph, and have no gradients.  The reference has no cache of this kind.
+
+Attention works in float32, and where ``block_size`` is a multiple of 8 on tensor cores: codes are exact there, the entries of a query head are whole
+numbers of 24 bits, off by 2^-23 of its largest magnitude at most, and a weight is a sum of two fp16 (over tokens of a bf16 ring of two bf16), off by
+2^-23 (2^-16) of itself.  That is as good as float32 unless a query's largest entries meet keys that are next to nothing there.
 """
 from __future__ import annotations
 
@@ -130,9 +134,10 @@ def _last_dim(tensor: torch.Tensor) -> torch.Tensor:
 def run_q8_paged_attention(*, query: torch.Tensor, packed_pages: torch.Tensor, page_table: torch.Tensor, window: torch.Tensor,
                            window_slots: torch.Tensor, lengths: torch.Tensor, scaling: float, gate: torch.Tensor | None = None,
                            blocks: torch.Tensor | None = None) -> torch.Tensor:
-    """Attention of the newest T tokens of every row: ``query`` ``[B, Hq, T, D]`` (any strides), ``lengths`` int64 ``[B]`` with the new
-    tokens among them; query ``t`` sees the keys up to position ``lengths[b] - T + t``, one that sees none gives zeros.  ``gate`` (shape and
-    dtype of the query): the output is multiplied by its sigmoid.
+    """Attention of the newest T tokens of every row: ``query`` ``[B, Hq, T, D]`` (any strides, ``Hq T`` below 2^20), ``lengths`` int64 ``[B]`` with
+    the new tokens among them; query ``t`` sees the keys up to position ``lengths[b] - T + t``, one that sees none gives zeros.  A length is cut at what table
+    and ring hold.  ``gate`` (shape and dtype of the query): the output is multiplied by its sigmoid.  An infinity or a NaN that a query sees shows in its
+    output, however small its weight.
 
     ``blocks``, int32 ``[B, Hkv, T, n]`` as ``run_q8_select_blocks`` gives them: of the full pages query ``t`` looks at those of its list
     alone, and at the unfinished page.  A list may be in any order; entries that are no full page of the row are left out, one that is named
